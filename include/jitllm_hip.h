@@ -438,6 +438,134 @@ int jl_gemm_xf16(jl_context *ctx, const jl_weight *const *weights, int count, co
 int jl_rms_apply_xf16(jl_context *ctx, float *X, const float *delta, const float *rms_weights, float eps,
                       int64_t rows, int64_t n, float *scales, uint16_t *out);
 
+/* ---- key-value cache in pages, and the attention that reads it ------------------------------- */
+/*
+ * What a layer runs between its q|k|v projection and its output projection.  One jl_kv_cache holds
+ * the keys and values of one layer in `pages` pages of `page_tokens` tokens; which pages a request
+ * has, and in which order, is in a block table that all layers share: entry b of a request's row is
+ * the page that holds its tokens b * page_tokens ... .  Positions, slots and tables are device int32
+ * arrays, so that a step's launches can be captured once and replayed while lengths grow.
+ *   slot      page * page_tokens + offset in the page: where a token's k and v lie in every layer
+ *   position  0, 1, ... inside its request: what the rotation turns by and the mask compares
+ * -1 in either means that the row has no token (padding of a captured batch, a request that got no
+ * page); such a row is skipped.
+ *
+ * Types.  JL_KV_F16: binary16.  JL_KV_Q8_0: blocks of 32 signed bytes with a binary16 scale d, as
+ * GGUF's Q8_0, of 53 % of the bytes; an element stands for the binary16 nearest to d * byte.
+ *
+ * Layout: [k, v][pages][kv_heads][part], where the part of one page and head is, for JL_KV_F16,
+ * [page_tokens][head_dim] binary16, and for JL_KV_Q8_0 [page_tokens][head_dim] bytes followed by
+ * [head_dim / 32][page_tokens] binary16 scales.  Heads of 64, 96, 128, 192 or 256 values (others:
+ * JL_ERR_UNSUPPORTED); pages of 16, 32, 64, 128 or 256 tokens; at most 2^31 - 1 tokens in all.
+ */
+typedef enum jl_kv_type { JL_KV_F16 = 1, JL_KV_Q8_0 = 8 } jl_kv_type;
+typedef struct jl_kv_cache jl_kv_cache;
+
+/* Device bytes of such a cache; 0 where jl_kv_cache_create would refuse it. */
+size_t jl_kv_cache_bytes(int kv_type, int64_t pages, int kv_heads, int head_dim, int page_tokens);
+/* Allocates the pages; what they hold is unspecified until it is written. */
+int jl_kv_cache_create(jl_context *ctx, int kv_type, int64_t pages, int kv_heads, int head_dim, int page_tokens,
+                       jl_kv_cache **out);
+/* The same over jl_kv_cache_bytes(...) bytes of device memory that the caller owns, 16-byte aligned. */
+int jl_kv_cache_wrap(jl_context *ctx, void *device_memory, int kv_type, int64_t pages, int kv_heads, int head_dim,
+                     int page_tokens, jl_kv_cache **out);
+int jl_kv_cache_free(jl_kv_cache *cache);
+void *jl_kv_cache_memory(const jl_kv_cache *cache);
+
+/*
+ * One step's pages, from request lengths that lie on the device: block tables, and for each of the
+ * step's rows (tokens, the requests' one behind the other) its request, position and slot.
+ *   past    [requests]  tokens each request has in the cache
+ *   fresh   [requests]  tokens it adds in this step: 1 where it decodes, a prompt's length where it
+ *                       begins, 0 where it waits; negative where it has ended
+ *   page_ring [pages], free_in [2], free_out [2]: the free pages, a ring.  free = {head, count}: the
+ *           next free page is page_ring[head], the others follow it cyclically.  All pages free at
+ *           the start: page_ring = 0, 1, ..., free = {0, pages}.  An impossible {head, count} is
+ *           taken as {0, 0}.
+ *   block_table [requests x table_stride]
+ *   lengths [requests], row_starts [requests + 1]; slots, positions, row_requests [max_rows]
+ * Request r takes rows row_starts[r] ... row_starts[r + 1] - 1, fresh[r] of them where that is
+ * positive; rows from row_starts[requests] on are padding (-1 in all three).  In request order, a
+ * request whose tokens fit its row of the table and the step's max_rows gets the pages it lacks from
+ * the ring while the ring has as many as it and those before it ask for; lengths[r] = past + fresh
+ * then.  One that does not (ring empty, table row or max_rows full, a `past` that no table row
+ * holds) gets nothing: lengths[r] = past[r], and its rows have slots and positions of -1.  An ended
+ * request's pages go behind the ring's last one, for the next step to take, and lengths[r] = 0.
+ * Only the table's new entries and the ring's returned pages are written; lengths may be past and
+ * free_out may be free_in, and with other arrays there the same call can be made again and leaves
+ * the same.  At most 8192 requests, 2^17 rows, 2^31 - 1 table entries.  One launch, or two where
+ * max_rows is large; the order of nothing depends on timing.
+ */
+int jl_kv_plan(jl_context *ctx, const int32_t *past, const int32_t *fresh, int64_t requests, int64_t pages,
+               int page_tokens, int32_t *page_ring, const int32_t *free_in, int32_t *free_out, int32_t *block_table,
+               int64_t table_stride, int32_t *lengths, int32_t *row_starts, int32_t *slots, int32_t *positions,
+               int32_t *row_requests, int64_t max_rows);
+
+/* Which elements of a head the rotation turns together: 2i and 2i + 1, or i and i + rotated / 2. */
+typedef enum jl_rope_style { JL_ROPE_PAIRS = 0, JL_ROPE_HALVES = 1 } jl_rope_style;
+
+/*
+ * Rotates q and k and writes k and v into the cache, `rows` tokens, in one launch.
+ *   q, k, v     fp32 rows of heads x head_dim and kv_heads x head_dim values, `ld*` floats apart: the
+ *               q|k|v that jl_gemv_qkv and jl_gemm leave, side by side or apart.  16-byte aligned,
+ *               strides a multiple of 4.  q null: only k and v (q_out is then not used).
+ *   q_out       the turned q, rows ldq_out floats apart; may be q (with ldq_out = ldq)
+ *   positions, slots  [rows]: a row whose position is negative is skipped altogether; one whose slot
+ *               is none of the cache's only leaves its q.  The slots of a call differ.
+ *   frequencies [rotated / 2] doubles on the device: pair i turns by positions[row] * frequencies[i]
+ *               radians (the angle is taken in double precision, as far positions need).  The first
+ *               `rotated` values of a head turn, a multiple of 16 up to head_dim; 0: none does, and
+ *               frequencies may be null.
+ *   q_norm, k_norm    [head_dim] fp32 or null: heads are normalised first, x <- w * (x / sqrt(sum x^2
+ *               / head_dim + eps)), as Qwen3's are
+ * A JL_KV_F16 element is the nearest binary16 (infinite where fp32 is beyond it).  A block of
+ * JL_KV_Q8_0 has d = the binary16 nearest to max |x| / 127 (at most 65504) and bytes rint(x / d)
+ * in -127 ... 127; 0 where d is 0 or x is NaN.
+ */
+int jl_kv_append(jl_context *ctx, jl_kv_cache *cache, const float *q, int heads, int64_t ldq, const float *k,
+                 int64_t ldk, const float *v, int64_t ldv, float *q_out, int64_t ldq_out, const int32_t *positions,
+                 const int32_t *slots, int64_t rows, const double *frequencies, int rotated, int rope_style,
+                 const float *q_norm, const float *k_norm, float eps);
+
+/*
+ * Decodes the k and v at `slots` ([rows]) to rows of kv_heads x head_dim values, binary16 (exact) or,
+ * with out_f16 == 0, fp32: the parity probe, and the way out of the cache for a prefix that is kept
+ * elsewhere.  Zeros where the slot is none of the cache's.  k_out and v_out 16-byte aligned; either
+ * may be null.
+ */
+int jl_kv_read(jl_context *ctx, const jl_kv_cache *cache, const int32_t *slots, int64_t rows, void *k_out,
+               void *v_out, int out_f16);
+
+/*
+ * Attention of one new token a row over its request's pages (grouped heads: query head h reads k / v
+ * head h / (heads / kv_heads)):
+ *   out[row][h] = sum_j p_j v_j,  p = softmax_j(scale * q[row][h] . k_j),  first <= j <= positions[row]
+ * with first = 0, or positions[row] - window + 1 where window > 0 and that is positive.
+ *   q    fp32 rows of heads x head_dim values, ldq floats apart (16-byte aligned, ldq a multiple of 4)
+ *   row_requests [rows]: the row of the block table that a row reads, or null: row i reads row i (and
+ *        requests >= rows).  Rows of one request may stand beside each other (a prompt's, a draft's):
+ *        each reads its own range.
+ *   out  fp32, or with out_f16 binary16 (rounded once, as the projections of jl_gemm_xf16 take it);
+ *        `ldo` of its values between rows; 16-byte aligned, ldo a multiple of 4 (fp32) or 8 (binary16)
+ * A row with nothing to read -- position -1, a request outside the table -- is zeros.  A position past
+ * the table's last token reads the tokens that the table holds.  A page outside the cache counts as
+ * one whose tokens are all masked.  What lies in the pages at masked tokens (other requests' or
+ * stale values, infinities, NaN) has no influence.  Scores, weights and sums are fp32 (q and the weights enter
+ * the matrix instructions as two binary16 parts each, 22 bits), so results are those of an fp32
+ * softmax.  The work is cut over the cache's length where rows are few or lengths differ, and
+ * joined in a fixed order: the same call gives the same bits, whose last few may differ between
+ * batches of other lengths.
+ * workspace: jl_kv_attention_workspace_bytes of the largest call that uses it, 16-byte aligned, for
+ * the parts that are joined; its contents need no preparation and do not outlive the call.  Calls
+ * that may run at the same time (graphs on two streams) need one each.
+ * At most 65535 rows; heads a multiple of kv_heads.
+ */
+size_t jl_kv_attention_workspace_bytes(int heads, int kv_heads, int head_dim);
+int jl_kv_attention(jl_context *ctx, const jl_kv_cache *cache, const float *q, int heads, int64_t ldq, int64_t rows,
+                    const int32_t *positions, const int32_t *row_requests, const int32_t *block_table,
+                    int64_t requests, int64_t table_stride, float scale, int64_t window, void *out, int out_f16,
+                    int64_t ldo, void *workspace, size_t workspace_bytes);
+
 /* ---- GGUF files: the caller either side of jl_weight_upload --------------------------------- */
 
 /*

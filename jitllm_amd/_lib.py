@@ -15,6 +15,8 @@ JL_OK = 0
 JL_ERR_INVALID, JL_ERR_UNSUPPORTED, JL_ERR_HIP, JL_ERR_OOM, JL_ERR_WORKSPACE = -1, -2, -3, -4, -5
 JL_STORE, JL_RESIDUAL, JL_SWIGLU = 0, 1, 2
 JL_MATH_DEFAULT, JL_MATH_F16, JL_MATH_INT8 = 0, 1, 2
+JL_KV_F16, JL_KV_Q8_0 = 1, 8
+JL_ROPE_PAIRS, JL_ROPE_HALVES = 0, 1
 ABI_VERSION = 1
 
 vp = C.c_void_p
@@ -68,6 +70,18 @@ SYMBOLS = {
     "jl_gemm_xf16": (C.c_int, [vp, C.POINTER(vp), C.c_int, vp, vp, C.c_int, i64, i64, i64, i64, C.c_int,
                                vp, C.c_size_t, vp, C.c_size_t, C.POINTER(C.c_int32)]),
     "jl_rms_apply_xf16": (C.c_int, [vp, vp, vp, vp, C.c_float, i64, i64, vp, vp]),
+    "jl_kv_cache_bytes": (C.c_size_t, [C.c_int, i64, C.c_int, C.c_int, C.c_int]),
+    "jl_kv_cache_create": (C.c_int, [vp, C.c_int, i64, C.c_int, C.c_int, C.c_int, C.POINTER(vp)]),
+    "jl_kv_cache_wrap": (C.c_int, [vp, vp, C.c_int, i64, C.c_int, C.c_int, C.c_int, C.POINTER(vp)]),
+    "jl_kv_cache_free": (C.c_int, [vp]),
+    "jl_kv_cache_memory": (vp, [vp]),
+    "jl_kv_plan": (C.c_int, [vp, vp, vp, i64, i64, C.c_int, vp, vp, vp, vp, i64, vp, vp, vp, vp, vp, i64]),
+    "jl_kv_append": (C.c_int, [vp, vp, vp, C.c_int, i64, vp, i64, vp, i64, vp, i64, vp, vp, i64, vp, C.c_int, C.c_int,
+                               vp, vp, C.c_float]),
+    "jl_kv_read": (C.c_int, [vp, vp, vp, i64, vp, vp, C.c_int]),
+    "jl_kv_attention_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int, C.c_int]),
+    "jl_kv_attention": (C.c_int, [vp, vp, vp, C.c_int, i64, i64, vp, vp, vp, i64, i64, C.c_float, i64, vp, C.c_int,
+                                  i64, vp, C.c_size_t]),
     "jl_gguf_open": (C.c_int, [C.c_char_p, C.POINTER(vp)]),
     "jl_gguf_close": (C.c_int, [vp]),
     "jl_gguf_version": (C.c_int, [vp]),

@@ -1,0 +1,258 @@
+"""The key-value cache in pages and the attention that reads it: host mirror of the jl_kv_* calls.
+
+What a decode step runs between the q|k|v projection and the output projection of
+``jitllm_amd.projections``::
+
+    tables = BlockTables(ctx, requests, blocksPerRequest, pages, pageTokens, maxRows)
+    caches = [PagedKvCache(ctx, KvType.F16, pages, kvHeads, headDim, pageTokens) for _ in layers]
+    rope = Rope.of_base(ctx, headDim, 500000.0)
+    attention = PagedAttention(ctx, maxRows, heads, kvHeads, headDim)
+    ...
+    tables.plan(fresh)                                   # once a step
+    for cache, layer in zip(caches, layers):             # in every layer
+        projections.fusedQKV(xb, qkv, layer.wq, layer.wk, layer.wv, rows)
+        cache.append(Rows(qkv, w, dim), Rows(qkv, w, dim + kv), tables.positions, tables.slots, rows, rope=rope,
+                     q=Rows(qkv, w), heads=heads)
+        attention.attend(cache, Rows(qkv, w), rows, tables.positions, tables.table, att, requests=requests,
+                         rowRequests=tables.rowRequests)
+        projections.projection(att, x, layer.wo, ...)
+
+Every array lies on the device, so the calls of a step can be captured into a graph once and replayed while
+the lengths grow.  The reference's own paged cache (J/backend/tornado/kernels/TransformerPagedKvKernels.java)
+is planned on the host; these calls plan, write and read on the device.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import enum
+import math
+
+import numpy as np
+
+from . import _lib as L
+from .runtime import Context, DeviceBuffer, HalfFloatArray
+
+
+class KvType(enum.IntEnum):
+    """What a cache keeps of an element (jl_kv_type)."""
+    F16 = L.JL_KV_F16
+    Q8_0 = L.JL_KV_Q8_0
+
+
+class RopeStyle(enum.IntEnum):
+    """Which elements of a head turn together: 2i and 2i + 1, or i and i + rotated / 2 (jl_rope_style)."""
+    PAIRS = L.JL_ROPE_PAIRS
+    HALVES = L.JL_ROPE_HALVES
+
+
+class IntArray(DeviceBuffer):
+    """int32 device array."""
+
+    def __init__(self, ctx: Context, size: int):
+        super().__init__(ctx, int(size) * 4)
+        self.size = int(size)
+
+    def set(self, values: np.ndarray) -> None:
+        values = np.ascontiguousarray(values, dtype=np.int32).reshape(-1)
+        if values.size != self.size:
+            raise ValueError(f"{values.size} values for an IntArray of {self.size}")
+        self.upload(values)
+
+    def get(self) -> np.ndarray:
+        return self.download(np.int32, self.size)
+
+
+class Rows:
+    """Rows of a device array that lie ``stride`` elements apart, the first ``offset`` elements in: the q, k
+    or v part of the rows that a fused projection leaves side by side."""
+
+    def __init__(self, array, stride: int, offset: int = 0):
+        self.array, self.stride, self.offset = array, int(stride), int(offset)
+        self.itemsize = array.nbytes // array.size if array.size else 4
+
+    def ptr(self, who: str, rows: int, width: int) -> int:
+        """Address of the first row; raises where ``rows`` rows of ``width`` elements are not the array's."""
+        if self.stride < width or self.offset < 0 or (rows and self.offset + (rows - 1) * self.stride + width > self.array.size):
+            raise ValueError(f"{who}: {rows} rows of {width} elements, {self.stride} apart from {self.offset} on, "
+                             f"in an array of {self.array.size}")
+        return _address(self.array) + self.offset * self.itemsize
+
+
+def _address(array) -> int:
+    return array.ptr.value or 0
+
+
+def _rows(value, width: int) -> Rows:
+    return value if isinstance(value, Rows) else Rows(value, width)
+
+
+def _ints(who: str, array, count: int) -> int:
+    if array.nbytes < 4 * count:
+        raise ValueError(f"{who}: {count} int32 values in an array of {array.nbytes} bytes")
+    return _address(array)
+
+
+class Rope:
+    """A rotation: ``rotated`` values of every head turn, pair i by position * frequencies[i] radians.
+
+    ``frequencies`` is a device array of ``rotated / 2`` doubles, so that any scaling of them is the caller's;
+    ``of_base`` makes the plain ones."""
+
+    def __init__(self, ctx: Context, frequencies, rotated: int, style: RopeStyle = RopeStyle.PAIRS):
+        if frequencies.nbytes < 4 * rotated:
+            raise ValueError(f"{rotated // 2} frequencies in an array of {frequencies.nbytes} bytes")
+        self.ctx, self.frequencies, self.rotated, self.style = ctx, frequencies, int(rotated), RopeStyle(style)
+
+    @classmethod
+    def of(cls, ctx: Context, frequencies, style: RopeStyle = RopeStyle.PAIRS) -> "Rope":
+        values = np.ascontiguousarray(frequencies, dtype=np.float64).reshape(-1)
+        memory = ctx.raw_buffer(values.nbytes)
+        memory.upload(values)
+        return cls(ctx, memory, 2 * values.size, style)
+
+    @classmethod
+    def of_base(cls, ctx: Context, rotated: int, base: float, style: RopeStyle = RopeStyle.PAIRS) -> "Rope":
+        return cls.of(ctx, float(base) ** (-np.arange(0, rotated, 2, dtype=np.float64) / rotated), style)
+
+
+class PagedKvCache:
+    """One layer's keys and values in pages (jl_kv_cache).  ``memory``: a device array that holds the pages
+    and stays the caller's; without one the cache allocates them."""
+
+    def __init__(self, ctx: Context, kvType: KvType, pages: int, kvHeads: int, headDim: int, pageTokens: int, memory=None):
+        self.ctx, self._lib = ctx, ctx._lib
+        self.type = KvType(kvType)
+        self.pages, self.kvHeads, self.headDim, self.pageTokens = int(pages), int(kvHeads), int(headDim), int(pageTokens)
+        self.memory = memory
+        h = C.c_void_p()
+        if memory is None:
+            L.check(self._lib.jl_kv_cache_create(ctx.handle, self.type, pages, kvHeads, headDim, pageTokens, C.byref(h)))
+        else:
+            want = self.bytes_for(self.type, pages, kvHeads, headDim, pageTokens)
+            if memory.nbytes < want:
+                raise ValueError(f"{memory.nbytes} bytes for a cache of {want}")
+            L.check(self._lib.jl_kv_cache_wrap(ctx.handle, memory.ptr, self.type, pages, kvHeads, headDim, pageTokens, C.byref(h)))
+        self.handle = h
+
+    @staticmethod
+    def bytes_for(kvType: KvType, pages: int, kvHeads: int, headDim: int, pageTokens: int) -> int:
+        return L.load().jl_kv_cache_bytes(int(kvType), pages, kvHeads, headDim, pageTokens)
+
+    @property
+    def nbytes(self) -> int:
+        return self.bytes_for(self.type, self.pages, self.kvHeads, self.headDim, self.pageTokens)
+
+    def free(self) -> None:
+        if self.handle and self.ctx.handle:
+            L.check(self._lib.jl_kv_cache_free(self.handle))
+        self.handle = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+    def append(self, k, v, positions, slots, rows: int, rope: Rope | None = None, q=None, qOut=None, heads: int = 0,
+               qNorm=None, kNorm=None, eps: float = 0.0) -> None:
+        """Turns q and k (normalised first where ``qNorm`` / ``kNorm`` are given) and writes k and v to
+        ``slots`` (jl_kv_append).  ``q`` is turned into ``qOut``, or in place without one."""
+        width, qWidth = self.kvHeads * self.headDim, heads * self.headDim
+        k, v = _rows(k, width), _rows(v, width)
+        q = _rows(q, qWidth) if q is not None else None
+        qOut = q if qOut is None else _rows(qOut, qWidth)
+        for name, norm in (("qNorm", qNorm), ("kNorm", kNorm)):
+            if norm is not None and norm.size != self.headDim:
+                raise ValueError(f"{name} has {norm.size} weights, a head {self.headDim} values")
+        L.check(self._lib.jl_kv_append(
+            self.ctx.handle, self.handle, q.ptr("q", rows, qWidth) if q else None, heads, q.stride if q else 0,
+            k.ptr("k", rows, width), k.stride, v.ptr("v", rows, width), v.stride, qOut.ptr("qOut", rows, qWidth) if q else None,
+            qOut.stride if q else 0, _ints("positions", positions, rows), _ints("slots", slots, rows), rows,
+            rope.frequencies.ptr if rope else None, rope.rotated if rope else 0, rope.style if rope else RopeStyle.PAIRS,
+            qNorm.ptr if qNorm is not None else None, kNorm.ptr if kNorm is not None else None, float(eps)))
+
+    def read(self, slots, rows: int, k=None, v=None) -> None:
+        """Decodes the k and v at ``slots`` into rows of kvHeads x headDim values, binary16 or fp32 by the
+        arrays' elements (jl_kv_read)."""
+        need = rows * self.kvHeads * self.headDim
+        half = None
+        for name, array in (("k", k), ("v", v)):
+            if array is None:
+                continue
+            if array.size < need:
+                raise ValueError(f"{name} has {array.size} elements, {need} are read")
+            size = array.nbytes // max(1, array.size)
+            if half is not None and half != (size == 2):
+                raise ValueError("k and v are read into elements of one type")
+            half = size == 2
+        L.check(self._lib.jl_kv_read(self.ctx.handle, self.handle, _ints("slots", slots, rows), rows,
+                                     k.ptr if k is not None else None, v.ptr if v is not None else None, int(bool(half))))
+
+
+class BlockTables:
+    """The pages of a batch's requests, and the rows of a step (jl_kv_plan).
+
+    Device arrays: ``table`` [requests x blocksPerRequest], ``lengths`` [requests], ``rowStarts``
+    [requests + 1], ``slots``, ``positions`` and ``rowRequests`` [maxRows], and the free pages, a ring
+    ``pageRing`` [pages] with ``freePages`` = {head, count}.  ``arrays`` gives some or all of them; those not
+    given are allocated, and start with no tokens and every page free."""
+
+    def __init__(self, ctx: Context, requests: int, blocksPerRequest: int, pages: int, pageTokens: int, maxRows: int, arrays=None):
+        self.ctx, self._lib = ctx, ctx._lib
+        self.requests, self.blocksPerRequest, self.pages = int(requests), int(blocksPerRequest), int(pages)
+        self.pageTokens, self.maxRows = int(pageTokens), int(maxRows)
+        sizes = {"table": requests * blocksPerRequest, "lengths": requests, "rowStarts": requests + 1, "slots": maxRows,
+                 "positions": maxRows, "rowRequests": maxRows, "pageRing": pages, "freePages": 2}
+        start = {"table": lambda n: np.full(n, -1), "pageRing": np.arange, "freePages": lambda n: np.array([0, pages])}
+        given = dict(arrays or {})
+        for name, size in sizes.items():
+            array = given.pop(name, None)
+            if array is None:
+                array = IntArray(ctx, size)
+                if size:
+                    array.set(start.get(name, np.zeros)(size))
+            elif array.nbytes < 4 * size:
+                raise ValueError(f"{name}: {array.nbytes} bytes for {size} int32 values")
+            setattr(self, name, array)
+        if given:
+            raise ValueError(f"no such arrays: {', '.join(sorted(given))}")
+
+    def plan(self, fresh, past=None, freeIn=None) -> None:
+        """One step: ``fresh`` [requests] new tokens of each request (negative: it has ended).  Lengths and
+        free pages move on in place; ``past`` / ``freeIn`` give others to start from."""
+        for name, array, count in (("fresh", fresh, self.requests), ("past", past, self.requests), ("freeIn", freeIn, 2)):
+            if array is not None:
+                _ints(name, array, count)
+        L.check(self._lib.jl_kv_plan(
+            self.ctx.handle, (past or self.lengths).ptr, fresh.ptr, self.requests, self.pages, self.pageTokens, self.pageRing.ptr,
+            (freeIn or self.freePages).ptr, self.freePages.ptr, self.table.ptr, self.blocksPerRequest, self.lengths.ptr,
+            self.rowStarts.ptr, self.slots.ptr, self.positions.ptr, self.rowRequests.ptr, self.maxRows))
+
+
+class PagedAttention:
+    """Attention of one new token a row over paged caches of one shape, with the workspace it joins in
+    (jl_kv_attention).  One object for every layer; calls that may run at the same time need one each."""
+
+    def __init__(self, ctx: Context, maxRows: int, heads: int, kvHeads: int, headDim: int):
+        self.ctx, self._lib = ctx, ctx._lib
+        self.maxRows, self.heads, self.kvHeads, self.headDim = int(maxRows), int(heads), int(kvHeads), int(headDim)
+        nbytes = self._lib.jl_kv_attention_workspace_bytes(heads, kvHeads, headDim)
+        if not nbytes:
+            raise ValueError(f"{heads} query heads over {kvHeads} of k and v, {headDim} values each")
+        self.workspace = ctx.raw_buffer(nbytes)
+
+    def attend(self, cache: PagedKvCache, q, rows: int, positions, table, out, requests: int, rowRequests=None,
+               scale: float | None = None, window: int = 0) -> None:
+        """``out[row] = softmax(scale * q[row] . k) v`` over the tokens up to ``positions[row]`` (the last
+        ``window`` of them where that is positive) of request ``rowRequests[row]``, or of request ``row``.
+        ``scale``: 1 / sqrt(headDim) unless given.  ``out``: a FloatArray or a HalfFloatArray."""
+        width = self.heads * self.headDim
+        if (cache.kvHeads, cache.headDim) != (self.kvHeads, self.headDim):
+            raise ValueError(f"a cache of {cache.kvHeads} heads of {cache.headDim}, attention over {self.kvHeads} of {self.headDim}")
+        q, out = _rows(q, width), _rows(out, width)
+        stride = table.nbytes // 4 // requests if requests else 0
+        L.check(self._lib.jl_kv_attention(
+            self.ctx.handle, cache.handle, q.ptr("q", rows, width), self.heads, q.stride, rows, _ints("positions", positions, rows),
+            _ints("rowRequests", rowRequests, rows) if rowRequests is not None else None, table.ptr, requests, max(1, stride),
+            float(scale if scale is not None else 1 / math.sqrt(self.headDim)), window, out.ptr("out", rows, width),
+            int(out.itemsize == 2), out.stride, self.workspace.ptr, self.workspace.nbytes))

@@ -1,0 +1,651 @@
+"""The paged key-value cache's operators on the GPU against numpy in 64 bits."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import kv_models as M
+from gpu_util import say
+
+pytestmark = pytest.mark.gpu
+
+HALF = 2.0 ** -11            # half a step of binary16, relative to the value
+ULP = 2.0 ** -24             # ... of fp32
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    from jitllm_amd.runtime import Context
+    c = Context(0)
+    yield c
+    c.close()
+
+
+def ints(ctx, values):
+    from jitllm_amd.attention import IntArray
+    values = np.asarray(values, np.int32).reshape(-1)
+    a = IntArray(ctx, max(1, values.size))
+    if values.size:
+        a.upload(values)
+    a.size = values.size
+    return a
+
+
+def random_pool(rng, q8, pages, heads, dim, page, spread=1.0):
+    """A cache's bytes: normal values, or blocks of uniform bytes with scales of their own."""
+    per = M.part_bytes(q8, dim, page)
+    if not q8:
+        return (spread * rng.standard_normal((2, pages, heads, page * dim))).astype(np.float16).view(np.uint8).reshape(-1)
+    raw = np.empty((2, pages, heads, per), np.uint8)
+    raw[..., :page * dim] = rng.integers(-127, 128, (2, pages, heads, page * dim)).astype(np.int8).view(np.uint8)
+    d = (spread * rng.uniform(0.004, 0.03, (2, pages, heads, page * dim // 32))).astype(np.float16)
+    raw[..., page * dim:] = d.view(np.uint8).reshape(2, pages, heads, -1)
+    return raw.reshape(-1)
+
+
+def cache_of(ctx, q8, pages, heads, dim, page, raw):
+    from jitllm_amd.attention import KvType, PagedKvCache
+    memory = ctx.raw_buffer(raw.nbytes)
+    memory.upload(raw)
+    return PagedKvCache(ctx, KvType.Q8_0 if q8 else KvType.F16, pages, heads, dim, page, memory=memory)
+
+
+def pool_bytes(cache):
+    return cache.memory.download(np.uint8, cache.nbytes)
+
+
+# ---- jl_kv_plan ----------------------------------------------------------------------------------
+
+NAMES = ("lengths", "rowStarts", "table", "pageRing", "freePages", "slots", "positions", "rowRequests")
+
+
+def run_plan(ctx, past, fresh, pages, page, ring, free, table, max_rows, in_place=False):
+    from jitllm_amd.attention import BlockTables
+    requests, stride = table.shape
+    t = BlockTables(ctx, requests, stride, pages, page, max_rows)
+    t.table.set(table), t.pageRing.set(ring)
+    if in_place:
+        t.lengths.set(past), t.freePages.set(free)
+        t.plan(ints(ctx, fresh))
+    else:
+        t.plan(ints(ctx, fresh), past=ints(ctx, past), freeIn=ints(ctx, free))
+    ctx.sync()
+    return t
+
+
+def check_plan(ctx, t, want):
+    for name in NAMES:
+        got = getattr(t, name).get() if getattr(t, name).size else np.zeros(0)
+        assert np.array_equal(got, want[name].reshape(-1)), name
+
+
+def random_step(rng, requests, page, stride, pages=None, prompts=0.1, free_share=1.5):
+    past = rng.integers(0, stride * page, requests)
+    fresh = rng.choice([1, 1, 1, 1, 1, 0, -1], requests)
+    begin = rng.random(requests) < prompts
+    past[begin], fresh[begin] = 0, rng.integers(1, stride * page + 1, int(begin.sum()))
+    had = -(-past // page)
+    need = np.maximum(0, -(-(past + np.maximum(fresh, 0)) // page) - had)
+    free = int(need.sum() * free_share)
+    pages = pages or int(had.sum()) + free + 3
+    order = rng.permutation(pages)
+    table = np.full((requests, stride), -1)
+    table[np.arange(stride) < had[:, None]] = order[:had.sum()]
+    head = int(rng.integers(0, pages))
+    ring = np.full(pages, -1)
+    ring[(head + np.arange(free)) % pages] = order[had.sum():had.sum() + free]
+    return past, fresh, pages, ring, np.array([head, free]), table
+
+
+@pytest.mark.parametrize("requests,page,stride,max_rows,free_share", [
+    (1, 16, 4, 64, 1.5), (64, 16, 256, 512, 1.5), (65, 32, 7, 300, 0.5), (1023, 64, 5, 20000, 1.0), (1025, 128, 9, 40000, 0.4),
+    (2500, 16, 3, 2500, 1.1), (4096, 256, 4, 131072, 1.5), (8192, 16, 2, 9000, 0.9), (200, 64, 100, 131072, 1.2)])
+def test_plan_is_the_sequential_one(ctx, requests, page, stride, max_rows, free_share):
+    say("plan", requests, page, stride, max_rows, free_share)
+    rng = np.random.default_rng(requests + page)
+    past, fresh, pages, ring, free, table = random_step(rng, requests, page, stride, free_share=free_share)
+    want = M.plan(past, fresh, pages, page, ring, free, table, max_rows)
+    t = run_plan(ctx, past, fresh, pages, page, ring, free, table, max_rows)
+    check_plan(ctx, t, want)
+    # the same call over what it left leaves the same
+    t.plan(ints(ctx, fresh), past=ints(ctx, past), freeIn=ints(ctx, free))
+    ctx.sync()
+    check_plan(ctx, t, want)
+    check_plan(ctx, run_plan(ctx, past, fresh, pages, page, ring, free, table, max_rows, in_place=True), want)
+
+
+PLAN_EDGES = {
+    # past, fresh, pages, ring, free, blocks a request, max_rows
+    "nothing waits": ([0, 0], [0, 0], 4, [0, 1, 2, 3], [0, 4], 2, 4),
+    "no rows": ([3], [1], 4, [1, 2, 3, 0], [0, 3], 2, 0),
+    "a page's last token, its first, the table's last": ([15, 16, 31, 32], [1, 1, 1, 1], 12, range(12), [0, 12], 2, 8),
+    "a prompt as long as the table row, one longer": ([0, 0], [32, 33], 8, range(8), [6, 8], 2, 80),
+    "ring empty: none but those with room go on": ([16, 5, 0, 7], [1, 1, 3, 2], 4, range(4), [2, 0], 2, 9),
+    "one page for two": ([16, 16, 3], [1, 1, 1], 4, range(4), [3, 1], 2, 9),
+    "a large request in front of small ones": ([0, 0, 0], [40, 3, 3], 8, range(8), [0, 2], 4, 64),
+    "lengths that no row holds": ([-1, 33, -5, 2**31 - 1], [1, 1, -1, 1], 8, range(8), [0, 8], 2, 8),
+    "a fresh of 2^31 - 1": ([0, 4], [2**31 - 1, 1], 8, range(8), [0, 8], 2, 8),
+    "no such ring": ([0, 4, 20], [1, 1, -1], 8, range(8), [9, 4], 2, 8),
+    "no such ring either": ([0, 4, 20], [1, 1, -1], 8, range(8), [1, 9], 2, 8),
+    "negative": ([0, 4, 20], [1, 1, -1], 8, range(8), [-1, 4], 2, 8),
+    "more comes back than was missing": ([32, 32, 32], [-1, -1, -1], 5, range(5), [4, 2], 2, 8),
+    "all end": ([32, 1, 0, 17], [-1, -7, -1, -2**31], 12, range(12), [5, 0], 2, 8),
+    "rows that pass the step's end": ([0, 0, 0], [5, 6, 2], 8, range(8), [0, 8], 2, 8),
+}
+
+
+@pytest.mark.parametrize("name", PLAN_EDGES)
+def test_plan_edges(ctx, name):
+    say("plan edge", name)
+    past, fresh, pages, ring, free, stride, max_rows = PLAN_EDGES[name]
+    requests = len(past)
+    # bad entries among the good: pages outside the cache give no slot
+    table = (np.arange(requests * stride).reshape(requests, stride) * 7) % (pages + 2) - 1
+    ring = np.array(list(ring))
+    want = M.plan(past, fresh, pages, 16, ring, free, table, max_rows)
+    check_plan(ctx, run_plan(ctx, np.array(past), np.array(fresh), pages, 16, ring, np.array(free), table, max_rows), want)
+
+
+def test_plan_of_no_requests(ctx):
+    from jitllm_amd.attention import BlockTables
+    t = BlockTables(ctx, 0, 4, 5, 16, 6)
+    t.plan(ints(ctx, []))
+    ctx.sync()
+    assert t.rowStarts.get().tolist() == [0] and t.freePages.get().tolist() == [0, 5]
+    assert t.slots.get().tolist() == t.positions.get().tolist() == t.rowRequests.get().tolist() == [-1] * 6
+
+
+def test_plan_many_steps_lose_no_page(ctx):
+    """A server's life: requests begin, decode, wait, end; in place, step after step, against the sequential one."""
+    from jitllm_amd.attention import BlockTables
+    rng = np.random.default_rng(8)
+    requests, stride, page, pages, max_rows = 40, 8, 16, 150, 400
+    t = BlockTables(ctx, requests, stride, pages, page, max_rows)
+    state = {"lengths": np.zeros(requests, int), "table": np.full((requests, stride), -1), "pageRing": np.arange(pages), "freePages": np.array([0, pages])}
+    for step in range(60):
+        fresh = np.where(state["lengths"] == 0, rng.integers(0, 60, requests) * (rng.random(requests) < 0.4),
+                         rng.choice([1, 1, 1, 0, -1], requests, p=[0.4, 0.3, 0.15, 0.1, 0.05]))
+        say("step", step)
+        t.plan(ints(ctx, fresh))
+        state = M.plan(state["lengths"], fresh, pages, page, state["pageRing"], state["freePages"], state["table"], max_rows)
+        ctx.sync()
+        check_plan(ctx, t, state)
+        held = [state["table"][r, :-(-state["lengths"][r] // page)] for r in range(requests)]
+        free = state["pageRing"][(state["freePages"][0] + np.arange(state["freePages"][1])) % pages]
+        assert sorted(np.concatenate(held + [free])) == list(range(pages))
+
+
+# ---- jl_kv_append and jl_kv_read -----------------------------------------------------------------
+
+def run_append(ctx, cache, x, heads, kv, dim, positions, slots, freq, halves, qn, kn, eps, apart=False, pad=0, in_place=False):
+    """x [rows][heads + 2 kv][dim] -> q as the call leaves it."""
+    from jitllm_amd.attention import Rope, RopeStyle, Rows
+    rows = len(x)
+    rope = Rope.of(ctx, freq, RopeStyle.HALVES if halves else RopeStyle.PAIRS) if len(freq) else None
+    norms = dict(qNorm=ctx.from_numpy(qn) if qn is not None else None, kNorm=ctx.from_numpy(kn) if kn is not None else None, eps=eps)
+    w = heads * dim
+    sentinel = np.float32(-77.25)
+    if apart:
+        q, k, v = (ctx.from_numpy(part) for part in (x[:, :heads], x[:, heads:heads + kv], x[:, heads + kv:]))
+        qr, kr, vr = Rows(q, w), Rows(k, kv * dim), Rows(v, kv * dim)
+    else:
+        stride = (heads + 2 * kv) * dim + pad
+        flat = np.full((rows, stride), sentinel, np.float32)
+        flat[:, :stride - pad] = x.reshape(rows, -1)
+        q = ctx.from_numpy(flat)
+        qr, kr, vr = Rows(q, stride), Rows(q, stride, w), Rows(q, stride, w + kv * dim)
+    out = q if in_place else ctx.float_array(rows * (w + pad), fill=float(sentinel))
+    outr = qr if in_place else Rows(out, w + pad)
+    cache.append(kr, vr, ints(ctx, positions), ints(ctx, slots), rows, rope=rope, q=qr if heads else None, qOut=outr if heads else None,
+                 heads=heads, **norms)
+    ctx.sync()
+    got = out.get()
+    if not heads:
+        return None
+    got = np.lib.stride_tricks.as_strided(got, (rows, w), (outr.stride * 4, 4)).copy()
+    if pad and not in_place:
+        rest = out.get().reshape(rows, -1)[:, w:]
+        assert (rest == sentinel).all()
+    return got.reshape(rows, heads, dim)
+
+
+APPENDS = [
+    # rows, heads, kv, dim, page, q8, halves, turned, norm, context
+    (1, 32, 8, 64, 16, False, False, 64, False, 1000), (1, 14, 2, 64, 16, True, True, 64, False, 5), (3, 28, 4, 128, 32, False, True, 128, False, 131072),
+    (64, 32, 8, 128, 32, True, True, 128, True, 8192), (65, 5, 5, 96, 16, True, False, 96, True, 700), (33, 3, 1, 96, 64, False, True, 48, True, 900),
+    (17, 8, 2, 192, 128, True, True, 96, False, 100000), (40, 16, 4, 256, 16, True, False, 256, True, 4096), (7, 71, 1, 64, 256, False, False, 32, False, 60),
+    (300, 4, 2, 128, 64, False, False, 128, False, 2000000), (20, 8, 8, 128, 16, True, False, 0, False, 50), (9, 0, 4, 128, 16, False, True, 64, True, 77)]
+
+
+@pytest.mark.parametrize("rows,heads,kv,dim,page,q8,halves,turned,norm,context", APPENDS)
+def test_append(ctx, rows, heads, kv, dim, page, q8, halves, turned, norm, context):
+    say("append", rows, heads, kv, dim, page, q8, halves, turned, norm, context)
+    rng = np.random.default_rng(rows + dim + page)
+    pages = rows // page + 3
+    x = rng.standard_normal((rows, heads + 2 * kv, dim)).astype(np.float32)
+    x[:, :, 3] *= 20                                           # a channel that stands out, as keys have
+    x[rows // 2, heads + 2 * kv - 1, :32] = 0                  # a block of zeros
+    raw = random_pool(rng, q8, pages, kv, dim, page)
+    cache = cache_of(ctx, q8, pages, kv, dim, page, raw)
+    slots = rng.permutation(pages * page)[:rows]
+    positions = rng.integers(0, context, rows)
+    freq = 500000.0 ** (-np.arange(0, turned, 2) / turned) if turned else np.zeros(0)
+    qn, kn = (1 + 0.1 * rng.standard_normal(dim).astype(np.float32) for _ in range(2)) if norm else (None, None)
+    eps = 1e-6
+    if rows > 2:
+        slots[1], positions[2] = -1, -1                        # no page; no token at all
+    if rows > 3:
+        slots[3] = pages * page                                # a slot behind the cache's last
+    apart = rows % 2 == 1
+    got = run_append(ctx, cache, x, heads, kv, dim, positions, slots, freq, halves, qn, kn, eps, apart=apart, pad=0 if apart else 8)
+    after = M.decode_pool(pool_bytes(cache), q8, pages, kv, dim, page)
+    before = M.decode_pool(raw, q8, pages, kv, dim, page)
+    live = positions >= 0
+    # A turned value is two products and a sum over cos and sin that are exact to fp32 but for the rounding of
+    # an angle below pi (2^-24 pi of it) and the functions' own few units: 10 ulp of |a| + |b| cover them, and
+    # a norm's sum of dim squares, division, root and products another dim / 2 + 8 of the value.
+    step = (10 + (dim / 2 + 8 if norm else 0)) * ULP
+    k = M.rotate(x[:, heads:heads + kv], np.maximum(positions, 0), freq, halves, kn, eps)
+    size = lambda y: np.abs(y).max(-1, keepdims=True) * 2      # noqa: E731  (|a| + |b| of any pair of the head)
+    if heads:
+        q = M.rotate(x[:, :heads], np.maximum(positions, 0), freq, halves, qn, eps)
+        assert (np.abs(got - q) <= step * size(q))[live].all()
+        assert (got[~live] == -77.25).all()
+    v = x[:, heads + kv:].astype(np.float64)
+    written = np.zeros((pages, page), bool)
+    for which, y, slack in ((0, k, step * size(k)), (1, v, 0.0 * size(v))):
+        for i in range(rows):
+            if not live[i] or not 0 <= slots[i] < pages * page:
+                continue
+            at = after[which, slots[i] // page, :, slots[i] % page]
+            written[slots[i] // page, slots[i] % page] = True
+            if not q8:
+                assert (np.abs(at - y[i]) <= slack[i] + HALF * np.abs(y[i]) + 2.0 ** -25).all()
+                continue
+            kept, d, _ = M.encode_blocks(y[i])
+            # half a step of the block's scale, which is half a binary16 step off max / 127 (an end is clamped by that);
+            # the value itself is rounded to binary16
+            d = np.repeat(d, 32, -1)
+            assert (np.abs(at - y[i]) <= d / 2 * (1 + 2 * HALF) + slack[i] + 2 * HALF * np.abs(y[i]) + 2.0 ** -24).all()
+            if which == 1:                                     # nothing but copies in front of it: the very bytes
+                assert np.array_equal(at, (kept * d).astype(np.float16).astype(np.float64))
+    keep = np.broadcast_to(~written[None, :, None, :, None], after.shape)
+    assert np.array_equal(after[keep], before[keep])
+
+
+def test_append_in_place_is_the_same(ctx):
+    rng = np.random.default_rng(3)
+    for halves in (False, True):
+        for dim, turned in ((64, 64), (96, 64), (256, 256)):
+            x = rng.standard_normal((37, 6, dim)).astype(np.float32)
+            raw = random_pool(rng, False, 4, 1, dim, 16)
+            freq = 1e4 ** (-np.arange(0, turned, 2) / turned)
+            slots, positions = np.arange(37), rng.integers(0, 9999, 37)
+            say("append in place", halves, dim, turned)
+            norm = rng.standard_normal(dim).astype(np.float32)
+            two = [run_append(ctx, cache_of(ctx, False, 4, 1, dim, 16, raw), x, 4, 1, dim, positions, slots, freq, halves, norm, None, 1e-5, in_place=p)
+                   for p in (False, True)]
+            assert np.array_equal(two[0], two[1])
+
+
+@pytest.mark.parametrize("q8", [False, True])
+def test_append_special_values(ctx, q8):
+    """Infinities, NaN, values past binary16, values below its smallest."""
+    dim, page = 64, 16
+    x = np.zeros((6, 3, dim), np.float32)
+    x[0, 2, :] = 1e6
+    x[1, 2, :] = np.nan
+    x[2, 2, 0], x[2, 2, 1], x[2, 2, 2] = np.inf, -np.inf, 5
+    x[3, 2, :] = 1e-9
+    x[4, 2, :32], x[4, 2, 5] = 2, np.nan
+    x[5, 2, :] = np.linspace(-1e38, 1e38, dim)
+    cache = cache_of(ctx, q8, 2, 1, dim, page, np.zeros(2 * 2 * M.part_bytes(q8, dim, page), np.uint8))
+    say("append special", q8)
+    run_append(ctx, cache, x, 1, 1, dim, np.zeros(6, int), np.arange(6), np.zeros(0), False, None, None, 0.0)
+    v = M.decode_pool(pool_bytes(cache), q8, 2, 1, dim, page)[1, 0, 0]
+    with np.errstate(over="ignore"):
+        plain = x[:, 2].astype(np.float16).astype(np.float64)
+    if not q8:
+        assert np.array_equal(v[:6], plain, equal_nan=True)
+        return
+    assert (v[0] == np.inf).all()                               # 127 x 7872, beyond binary16
+    assert (v[1] == 0).all()                                    # nothing but NaN: a scale of 0
+    assert v[2, 0] == np.inf and v[2, 1] == -np.inf and v[2, 2] == 0
+    assert (v[3] == 0).all()
+    assert v[4, 5] == 0 and np.allclose(np.delete(v[4, :32], 5), 2, rtol=2 * HALF)
+    assert np.isinf(v[5][[0, -1]]).all()
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("dim,kv,page", [(64, 3, 16), (96, 2, 256), (128, 8, 32), (192, 1, 64), (256, 5, 128)])
+def test_read(ctx, q8, dim, kv, page):
+    say("read", q8, dim, kv, page)
+    rng = np.random.default_rng(dim)
+    pages, rows = 5, 23
+    raw = random_pool(rng, q8, pages, kv, dim, page)
+    cache = cache_of(ctx, q8, pages, kv, dim, page, raw)
+    slots = rng.integers(0, pages * page, rows)                # one twice is fine here
+    slots[4], slots[9], slots[11] = -1, pages * page, 2**31 - 1
+    pool = M.decode_pool(raw, q8, pages, kv, dim, page)
+    ok = (slots >= 0) & (slots < pages * page)
+    at = np.where(ok, slots, 0)
+    want = np.where(ok[:, None, None, None], pool[:, at // page, :, at % page], 0)      # [rows][2][kv][dim]
+    if want.shape[0] == 2:
+        want = np.swapaxes(want, 0, 1)
+    for make in (ctx.half_array, ctx.float_array):
+        k, v = make(rows * kv * dim), make(rows * kv * dim)
+        cache.read(ints(ctx, slots), rows, k, v)
+        ctx.sync()
+        for which, a in enumerate((k, v)):
+            assert np.array_equal(a.get().astype(np.float64).reshape(rows, kv, dim), want[:, which])
+    only = ctx.float_array(rows * kv * dim)
+    cache.read(ints(ctx, slots), rows, v=only)
+    ctx.sync()
+    assert np.array_equal(only.get().astype(np.float64).reshape(rows, kv, dim), want[:, 1])
+
+
+# ---- jl_kv_attention -----------------------------------------------------------------------------
+
+def make_tables(rng, lengths, page, requests_of=None, requests=None, spare=2):
+    """A table whose rows hold the requests' pages in no order, -1 behind them; (table, pages)."""
+    rows = len(lengths)
+    requests = requests or rows
+    need = np.zeros(requests, int)
+    for i, n in enumerate(lengths):
+        r = i if requests_of is None else requests_of[i]
+        need[r] = max(need[r], -(-n // page))
+    pages = int(need.sum()) + spare
+    table = np.full((requests, max(1, need.max())), -1)
+    order = rng.permutation(pages)[:need.sum()]
+    table[np.arange(table.shape[1]) < need[:, None]] = order
+    return table, pages
+
+
+def run_attend(ctx, cache, q, positions, requests_of, table, scale=None, window=0, half=False, pad=0, workspace=None, attention=None):
+    from jitllm_amd.attention import PagedAttention, Rows
+    rows, heads, dim = q.shape
+    attention = attention or PagedAttention(ctx, rows, heads, cache.kvHeads, dim)
+    if workspace is not None:
+        attention.workspace.upload(np.full(attention.workspace.nbytes, workspace, np.uint8))
+    stride = heads * dim + pad
+    flat = np.full((rows, stride), np.nan, np.float32)
+    flat[:, :heads * dim] = q.reshape(rows, -1)
+    out = (ctx.half_from_numpy if half else ctx.from_numpy)(np.full((rows + 2) * stride, -5.5))
+    qa = ctx.from_numpy(flat)
+    attention.attend(cache, Rows(qa, stride), rows, ints(ctx, positions), ints(ctx, table), Rows(out, stride), requests=table.shape[0],
+                     rowRequests=ints(ctx, requests_of) if requests_of is not None else None, scale=scale, window=window)
+    ctx.sync()
+    got = out.get().reshape(rows + 2, stride)
+    assert (got[rows:] == -5.5).all() and (got[:, heads * dim:] == -5.5).all()   # rows behind, columns between
+    return got[:rows, :heads * dim].astype(np.float64).reshape(rows, heads, dim)
+
+
+def check_attend(got, want, weight, reach, lengths, dim, half=False):
+    """An element is sum p v.  A score is off by at most the rounding of the 2 dim products and sums of its two
+    binary16 parts, (2 dim + 8) half steps of scale * sum |q k|, and its weight by twice that (itself, and the sum
+    of all weights) and the power's own 4; the sums over n tokens add n + 64 half steps of sum p |v|.  Roundings of
+    either sign: all outputs together are held to 2e-6 of their norm and a hundredth of the sum of those bounds,
+    which one operand rounded to binary16 (2^-11) would pass ten times over."""
+    n = np.maximum(np.asarray(lengths, float), 1)[:, None, None]
+    bound = ((2 * (2 * dim + 8) * reach[..., None] + 8) + n + 64) * ULP * weight
+    if half:
+        bound = bound + HALF * np.abs(want) + 2.0 ** -25
+    assert np.isfinite(got).all()
+    assert (np.abs(got - want) <= bound).all(), np.max(np.abs(got - want) / np.maximum(bound, 1e-300))
+    if not half:
+        assert np.linalg.norm(got - want) <= 2e-6 * np.linalg.norm(want) + 0.01 * np.linalg.norm(bound) + 1e-12
+
+
+ATTENDS = [
+    # lengths, heads, kv, dim, page, q8, window, half
+    ([201], 32, 8, 64, 16, False, 0, False), ([1], 14, 2, 64, 16, True, 0, True), ([1, 2, 15, 16, 17, 31, 32, 33, 0, 64, 65], 4, 2, 128, 16, False, 0, False),
+    ([127, 128, 129, 255, 256, 257, 1000], 28, 4, 128, 32, True, 0, False), ([950, 3, 511, 512, 513], 6, 6, 128, 16, False, 0, True),
+    ([4096], 16, 4, 256, 16, True, 1024, False), ([700, 40, 90], 16, 4, 256, 64, False, 100, False), ([333, 1, 77], 9, 3, 96, 16, True, 0, False),
+    ([1300, 64], 3, 3, 96, 128, False, 1, False), ([260, 511], 24, 2, 192, 256, False, 0, True), ([900, 5], 12, 2, 192, 16, True, 17, False),
+    ([2000, 7], 71, 1, 64, 32, False, 0, False), ([129], 48, 1, 128, 16, True, 0, True), ([9000], 32, 8, 128, 64, False, 0, False),
+    ([5000, 1, 300], 8, 8, 64, 16, True, 0, False)]
+
+
+@pytest.mark.parametrize("lengths,heads,kv,dim,page,q8,window,half", ATTENDS)
+def test_attend(ctx, lengths, heads, kv, dim, page, q8, window, half):
+    say("attend", lengths, heads, kv, dim, page, q8, window, half)
+    rng = np.random.default_rng(sum(lengths) + dim)
+    rows = len(lengths)
+    table, pages = make_tables(rng, lengths, page)
+    raw = random_pool(rng, q8, pages, kv, dim, page)
+    cache = cache_of(ctx, q8, pages, kv, dim, page, raw)
+    q = (2 * rng.standard_normal((rows, heads, dim))).astype(np.float32)
+    positions = np.array(lengths) - 1
+    scale = dim ** -0.5
+    got = run_attend(ctx, cache, q, positions, None, table, scale, window, half, pad=8 if rows > 1 else 0, workspace=0xff)
+    want = M.attend(M.decode_pool(raw, q8, pages, kv, dim, page), q, positions, None, table, scale, window)
+    check_attend(got, *want, np.minimum(lengths, window or max(lengths)), dim, half)
+
+
+@pytest.mark.parametrize("rows,longest,heads,kv,dim,q8", [(70, 400, 8, 2, 64, False), (300, 60, 4, 4, 128, True), (1030, 20, 4, 1, 64, False),
+                                                          (40, 3000, 7, 1, 128, False), (5, 20000, 4, 1, 64, True)])
+def test_attend_ragged_batches(ctx, rows, longest, heads, kv, dim, q8):
+    """Many rows of all lengths, empty ones among them, that read the table's rows in another order."""
+    say("attend ragged", rows, longest, heads, kv, dim, q8)
+    rng = np.random.default_rng(rows)
+    page = 16
+    lengths = (longest * rng.random(rows) ** 2).astype(int)
+    lengths[rng.integers(0, rows)] = longest
+    requests = rows + 5
+    requests_of = rng.permutation(requests)[:rows]
+    table, pages = make_tables(rng, lengths, page, requests_of, requests)
+    raw = random_pool(rng, q8, pages, kv, dim, page)
+    cache = cache_of(ctx, q8, pages, kv, dim, page, raw)
+    q = (2 * rng.standard_normal((rows, heads, dim))).astype(np.float32)
+    got = run_attend(ctx, cache, q, lengths - 1, requests_of, table, workspace=0x7f)
+    want = M.attend(M.decode_pool(raw, q8, pages, kv, dim, page), q, lengths - 1, requests_of, table, dim ** -0.5)
+    check_attend(got, *want, lengths, dim)
+    assert (got[lengths == 0] == 0).all()
+
+
+def test_attend_rows_of_one_request(ctx):
+    """A prompt's rows, each up to its own position, and rows of requests that the table does not have."""
+    rng = np.random.default_rng(4)
+    dim, page, kv, heads = 64, 16, 2, 8
+    table, pages = make_tables(rng, [50, 130], page)
+    raw = random_pool(rng, False, pages, kv, dim, page)
+    cache = cache_of(ctx, False, pages, kv, dim, page, raw)
+    positions = np.concatenate([np.arange(50), np.arange(100, 130), [5, 5, -1, -7]])
+    requests_of = np.concatenate([np.zeros(50, int), np.ones(30, int), [-1, 2, 0, 1]])
+    q = rng.standard_normal((len(positions), heads, dim)).astype(np.float32)
+    say("attend prompt rows")
+    got = run_attend(ctx, cache, q, positions, requests_of, table)
+    want = M.attend(M.decode_pool(raw, False, pages, kv, dim, page), q, positions, requests_of, table, dim ** -0.5)
+    check_attend(got, *want, np.maximum(positions + 1, 0), dim)
+    assert (got[-4:] == 0).all()
+
+
+@pytest.mark.parametrize("q8", [False, True])
+def test_attend_masked_places_have_no_influence(ctx, q8):
+    """NaN and infinities behind a row's last token, before its window, and in pages of others."""
+    rng = np.random.default_rng(11)
+    dim, page, kv, heads = 128, 32, 2, 6
+    lengths = np.array([1, 16, 33, 95, 300])
+    for window in (0, 40):
+        table, pages = make_tables(rng, lengths, page)
+        raw = random_pool(rng, q8, pages, kv, dim, page)
+        clean = cache_of(ctx, q8, pages, kv, dim, page, raw)
+        q = rng.standard_normal((5, heads, dim)).astype(np.float32)
+        seen = np.zeros((pages, page), bool)
+        for i, n in enumerate(lengths):
+            j = np.arange(max(0, n - window) if window else 0, n)
+            seen[table[i, j // page], j % page] = True
+        dirty = raw.reshape(2, pages, kv, -1).copy()
+        if q8:
+            scales = dirty[..., page * dim:].view(np.float16).reshape(2, pages, kv, dim // 32, page)
+            for which, bad in ((0, np.nan), (1, np.inf)):
+                scales[which] = np.where(seen[:, None, None, :], scales[which], np.float16(bad))
+        else:
+            values = dirty.view(np.float16).reshape(2, pages, kv, page, dim)
+            for which, bad in ((0, np.nan), (1, -np.inf)):
+                values[which] = np.where(seen[:, None, :, None], values[which], np.float16(bad))
+            values[1, ~seen.any(1)] = np.nan
+        other = cache_of(ctx, q8, pages, kv, dim, page, dirty.reshape(-1))
+        say("attend masked", q8, window)
+        a, b = (run_attend(ctx, c, q, lengths - 1, None, table, window=window) for c in (clean, other))
+        assert np.array_equal(a, b) and np.isfinite(b).all()
+
+
+def test_attend_pages_outside_the_cache_count_as_masked(ctx):
+    rng = np.random.default_rng(12)
+    dim, page, kv, heads = 64, 16, 1, 4
+    lengths = [100, 100, 40, 300]
+    table, pages = make_tables(rng, lengths, page)
+    table[0, [0, 3]], table[1, 6], table[2, :3], table[3, 5:12] = -1, pages, 2**31 - 1, -2**31
+    raw = random_pool(rng, False, pages, kv, dim, page)
+    cache = cache_of(ctx, False, pages, kv, dim, page, raw)
+    q = rng.standard_normal((4, heads, dim)).astype(np.float32)
+    positions = np.array([99, 99, 39, 2**31 - 1])              # ... and a position past the table's last token
+    say("attend bad pages")
+    got = run_attend(ctx, cache, q, positions, None, table)
+    want = M.attend(M.decode_pool(raw, False, pages, kv, dim, page), q, positions, None, table, dim ** -0.5)
+    check_attend(got, *want, [100, 100, 1, 304], dim)
+    assert (got[2] == 0).all()
+
+
+def test_attend_large_and_extreme_scores(ctx):
+    """Scores thousands apart, all equal, of one sign; queries past binary16 and below it; infinities in q."""
+    rng = np.random.default_rng(13)
+    dim, page, kv = 64, 16, 1
+    n = 700
+    table, pages = make_tables(rng, [n] * 7, page)
+    raw = random_pool(rng, False, pages, kv, dim, page)
+    pool = M.decode_pool(raw, False, pages, kv, dim, page)
+    cache = cache_of(ctx, False, pages, kv, dim, page, raw)
+    q = rng.standard_normal((7, 4, dim)).astype(np.float32)
+    q[0] *= 3000
+    q[1] = 0
+    q[2] *= 1e7
+    q[3] *= 1e-9
+    q[4] *= np.exp(rng.uniform(-20, 5, (4, dim))).astype(np.float32)
+    q[5] = 2.0 ** -140
+    say("attend extreme")
+    got = run_attend(ctx, cache, q, np.full(7, n - 1), None, table)
+    want = M.attend(pool, q, np.full(7, n - 1), None, table, dim ** -0.5)
+    # rows whose scores are off by more than a weight can say (1e7 * 64 * 2^-24 ...) are held by their largest weight
+    for i in (0, 1, 3, 4, 5, 6):
+        check_attend(got[i:i + 1], *(w[i:i + 1] for w in want), [n], dim)
+    assert np.isfinite(got[2]).all()
+    assert np.abs(got[2] - want[0][2]).max() <= 1e-3           # the winner stands alone: scores are 1e6 apart
+    bad = q[:1].copy()
+    bad[0, 1, 5], bad[0, 2, 7] = np.inf, np.nan
+    got = run_attend(ctx, cache, bad, np.array([n - 1]), None, table[:1])
+    assert np.isnan(got[0, 1]).all() and np.isnan(got[0, 2]).all()
+    check_attend(got[:, [0, 3]], *(w[:1, [0, 3]] for w in want), [n], dim)
+
+
+def test_attend_is_the_same_every_time_and_with_any_workspace(ctx):
+    rng = np.random.default_rng(14)
+    lengths = np.array([5000, 12, 800, 0, 3333])
+    table, pages = make_tables(rng, lengths, 16)
+    raw = random_pool(rng, False, pages, 2, 128, 16)
+    cache = cache_of(ctx, False, pages, 2, 128, 16, raw)
+    q = rng.standard_normal((5, 8, 128)).astype(np.float32)
+    say("attend repeats")
+    runs = [run_attend(ctx, cache, q, lengths - 1, None, table, workspace=w) for w in (0, 0xff, 0x7f, None)]
+    for r in runs[1:]:
+        assert np.array_equal(r, runs[0])
+
+
+def test_attend_past_32_bit_offsets(ctx):
+    """A cache of over 4 GiB: its last pages are read and written where they lie."""
+    from jitllm_amd.attention import KvType, PagedAttention, PagedKvCache
+    rng = np.random.default_rng(15)
+    kv, dim, page, heads = 8, 256, 256, 8
+    pages = 2600                                               # 1 MiB a page for k, and for v
+    say("attend past 4 GiB")
+    cache = PagedKvCache(ctx, KvType.F16, pages, kv, dim, page)
+    assert cache.nbytes > 5 << 30
+    rows = 40
+    x = rng.standard_normal((rows, heads + 2 * kv, dim)).astype(np.float32)
+    slots = (pages - 1 - np.arange(rows) // 8 * 500) * page + np.arange(rows) % 8
+    table = (pages - 1 - np.arange(5) * 500).reshape(5, 1)
+    got_q = run_append(ctx, cache, x, heads, kv, dim, np.arange(rows) % 8, slots, np.zeros(0), False, None, None, 0.0)
+    assert np.array_equal(got_q, x[:, :heads])
+    out = run_attend(ctx, cache, np.ascontiguousarray(x[7::8, :heads]), np.full(5, 7), None, table)
+    kv16 = x[:, heads:].astype(np.float16).astype(np.float64).reshape(5, 8, 2, kv, dim)
+    pool = np.zeros((2, 5, kv, page, dim))
+    pool[:, :, :, :8] = kv16.transpose(2, 0, 3, 1, 4)
+    want = M.attend(pool, x[7::8, :heads], np.full(5, 7), None, np.arange(5).reshape(5, 1), dim ** -0.5)
+    check_attend(out, *want, [8] * 5, dim)
+    cache.free()
+
+
+# ---- together ------------------------------------------------------------------------------------
+
+class Layer:
+    """A small layer's attention half through the framework, and the same in float64."""
+
+    def __init__(self, ctx, rng, q8, halves, dim=256, heads=4, kv=2, head_dim=64):
+        from jitllm_amd import synthetic
+        from jitllm_amd.ggml import GGMLType
+        self.dim, self.heads, self.kv, self.head_dim = dim, heads, kv, head_dim
+        t = GGMLType.Q8_0
+        self.raw = [synthetic.weight(t, d, n, seed=int(rng.integers(1 << 30)))
+                    for d, n in ((heads * head_dim, dim), (kv * head_dim, dim), (kv * head_dim, dim), (dim, heads * head_dim))]
+        self.w = [ctx.load_weight(t, raw, d, n) for raw, (d, n) in
+                  zip(self.raw, ((heads * head_dim, dim), (kv * head_dim, dim), (kv * head_dim, dim), (dim, heads * head_dim)))]
+        self.dense = [w.dequantize().astype(np.float64) for w in self.w]
+
+
+@pytest.mark.parametrize("q8,half", [(False, False), (True, False), (False, True)])
+def test_decode_steps_through_a_layer(ctx, q8, half):
+    """plan -> q|k|v -> append -> attend -> output projection, step after step: prompts of three lengths, decoding,
+    one that ends and one that takes its pages; against float64 over the unquantised history."""
+    from jitllm_amd.attention import BlockTables, KvType, PagedAttention, PagedKvCache, Rope, RopeStyle, Rows
+    from jitllm_amd.projections import QuantizedBatchProjections
+    rng = np.random.default_rng(21)
+    y = Layer(ctx, rng, q8, True)
+    requests, stride, page, pages, max_rows = 4, 6, 16, 14, 64
+    w, hd = (y.heads + 2 * y.kv) * y.head_dim, y.heads * y.head_dim
+    freq = 1e4 ** (-np.arange(0, y.head_dim, 2) / y.head_dim)
+    rope = Rope.of_base(ctx, y.head_dim, 1e4, RopeStyle.HALVES)
+    tables = BlockTables(ctx, requests, stride, pages, page, max_rows)
+    cache = PagedKvCache(ctx, KvType.Q8_0 if q8 else KvType.F16, pages, y.kv, y.head_dim, page)
+    attention = PagedAttention(ctx, max_rows, y.heads, y.kv, y.head_dim)
+    proj = QuantizedBatchProjections(ctx, max_rows, max(y.dim, hd), w)
+    history = [[] for _ in range(requests)]                    # (k, v) of every token, float64
+    steps = [[20, 7, 33, 0], [1, 1, 1, 0], [1, -1, 1, 0], [1, 0, 1, 29], [1, 0, 0, 1], [1, 16, 1, 1]]
+    qkv = ctx.float_array(max_rows * w, fill=0.0)
+    att = ctx.half_array(max_rows * hd) if half else ctx.float_array(max_rows * hd, fill=0.0)
+    for step, fresh in enumerate(steps):
+        rows = sum(max(f, 0) for f in fresh)
+        x = rng.standard_normal((max_rows, y.dim)).astype(np.float32)
+        X, out = ctx.from_numpy(x), ctx.float_array(max_rows * y.dim, fill=0.0)
+        say("layer step", step, fresh)
+        tables.plan(ints(ctx, fresh))
+        proj.fusedQKV(X, qkv, y.w[0], y.w[1], y.w[2], rows)
+        cache.append(Rows(qkv, w, hd), Rows(qkv, w, hd + y.kv * y.head_dim), tables.positions, tables.slots, rows, rope=rope,
+                     q=Rows(qkv, w), heads=y.heads)
+        attention.attend(cache, Rows(qkv, w), rows, tables.positions, tables.table, att, requests=requests, rowRequests=tables.rowRequests)
+        proj.projection(att, out, y.w[3], hd, y.dim, False, rows)
+        ctx.sync()
+        got = out.get().reshape(max_rows, y.dim)[:rows]
+        row = 0
+        for r, f in enumerate(fresh):
+            if f < 0:
+                history[r] = []
+            for _ in range(max(f, 0)):
+                xx = x[row].astype(np.float64)
+                pos = np.array([len(history[r])])
+                q, k, v = ((m @ xx).reshape(1, -1, y.head_dim) for m in y.dense[:3])
+                q, k = M.rotate(q, pos, freq, True), M.rotate(k, pos, freq, True)
+                history[r].append((k[0], v[0]))
+                K, V = (np.array([h[i] for h in history[r]]) for i in (0, 1))
+                o = np.zeros((y.heads, y.head_dim))
+                for h in range(y.heads):
+                    s = K[:, h // 2] @ q[0, h] * y.head_dim ** -0.5
+                    p = np.exp(s - s.max())
+                    o[h] = (p / p.sum()) @ V[:, h // 2]
+                want = y.dense[3] @ o.reshape(-1)
+                # fp16 products inside the projections (2e-3 of the magnitude, as the path is held to) and a cache
+                # of 11 or 7 bits, whose scores move by up to that share of a few units
+                size = np.abs(y.dense[3]) @ np.abs(o.reshape(-1))
+                assert np.abs(got[row] - want).max() <= (0.15 if q8 else 0.03) * size.max(), (step, r, row)
+                row += 1
+    assert tables.lengths.get().tolist() == [25, 16, 37, 31]   # 20 + 5, 16, 33 + 4, 29 + 2
