@@ -74,9 +74,11 @@ __device__ __forceinline__ Range range_of(const AttentionArgs &p, int row) {
     return r;
 }
 
+// k and v pass once: loads that do not stay in the caches (512 MB in 16 KB pieces, nothing else done: 90 us with ordinary
+// loads, 80 with these).
 template <typename T>
 __device__ __forceinline__ T load_at(const uint8_t *base, uint32_t offset) {
-    return *(const T *)(base + offset);
+    return __builtin_nontemporal_load((const T *)(base + offset));
 }
 __device__ __forceinline__ jl_half2v as_half2(uint32_t x) { return __builtin_bit_cast(jl_half2v, x); }
 __device__ __forceinline__ uint32_t as_u32(jl_half2v x) { return __builtin_bit_cast(uint32_t, x); }
