@@ -555,12 +555,14 @@ int jl_kv_read(jl_context *ctx, const jl_kv_cache *cache, const int32_t *slots, 
  * softmax.  The work is cut over the cache's length where rows are few or lengths differ, and
  * joined in a fixed order: the same call gives the same bits, whose last few may differ between
  * batches of other lengths.
- * workspace: jl_kv_attention_workspace_bytes of the largest call that uses it, 16-byte aligned, for
- * the parts that are joined; its contents need no preparation and do not outlive the call.  Calls
- * that may run at the same time (graphs on two streams) need one each.
+ * workspace: jl_kv_attention_workspace_bytes of the largest call that uses it, 16-byte aligned, which
+ * jl_kv_attention_workspace_init has been over once (on the stream, before the first call; every call
+ * leaves it as it needs it).  Parts of rows that are cut are joined there.  Calls that may run at the
+ * same time -- contexts, graphs on two streams -- need one each.
  * At most 65535 rows; heads a multiple of kv_heads.
  */
 size_t jl_kv_attention_workspace_bytes(int heads, int kv_heads, int head_dim);
+int jl_kv_attention_workspace_init(jl_context *ctx, void *workspace, size_t workspace_bytes);
 int jl_kv_attention(jl_context *ctx, const jl_kv_cache *cache, const float *q, int heads, int64_t ldq, int64_t rows,
                     const int32_t *positions, const int32_t *row_requests, const int32_t *block_table,
                     int64_t requests, int64_t table_stride, float scale, int64_t window, void *out, int out_f16,

@@ -80,6 +80,7 @@ SYMBOLS = {
                                vp, vp, C.c_float]),
     "jl_kv_read": (C.c_int, [vp, vp, vp, i64, vp, vp, C.c_int]),
     "jl_kv_attention_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int, C.c_int]),
+    "jl_kv_attention_workspace_init": (C.c_int, [vp, vp, C.c_size_t]),
     "jl_kv_attention": (C.c_int, [vp, vp, vp, C.c_int, i64, i64, vp, vp, vp, i64, i64, C.c_float, i64, vp, C.c_int,
                                   i64, vp, C.c_size_t]),
     "jl_gguf_open": (C.c_int, [C.c_char_p, C.POINTER(vp)]),

@@ -240,6 +240,7 @@ class PagedAttention:
         if not nbytes:
             raise ValueError(f"{heads} query heads over {kvHeads} of k and v, {headDim} values each")
         self.workspace = ctx.raw_buffer(nbytes)
+        L.check(self._lib.jl_kv_attention_workspace_init(ctx.handle, self.workspace.ptr, nbytes))
 
     def attend(self, cache: PagedKvCache, q, rows: int, positions, table, out, requests: int, rowRequests=None,
                scale: float | None = None, window: int = 0) -> None:

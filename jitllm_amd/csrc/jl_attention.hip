@@ -17,8 +17,8 @@
 //
 // Work.  The tiles of all (row, head of k and v, 16 query heads) are one long list, cut into equal spans for the
 // launch's workgroups whatever the rows' lengths are; a workgroup's four waves take a span's tiles in turn and
-// join in LDS.  A row's head that a cut goes through leaves its parts in the workspace, and a second launch joins them
-// in their order.
+// join in LDS.  A head that a cut goes through leaves its parts in the workspace, and the workgroup that is done last
+// with it joins them, in their order whoever that is (nobody waits for anybody).
 #include <algorithm>
 #include <climits>
 #include <cmath>
@@ -28,25 +28,29 @@
 namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / JL_WAVE;
-constexpr int kTile = 32;                 // tokens
-constexpr int kLeastSpan = kWaves;        // tiles: one a wave
 constexpr int kMostGroups = 1024;         // workgroups of a launch, and spans
+constexpr int kWholeTokens = 512;         // rows no longer than this are never cut
 constexpr float kNone = -3.0e38f;         // the running maximum of nothing: finite, so that differences are numbers
+
+template <bool Q8, int DIM>
+struct Shape {
+    // 16-token halves of a wave's tile: 64 tokens of 8-bit blocks are the registers, and the bytes in flight, of 32 of binary16
+    static constexpr int kHalves = Q8 && DIM <= 128 ? 4 : 2, kTile = 16 * kHalves;
+    static constexpr int kPerUnit = DIM == 256 ? 1 : 2;   // workgroups that a compute unit holds at a time
+};
 
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
 typedef uint32_t uintx2 __attribute__((ext_vector_type(2)));
-
-struct Part {             // a row's head that is cut: its parts are spans `group` ... group + count - 1
-    int row, head, group, count;
-};
 
 struct AttentionArgs {
     JlKvView cache;
     const float *q;
     int64_t ldq, ldo;
     const int32_t *positions, *row_requests, *table;
-    int64_t requests, table_stride;
+    int64_t table_stride;
+    int requests;
+    int table_tokens;     // of a row of the table, at most 2^31 - 64
     float scale;          // times log2(e): weights are powers of two
     int window;           // 0: none
     int group;            // query heads to a head of k and v
@@ -54,24 +58,47 @@ struct AttentionArgs {
     int rows;
     void *out;
     bool out_f16;
-    bool by_head;         // `cut` has an entry per row and head instead of one per span
-    Part *cut;
+    uint32_t *arrived;    // [kMostGroups], all 0 between calls
     float *parts;         // [2 * spans][16 * (DIM + 2)]
 };
 
-// The tokens [first, end) that a row sees.
+// The tokens [first, end) of its request that a row sees.
 struct Range {
-    int first, end;
-    __device__ int tiles() const { return end > first ? (end + kTile - 1) / kTile - first / kTile : 0; }
+    int first, end, request;
+    template <int TILE>
+    __device__ int tiles() const { return end > first ? (end + TILE - 1) / TILE - first / TILE : 0; }
 };
 __device__ __forceinline__ Range range_of(const AttentionArgs &p, int row) {
     const int position = p.positions[row];
-    const int request = p.row_requests ? p.row_requests[row] : row;
-    const int64_t held = min((int64_t)p.table_stride << p.cache.page_shift, (int64_t)INT_MAX);
     Range r;
-    r.end = position >= 0 && request >= 0 && request < p.requests ? (int)min((int64_t)position + 1, held) : 0;
+    r.request = p.row_requests ? p.row_requests[row] : row;
+    r.end = position >= 0 && r.request >= 0 && r.request < p.requests ? min(position, p.table_tokens - 1) + 1 : 0;
     r.first = p.window > 0 ? max(position - p.window + 1, 0) : 0;
     return r;
+}
+
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// Parts go to the workgroup that joins them through device scope: past the XCD's own second-level cache.
+__device__ __forceinline__ void agent_store(float *to, float v) {
+    __hip_atomic_store(to, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void agent_store4(float *to, floatx4 v) {
+    uint64_t two[2];
+    __builtin_memcpy(two, &v, 16);
+    __hip_atomic_store((uint64_t *)to, two[0], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_store((uint64_t *)to + 1, two[1], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float agent_load(const float *from) {
+    return __hip_atomic_load(from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ floatx4 agent_load4(const float *from) {
+    uint64_t two[2];
+    two[0] = __hip_atomic_load((const uint64_t *)from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    two[1] = __hip_atomic_load((const uint64_t *)from + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    floatx4 v;
+    __builtin_memcpy(&v, two, 16);
+    return v;
 }
 
 // k and v pass once: loads that do not stay in the caches (512 MB in 16 KB pieces, nothing else done: 90 us with ordinary
@@ -91,12 +118,13 @@ struct Raw;
 
 template <int DIM>
 struct Raw<false, DIM> {
+    static constexpr int kHalves = Shape<false, DIM>::kHalves;
     static constexpr int kSteps = DIM / 32;
     static constexpr int kWide = DIM / 128, kMid = DIM % 128 / 64, kThin = DIM % 64 / 32;
-    uintx4 k[2][kSteps];
-    uintx4 v4[2][4][kWide ? kWide : 1];
-    uintx2 v2[2][4];
-    uint32_t v1[2][4];
+    uintx4 k[kHalves][kSteps];
+    uintx4 v4[kHalves][4][kWide ? kWide : 1];
+    uintx2 v2[kHalves][4];
+    uint32_t v1[kHalves][4];
     __device__ static int element(int step, int g) { return 32 * step + 8 * g; }   // first of the eight of k step `step`
     __device__ void load_k(int half, const uint8_t *part, int in_page, int, int g, int m) {
 #pragma unroll
@@ -114,9 +142,9 @@ struct Raw<false, DIM> {
     }
     __device__ jl_half8 k_operand(int half, int step) const { return __builtin_bit_cast(jl_half8, k[half][step]); }
     // masked tokens' values are nothing, whatever lies there
-    __device__ void mask_v(const bool (&seen)[2][4]) {
+    __device__ void mask_v(const bool (&seen)[kHalves][4]) {
 #pragma unroll
-        for (int h = 0; h < 2; h++)
+        for (int h = 0; h < kHalves; h++)
 #pragma unroll
             for (int i = 0; i < 4; i++) {
 #pragma unroll
@@ -127,14 +155,14 @@ struct Raw<false, DIM> {
                 if constexpr (kThin) v1[h][i] = seen[h][i] ? v1[h][i] : 0;
             }
     }
-    // eight tokens of the column that output block `block` takes of this lane
-    __device__ jl_half8 v_operand(int block) const {
+    // eight tokens (of both halves of 32) of the column that output block `block` takes of this lane
+    __device__ jl_half8 v_operand(int sub, int block) const {
         uintx4 r;
         const int word = block / 2;
         const uint32_t pick = block % 2 ? 0x07060302u : 0x05040100u;
 #pragma unroll
         for (int pair = 0; pair < 4; pair++) {
-            const int h = pair / 2, i = pair % 2 * 2;
+            const int h = 2 * sub + pair / 2, i = pair % 2 * 2;
             uint32_t a, b;
             if (word < 4 * kWide) a = v4[h][i][word / 4][word % 4], b = v4[h][i + 1][word / 4][word % 4];
             else if (word < 4 * kWide + 2 * kMid) a = v2[h][i][word % 2], b = v2[h][i + 1][word % 2];
@@ -147,16 +175,17 @@ struct Raw<false, DIM> {
 
 template <int DIM>
 struct Raw<true, DIM> {
+    static constexpr int kHalves = Shape<true, DIM>::kHalves;
     static constexpr int kSteps = DIM / 32, kPairs = DIM / 64, kTail = DIM % 64 / 32;
     static constexpr int kWide = DIM / 128, kMid = DIM % 128 / 64, kThin = DIM % 64 / 32;
     static constexpr int kPieces = kWide + kMid + kThin;
-    uintx4 k[2][kPairs];
-    uintx2 k_tail[2];
-    uint16_t k_scale[2][kPairs + kTail];
-    uintx2 v2[2][4][kWide ? kWide : 1];
-    uint32_t v1[2][4];
-    uint16_t v0[2][4];
-    uintx2 v_scale[2][kPieces];
+    uintx4 k[kHalves][kPairs];
+    uintx2 k_tail[kHalves];
+    uint16_t k_scale[kHalves][kPairs + kTail];
+    uintx2 v2[kHalves][4][kWide ? kWide : 1];
+    uint32_t v1[kHalves][4];
+    uint16_t v0[kHalves][4];
+    uintx2 v_scale[kHalves][kPieces];
     // (16 consecutive bytes serve two steps: a lane's loads stay 16 bytes wide)
     __device__ static int element(int step, int g) {
         return step < 2 * kPairs ? 64 * (step / 2) + 16 * g + 8 * (step % 2) : 64 * kPairs + 8 * g;
@@ -201,21 +230,21 @@ struct Raw<true, DIM> {
         return jl_half8{a.x, a.y, b.x, b.y, c.x, c.y, e.x, e.y};
     }
     // (a byte times a scale of 0; the scale alone can be an infinity or NaN)
-    __device__ void mask_v(const bool (&seen)[2][4]) {
+    __device__ void mask_v(const bool (&seen)[kHalves][4]) {
 #pragma unroll
-        for (int h = 0; h < 2; h++)
+        for (int h = 0; h < kHalves; h++)
 #pragma unroll
             for (int w = 0; w < kPieces; w++)
 #pragma unroll
                 for (int c = 0; c < 2; c++)
                     v_scale[h][w][c] &= (seen[h][2 * c] ? 0xffffu : 0u) | (seen[h][2 * c + 1] ? 0xffff0000u : 0u);
     }
-    __device__ jl_half8 v_operand(int block) const {
+    __device__ jl_half8 v_operand(int sub, int block) const {
         uintx4 r;
         const int piece = block < 8 * kWide ? block / 8 : block < 8 * kWide + 4 * kMid ? kWide : kWide + kMid;
 #pragma unroll
         for (int pair = 0; pair < 4; pair++) {
-            const int h = pair / 2, i = pair % 2 * 2;
+            const int h = 2 * sub + pair / 2, i = pair % 2 * 2;
             uint32_t a, b;
             int byte;
             if (block < 8 * kWide) a = v2[h][i][block / 8][block % 8 / 4], b = v2[h][i + 1][block / 8][block % 8 / 4], byte = block % 4;
@@ -257,80 +286,196 @@ __device__ __forceinline__ void store_out(const AttentionArgs &p, int64_t at, co
     else *(floatx4 *)((float *)p.out + at) = v;
 }
 
+// A piece of a workgroup's list: tiles tile ... tile + count - 1 of a row's head, and what the row sees.
+struct Piece {
+    int row, head, tile, count, tiles;
+    int first, end, request;
+    uint32_t left;    // tiles of the span, this piece's included; 0: no such piece
+};
+
 template <bool Q8, int DIM>
-__global__ void __launch_bounds__(kThreads, DIM == 256 ? 1 : 2) jl_kv_attention_kernel(AttentionArgs p) {
+__global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_attention_kernel(AttentionArgs p) {
     constexpr int kSteps = DIM / 32, kBlocks = DIM / 16;
+    constexpr int kHalves = Shape<Q8, DIM>::kHalves, kTile = Shape<Q8, DIM>::kTile, kSubs = kHalves / 2;
     constexpr int kRound = DIM == 256 ? 128 : DIM;            // elements that are joined at a time: 64 KB of LDS at most
     constexpr int kStride = kRound + 4;                       // (four floats on: rows start on other banks)
+    constexpr int kSlot = 16 * (DIM + 2);
     __shared__ float joined[kWaves][16][kStride];
     __shared__ float joined_max[kWaves][16], joined_sum[kWaves][16];
-    __shared__ int64_t scan[kWaves];
-    __shared__ int64_t start_tiles;
+    __shared__ uint32_t scan[kWaves];
+    __shared__ uint32_t start_tiles, before_me;
     __shared__ int start_row;
-    const int tid = threadIdx.x, lane = tid % JL_WAVE, wave = __builtin_amdgcn_readfirstlane(tid / JL_WAVE);
+    const int tid = threadIdx.x, lane = tid % JL_WAVE, wave = uniform(tid / JL_WAVE);
     const int g = lane / 16, m = lane % 16;
     const int heads = p.cache.kv_heads * p.blocks_of_16;      // of a row's list
-    const int width = p.cache.kv_heads * p.group * DIM;
+    const int page_shift = p.cache.page_shift, in_page_mask = (1 << page_shift) - 1;
 
-    // ---- this workgroup's span of the list of tiles
-    const int per = (p.rows + kThreads - 1) / kThreads;
-    int64_t mine = 0;
-    for (int i = 0; i < per; i++) {
-        const int r = tid * per + i;
-        if (r < p.rows) mine += range_of(p, r).tiles();
-    }
-    int64_t through = mine;
+    // ---- the rows' ranges, 64 at a time in the lanes of every wave
+    int window_row = 0;
+    Range in_lane;
+    auto load_window = [&](int from) {
+        window_row = from;
+        in_lane = from + lane < p.rows ? range_of(p, from + lane) : Range{0, 0, 0};
+    };
+
+    // ---- this workgroup's share of the list: whole (row, head) pairs one after the other where all rows are short, else
+    // an equal span of tiles.  (All tiles together are fewer than 2^32: jl_kv_attention.)
+    load_window(0);
+    const uint32_t mine = in_lane.tiles<kTile>();
+    uint32_t all, through = mine;                             // tiles of all rows; of those up to this lane's (this thread's last)
+    bool whole;
+    if (p.rows <= JL_WAVE) {
 #pragma unroll
-    for (int off = 1; off < JL_WAVE; off <<= 1) {
-        const int64_t other = __shfl_up(through, off, JL_WAVE);
-        if (lane >= off) through += other;
-    }
-    if (lane == JL_WAVE - 1) scan[wave] = through;
-    __syncthreads();
-    int64_t all = 0;
-    for (int w = 0; w < kWaves; w++) {
-        if (w < wave) through += scan[w];
-        all += scan[w];
-    }
-    const int64_t total = all * heads;
-    int64_t span = (total + gridDim.x - 1) / gridDim.x;
-    if (span < kLeastSpan) span = kLeastSpan;
-    const int64_t begin = span * blockIdx.x;
-    // rows with nothing to read
-    for (int r = blockIdx.x; r < p.rows; r += gridDim.x) {
-        if (range_of(p, r).tiles() > 0) continue;
-        for (int c = 4 * tid; c < width; c += 4 * kThreads) store_out(p, r * p.ldo + c, floatx4{0.f, 0.f, 0.f, 0.f});
-        if (p.by_head)
-            for (int h = tid; h < heads; h += kThreads) p.cut[r * heads + h].count = 0;
-    }
-    if (!p.by_head && tid == 0) p.cut[blockIdx.x].count = 0;
-    if (begin >= total) return;
-    {
-        const int64_t from = begin / heads;
-        if (from >= through - mine && from < through) {
-            int64_t before = through - mine;
-            int r = tid * per;
-            for (int n; before + (n = range_of(p, r).tiles()) <= from; r++) before += n;
-            start_row = r;
-            start_tiles = before;
+        for (int off = 1; off < JL_WAVE; off <<= 1) {
+            const uint32_t other = __shfl_up(through, off, JL_WAVE);
+            if (lane >= off) through += other;
         }
+        all = __builtin_amdgcn_readlane(through, JL_WAVE - 1);
+        whole = !__any(mine > kWholeTokens / kTile);
+    } else {
+        const int per = (p.rows + kThreads - 1) / kThreads;
+        bool longer = false;
+        through = 0;
+        for (int r = tid * per; r < min((tid + 1) * per, p.rows); r++) {
+            const int n = range_of(p, r).tiles<kTile>();
+            through += n;
+            longer |= n > kWholeTokens / kTile;
+        }
+        const uint32_t own = through;
+#pragma unroll
+        for (int off = 1; off < JL_WAVE; off <<= 1) {
+            const uint32_t other = __shfl_up(through, off, JL_WAVE);
+            if (lane >= off) through += other;
+        }
+        if (lane == JL_WAVE - 1) scan[wave] = through;
+        whole = !__syncthreads_or(longer);
+        all = 0;
+        for (int w = 0; w < kWaves; w++) {
+            if (w < wave) through += scan[w];
+            all += scan[w];
+        }
+        all = uniform(all);
+        const uint32_t from = (all * heads + gridDim.x - 1) / gridDim.x * blockIdx.x / heads;
+        if (!whole && from >= through - own && from < through) {
+            uint32_t before = through - own;
+            int r = tid * per;
+            for (uint32_t n; before + (n = range_of(p, r).tiles<kTile>()) <= from; r++) before += n;
+            start_row = r, start_tiles = before;
+        }
+        __syncthreads();
     }
-    __syncthreads();
-    int row = __builtin_amdgcn_readfirstlane(start_row);
-    Range range = range_of(p, row);
-    int tiles = range.tiles();
-    const int64_t into = begin - start_tiles * heads;
-    int head = (int)(into / tiles), tile = (int)(into % tiles);
-    int64_t left = min(span, total - begin);
 
-    while (left > 0) {
-        row = __builtin_amdgcn_readfirstlane(row), head = __builtin_amdgcn_readfirstlane(head), tile = __builtin_amdgcn_readfirstlane(tile);
-        const int count = __builtin_amdgcn_readfirstlane((int)min((int64_t)(tiles - tile), left));
-        const int first = __builtin_amdgcn_readfirstlane(range.first), end = __builtin_amdgcn_readfirstlane(range.end);
-        const int kv_head = head / p.blocks_of_16, block_of_16 = head % p.blocks_of_16;
+    // rows with nothing to read
+    const int width = p.cache.kv_heads * p.group * DIM;
+    for (int r = blockIdx.x; r < p.rows; r += gridDim.x) {
+        const int n = p.rows <= JL_WAVE ? __builtin_amdgcn_readlane(in_lane.tiles<kTile>(), r) : range_of(p, r).tiles<kTile>();
+        if (n == 0)
+            for (int c = 4 * tid; c < width; c += 4 * kThreads) store_out(p, r * p.ldo + c, floatx4{0.f, 0.f, 0.f, 0.f});
+    }
+
+    const uint32_t total = all * heads, span = (total + gridDim.x - 1) / gridDim.x, begin = whole ? 0 : span * blockIdx.x;
+    const int row_step = gridDim.x / heads, head_step = gridDim.x % heads;    // from one whole pair of a workgroup to its next
+    Piece next;
+    if (whole) {
+        next.row = blockIdx.x / heads, next.head = blockIdx.x % heads, next.tile = 0;
+        next.left = 1;
+    } else {
+        if (begin >= total) return;
+        const uint32_t from = begin / heads;
+        uint32_t before;
+        if (p.rows <= JL_WAVE) {
+            next.row = __popcll(__ballot(through <= from));
+            before = next.row == 0 ? 0 : __builtin_amdgcn_readlane(through, uniform(next.row - 1));
+        } else {
+            next.row = uniform(start_row), before = uniform(start_tiles);
+        }
+        next.head = begin - before * heads;                   // (its tile in the row's list, taken apart below)
+        next.tile = -1;
+        next.left = min(span, total - begin);
+    }
+    // Completes `next` from its row, head and tile, going on to the first row that has tiles.
+    auto complete = [&]() {
+        next.row = uniform(next.row), next.head = uniform(next.head), next.tile = uniform(next.tile), next.left = uniform(next.left);
+        while (next.left > 0) {
+            if (next.row >= p.rows) {
+                next.left = 0;
+                break;
+            }
+            if (next.row < window_row || next.row >= window_row + JL_WAVE) load_window(next.row);
+            const int at = uniform(next.row - window_row);
+            next.first = __builtin_amdgcn_readlane(in_lane.first, at);
+            next.end = __builtin_amdgcn_readlane(in_lane.end, at);
+            next.request = __builtin_amdgcn_readlane(in_lane.request, at);
+            next.tiles = Range{next.first, next.end, 0}.tiles<kTile>();
+            if (next.tiles > 0) break;
+            if (whole) {
+                next.row += row_step, next.head += head_step;
+                if (next.head >= heads) next.head -= heads, next.row++;
+            } else {
+                next.row++;
+            }
+        }
+        if (next.tile < 0 && next.left > 0) {
+            const int into = next.head;
+            next.head = uniform((uint32_t)into / next.tiles);
+            next.tile = into - next.head * next.tiles;
+        }
+        next.count = whole ? next.tiles : min((uint32_t)(next.tiles - next.tile), next.left);
+    };
+
+    // k and v of a tile go from memory to `raw`; `page` are the pages of its halves, and one behind the last token, or one
+    // outside the cache, is -1
+    Raw<Q8, DIM> raw;
+    bool loaded = false;
+    uint32_t paged = 0;           // bit h: half h of the tile in `raw` has a page of the cache
+    int page[kHalves];
+    auto find_pages = [&](const Piece &c, int t) {
+        const int32_t *table = p.table + c.request * p.table_stride;
+#pragma unroll
+        for (int h = 0; h < kHalves; h++) {
+            const int token = t * kTile + 16 * h;
+            page[h] = token < c.end ? table[token >> page_shift] : -1;
+        }
+    };
+    auto issue = [&](int kv_head, int t, bool values) {
+        if (values) paged = 0;
+#pragma unroll
+        for (int h = 0; h < kHalves; h++) {
+            const bool real = (unsigned)page[h] < (unsigned)p.cache.pages;
+            const uint8_t *part = p.cache.k + ((int64_t)(real ? page[h] : 0) * p.cache.kv_heads + kv_head) * p.cache.part_bytes;
+            const int in_page = (t * kTile + 16 * h) & in_page_mask;
+            if (values) {
+                raw.load_v(h, part + p.cache.v_offset, in_page, page_shift, g, m);
+                paged |= real ? 1u << h : 0u;
+            } else {
+                raw.load_k(h, part, in_page, page_shift, g, m);
+            }
+        }
+    };
+    const bool one_block = p.blocks_of_16 == 1;
+    auto kv_head_of = [&](int head) { return one_block ? head : head / p.blocks_of_16; };
+
+    for (complete(); next.left > 0;) {
+        const Piece cur = next;
+        // the piece behind this one: the loads of its first tiles go out with this one's last
+        next.left = whole ? 1 : next.left - next.count;
+        next.tile = 0;
+        if (whole) next.row += row_step, next.head += head_step;
+        else next.head++;
+        if (next.head >= heads) next.head -= heads, next.row++;
+        complete();
+        const int count = cur.count, row = cur.row;
+        const int kv_head = kv_head_of(cur.head), block_of_16 = cur.head - kv_head * p.blocks_of_16;
+        // (a row's tiles begin with the one of its first token)
+        const int from_tile = cur.first / kTile + cur.tile, last = from_tile + count;
+        const int next_tile = next.left > 0 ? next.first / kTile + next.tile + wave : 0, next_last = next_tile - wave + next.count;
+        if (!loaded && from_tile + wave < last) {
+            find_pages(cur, from_tile + wave);
+            issue(kv_head, from_tile + wave, false);
+            issue(kv_head, from_tile + wave, true);
+        }
+        loaded = false;
         const int q_head = kv_head * p.group + 16 * block_of_16, q_heads = min(p.group - 16 * block_of_16, 16);
-        const int request = p.row_requests ? p.row_requests[row] : row;
-        const int32_t *table = p.table + request * p.table_stride;
 
         // ---- q, times a power of two that brings its largest value to 2^10 ... 2^11: both parts are then binary16
         // numbers of full precision however large or small the row is
@@ -369,81 +514,59 @@ __global__ void __launch_bounds__(kThreads, DIM == 256 ? 1 : 2) jl_kv_attention_
         for (int b = 0; b < kBlocks; b++) o[b] = floatx4{0.f, 0.f, 0.f, 0.f};
         float top = kNone, sum = 0.f;
 
-        // the pages of a tile's two halves; a half behind the last token, and a page outside the cache, is -1
-        auto pages_of = [&](int t, int (&page)[2]) {
+        for (int t = from_tile + wave; t < last; t += kWaves) {
+            const uint32_t here = paged;
+            // what is loaded next: this piece's next tile of the wave, or the next piece's first
+            const bool more = t + kWaves < last;
+            loaded = more || (next.left > 0 && next_tile < next_last);
+            const int load_tile = more ? t + kWaves : next_tile, load_head = more ? kv_head : kv_head_of(next.head);
+            if (loaded) find_pages(more ? cur : next, load_tile);
+            floatx4 s[kHalves];
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const int token = t * kTile + 16 * h;
-                page[h] = token < end ? table[token >> p.cache.page_shift] : -1;
-                if ((unsigned)page[h] >= (unsigned)p.cache.pages) page[h] = -1;
+            for (int h = 0; h < kHalves; h++) {
+                s[h] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < kSteps; i++) {
+                    const jl_half8 k = raw.k_operand(h, i);
+                    s[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q_lo[i], s[h], 0, 0, 0);
+                    s[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q_hi[i], s[h], 0, 0, 0);
+                }
             }
-        };
-        auto part_of = [&](int page) {
-            return p.cache.k + ((int64_t)(page < 0 ? 0 : page) * p.cache.kv_heads + kv_head) * p.cache.part_bytes;
-        };
-        const int in_page_mask = (1 << p.cache.page_shift) - 1;
-        Raw<Q8, DIM> raw;
-        const int last = first / kTile + tile + count;        // (the list's tiles of a row begin with the one of its first token)
-        int t = first / kTile + tile + wave;
-        if (t < last) {
-            int page[2], next[2] = {-1, -1};
-            pages_of(t, page);
+            if (loaded) issue(load_head, load_tile, false);   // k of the next tile goes out as soon as this one's is used
+            const bool all_seen = t * kTile >= cur.first && t * kTile + kTile <= cur.end && here == (1u << kHalves) - 1;
+            float x[4 * kHalves];
 #pragma unroll
-            for (int h = 0; h < 2; h++) raw.load_k(h, part_of(page[h]), (t * kTile + 16 * h) & in_page_mask, p.cache.page_shift, g, m);
+            for (int i = 0; i < 4 * kHalves; i++) x[i] = s[i / 4][i % 4] * undo;
+            if (!all_seen) {
+                bool seen[kHalves][4];
 #pragma unroll
-            for (int h = 0; h < 2; h++)
-                raw.load_v(h, part_of(page[h]) + p.cache.v_offset, (t * kTile + 16 * h) & in_page_mask, p.cache.page_shift, g, m);
-            if (t + kWaves < last) pages_of(t + kWaves, next);
-            for (; t < last; t += kWaves) {
-                const bool more = t + kWaves < last;
-                // S
-                floatx4 s[2];
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    s[h] = floatx4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int i = 0; i < kSteps; i++) {
-                        const jl_half8 k = raw.k_operand(h, i);
-                        s[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q_lo[i], s[h], 0, 0, 0);
-                        s[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q_hi[i], s[h], 0, 0, 0);
-                    }
+                for (int i = 0; i < 4 * kHalves; i++) {
+                    const int token = t * kTile + 16 * (i / 4) + 4 * g + i % 4;
+                    seen[i / 4][i % 4] = token >= cur.first && token < cur.end && (here >> (i / 4) & 1);
+                    x[i] = seen[i / 4][i % 4] ? x[i] : -INFINITY;
                 }
-                // k of the next tile goes out as soon as this one's is used
-                if (more) {
+                raw.mask_v(seen);
+            }
+            float most = x[0];
 #pragma unroll
-                    for (int h = 0; h < 2; h++)
-                        raw.load_k(h, part_of(next[h]), ((t + kWaves) * kTile + 16 * h) & in_page_mask, p.cache.page_shift, g, m);
-                }
-                const bool whole = t * kTile >= first && t * kTile + kTile <= end && page[0] >= 0 && page[1] >= 0;
-                float x[8];
+            for (int i = 1; i < 4 * kHalves; i++) most = fmaxf(most, x[i]);
+            most = over_groups_max(most);
+            // The maximum may fall behind by a factor of 2^8 before everything is brought to the new one: weights
+            // stay far inside binary16, and after a row's first tiles this is rare.
+            if (__any(most > top + 8.f)) {
+                const float next_top = fmaxf(top, most);
+                const float keep = __builtin_amdgcn_exp2f(top - next_top);
+                top = next_top;
+                sum *= keep;
 #pragma unroll
-                for (int i = 0; i < 8; i++) x[i] = s[i / 4][i % 4] * undo;
-                if (!whole) {
-                    bool seen[2][4];
+                for (int b = 0; b < kBlocks; b++) o[b] *= keep;
+            }
 #pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const int token = t * kTile + 16 * (i / 4) + 4 * g + i % 4;
-                        seen[i / 4][i % 4] = token >= first && token < end && page[i / 4] >= 0;
-                        x[i] = seen[i / 4][i % 4] ? x[i] : -INFINITY;
-                    }
-                    raw.mask_v(seen);
-                }
-                float most = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-                most = over_groups_max(most);
-                // The maximum may fall behind by a factor of 2^8 before everything is brought to the new one: weights
-                // stay far inside binary16, and after a row's first tiles this is rare.
-                if (__any(most > top + 8.f)) {
-                    const float next_top = fmaxf(top, most);
-                    const float keep = __builtin_amdgcn_exp2f(top - next_top);
-                    top = next_top;
-                    sum *= keep;
-#pragma unroll
-                    for (int b = 0; b < kBlocks; b++) o[b] *= keep;
-                }
+            for (int sub = 0; sub < kSubs; sub++) {
                 uintx4 hi, lo;
 #pragma unroll
                 for (int i = 0; i < 8; i += 2) {
-                    const float a = __builtin_amdgcn_exp2f(x[i] - top), b = __builtin_amdgcn_exp2f(x[i + 1] - top);
+                    const float a = __builtin_amdgcn_exp2f(x[8 * sub + i] - top), b = __builtin_amdgcn_exp2f(x[8 * sub + i + 1] - top);
                     sum += a + b;
                     const auto two = __builtin_amdgcn_cvt_pkrtz(a, b);
                     hi[i / 2] = __builtin_bit_cast(uint32_t, two);
@@ -452,18 +575,12 @@ __global__ void __launch_bounds__(kThreads, DIM == 256 ? 1 : 2) jl_kv_attention_
                 const jl_half8 p_hi = __builtin_bit_cast(jl_half8, hi), p_lo = __builtin_bit_cast(jl_half8, lo);
 #pragma unroll
                 for (int b = 0; b < kBlocks; b++) {
-                    const jl_half8 v = raw.v_operand(b);
+                    const jl_half8 v = raw.v_operand(sub, b);
                     o[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p_lo, o[b], 0, 0, 0);
                     o[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p_hi, o[b], 0, 0, 0);
                 }
-                if (more) {
-                    page[0] = next[0], page[1] = next[1];
-#pragma unroll
-                    for (int h = 0; h < 2; h++)
-                        raw.load_v(h, part_of(page[h]) + p.cache.v_offset, ((t + kWaves) * kTile + 16 * h) & in_page_mask, p.cache.page_shift, g, m);
-                    if (t + 2 * kWaves < last) pages_of(t + 2 * kWaves, next);
-                }
             }
+            if (loaded) issue(load_head, load_tile, true);
         }
 
         // ---- the four waves' parts into one
@@ -472,8 +589,18 @@ __global__ void __launch_bounds__(kThreads, DIM == 256 ? 1 : 2) jl_kv_attention_
         __syncthreads();
         const float together = fmaxf(fmaxf(joined_max[0][m], joined_max[1][m]), fmaxf(joined_max[2][m], joined_max[3][m]));
         const float share = __builtin_amdgcn_exp2f(top - together);
-        const bool opens = tile == 0, closes = tile + count == tiles;
-        float *slot = p.parts + (int64_t)(2 * blockIdx.x + (opens ? 1 : 0)) * (16 * (DIM + 2));
+        const bool opens = cur.tile == 0, closes = cur.tile + count == cur.tiles;
+        float *slot = p.parts + (int64_t)(2 * blockIdx.x + (opens ? 1 : 0)) * kSlot;
+        // (the most and the sum of a head of the sixteen)
+        auto of_waves = [&](int h, float &most, float &l) {
+            most = fmaxf(fmaxf(joined_max[0][h], joined_max[1][h]), fmaxf(joined_max[2][h], joined_max[3][h]));
+            l = 0.f;
+#pragma unroll
+            for (int w = 0; w < kWaves; w++) l += joined_sum[w][h] * __builtin_amdgcn_exp2f(joined_max[w][h] - most);
+        };
+        auto finish = [&](int h, int d, floatx4 v, float l) {
+            store_out(p, row * p.ldo + (int64_t)(q_head + h) * DIM + d, l == 0.f ? floatx4{0.f, 0.f, 0.f, 0.f} : v / l);
+        };
 #pragma unroll
         for (int from = 0; from < DIM; from += kRound) {
             if (from > 0) __syncthreads();
@@ -486,114 +613,114 @@ __global__ void __launch_bounds__(kThreads, DIM == 256 ? 1 : 2) jl_kv_attention_
             __syncthreads();
             for (int c = 4 * tid; c < q_heads * kRound; c += 4 * kThreads) {
                 const int h = c / kRound, d = c % kRound;
-                floatx4 v = *(const floatx4 *)&joined[0][h][d] + *(const floatx4 *)&joined[1][h][d] +
-                            *(const floatx4 *)&joined[2][h][d] + *(const floatx4 *)&joined[3][h][d];
+                const floatx4 v = *(const floatx4 *)&joined[0][h][d] + *(const floatx4 *)&joined[1][h][d] +
+                                  *(const floatx4 *)&joined[2][h][d] + *(const floatx4 *)&joined[3][h][d];
                 if (opens && closes) {
-                    const float most = fmaxf(fmaxf(joined_max[0][h], joined_max[1][h]), fmaxf(joined_max[2][h], joined_max[3][h]));
-                    float l = 0.f;
-#pragma unroll
-                    for (int w = 0; w < kWaves; w++) l += joined_sum[w][h] * __builtin_amdgcn_exp2f(joined_max[w][h] - most);
-                    v = l == 0.f ? floatx4{0.f, 0.f, 0.f, 0.f} : v / l;
-                    store_out(p, row * p.ldo + (int64_t)(q_head + h) * DIM + from + d, v);
+                    float most, l;
+                    of_waves(h, most, l);
+                    finish(h, from + d, v, l);
                 } else {
-                    *(floatx4 *)(slot + h * DIM + from + d) = v;
+                    agent_store4(slot + h * DIM + from + d, v);
                 }
             }
         }
-        if (!(opens && closes) && tid < q_heads) {
-            const float most = fmaxf(fmaxf(joined_max[0][tid], joined_max[1][tid]), fmaxf(joined_max[2][tid], joined_max[3][tid]));
-            float l = 0.f;
+        if (!(opens && closes)) {
+            // ---- a part of a head that others have parts of: the last of them to be done joins all, in their order
+            if (tid < q_heads) {
+                float most, l;
+                of_waves(tid, most, l);
+                agent_store(slot + 16 * DIM + tid, most);
+                agent_store(slot + 16 * DIM + 16 + tid, l);
+            }
+            const uint32_t head_begin = begin + min(span, total - begin) - cur.left - cur.tile;   // in the list of all tiles
+            const int opener = head_begin / span, parts = (head_begin + cur.tiles - 1) / span - opener + 1;
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's stores have arrived
+            __syncthreads();
+            if (tid == 0) {
+                const uint32_t before = __hip_atomic_fetch_add(p.arrived + opener, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                if (before == (uint32_t)(parts - 1)) __hip_atomic_store(p.arrived + opener, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                before_me = before;
+            }
+            __syncthreads();
+            if (before_me == (uint32_t)(parts - 1)) {
+                // part 0 is what its span opened, the others what theirs went on with
+                auto slot_of = [&](int i) { return p.parts + (int64_t)(2 * (opener + i) + (i == 0 ? 1 : 0)) * kSlot; };
+                float *most_of = &joined[0][0][0], *sum_of = most_of + 256, *top_of = most_of + 512, *l_of = most_of + 528;
+                {
+                    const int h = tid % 16;
+                    float most = kNone, l = 0.f;
+                    if (h < q_heads) {
+                        for (int i = tid / 16; i < parts; i += kThreads / 16) {
+                            const float a = agent_load(slot_of(i) + 16 * DIM + h), b = agent_load(slot_of(i) + 16 * DIM + 16 + h);
+                            const float next = fmaxf(most, a);
+                            l = l * __builtin_amdgcn_exp2f(most - next) + b * __builtin_amdgcn_exp2f(a - next);
+                            most = next;
+                        }
+                    }
+                    most_of[tid] = most, sum_of[tid] = l;
+                    __syncthreads();
+                    if (tid < 16) {
+                        for (int i = 1; i < kThreads / 16; i++) most = fmaxf(most, most_of[16 * i + tid]);
+                        l = 0.f;
+                        for (int i = 0; i < kThreads / 16; i++) l += sum_of[16 * i + tid] * __builtin_amdgcn_exp2f(most_of[16 * i + tid] - most);
+                        top_of[tid] = most, l_of[tid] = l;
+                    }
+                    __syncthreads();
+                }
+                // threads across the heads' elements, and across the parts where there are threads enough
+                const int quads = q_heads * (DIM / 4), sets = max(kThreads / quads, 1);
+                float *folded = &joined[1][0][0];             // [sets][quads] of four
+                for (int base = 0; base < quads; base += kThreads) {
+                    const int at = sets > 1 ? tid % quads : base + tid, set = sets > 1 ? tid / quads : 0;
+                    floatx4 v = {0.f, 0.f, 0.f, 0.f};
+                    const int h = at / (DIM / 4);
+                    if (at < quads && set < sets) {
+                        const float top_here = top_of[h];
+                        // (eight parts' loads are under way together: a loop that waits for each took 17 us over 64 parts)
+                        for (int i = set; i < parts; i += 8 * sets) {
+                            floatx4 part[8];
+                            float most[8];
 #pragma unroll
-            for (int w = 0; w < kWaves; w++) l += joined_sum[w][tid] * __builtin_amdgcn_exp2f(joined_max[w][tid] - most);
-            slot[16 * DIM + tid] = most;
-            slot[16 * DIM + 16 + tid] = l;
-        }
-        if (opens && tid == 0 && (p.by_head || !closes)) {
-            Part *cut = p.cut + (p.by_head ? row * heads + head : blockIdx.x);
-            const int64_t here = begin + (min(span, total - begin) - left);   // the head's first tile in the list
-            *cut = Part{row, head, (int)blockIdx.x, closes ? 0 : (int)((here + tiles - 1) / span) - (int)blockIdx.x + 1};
+                            for (int j = 0; j < 8; j++) {
+                                const float *slot = slot_of(min(i + j * sets, parts - 1));
+                                most[j] = agent_load(slot + 16 * DIM + h), part[j] = agent_load4(slot + 4 * at);
+                            }
+#pragma unroll
+                            for (int j = 0; j < 8; j++)
+                                if (i + j * sets < parts) v += __builtin_amdgcn_exp2f(most[j] - top_here) * part[j];
+                        }
+                        if (sets > 1) *(floatx4 *)(folded + 4 * (set * quads + at)) = v;
+                    }
+                    if (sets > 1) __syncthreads();
+                    if (at < quads && set == 0) {
+                        for (int i = 1; i < sets; i++) v += *(const floatx4 *)(folded + 4 * (i * quads + at));
+                        finish(h, 4 * (at % (DIM / 4)), v, l_of[h]);
+                    }
+                }
+            }
         }
         __syncthreads();
-        left -= count;
-        tile = 0;
-        if (closes && ++head == heads) {
-            head = 0;
-            do {
-                row++;
-                if (row >= p.rows) break;
-                range = range_of(p, row);
-                tiles = range.tiles();
-            } while (tiles == 0);
-        }
-    }
-}
-
-// Joins the parts of the row's head in cut[blockIdx.x], query head blockIdx.y of the sixteen.
-template <int DIM>
-__global__ void __launch_bounds__(256) jl_kv_attention_join_kernel(AttentionArgs p) {
-    constexpr int kLanes = DIM / 4, kSets = 256 / kLanes;      // threads across a row; parts summed side by side
-    __shared__ float most[kMostGroups], sums[kMostGroups];
-    __shared__ floatx4 folded[kSets][kLanes];
-    __shared__ float fold[8];
-    const Part cut = p.cut[blockIdx.x];
-    if (cut.count <= 0) return;
-    const int kv_head = cut.head / p.blocks_of_16, block_of_16 = cut.head % p.blocks_of_16, h = blockIdx.y;
-    if (16 * block_of_16 + h >= p.group) return;
-    const int tid = threadIdx.x;
-    // part 0 is what its span opened, the others what theirs went on with
-    auto slot = [&](int part) { return p.parts + (int64_t)(2 * (cut.group + part) + (part == 0 ? 1 : 0)) * (16 * (DIM + 2)); };
-    float top = kNone;
-    for (int i = tid; i < cut.count; i += 256) {
-        most[i] = slot(i)[16 * DIM + h];
-        sums[i] = slot(i)[16 * DIM + 16 + h];
-        top = fmaxf(top, most[i]);
-    }
-#pragma unroll
-    for (int off = 32; off; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, JL_WAVE));
-    if (tid % JL_WAVE == 0) fold[tid / JL_WAVE] = top;
-    __syncthreads();
-    top = fmaxf(fmaxf(fold[0], fold[1]), fmaxf(fold[2], fold[3]));
-    const int at = tid % kLanes, set = tid / kLanes;
-    floatx4 v = {0.f, 0.f, 0.f, 0.f};
-    float l = 0.f;
-    if (set < kSets) {
-        for (int i = set; i < cut.count; i += kSets) {
-            const float share = __builtin_amdgcn_exp2f(most[i] - top);
-            v += share * *(const floatx4 *)(slot(i) + h * DIM + 4 * at);
-        }
-        folded[set][at] = v;
-    }
-    for (int i = 0; i < cut.count; i++) l += sums[i] * __builtin_amdgcn_exp2f(most[i] - top);
-    __syncthreads();
-    if (tid < kLanes) {
-        v = folded[0][tid];
-        for (int i = 1; i < kSets; i++) v += folded[i][tid];
-        v = l == 0.f ? floatx4{0.f, 0.f, 0.f, 0.f} : v / l;
-        store_out(p, cut.row * p.ldo + (int64_t)(kv_head * p.group + 16 * block_of_16 + h) * DIM + 4 * tid, v);
     }
 }
 
 template <bool Q8, int DIM>
-hipError_t launch(const AttentionArgs &a, int groups, int cuts, hipStream_t stream) {
+hipError_t launch(const AttentionArgs &a, int compute_units, hipStream_t stream) {
+    const int groups = std::min(Shape<Q8, DIM>::kPerUnit * compute_units, kMostGroups);
     hipLaunchKernelGGL((jl_kv_attention_kernel<Q8, DIM>), dim3((unsigned)groups), dim3(kThreads), 0, stream, a);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((jl_kv_attention_join_kernel<DIM>), dim3((unsigned)cuts, (unsigned)(a.group < 16 ? a.group : 16)), dim3(256), 0,
-                       stream, a);
     return hipGetLastError();
 }
 template <bool Q8>
-hipError_t launch_dim(const AttentionArgs &a, int head_dim, int groups, int cuts, hipStream_t stream) {
+hipError_t launch_dim(const AttentionArgs &a, int head_dim, int compute_units, hipStream_t stream) {
     switch (head_dim) {
-        case 64: return launch<Q8, 64>(a, groups, cuts, stream);
-        case 96: return launch<Q8, 96>(a, groups, cuts, stream);
-        case 128: return launch<Q8, 128>(a, groups, cuts, stream);
-        case 192: return launch<Q8, 192>(a, groups, cuts, stream);
-        default: return launch<Q8, 256>(a, groups, cuts, stream);
+        case 64: return launch<Q8, 64>(a, compute_units, stream);
+        case 96: return launch<Q8, 96>(a, compute_units, stream);
+        case 128: return launch<Q8, 128>(a, compute_units, stream);
+        case 192: return launch<Q8, 192>(a, compute_units, stream);
+        default: return launch<Q8, 256>(a, compute_units, stream);
     }
 }
 
-constexpr size_t kCutBytes = kMostGroups * sizeof(Part);
+constexpr size_t kArrivedBytes = kMostGroups * sizeof(uint32_t);
 
 bool aligned(const void *p, int to) { return ((uintptr_t)p & (to - 1)) == 0; }
 
@@ -603,7 +730,17 @@ extern "C" {
 
 size_t jl_kv_attention_workspace_bytes(int heads, int kv_heads, int head_dim) {
     if (kv_heads <= 0 || heads <= 0 || heads % kv_heads || head_dim <= 0) return 0;
-    return kCutBytes + (size_t)2 * kMostGroups * 16 * (head_dim + 2) * sizeof(float);
+    return kArrivedBytes + (size_t)2 * kMostGroups * 16 * (head_dim + 2) * sizeof(float);
+}
+
+int jl_kv_attention_workspace_init(jl_context *ctx, void *workspace, size_t workspace_bytes) {
+    JL_REQUIRE(ctx && workspace, "jl_kv_attention_workspace_init: null argument");
+    JL_REQUIRE(aligned(workspace, 16), "jl_kv_attention_workspace_init: the workspace must be 16-byte aligned");
+    if (workspace_bytes < kArrivedBytes)
+        return jl_fail(JL_ERR_WORKSPACE, "jl_kv_attention_workspace_init: workspace of %zu bytes", workspace_bytes);
+    const JlOnDevice on(ctx);
+    JL_HIP(on.status);
+    return jl_launch_fill(ctx, (float *)workspace, 0.f, kArrivedBytes / sizeof(float));
 }
 
 int jl_kv_attention(jl_context *ctx, const jl_kv_cache *cache, const float *q, int heads, int64_t ldq, int64_t rows,
@@ -620,6 +757,11 @@ int jl_kv_attention(jl_context *ctx, const jl_kv_cache *cache, const float *q, i
     JL_REQUIRE(requests >= 0 && requests <= INT32_MAX && (row_requests || requests >= rows),
                "jl_kv_attention: %lld rows of %lld requests", (long long)rows, (long long)requests);
     JL_REQUIRE(table_stride > 0 && table_stride <= INT32_MAX, "jl_kv_attention: block table rows of %lld entries", (long long)table_stride);
+    // (a row's list of tiles of 32 tokens, times its heads, all rows together: a 32-bit number)
+    const int64_t table_tokens = std::min(table_stride * cache->page_tokens, (int64_t)INT_MAX - 64);
+    const int64_t lists = rows * cache->kv_heads * ((heads / cache->kv_heads + 15) / 16);
+    JL_REQUIRE(lists <= 0 || table_tokens / 32 + 2 <= (int64_t)(UINT32_MAX - 2 * kMostGroups) / lists,
+               "jl_kv_attention: %lld rows of %d heads over %lld tokens in one call", (long long)rows, heads, (long long)table_tokens);
     JL_REQUIRE(std::isfinite(scale), "jl_kv_attention: scale %g", (double)scale);
     JL_REQUIRE(window >= 0, "jl_kv_attention: window %lld", (long long)window);
     const int64_t width = (int64_t)heads * dim;
@@ -637,20 +779,17 @@ int jl_kv_attention(jl_context *ctx, const jl_kv_cache *cache, const float *q, i
     a.cache = jl_kv_view(cache);
     a.q = q, a.ldq = ldq, a.ldo = ldo;
     a.positions = positions, a.row_requests = row_requests, a.table = block_table;
-    a.requests = requests, a.table_stride = table_stride;
+    a.requests = (int)requests, a.table_stride = table_stride, a.table_tokens = (int)table_tokens;
     a.scale = scale * 1.44269504088896340736f;
     a.window = window > INT32_MAX ? 0 : (int)window;   // one that reaches behind every position
     a.group = heads / cache->kv_heads;
     a.blocks_of_16 = (a.group + 15) / 16;
     a.rows = (int)rows;
     a.out = out, a.out_f16 = out_f16 != 0;
-    a.cut = (Part *)workspace;
-    a.parts = (float *)((uint8_t *)workspace + kCutBytes);
-    const int groups = std::min(2 * ctx->compute_units, kMostGroups);
-    const int64_t row_heads = rows * cache->kv_heads * a.blocks_of_16;
-    a.by_head = row_heads <= groups;
-    const int cuts = a.by_head ? (int)row_heads : groups;
-    JL_HIP(cache->type == JL_KV_Q8_0 ? launch_dim<true>(a, dim, groups, cuts, ctx->stream) : launch_dim<false>(a, dim, groups, cuts, ctx->stream));
+    a.arrived = (uint32_t *)workspace;
+    a.parts = (float *)((uint8_t *)workspace + kArrivedBytes);
+    JL_HIP(cache->type == JL_KV_Q8_0 ? launch_dim<true>(a, dim, ctx->compute_units, ctx->stream)
+                                     : launch_dim<false>(a, dim, ctx->compute_units, ctx->stream));
     return JL_OK;
 }
 

@@ -362,11 +362,13 @@ def make_tables(rng, lengths, page, requests_of=None, requests=None, spare=2):
 
 
 def run_attend(ctx, cache, q, positions, requests_of, table, scale=None, window=0, half=False, pad=0, workspace=None, attention=None):
+    from jitllm_amd import _lib as L
     from jitllm_amd.attention import PagedAttention, Rows
     rows, heads, dim = q.shape
     attention = attention or PagedAttention(ctx, rows, heads, cache.kvHeads, dim)
     if workspace is not None:
         attention.workspace.upload(np.full(attention.workspace.nbytes, workspace, np.uint8))
+        L.check(ctx._lib.jl_kv_attention_workspace_init(ctx.handle, attention.workspace.ptr, attention.workspace.nbytes))
     stride = heads * dim + pad
     flat = np.full((rows, stride), np.nan, np.float32)
     flat[:, :heads * dim] = q.reshape(rows, -1)
