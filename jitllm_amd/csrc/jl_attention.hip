@@ -29,7 +29,9 @@ namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / JL_WAVE;
 constexpr int kMostGroups = 1024;         // workgroups of a launch, and spans
-constexpr int kWholeTokens = 512;         // rows no longer than this are never cut
+constexpr int kStart = 4;                 // what beginning a (row, head) pair takes, in tiles
+constexpr uint32_t kMostParts = 32;       // of a head
+constexpr int kDeviceScope = 16;          // a buffer load's policy: sc1
 constexpr float kNone = -3.0e38f;         // the running maximum of nothing: finite, so that differences are numbers
 
 template <bool Q8, int DIM>
@@ -37,6 +39,9 @@ struct Shape {
     // 16-token halves of a wave's tile: 64 tokens of 8-bit blocks are the registers, and the bytes in flight, of 32 of binary16
     static constexpr int kHalves = Q8 && DIM <= 128 ? 4 : 2, kTile = 16 * kHalves;
     static constexpr int kPerUnit = DIM == 256 ? 1 : 2;   // workgroups that a compute unit holds at a time
+    // Tiles that the whole chip reads (6 TB/s) in the time that a workgroup alone takes for one (half a microsecond).
+    static constexpr int kTileBytes = Q8 ? 2 * kTile * (DIM + DIM / 16) : 2 * kTile * DIM * 2;
+    static constexpr float kTilesAtOnce = 3.0e6f / kTileBytes;
 };
 
 typedef float floatx4 __attribute__((ext_vector_type(4)));
@@ -89,18 +94,6 @@ __device__ __forceinline__ void agent_store4(float *to, floatx4 v) {
     __hip_atomic_store((uint64_t *)to, two[0], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __hip_atomic_store((uint64_t *)to + 1, two[1], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-__device__ __forceinline__ float agent_load(const float *from) {
-    return __hip_atomic_load(from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ floatx4 agent_load4(const float *from) {
-    uint64_t two[2];
-    two[0] = __hip_atomic_load((const uint64_t *)from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    two[1] = __hip_atomic_load((const uint64_t *)from + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    floatx4 v;
-    __builtin_memcpy(&v, two, 16);
-    return v;
-}
-
 // k and v pass once: loads that do not stay in the caches (512 MB in 16 KB pieces, nothing else done: 90 us with ordinary
 // loads, 80 with these).
 template <typename T>
@@ -286,11 +279,20 @@ __device__ __forceinline__ void store_out(const AttentionArgs &p, int64_t at, co
     else *(floatx4 *)((float *)p.out + at) = v;
 }
 
+// Units of a head in the list of all work: its tiles, and what beginning it takes.
+__device__ __forceinline__ uint32_t units_of(int tiles) { return tiles > 0 ? tiles + kStart : 0; }
+
 // A piece of a workgroup's list: tiles tile ... tile + count - 1 of a row's head, and what the row sees.
 struct Piece {
     int row, head, tile, count, tiles;
     int first, end, request;
-    uint32_t left;    // tiles of the span, this piece's included; 0: no such piece
+    int unit;         // where the piece begins in its head
+    uint32_t left;    // units of the span, this piece's included; 0: no such piece
+};
+
+// A head that the workgroup has one of several parts of: those of spans group ... group + parts - 1.
+struct Cut {
+    int row, kv_head, block_of_16, group, parts;
 };
 
 template <bool Q8, int DIM>
@@ -302,8 +304,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
     constexpr int kSlot = 16 * (DIM + 2);
     __shared__ float joined[kWaves][16][kStride];
     __shared__ float joined_max[kWaves][16], joined_sum[kWaves][16];
-    __shared__ uint32_t scan[kWaves];
-    __shared__ uint32_t start_tiles, before_me;
+    __shared__ uint32_t scan[kWaves], scan_longest[kWaves], start_units, arrived[2];
     __shared__ int start_row;
     const int tid = threadIdx.x, lane = tid % JL_WAVE, wave = uniform(tid / JL_WAVE);
     const int g = lane / 16, m = lane % 16;
@@ -321,46 +322,53 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
     // ---- this workgroup's share of the list: whole (row, head) pairs one after the other where all rows are short, else
     // an equal span of tiles.  (All tiles together are fewer than 2^32: jl_kv_attention.)
     load_window(0);
-    const uint32_t mine = in_lane.tiles<kTile>();
+    const uint32_t mine = units_of(in_lane.tiles<kTile>());
     uint32_t all, through = mine;                             // tiles of all rows; of those up to this lane's (this thread's last)
-    bool whole;
-    if (p.rows <= JL_WAVE) {
-#pragma unroll
-        for (int off = 1; off < JL_WAVE; off <<= 1) {
-            const uint32_t other = __shfl_up(through, off, JL_WAVE);
-            if (lane >= off) through += other;
-        }
-        all = __builtin_amdgcn_readlane(through, JL_WAVE - 1);
-        whole = !__any(mine > kWholeTokens / kTile);
-    } else {
-        const int per = (p.rows + kThreads - 1) / kThreads;
-        bool longer = false;
-        through = 0;
+    uint32_t longest = mine, own = mine;
+    const int per = (p.rows + kThreads - 1) / kThreads;       // rows a thread, where a wave does not hold them all
+    if (p.rows > JL_WAVE) {
+        own = longest = 0;
         for (int r = tid * per; r < min((tid + 1) * per, p.rows); r++) {
-            const int n = range_of(p, r).tiles<kTile>();
-            through += n;
-            longer |= n > kWholeTokens / kTile;
+            const uint32_t n = units_of(range_of(p, r).tiles<kTile>());
+            own += n;
+            longest = max(longest, n);
         }
-        const uint32_t own = through;
+        through = own;
+    }
 #pragma unroll
-        for (int off = 1; off < JL_WAVE; off <<= 1) {
-            const uint32_t other = __shfl_up(through, off, JL_WAVE);
-            if (lane >= off) through += other;
-        }
-        if (lane == JL_WAVE - 1) scan[wave] = through;
-        whole = !__syncthreads_or(longer);
+    for (int off = 1; off < JL_WAVE; off <<= 1) {
+        const uint32_t other = __shfl_up(through, off, JL_WAVE);
+        if (lane >= off) through += other;
+    }
+#pragma unroll
+    for (int off = JL_WAVE / 2; off; off >>= 1) longest = max(longest, (uint32_t)__shfl_xor(longest, off, JL_WAVE));
+    all = __builtin_amdgcn_readlane(through, JL_WAVE - 1);
+    if (p.rows > JL_WAVE) {
+        if (lane == 0) scan[wave] = all, scan_longest[wave] = longest;
+        __syncthreads();
         all = 0;
         for (int w = 0; w < kWaves; w++) {
             if (w < wave) through += scan[w];
             all += scan[w];
+            longest = max(longest, scan_longest[w]);
         }
-        all = uniform(all);
-        const uint32_t from = (all * heads + gridDim.x - 1) / gridDim.x * blockIdx.x / heads;
-        if (!whole && from >= through - own && from < through) {
+    }
+    all = uniform(all), longest = uniform(longest);
+    // Pairs are not cut where a workgroup is done with its whole ones in the time that all take to read anyway, or in what
+    // joining parts takes besides, ten tiles' worth.  (32 rows of 8 heads, 1000 tokens each: 27.8 us whole, 31.6 cut; 8 heads
+    // of 1000 tokens: 20.2 whole, 10.2 cut; of 256 tokens: 9.1 and 9.7.)
+    const uint32_t most_units = longest * ((p.rows * heads + gridDim.x - 1) / gridDim.x);
+    const bool whole = (float)((int)most_units - kStart - 10) * Shape<Q8, DIM>::kTilesAtOnce <= (float)all * heads;
+    const uint32_t total = all * heads;
+    const uint32_t span = max((total + gridDim.x - 1) / gridDim.x, (longest + kMostParts - 1) / kMostParts);
+    const uint32_t begin = whole ? 0 : span * blockIdx.x;
+    if (p.rows > JL_WAVE) {
+        const uint32_t from = begin / heads;
+        if (!whole && begin < total && from >= through - own && from < through) {
             uint32_t before = through - own;
             int r = tid * per;
-            for (uint32_t n; before + (n = range_of(p, r).tiles<kTile>()) <= from; r++) before += n;
-            start_row = r, start_tiles = before;
+            for (uint32_t n; before + (n = units_of(range_of(p, r).tiles<kTile>())) <= from; r++) before += n;
+            start_row = r, start_units = before;
         }
         __syncthreads();
     }
@@ -373,11 +381,10 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
             for (int c = 4 * tid; c < width; c += 4 * kThreads) store_out(p, r * p.ldo + c, floatx4{0.f, 0.f, 0.f, 0.f});
     }
 
-    const uint32_t total = all * heads, span = (total + gridDim.x - 1) / gridDim.x, begin = whole ? 0 : span * blockIdx.x;
     const int row_step = gridDim.x / heads, head_step = gridDim.x % heads;    // from one whole pair of a workgroup to its next
     Piece next;
     if (whole) {
-        next.row = blockIdx.x / heads, next.head = blockIdx.x % heads, next.tile = 0;
+        next.row = blockIdx.x / heads, next.head = blockIdx.x % heads, next.unit = 0;
         next.left = 1;
     } else {
         if (begin >= total) return;
@@ -387,15 +394,15 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
             next.row = __popcll(__ballot(through <= from));
             before = next.row == 0 ? 0 : __builtin_amdgcn_readlane(through, uniform(next.row - 1));
         } else {
-            next.row = uniform(start_row), before = uniform(start_tiles);
+            next.row = uniform(start_row), before = uniform(start_units);
         }
-        next.head = begin - before * heads;                   // (its tile in the row's list, taken apart below)
-        next.tile = -1;
+        next.head = begin - before * heads;                   // (its unit in the row's list, taken apart below)
+        next.unit = -1;
         next.left = min(span, total - begin);
     }
     // Completes `next` from its row, head and tile, going on to the first row that has tiles.
     auto complete = [&]() {
-        next.row = uniform(next.row), next.head = uniform(next.head), next.tile = uniform(next.tile), next.left = uniform(next.left);
+        next.row = uniform(next.row), next.head = uniform(next.head), next.unit = uniform(next.unit), next.left = uniform(next.left);
         while (next.left > 0) {
             if (next.row >= p.rows) {
                 next.left = 0;
@@ -415,12 +422,15 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
                 next.row++;
             }
         }
-        if (next.tile < 0 && next.left > 0) {
-            const int into = next.head;
-            next.head = uniform((uint32_t)into / next.tiles);
-            next.tile = into - next.head * next.tiles;
+        if (next.unit < 0 && next.left > 0) {
+            const int into = next.head, units = units_of(next.tiles);
+            next.head = uniform((uint32_t)into / units);
+            next.unit = into - next.head * units;
         }
-        next.count = whole ? next.tiles : min((uint32_t)(next.tiles - next.tile), next.left);
+        // (a head's first units are its beginning, not tiles: a span that ends there has none of it)
+        const int until = whole ? next.tiles + kStart : min(next.unit + next.left, (uint32_t)next.tiles + kStart);
+        next.tile = max(next.unit - kStart, 0);
+        next.count = max(until - kStart, 0) - next.tile;
     };
 
     // k and v of a tile go from memory to `raw`; `page` are the pages of its halves, and one behind the last token, or one
@@ -430,7 +440,9 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
     uint32_t paged = 0;           // bit h: half h of the tile in `raw` has a page of the cache
     int page[kHalves];
     auto find_pages = [&](const Piece &c, int t) {
-        const int32_t *table = p.table + c.request * p.table_stride;
+        // (scalar loads: vector loads come back in order, and these would wait for the tile that is under way)
+        typedef const __attribute__((address_space(4))) int32_t constant_int;
+        constant_int *table = (constant_int *)(uintptr_t)(p.table + c.request * p.table_stride);
 #pragma unroll
         for (int h = 0; h < kHalves; h++) {
             const int token = t * kTile + 16 * h;
@@ -455,24 +467,27 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
     const bool one_block = p.blocks_of_16 == 1;
     auto kv_head_of = [&](int head) { return one_block ? head : head / p.blocks_of_16; };
 
+    Cut went_on, opened;
+    went_on.parts = opened.parts = 0;
     for (complete(); next.left > 0;) {
         const Piece cur = next;
         // the piece behind this one: the loads of its first tiles go out with this one's last
-        next.left = whole ? 1 : next.left - next.count;
-        next.tile = 0;
+        next.left = whole ? 1 : next.left - min(next.left, units_of(cur.tiles) - cur.unit);
+        next.unit = 0;
         if (whole) next.row += row_step, next.head += head_step;
         else next.head++;
         if (next.head >= heads) next.head -= heads, next.row++;
         complete();
         const int count = cur.count, row = cur.row;
+        if (count == 0) continue;
         const int kv_head = kv_head_of(cur.head), block_of_16 = cur.head - kv_head * p.blocks_of_16;
         // (a row's tiles begin with the one of its first token)
-        const int from_tile = cur.first / kTile + cur.tile, last = from_tile + count;
-        const int next_tile = next.left > 0 ? next.first / kTile + next.tile + wave : 0, next_last = next_tile - wave + next.count;
-        if (!loaded && from_tile + wave < last) {
-            find_pages(cur, from_tile + wave);
-            issue(kv_head, from_tile + wave, false);
-            issue(kv_head, from_tile + wave, true);
+        const int list_tile = cur.first / kTile + cur.tile, last = list_tile + count, from_tile = list_tile + wave;
+        const int next_list = next.left > 0 ? next.first / kTile + next.tile : 0, next_last = next_list + next.count, next_tile = next_list + wave;
+        if (!loaded && from_tile < last) {
+            find_pages(cur, from_tile);
+            issue(kv_head, from_tile, false);
+            issue(kv_head, from_tile, true);
         }
         loaded = false;
         const int q_head = kv_head * p.group + 16 * block_of_16, q_heads = min(p.group - 16 * block_of_16, 16);
@@ -514,7 +529,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
         for (int b = 0; b < kBlocks; b++) o[b] = floatx4{0.f, 0.f, 0.f, 0.f};
         float top = kNone, sum = 0.f;
 
-        for (int t = from_tile + wave; t < last; t += kWaves) {
+        for (int t = from_tile; t < last; t += kWaves) {
             const uint32_t here = paged;
             // what is loaded next: this piece's next tile of the wave, or the next piece's first
             const bool more = t + kWaves < last;
@@ -586,18 +601,8 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
         // ---- the four waves' parts into one
         sum = over_groups_sum(sum);
         if (g == 0) joined_max[wave][m] = top, joined_sum[wave][m] = sum;
-        __syncthreads();
-        const float together = fmaxf(fmaxf(joined_max[0][m], joined_max[1][m]), fmaxf(joined_max[2][m], joined_max[3][m]));
-        const float share = __builtin_amdgcn_exp2f(top - together);
         const bool opens = cur.tile == 0, closes = cur.tile + count == cur.tiles;
         float *slot = p.parts + (int64_t)(2 * blockIdx.x + (opens ? 1 : 0)) * kSlot;
-        // (the most and the sum of a head of the sixteen)
-        auto of_waves = [&](int h, float &most, float &l) {
-            most = fmaxf(fmaxf(joined_max[0][h], joined_max[1][h]), fmaxf(joined_max[2][h], joined_max[3][h]));
-            l = 0.f;
-#pragma unroll
-            for (int w = 0; w < kWaves; w++) l += joined_sum[w][h] * __builtin_amdgcn_exp2f(joined_max[w][h] - most);
-        };
         auto finish = [&](int h, int d, floatx4 v, float l) {
             store_out(p, row * p.ldo + (int64_t)(q_head + h) * DIM + d, l == 0.f ? floatx4{0.f, 0.f, 0.f, 0.f} : v / l);
         };
@@ -608,95 +613,118 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
 #pragma unroll
                 for (int b = from / 16; b < (from + kRound) / 16; b++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) joined[wave][m][out_element<DIM>(b, 4 * g + i) - from] = o[b][i] * share;
+                    for (int i = 0; i < 4; i++) joined[wave][m][out_element<DIM>(b, 4 * g + i) - from] = o[b][i];
             }
             __syncthreads();
             for (int c = 4 * tid; c < q_heads * kRound; c += 4 * kThreads) {
                 const int h = c / kRound, d = c % kRound;
-                const floatx4 v = *(const floatx4 *)&joined[0][h][d] + *(const floatx4 *)&joined[1][h][d] +
-                                  *(const floatx4 *)&joined[2][h][d] + *(const floatx4 *)&joined[3][h][d];
+                const float most = fmaxf(fmaxf(joined_max[0][h], joined_max[1][h]), fmaxf(joined_max[2][h], joined_max[3][h]));
+                floatx4 v = {0.f, 0.f, 0.f, 0.f};
+                float l = 0.f;
+#pragma unroll
+                for (int w = 0; w < kWaves; w++) {
+                    const float share = __builtin_amdgcn_exp2f(joined_max[w][h] - most);
+                    v += share * *(const floatx4 *)&joined[w][h][d];
+                    l += share * joined_sum[w][h];
+                }
                 if (opens && closes) {
-                    float most, l;
-                    of_waves(h, most, l);
                     finish(h, from + d, v, l);
                 } else {
                     agent_store4(slot + h * DIM + from + d, v);
+                    if (from + d == 0) agent_store(slot + 16 * DIM + h, most), agent_store(slot + 16 * DIM + 16 + h, l);
                 }
             }
         }
         if (!(opens && closes)) {
-            // ---- a part of a head that others have parts of: the last of them to be done joins all, in their order
-            if (tid < q_heads) {
-                float most, l;
-                of_waves(tid, most, l);
-                agent_store(slot + 16 * DIM + tid, most);
-                agent_store(slot + 16 * DIM + 16 + tid, l);
-            }
-            const uint32_t head_begin = begin + min(span, total - begin) - cur.left - cur.tile;   // in the list of all tiles
-            const int opener = head_begin / span, parts = (head_begin + cur.tiles - 1) / span - opener + 1;
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's stores have arrived
-            __syncthreads();
-            if (tid == 0) {
-                const uint32_t before = __hip_atomic_fetch_add(p.arrived + opener, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                if (before == (uint32_t)(parts - 1)) __hip_atomic_store(p.arrived + opener, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                before_me = before;
-            }
-            __syncthreads();
-            if (before_me == (uint32_t)(parts - 1)) {
-                // part 0 is what its span opened, the others what theirs went on with
-                auto slot_of = [&](int i) { return p.parts + (int64_t)(2 * (opener + i) + (i == 0 ? 1 : 0)) * kSlot; };
-                float *most_of = &joined[0][0][0], *sum_of = most_of + 256, *top_of = most_of + 512, *l_of = most_of + 528;
-                {
-                    const int h = tid % 16;
-                    float most = kNone, l = 0.f;
-                    if (h < q_heads) {
-                        for (int i = tid / 16; i < parts; i += kThreads / 16) {
-                            const float a = agent_load(slot_of(i) + 16 * DIM + h), b = agent_load(slot_of(i) + 16 * DIM + 16 + h);
-                            const float next = fmaxf(most, a);
-                            l = l * __builtin_amdgcn_exp2f(most - next) + b * __builtin_amdgcn_exp2f(a - next);
-                            most = next;
+            const uint32_t head_begin = begin + min(span, total - begin) - cur.left - cur.unit;   // in the list of all units
+            Cut &c = opens ? opened : went_on;
+            c.row = row, c.kv_head = kv_head, c.block_of_16 = block_of_16;
+            // the spans that have tiles of it: from the one of its first tile on
+            c.group = (head_begin + kStart) / span, c.parts = (head_begin + kStart + cur.tiles - 1) / span - c.group + 1;
+        }
+        __syncthreads();
+    }
+
+    // ---- heads that others have parts of: the workgroup that is the last to be done with its part joins all, in their
+    // order.  (Two at most: one that the span begins in, one that it ends in.)
+    if (went_on.parts == 0 && opened.parts == 0) return;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");          // this wave's stores have arrived
+    __syncthreads();
+    if (tid < 2) {
+        const int group = tid ? opened.group : went_on.group, parts = tid ? opened.parts : went_on.parts;
+        uint32_t before = 0;
+        if (parts > 0) {
+            before = __hip_atomic_fetch_add(p.arrived + group, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1;
+            if (before == (uint32_t)parts) __hip_atomic_store(p.arrived + group, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        arrived[tid] = before;
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int which = 0; which < 2; which++) {
+        const Cut c = which ? opened : went_on;
+        if (c.parts == 0 || arrived[which] != (uint32_t)c.parts) continue;
+        const int q_head = c.kv_head * p.group + 16 * c.block_of_16, q_heads = min(p.group - 16 * c.block_of_16, 16), parts = c.parts;
+        // (the parts were written past the second-level caches and are read past this XCD's own, which may hold an earlier
+        // call's: buffer loads with the bit for that.  A fence would empty the cache for everybody: 40 us instead of 32 where
+        // 256 heads are joined at once)
+        const auto parts_at = __builtin_amdgcn_make_buffer_rsrc((void *)p.parts, 0, -1, 0x00020000);
+        auto read4 = [&](int at) {
+            return __builtin_bit_cast(floatx4, __builtin_amdgcn_raw_buffer_load_b128(parts_at, 4 * at, 0, kDeviceScope));
+        };
+        auto read1 = [&](int at) {
+            return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(parts_at, 4 * at, 0, kDeviceScope));
+        };
+        // part 0 is what its span opened, the others what theirs went on with
+        auto slot_of = [&](int i) { return (2 * (c.group + i) + (i == 0 ? 1 : 0)) * kSlot; };
+        // Threads across the heads' elements, and across the parts where there are threads enough.  The loads of
+        // a batch of parts are under way together, their maxima and sums with them (64 parts: 17 us with a loop
+        // that waits for each).
+        constexpr int kBatch = 16;
+        const int quads = q_heads * (DIM / 4), sets = max(kThreads / quads, 1);
+        float *folded = &joined[0][0][0];             // [sets][quads]: four elements, the maximum, the sum
+        for (int base = 0; base < quads; base += kThreads) {
+            const int at = sets > 1 ? tid % quads : base + tid, set = sets > 1 ? tid / quads : 0;
+            const int h = at / (DIM / 4);
+            floatx4 v = {0.f, 0.f, 0.f, 0.f};
+            float most = kNone, l = 0.f;
+            if (at < quads && set < sets) {
+                for (int i = set; i < parts; i += kBatch * sets) {
+                    floatx4 part[kBatch];
+                    float part_most[kBatch], part_sum[kBatch];
+#pragma unroll
+                    for (int j = 0; j < kBatch; j++) {
+                        const int from = slot_of(min(i + j * sets, parts - 1));
+                        part_most[j] = read1(from + 16 * DIM + h), part_sum[j] = read1(from + 16 * DIM + 16 + h);
+                        part[j] = read4(from + 4 * at);
+                    }
+                    float next_most = most;
+#pragma unroll
+                    for (int j = 0; j < kBatch; j++) next_most = fmaxf(next_most, part_most[j]);
+                    const float keep = __builtin_amdgcn_exp2f(most - next_most);
+                    most = next_most, v *= keep, l *= keep;
+#pragma unroll
+                    for (int j = 0; j < kBatch; j++) {
+                        if (i + j * sets < parts) {
+                            const float share = __builtin_amdgcn_exp2f(part_most[j] - most);
+                            v += share * part[j], l += share * part_sum[j];
                         }
                     }
-                    most_of[tid] = most, sum_of[tid] = l;
-                    __syncthreads();
-                    if (tid < 16) {
-                        for (int i = 1; i < kThreads / 16; i++) most = fmaxf(most, most_of[16 * i + tid]);
-                        l = 0.f;
-                        for (int i = 0; i < kThreads / 16; i++) l += sum_of[16 * i + tid] * __builtin_amdgcn_exp2f(most_of[16 * i + tid] - most);
-                        top_of[tid] = most, l_of[tid] = l;
-                    }
-                    __syncthreads();
                 }
-                // threads across the heads' elements, and across the parts where there are threads enough
-                const int quads = q_heads * (DIM / 4), sets = max(kThreads / quads, 1);
-                float *folded = &joined[1][0][0];             // [sets][quads] of four
-                for (int base = 0; base < quads; base += kThreads) {
-                    const int at = sets > 1 ? tid % quads : base + tid, set = sets > 1 ? tid / quads : 0;
-                    floatx4 v = {0.f, 0.f, 0.f, 0.f};
-                    const int h = at / (DIM / 4);
-                    if (at < quads && set < sets) {
-                        const float top_here = top_of[h];
-                        // (eight parts' loads are under way together: a loop that waits for each took 17 us over 64 parts)
-                        for (int i = set; i < parts; i += 8 * sets) {
-                            floatx4 part[8];
-                            float most[8];
-#pragma unroll
-                            for (int j = 0; j < 8; j++) {
-                                const float *slot = slot_of(min(i + j * sets, parts - 1));
-                                most[j] = agent_load(slot + 16 * DIM + h), part[j] = agent_load4(slot + 4 * at);
-                            }
-#pragma unroll
-                            for (int j = 0; j < 8; j++)
-                                if (i + j * sets < parts) v += __builtin_amdgcn_exp2f(most[j] - top_here) * part[j];
-                        }
-                        if (sets > 1) *(floatx4 *)(folded + 4 * (set * quads + at)) = v;
-                    }
-                    if (sets > 1) __syncthreads();
-                    if (at < quads && set == 0) {
-                        for (int i = 1; i < sets; i++) v += *(const floatx4 *)(folded + 4 * (i * quads + at));
-                        finish(h, 4 * (at % (DIM / 4)), v, l_of[h]);
-                    }
+                if (sets > 1) {
+                    float *to = folded + 8 * (set * quads + at);
+                    *(floatx4 *)to = v, to[4] = most, to[5] = l;
                 }
+            }
+            if (sets > 1) __syncthreads();
+            if (at < quads && set == 0) {
+                for (int i = 1; i < sets; i++) {
+                    const float *from = folded + 8 * (i * quads + at);
+                    const float next_most = fmaxf(most, from[4]);
+                    const float keep = __builtin_amdgcn_exp2f(most - next_most), share = __builtin_amdgcn_exp2f(from[4] - next_most);
+                    v = keep * v + share * *(const floatx4 *)from, l = keep * l + share * from[5], most = next_most;
+                }
+                store_out(p, c.row * p.ldo + (int64_t)q_head * DIM + 4 * at, l == 0.f ? floatx4{0.f, 0.f, 0.f, 0.f} : v / l);
             }
         }
         __syncthreads();
@@ -760,7 +788,7 @@ int jl_kv_attention(jl_context *ctx, const jl_kv_cache *cache, const float *q, i
     // (a row's list of tiles of 32 tokens, times its heads, all rows together: a 32-bit number)
     const int64_t table_tokens = std::min(table_stride * cache->page_tokens, (int64_t)INT_MAX - 64);
     const int64_t lists = rows * cache->kv_heads * ((heads / cache->kv_heads + 15) / 16);
-    JL_REQUIRE(lists <= 0 || table_tokens / 32 + 2 <= (int64_t)(UINT32_MAX - 2 * kMostGroups) / lists,
+    JL_REQUIRE(lists <= 0 || table_tokens / 32 + 2 + kStart <= (int64_t)(UINT32_MAX - 2 * kMostGroups) / lists,
                "jl_kv_attention: %lld rows of %d heads over %lld tokens in one call", (long long)rows, heads, (long long)table_tokens);
     JL_REQUIRE(std::isfinite(scale), "jl_kv_attention: scale %g", (double)scale);
     JL_REQUIRE(window >= 0, "jl_kv_attention: window %lld", (long long)window);
