@@ -1,7 +1,9 @@
 // The paged key-value cache: its memory, the pages of a step (jl_kv_plan), and what is written to and read from
 // pages (jl_kv_append, jl_kv_read).  The attention over it is in jl_attention.hip.
+#include <algorithm>
 #include <climits>
 #include <new>
+#include <type_traits>
 
 #include "jl_kv.h"
 
@@ -9,8 +11,9 @@ namespace {
 
 // ---- jl_kv_plan ----------------------------------------------------------------------------------
 
-constexpr int kPlanThreads = 1024;
 constexpr int kPlanMaxRequests = 8192, kPlanMaxRows = 1 << 17;
+// Up to this many rows the requests' workgroup fills the rows' arrays itself; more are spread over a second launch.
+constexpr int kPlanRowsAtOnce = 4096;
 
 struct PlanArgs {
     const int32_t *past, *fresh, *free_in;
@@ -18,103 +21,241 @@ struct PlanArgs {
     int requests, pages, page_shift, table_stride, max_rows;
 };
 
-// Inclusive sums over the workgroup's threads of three values at once; `sums` [3][waves] in LDS.
-__device__ __forceinline__ void scan3(int (&v)[3], int (&total)[3], int (*sums)[kPlanThreads / JL_WAVE]) {
-    const int lane = threadIdx.x & (JL_WAVE - 1), wave = threadIdx.x / JL_WAVE;
-#pragma unroll
-    for (int off = 1; off < JL_WAVE; off <<= 1) {
-#pragma unroll
-        for (int i = 0; i < 3; i++) {
-            const int other = __shfl_up(v[i], off, JL_WAVE);
-            if (lane >= off) v[i] += other;
-        }
-    }
-    if (lane == JL_WAVE - 1)
-        for (int i = 0; i < 3; i++) sums[i][wave] = v[i];
-    __syncthreads();
-    for (int i = 0; i < 3; i++) {
-        int before = 0;
-        total[i] = 0;
-        for (int w = 0; w < kPlanThreads / JL_WAVE; w++) {
-            if (w < wave) before += sums[i][w];
-            total[i] += sums[i][w];
-        }
-        v[i] += before;
-    }
-    __syncthreads();
+// Inclusive sum over a wave's lanes: within rows of sixteen, then rows' last lanes handed on.
+__device__ __forceinline__ int wave_sum_through(int v) {
+#define JL_ADD_DPP(CONTROL, ROWS) v += __builtin_amdgcn_update_dpp(0, v, CONTROL, ROWS, 0xF, false)
+    JL_ADD_DPP(0x111, 0xF);   // row_shr 1, 2, 4, 8
+    JL_ADD_DPP(0x112, 0xF);
+    JL_ADD_DPP(0x114, 0xF);
+    JL_ADD_DPP(0x118, 0xF);
+    JL_ADD_DPP(0x142, 0xA);   // row_bcast 15 into rows 1 and 3, 31 into rows 2 and 3
+    JL_ADD_DPP(0x143, 0xC);
+#undef JL_ADD_DPP
+    return v;
 }
 
-// One workgroup, a thread a request: sums over the requests (rows, pages taken, pages returned) give each its place.
-__global__ void __launch_bounds__(kPlanThreads) jl_kv_plan_kernel(PlanArgs p) {
-    __shared__ int sums[3][kPlanThreads / JL_WAVE];
+// The sum of `v` over the threads before this one, and over all; `sums` [waves] in LDS, one per call.
+template <int THREADS>
+__device__ __forceinline__ int sum_before(int v, int &total, int *sums) {
+    const int lane = threadIdx.x % JL_WAVE, wave = threadIdx.x / JL_WAVE;
+    const int through = wave_sum_through(v);
+    if (lane == JL_WAVE - 1) sums[wave] = through;
+    __syncthreads();
+    int before = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / JL_WAVE; w++) {
+        if (w < wave) before += sums[w];
+        total += sums[w];
+    }
+    return before + through - v;
+}
+
+// The first of n ascending sums that is larger than x[j], for K numbers side by side; `most`: the smallest power of two
+// above n.  (Their steps wait for LDS together.)
+template <int K>
+__device__ __forceinline__ void first_above(const int *const (&through)[K], int n, int most, const int (&x)[K], int (&at)[K]) {
+#pragma unroll
+    for (int j = 0; j < K; j++) at[j] = 0;
+    for (int step = most >> 1; step > 0; step >>= 1) {
+#pragma unroll
+        for (int j = 0; j < K; j++) {
+            const int to = at[j] + step;
+            if (to <= n && through[j][to - 1] <= x[j]) at[j] = to;
+        }
+    }
+}
+__device__ __forceinline__ int power_above(int n) { return n > 0 ? 2 << (31 - __clz(n)) : 1; }
+
+__device__ __forceinline__ int wrapped(int64_t at, int pages) { return (int)(at < pages ? at : at - pages); }   // 0 <= at < 2 pages
+
+__device__ __forceinline__ int slot_in(const PlanArgs &p, int page, int position) {
+    return (unsigned)page < (unsigned)p.pages ? (page << p.page_shift) + (position & ((1 << p.page_shift) - 1)) : -1;
+}
+
+// One workgroup, ITEMS consecutive requests a thread.  Sums over the requests give each its rows and pages; what a
+// request has many of -- rows of a prompt, pages of one that begins or ends -- is dealt to all threads alike, each
+// finding its request by bisection in LDS.  Latency: of the lengths' loads, two sums over the workgroup, and the loads
+// of page numbers that hang on them.
+template <int THREADS, int ITEMS, bool ROWS>
+__global__ void __launch_bounds__(THREADS) jl_kv_plan_kernel(PlanArgs p) {
+    extern __shared__ int lds[];
+    int *rows_through = lds, *taken_through = lds + p.requests, *back_through = lds + 2 * p.requests, *first_position = lds + 3 * p.requests;
+    __shared__ int sums[3][THREADS / JL_WAVE], granted_pages, most_rows;
     const int tid = threadIdx.x, page = 1 << p.page_shift;
+    if (tid == 0) granted_pages = most_rows = 0;
     int head = p.free_in[0], count = p.free_in[1];
     if (head < 0 || head >= p.pages || count < 0 || count > p.pages) head = count = 0;
-    const int64_t table_tokens = min((int64_t)p.table_stride << p.page_shift, (int64_t)INT_MAX);   // positions are int32
-    int carry[3] = {0, 0, 0}, granted_pages = 0;
-    for (int base = 0; base < p.requests; base += kPlanThreads) {
-        const int r = base + tid;
-        const bool real = r < p.requests;
-        const int past = real ? p.past[r] : 0, fresh = real ? p.fresh[r] : 0;
-        const int wanted = min(max(fresh, 0), p.max_rows + 1);
-        const bool held = past >= 0 && past <= table_tokens;
-        const int had = held ? (int)(((int64_t)past + page - 1) >> p.page_shift) : 0;
-        // rows first: whether a request's rows fit decides whether it asks for pages
-        int v[3] = {wanted, 0, 0}, total[3];
-        scan3(v, total, sums);
-        const int row_end = carry[0] + v[0];
-        const bool fits = held && wanted == max(fresh, 0) && row_end <= p.max_rows && (int64_t)past + wanted <= table_tokens;
-        const int need = fits ? (int)(((int64_t)past + wanted + page - 1) >> p.page_shift) - had : 0;
-        const int back = fresh < 0 ? had : 0;
-        v[0] = 0, v[1] = need, v[2] = back;
-        const int rows_here = total[0];
-        scan3(v, total, sums);
-        const int need_end = carry[1] + v[1];
-        const bool granted = fits && wanted > 0 && (need == 0 || need_end <= count);
-        if (real) {
-            p.lengths[r] = fresh < 0 ? 0 : granted ? past + wanted : past;
-            p.row_starts[r + 1] = min(row_end, p.max_rows);
-            if (r == 0) p.row_starts[0] = 0;
-            for (int i = 0; i < wanted; i++) {
-                const int row = row_end - wanted + i;
-                if (row < p.max_rows) {
+    const int table_tokens = (int)min((int64_t)p.table_stride << p.page_shift, (int64_t)INT_MAX);   // positions are int32
+    int past[ITEMS], fresh[ITEMS], wanted[ITEMS], need[ITEMS], back[ITEMS];
+    int rows = 0;
+#pragma unroll
+    for (int j = 0; j < ITEMS; j++) {
+        const int r = tid * ITEMS + j;
+        past[j] = r < p.requests ? p.past[r] : 0, fresh[j] = r < p.requests ? p.fresh[r] : 0;
+        wanted[j] = min(max(fresh[j], 0), p.max_rows + 1);
+        rows += wanted[j];
+    }
+    int all_rows, all_need, all_back;
+    int row = sum_before<THREADS>(rows, all_rows, sums[0]);
+    // whether its rows fit decides whether a request asks for pages
+    int needs = 0, backs = 0, at = row;
+#pragma unroll
+    for (int j = 0; j < ITEMS; j++) {
+        at += wanted[j];
+        const bool held = past[j] >= 0 && past[j] <= table_tokens;
+        const int had = held ? (int)(((int64_t)past[j] + page - 1) >> p.page_shift) : 0;
+        const bool fits = held && wanted[j] == max(fresh[j], 0) && at <= p.max_rows && (int64_t)past[j] + wanted[j] <= table_tokens;
+        need[j] = fits ? (int)(((int64_t)past[j] + wanted[j] + page - 1) >> p.page_shift) - had : -1;    // -1: does not fit
+        back[j] = fresh[j] < 0 ? had : 0;
+        needs += max(need[j], 0), backs += back[j];
+    }
+    int asked = sum_before<THREADS>(needs, all_need, sums[1]);
+    int returned = sum_before<THREADS>(backs, all_back, sums[2]);
+    int granted_through = 0, widest = 0;
+#pragma unroll
+    for (int j = 0; j < ITEMS; j++) {
+        const int r = tid * ITEMS + j;
+        const int take = max(need[j], 0), had = need[j] >= 0 ? (int)(((int64_t)past[j] + page - 1) >> p.page_shift) : 0;
+        asked += take, returned += back[j];
+        const bool granted = need[j] >= 0 && wanted[j] > 0 && (take == 0 || asked <= count);
+        if (granted && take > 0) granted_through = asked;
+        widest = max(widest, wanted[j]);
+        if (r < p.requests) {
+            rows_through[r] = row + wanted[j];
+            taken_through[r] = granted ? asked : min(asked, count);      // (nothing behind the last one granted is taken)
+            back_through[r] = returned;
+            first_position[r] = granted ? past[j] : -1;
+            p.lengths[r] = fresh[j] < 0 ? 0 : granted ? past[j] + wanted[j] : past[j];
+            p.row_starts[r + 1] = min(row + wanted[j], p.max_rows);
+            if (wanted[j] > 0 && row < p.max_rows) {
+                // its first row; a second launch takes the position from here for the others
+                p.positions[row] = granted ? past[j] : -1;
+                if constexpr (ROWS) {
+                    const int b = past[j] >> p.page_shift;
+                    int of = -1;
+                    if (granted) of = b < had ? p.table[(int64_t)r * p.table_stride + b] : p.ring[wrapped((int64_t)head + asked - take + b - had, p.pages)];
                     p.row_requests[row] = r;
-                    p.positions[row] = granted ? past + i : -1;
-                    int slot = -1;
-                    if (granted) {
-                        const int b = (past + i) >> p.page_shift;
-                        const int at = b < had ? p.table[(int64_t)r * p.table_stride + b]
-                                               : p.ring[(int)(((int64_t)head + need_end - need + b - had) % p.pages)];
-                        if (at >= 0 && at < p.pages) slot = (at << p.page_shift) + ((past + i) & (page - 1));
-                    }
-                    p.slots[row] = slot;
-                }
-            }
-            if (granted)
-                for (int i = 0; i < need; i++)
-                    p.table[(int64_t)r * p.table_stride + had + i] = p.ring[(int)(((int64_t)head + need_end - need + i) % p.pages)];
-            if (back) {
-                for (int i = 0; i < back; i++) {
-                    const int64_t behind = (int64_t)carry[2] + v[2] - back + i;
-                    if (behind < p.pages - count)
-                        p.ring[(int)((head + count + behind) % p.pages)] = p.table[(int64_t)r * p.table_stride + i];
+                    p.slots[row] = slot_in(p, of, past[j]);
                 }
             }
         }
-        int g[3] = {granted ? need : 0, 0, 0}, gt[3];
-        scan3(g, gt, sums);
-        granted_pages += gt[0];
-        carry[0] += rows_here;
-        carry[1] += total[1];
-        carry[2] += total[2];
+        row += wanted[j];
     }
-    for (int row = carry[0] + tid; row < p.max_rows; row += kPlanThreads) p.slots[row] = p.positions[row] = p.row_requests[row] = -1;
+    if (tid == 0) p.row_starts[0] = 0;
+    if (granted_through > 0) atomicMax(&granted_pages, granted_through);
+    if (widest > 1) atomicMax(&most_rows, widest);
+    __syncthreads();
+    const int taken = granted_pages, put_back = min(all_back, p.pages - count);
+    // Everything that is moved is one list -- pages taken, pages returned, rows -- dealt to the threads: all searches run
+    // together, and then all loads.
+    const int most = power_above(p.requests), behind = wrapped((int64_t)head + count, p.pages);
+    const int used = min(all_rows, p.max_rows), rows_listed = ROWS && most_rows > 1 ? used : 0;
+    const int listed = taken + put_back + rows_listed;
+    auto move = [&](auto batch, int base) {
+        constexpr int K = decltype(batch)::value;
+        int kind[K], i[K], r[K], of[K], position[K];
+        const int *through[K];
+#pragma unroll
+        for (int j = 0; j < K; j++) {
+            const int e = min(base + j * THREADS + tid, listed - 1);
+            kind[j] = e < taken ? 0 : e < taken + put_back ? 1 : 2;
+            i[j] = e - (kind[j] == 0 ? 0 : kind[j] == 1 ? taken : taken + put_back);
+            through[j] = kind[j] == 0 ? taken_through : kind[j] == 1 ? back_through : rows_through;
+        }
+        first_above(through, p.requests, most, i, r);
+#pragma unroll
+        for (int j = 0; j < K; j++) {
+            const int into = i[j] - (r[j] > 0 ? through[j][r[j] - 1] : 0), first = first_position[r[j]];
+            const int had = (int)(((int64_t)first + page - 1) >> p.page_shift);
+            int32_t *row_of_table = p.table + (int64_t)r[j] * p.table_stride;
+            const int32_t *from;
+            if (kind[j] == 0) {
+                from = p.ring + wrapped((int64_t)head + i[j], p.pages);
+                position[j] = had + into;                     // the entry that it becomes
+            } else if (kind[j] == 1) {
+                from = row_of_table + into;
+                position[j] = 0;
+            } else {
+                position[j] = first < 0 ? -1 : first + into;
+                const int b = max(position[j], 0) >> p.page_shift;
+                from = b < had ? row_of_table + b : p.ring + wrapped((int64_t)head + (r[j] > 0 ? taken_through[r[j] - 1] : 0) + b - had, p.pages);
+            }
+            of[j] = kind[j] == 2 && first < 0 ? -1 : *from;
+        }
+#pragma unroll
+        for (int j = 0; j < K; j++) {
+            if (base + j * THREADS + tid >= listed) continue;
+            if (kind[j] == 0) {
+                p.table[(int64_t)r[j] * p.table_stride + position[j]] = of[j];
+            } else if (kind[j] == 1) {
+                // (places that no page is taken from: together with those they are at most the ring's)
+                p.ring[wrapped((int64_t)behind + i[j], p.pages)] = of[j];
+            } else {
+                p.row_requests[i[j]] = r[j];
+                p.positions[i[j]] = position[j];
+                p.slots[i[j]] = slot_in(p, of[j], position[j]);
+            }
+        }
+    };
+    int base = 0;
+    for (; listed - base > THREADS; base += 4 * THREADS) move(std::integral_constant<int, 4>{}, base);
+    if (listed > base) move(std::integral_constant<int, 1>{}, base);
+    if constexpr (ROWS)
+        for (int i = used + tid; i < p.max_rows; i += THREADS) p.slots[i] = p.positions[i] = p.row_requests[i] = -1;
     if (tid == 0) {
-        if (p.requests == 0) p.row_starts[0] = 0;
-        const int returned = min(carry[2], p.pages - count);
-        p.free_out[0] = (int)(((int64_t)head + granted_pages) % p.pages);
-        p.free_out[1] = count - granted_pages + returned;
+        p.free_out[0] = wrapped((int64_t)head + taken, p.pages);
+        p.free_out[1] = count - taken + put_back;
     }
+}
+
+// The rows of many: request, position and slot of each, from what the first launch left (row_starts, the table, and the
+// position of every request's first row).
+__global__ void __launch_bounds__(256) jl_kv_plan_rows_kernel(PlanArgs p) {
+    extern __shared__ int lds[];
+    for (int r = threadIdx.x; r < p.requests; r += 256) lds[r] = p.row_starts[r + 1];
+    __syncthreads();
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    if (i < p.max_rows) {
+        const int *const ends[1] = {lds};
+        const int mine[1] = {i};
+        int found[1];
+        first_above(ends, p.requests, power_above(p.requests), mine, found);
+        const int r = found[0];
+        int position = -1, slot = -1;
+        if (r < p.requests) {
+            // (the first row's thread writes the value that the others read)
+            const int start = r > 0 ? lds[r - 1] : 0, first = __hip_atomic_load(p.positions + start, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (first >= 0) {
+                position = first + i - start;
+                slot = slot_in(p, p.table[(int64_t)r * p.table_stride + (position >> p.page_shift)], position);
+            }
+        }
+        p.row_requests[i] = r < p.requests ? r : -1;
+        __hip_atomic_store(p.positions + i, position, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        p.slots[i] = slot;
+    }
+}
+
+template <int THREADS, int ITEMS>
+int launch_plan(jl_context *ctx, const PlanArgs &p) {
+    const int lds = std::max(4 * p.requests * (int)sizeof(int), 16);
+    const bool rows = p.max_rows <= kPlanRowsAtOnce;
+    const void *kernel = rows ? (const void *)jl_kv_plan_kernel<THREADS, ITEMS, true> : (const void *)jl_kv_plan_kernel<THREADS, ITEMS, false>;
+    if (lds > 60 * 1024) {
+        static jl_lds_limit_flags raised[2];
+        const int st = jl_raise_lds_limit(raised[rows], ctx->device, kernel, 4 * THREADS * ITEMS * (int)sizeof(int));
+        if (st != JL_OK) return st;
+    }
+    if (rows) {
+        hipLaunchKernelGGL((jl_kv_plan_kernel<THREADS, ITEMS, true>), dim3(1), dim3(THREADS), lds, ctx->stream, p);
+    } else {
+        hipLaunchKernelGGL((jl_kv_plan_kernel<THREADS, ITEMS, false>), dim3(1), dim3(THREADS), lds, ctx->stream, p);
+        JL_HIP(hipGetLastError());
+        hipLaunchKernelGGL(jl_kv_plan_rows_kernel, dim3((unsigned)((p.max_rows + 255) / 256)), dim3(256), std::max(4 * p.requests, 16), ctx->stream, p);
+    }
+    JL_HIP(hipGetLastError());
+    return JL_OK;
 }
 
 // ---- jl_kv_append --------------------------------------------------------------------------------
@@ -368,9 +509,9 @@ int jl_kv_plan(jl_context *ctx, const int32_t *past, const int32_t *fresh, int64
     p.slots = slots, p.positions = positions, p.row_requests = row_requests;
     p.requests = (int)requests, p.pages = (int)pages, p.page_shift = __builtin_ctz((unsigned)page_tokens);
     p.table_stride = (int)table_stride, p.max_rows = (int)max_rows;
-    hipLaunchKernelGGL(jl_kv_plan_kernel, dim3(1), dim3(kPlanThreads), 0, ctx->stream, p);
-    JL_HIP(hipGetLastError());
-    return JL_OK;
+    if (requests <= 1024) return launch_plan<1024, 1>(ctx, p);
+    if (requests <= 4096) return launch_plan<1024, 4>(ctx, p);
+    return launch_plan<1024, 8>(ctx, p);
 }
 
 int jl_kv_append(jl_context *ctx, jl_kv_cache *cache, const float *q, int heads, int64_t ldq, const float *k,
