@@ -66,30 +66,30 @@ class Rows:
     """Rows of a device array that lie ``stride`` elements apart, the first ``offset`` elements in: the q, k
     or v part of the rows that a fused projection leaves side by side."""
 
+    __slots__ = ("array", "stride", "offset")
+
     def __init__(self, array, stride: int, offset: int = 0):
-        self.array, self.stride, self.offset = array, int(stride), int(offset)
-        self.itemsize = array.nbytes // array.size if array.size else 4
-
-    def ptr(self, who: str, rows: int, width: int) -> int:
-        """Address of the first row; raises where ``rows`` rows of ``width`` elements are not the array's."""
-        if self.stride < width or self.offset < 0 or (rows and self.offset + (rows - 1) * self.stride + width > self.array.size):
-            raise ValueError(f"{who}: {rows} rows of {width} elements, {self.stride} apart from {self.offset} on, "
-                             f"in an array of {self.array.size}")
-        return _address(self.array) + self.offset * self.itemsize
+        self.array, self.stride, self.offset = array, stride, offset
 
 
-def _address(array) -> int:
-    return array.ptr.value or 0
-
-
-def _rows(value, width: int) -> Rows:
-    return value if isinstance(value, Rows) else Rows(value, width)
+def _place(who: str, value, rows: int, width: int):
+    """(address, stride) of ``rows`` rows of ``width`` elements; raises where they are not the array's.  An
+    array in place of Rows: its rows lie behind one another."""
+    if value.__class__ is Rows:
+        array, stride, offset = value.array, value.stride, value.offset
+    else:
+        array, stride, offset = value, width, 0
+    size = array.size
+    if stride < width or offset < 0 or (rows > 0 and offset + (rows - 1) * stride + width > size):
+        raise ValueError(f"{who}: {rows} rows of {width} elements, {stride} apart from {offset} on, in an array of {size}")
+    address = array.ptr.value or 0
+    return (address + offset * (array.nbytes // size) if offset else address), stride
 
 
 def _ints(who: str, array, count: int) -> int:
     if array.nbytes < 4 * count:
         raise ValueError(f"{who}: {count} int32 values in an array of {array.nbytes} bytes")
-    return _address(array)
+    return array.ptr.value or 0
 
 
 class Rope:
@@ -102,6 +102,7 @@ class Rope:
         if frequencies.nbytes < 4 * rotated:
             raise ValueError(f"{rotated // 2} frequencies in an array of {frequencies.nbytes} bytes")
         self.ctx, self.frequencies, self.rotated, self.style = ctx, frequencies, int(rotated), RopeStyle(style)
+        self._args = (frequencies.ptr.value, self.rotated, int(self.style))
 
     @classmethod
     def of(cls, ctx: Context, frequencies, style: RopeStyle = RopeStyle.PAIRS) -> "Rope":
@@ -113,6 +114,9 @@ class Rope:
     @classmethod
     def of_base(cls, ctx: Context, rotated: int, base: float, style: RopeStyle = RopeStyle.PAIRS) -> "Rope":
         return cls.of(ctx, float(base) ** (-np.arange(0, rotated, 2, dtype=np.float64) / rotated), style)
+
+
+_NO_ROPE = (None, 0, int(RopeStyle.PAIRS))
 
 
 class PagedKvCache:
@@ -157,19 +161,25 @@ class PagedKvCache:
                qNorm=None, kNorm=None, eps: float = 0.0) -> None:
         """Turns q and k (normalised first where ``qNorm`` / ``kNorm`` are given) and writes k and v to
         ``slots`` (jl_kv_append).  ``q`` is turned into ``qOut``, or in place without one."""
-        width, qWidth = self.kvHeads * self.headDim, heads * self.headDim
-        k, v = _rows(k, width), _rows(v, width)
-        q = _rows(q, qWidth) if q is not None else None
-        qOut = q if qOut is None else _rows(qOut, qWidth)
-        for name, norm in (("qNorm", qNorm), ("kNorm", kNorm)):
+        width = self.kvHeads * self.headDim
+        k, ldk = _place("k", k, rows, width)
+        v, ldv = _place("v", v, rows, width)
+        if q is None:
+            q = ldq = out = ldOut = heads = 0
+        else:
+            width = heads * self.headDim
+            out, ldOut = _place("qOut", q if qOut is None else qOut, rows, width)
+            q, ldq = _place("q", q, rows, width)
+        for name, norm in (("qNorm", qNorm), ("kNorm", kNorm)) if qNorm is not None or kNorm is not None else ():
             if norm is not None and norm.size != self.headDim:
                 raise ValueError(f"{name} has {norm.size} weights, a head {self.headDim} values")
-        L.check(self._lib.jl_kv_append(
-            self.ctx.handle, self.handle, q.ptr("q", rows, qWidth) if q else None, heads, q.stride if q else 0,
-            k.ptr("k", rows, width), k.stride, v.ptr("v", rows, width), v.stride, qOut.ptr("qOut", rows, qWidth) if q else None,
-            qOut.stride if q else 0, _ints("positions", positions, rows), _ints("slots", slots, rows), rows,
-            rope.frequencies.ptr if rope else None, rope.rotated if rope else 0, rope.style if rope else RopeStyle.PAIRS,
-            qNorm.ptr if qNorm is not None else None, kNorm.ptr if kNorm is not None else None, float(eps)))
+        frequencies, rotated, style = rope._args if rope is not None else _NO_ROPE
+        status = self._lib.jl_kv_append(
+            self.ctx.handle, self.handle, q, heads, ldq, k, ldk, v, ldv, out, ldOut, _ints("positions", positions, rows),
+            _ints("slots", slots, rows), rows, frequencies, rotated, style, qNorm.ptr if qNorm is not None else None,
+            kNorm.ptr if kNorm is not None else None, eps)
+        if status:
+            L.check(status)
 
     def read(self, slots, rows: int, k=None, v=None) -> None:
         """Decodes the k and v at ``slots`` into rows of kvHeads x headDim values, binary16 or fp32 by the
@@ -220,13 +230,13 @@ class BlockTables:
     def plan(self, fresh, past=None, freeIn=None) -> None:
         """One step: ``fresh`` [requests] new tokens of each request (negative: it has ended).  Lengths and
         free pages move on in place; ``past`` / ``freeIn`` give others to start from."""
-        for name, array, count in (("fresh", fresh, self.requests), ("past", past, self.requests), ("freeIn", freeIn, 2)):
-            if array is not None:
-                _ints(name, array, count)
-        L.check(self._lib.jl_kv_plan(
-            self.ctx.handle, (past or self.lengths).ptr, fresh.ptr, self.requests, self.pages, self.pageTokens, self.pageRing.ptr,
-            (freeIn or self.freePages).ptr, self.freePages.ptr, self.table.ptr, self.blocksPerRequest, self.lengths.ptr,
-            self.rowStarts.ptr, self.slots.ptr, self.positions.ptr, self.rowRequests.ptr, self.maxRows))
+        n = self.requests
+        status = self._lib.jl_kv_plan(
+            self.ctx.handle, _ints("past", self.lengths if past is None else past, n), _ints("fresh", fresh, n), n, self.pages, self.pageTokens,
+            self.pageRing.ptr, _ints("freeIn", self.freePages if freeIn is None else freeIn, 2), self.freePages.ptr, self.table.ptr,
+            self.blocksPerRequest, self.lengths.ptr, self.rowStarts.ptr, self.slots.ptr, self.positions.ptr, self.rowRequests.ptr, self.maxRows)
+        if status:
+            L.check(status)
 
 
 class PagedAttention:
@@ -236,6 +246,7 @@ class PagedAttention:
     def __init__(self, ctx: Context, maxRows: int, heads: int, kvHeads: int, headDim: int):
         self.ctx, self._lib = ctx, ctx._lib
         self.maxRows, self.heads, self.kvHeads, self.headDim = int(maxRows), int(heads), int(kvHeads), int(headDim)
+        self.width, self.scale = self.heads * self.headDim, 1 / math.sqrt(self.headDim) if headDim > 0 else 0.0
         nbytes = self._lib.jl_kv_attention_workspace_bytes(heads, kvHeads, headDim)
         if not nbytes:
             raise ValueError(f"{heads} query heads over {kvHeads} of k and v, {headDim} values each")
@@ -247,13 +258,17 @@ class PagedAttention:
         """``out[row] = softmax(scale * q[row] . k) v`` over the tokens up to ``positions[row]`` (the last
         ``window`` of them where that is positive) of request ``rowRequests[row]``, or of request ``row``.
         ``scale``: 1 / sqrt(headDim) unless given.  ``out``: a FloatArray or a HalfFloatArray."""
-        width = self.heads * self.headDim
-        if (cache.kvHeads, cache.headDim) != (self.kvHeads, self.headDim):
+        if cache.kvHeads != self.kvHeads or cache.headDim != self.headDim:
             raise ValueError(f"a cache of {cache.kvHeads} heads of {cache.headDim}, attention over {self.kvHeads} of {self.headDim}")
-        q, out = _rows(q, width), _rows(out, width)
-        stride = table.nbytes // 4 // requests if requests else 0
-        L.check(self._lib.jl_kv_attention(
-            self.ctx.handle, cache.handle, q.ptr("q", rows, width), self.heads, q.stride, rows, _ints("positions", positions, rows),
-            _ints("rowRequests", rowRequests, rows) if rowRequests is not None else None, table.ptr, requests, max(1, stride),
-            float(scale if scale is not None else 1 / math.sqrt(self.headDim)), window, out.ptr("out", rows, width),
-            int(out.itemsize == 2), out.stride, self.workspace.ptr, self.workspace.nbytes))
+        width = self.width
+        array = out.array if out.__class__ is Rows else out
+        half = array.nbytes == 2 * array.size
+        q, ldq = _place("q", q, rows, width)
+        out, ldOut = _place("out", out, rows, width)
+        status = self._lib.jl_kv_attention(
+            self.ctx.handle, cache.handle, q, self.heads, ldq, rows, _ints("positions", positions, rows),
+            _ints("rowRequests", rowRequests, rows) if rowRequests is not None else None, table.ptr, requests,
+            table.nbytes // 4 // requests if requests > 0 else 1, self.scale if scale is None else scale, window, out, half, ldOut,
+            self.workspace.ptr, self.workspace.nbytes)
+        if status:
+            L.check(status)

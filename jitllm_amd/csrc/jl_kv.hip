@@ -261,6 +261,7 @@ int launch_plan(jl_context *ctx, const PlanArgs &p) {
 // ---- jl_kv_append --------------------------------------------------------------------------------
 
 constexpr int kAppendThreads = 256;
+constexpr int kAppendPer = 2;   // heads a thread has (2048 tokens of 48 heads of 128: 18.8 us with one, 17.8 with two, 18.2 with four)
 
 struct AppendArgs {
     JlKvView cache;
@@ -272,111 +273,125 @@ struct AppendArgs {
     const float *q_norm, *k_norm;
     float eps;
     int heads, head_dim, rotated;   // heads: 0 without q
-    bool halves;
 };
 
-// LANES consecutive lanes have a head, eight values each (those past head_dim / 8 idle); a wave has 64 / LANES heads at
-// a time, a workgroup the q, k and v heads [blockIdx.y * 256 / LANES, ...) of a token.
-template <bool Q8, int LANES>
+// LANES consecutive lanes have a head, eight values each (those past head_dim / 8 idle); a workgroup has kAppendPer times
+// 256 / LANES of a token's q, k and v heads, and all their loads are on their way before anything else is done.
+// Bound: the bytes.  The angles' cosines and sines are worked out once per workgroup, in LDS, while the loads come in.
+template <bool Q8, int LANES, bool HALVES>
 __global__ void __launch_bounds__(kAppendThreads) jl_kv_append_kernel(AppendArgs p) {
     __shared__ float2 turn[128];    // (cos, sin) of the token's pairs
     const int row = blockIdx.x, tid = threadIdx.x;
     const int position = p.positions[row];
     if (position < 0) return;
+    const int slot = p.slots[row];
+    const int kv_heads = p.cache.kv_heads, units = p.heads + 2 * kv_heads;
+    const int first_unit = blockIdx.y * (kAppendPer * (kAppendThreads / LANES)) + tid / LANES, chunk = tid % LANES;
+    const bool in_head = chunk < p.head_dim / 8;
+    // where the partners of this lane's values lie: half the turned part on, or back
+    const int half_chunks = p.rotated / 16;
+    const bool turns = 8 * chunk < p.rotated, first_half = chunk < half_chunks;
+    const int partner = !HALVES || !turns ? chunk : first_half ? chunk + half_chunks : chunk - half_chunks;
+    float4 own[kAppendPer][2], other[kAppendPer][2];
+#pragma unroll
+    for (int j = 0; j < kAppendPer; j++) {
+        const int unit = first_unit + j * (kAppendThreads / LANES);
+        if (unit < units && in_head) {
+            const float *x = unit < p.heads              ? p.q + row * p.ldq + unit * p.head_dim
+                             : unit < p.heads + kv_heads ? p.k + row * p.ldk + (unit - p.heads) * p.head_dim
+                                                         : p.v + row * p.ldv + (unit - p.heads - kv_heads) * p.head_dim;
+            own[j][0] = *(const float4 *)(x + 8 * chunk), own[j][1] = *(const float4 *)(x + 8 * chunk + 4);
+            if (HALVES && unit < p.heads + kv_heads)
+                other[j][0] = *(const float4 *)(x + 8 * partner), other[j][1] = *(const float4 *)(x + 8 * partner + 4);
+        }
+    }
     for (int i = tid; i < p.rotated / 2; i += kAppendThreads) {
         // whole turns are dropped in double precision; what is left needs 24 bits
-        const double turns = (double)position * p.frequencies[i] * 0.15915494309189533577;
+        const double turns_of = (double)position * p.frequencies[i] * 0.15915494309189533577;
         float s, c;
-        sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
+        sincospif(2.0f * (float)(turns_of - rint(turns_of)), &s, &c);
         turn[i] = make_float2(c, s);
     }
     __syncthreads();
-    const int unit = blockIdx.y * (kAppendThreads / LANES) + tid / LANES, chunk = tid % LANES;
-    const int kv_heads = p.cache.kv_heads;
-    if (unit >= p.heads + 2 * kv_heads) return;
-    const bool live = chunk < p.head_dim / 8;
-    const bool is_q = unit < p.heads, is_v = unit >= p.heads + kv_heads;
-    const float *x = is_q ? p.q + row * p.ldq + unit * p.head_dim
-                   : is_v ? p.v + row * p.ldv + (unit - p.heads - kv_heads) * p.head_dim
-                          : p.k + row * p.ldk + (unit - p.heads) * p.head_dim;
-    const float *norm = is_q ? p.q_norm : is_v ? nullptr : p.k_norm;
-    const int rotated = is_v ? 0 : p.rotated;
-    float a[8], b[8];               // the lane's values, and those they turn with (halves)
-    // where the partners of this lane's values lie: half the turned part on, or back
-    const int half_chunks = rotated / 16;
-    const int partner = !p.halves || 8 * chunk >= rotated ? chunk : chunk < half_chunks ? chunk + half_chunks : chunk - half_chunks;
 #pragma unroll
-    for (int i = 0; i < 8; i++) a[i] = live ? x[8 * chunk + i] : 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; i++) b[i] = live ? x[8 * partner + i] : 0.f;
-    if (norm) {
-        float ss = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; i++) ss = fmaf(a[i], a[i], ss);
-        ss = jl_group_sum<LANES>(ss);
-        const float root = sqrtf(ss / (float)p.head_dim + p.eps);
+    for (int j = 0; j < kAppendPer; j++) {
+        const int unit = first_unit + j * (kAppendThreads / LANES);
+        if (unit >= units) return;                            // (a head's lanes together)
+        const bool is_q = unit < p.heads, is_v = unit >= p.heads + kv_heads;
+        const float *norm = is_q ? p.q_norm : is_v ? nullptr : p.k_norm;
+        float a[8], b[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            a[i] = live ? a[i] / root * norm[8 * chunk + i] : 0.f;
-            b[i] = live ? b[i] / root * norm[8 * partner + i] : 0.f;
+            a[i] = in_head ? (&own[j][i / 4].x)[i % 4] : 0.f;
+            if constexpr (HALVES) b[i] = in_head && !is_v ? (&other[j][i / 4].x)[i % 4] : 0.f;
         }
-    }
-    if (live && 8 * chunk < rotated) {
-        if (p.halves) {
-            const bool first = chunk < half_chunks;
+        if (norm) {
+            float ss = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; i++) ss = fmaf(a[i], a[i], ss);
+            ss = jl_group_sum<LANES>(ss);
+            const float root = sqrtf(ss / (float)p.head_dim + p.eps);
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const float2 t = turn[8 * (first ? chunk : partner) + i];
-                a[i] = first ? a[i] * t.x - b[i] * t.y : b[i] * t.y + a[i] * t.x;
+                if (in_head) a[i] = a[i] / root * norm[8 * chunk + i];
+                if (HALVES && in_head) b[i] = b[i] / root * norm[8 * partner + i];
             }
+        }
+        if (in_head && turns && !is_v) {
+            if constexpr (HALVES) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float2 t = turn[8 * (first_half ? chunk : partner) + i];
+                    a[i] = first_half ? a[i] * t.x - b[i] * t.y : b[i] * t.y + a[i] * t.x;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i += 2) {
+                    const float2 t = turn[4 * chunk + i / 2];
+                    const float even = a[i], odd = a[i + 1];
+                    a[i] = even * t.x - odd * t.y;
+                    a[i + 1] = even * t.y + odd * t.x;
+                }
+            }
+        }
+        if (is_q) {
+            float *out = p.q_out + row * p.ldq_out + unit * p.head_dim + 8 * chunk;
+            if (in_head) {
+                *(float4 *)out = make_float4(a[0], a[1], a[2], a[3]);
+                *(float4 *)(out + 4) = make_float4(a[4], a[5], a[6], a[7]);
+            }
+            continue;
+        }
+        if (slot < 0 || (slot >> p.cache.page_shift) >= p.cache.pages) continue;
+        const int page = slot >> p.cache.page_shift, token = slot & ((1 << p.cache.page_shift) - 1);
+        uint8_t *part = p.cache.k + (is_v ? p.cache.v_offset : 0) +
+                        ((int64_t)page * kv_heads + (is_v ? unit - p.heads - kv_heads : unit - p.heads)) * p.cache.part_bytes;
+        if constexpr (!Q8) {
+            jl_half8 h;
+#pragma unroll
+            for (int i = 0; i < 8; i++) h[i] = (_Float16)a[i];
+            if (in_head) *(jl_half8 *)(part + (token * p.head_dim + 8 * chunk) * 2) = h;
         } else {
+            float most = 0.f;
 #pragma unroll
-            for (int i = 0; i < 8; i += 2) {
-                const float2 t = turn[4 * chunk + i / 2];
-                const float even = a[i], odd = a[i + 1];
-                a[i] = even * t.x - odd * t.y;
-                a[i + 1] = even * t.y + odd * t.x;
+            for (int i = 0; i < 8; i++) most = fmaxf(most, fabsf(a[i]));
+            most = fmaxf(most, __shfl_xor(most, 1, JL_WAVE));   // a block is four lanes' values
+            most = fmaxf(most, __shfl_xor(most, 2, JL_WAVE));
+            const _Float16 d16 = (_Float16)fminf(most / 127.f, 65504.f);
+            const float d = (float)d16;
+            uint32_t word[2] = {0, 0};
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                // (NaN: both comparisons fall to the other operand's side, so it is taken out first)
+                const float y = d > 0.f && a[i] == a[i] ? fminf(fmaxf(rintf(a[i] / d), -127.f), 127.f) : 0.f;
+                word[i / 4] |= (uint32_t)((int)y & 255) << (8 * (i % 4));
             }
-        }
-    }
-    if (is_q) {
-        float *out = p.q_out + row * p.ldq_out + unit * p.head_dim + 8 * chunk;
-        if (live) {
-            *(float4 *)out = make_float4(a[0], a[1], a[2], a[3]);
-            *(float4 *)(out + 4) = make_float4(a[4], a[5], a[6], a[7]);
-        }
-        return;
-    }
-    const int slot = p.slots[row];
-    if (slot < 0 || (slot >> p.cache.page_shift) >= p.cache.pages) return;
-    const int page = slot >> p.cache.page_shift, token = slot & ((1 << p.cache.page_shift) - 1);
-    uint8_t *part = p.cache.k + (is_v ? p.cache.v_offset : 0) +
-                    ((int64_t)page * kv_heads + (is_v ? unit - p.heads - kv_heads : unit - p.heads)) * p.cache.part_bytes;
-    if constexpr (!Q8) {
-        jl_half8 h;
-#pragma unroll
-        for (int i = 0; i < 8; i++) h[i] = (_Float16)a[i];
-        if (live) *(jl_half8 *)(part + (token * p.head_dim + 8 * chunk) * 2) = h;
-    } else {
-        float most = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; i++) most = fmaxf(most, fabsf(a[i]));
-        most = fmaxf(most, __shfl_xor(most, 1, JL_WAVE));   // a block is four lanes' values
-        most = fmaxf(most, __shfl_xor(most, 2, JL_WAVE));
-        const _Float16 d16 = (_Float16)fminf(most / 127.f, 65504.f);
-        const float d = (float)d16;
-        uint32_t word[2] = {0, 0};
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            // (NaN: both comparisons fall to the other operand's side, so it is taken out first)
-            const float y = d > 0.f && a[i] == a[i] ? fminf(fmaxf(rintf(a[i] / d), -127.f), 127.f) : 0.f;
-            word[i / 4] |= (uint32_t)((int)y & 255) << (8 * (i % 4));
-        }
-        if (live) {
-            *(uint2 *)(part + token * p.head_dim + 8 * chunk) = make_uint2(word[0], word[1]);
-            if (chunk % 4 == 0) {
-                _Float16 *scales = (_Float16 *)(part + ((int64_t)p.head_dim << p.cache.page_shift));
-                scales[((chunk / 4) << p.cache.page_shift) + token] = d16;
+            if (in_head) {
+                *(uint2 *)(part + token * p.head_dim + 8 * chunk) = make_uint2(word[0], word[1]);
+                if (chunk % 4 == 0) {
+                    _Float16 *scales = (_Float16 *)(part + ((int64_t)p.head_dim << p.cache.page_shift));
+                    scales[((chunk / 4) << p.cache.page_shift) + token] = d16;
+                }
             }
         }
     }
@@ -443,14 +458,16 @@ int cache_make(const char *who, jl_context *ctx, void *memory, int kv_type, int6
     return JL_OK;
 }
 
-template <bool Q8>
+template <bool Q8, int LANES, bool HALVES>
+void launch_append_lanes(const AppendArgs &a, unsigned rows, hipStream_t stream) {
+    const int units = a.heads + 2 * a.cache.kv_heads, per = kAppendPer * (kAppendThreads / LANES);
+    hipLaunchKernelGGL((jl_kv_append_kernel<Q8, LANES, HALVES>), dim3(rows, (unsigned)((units + per - 1) / per)), dim3(kAppendThreads), 0, stream, a);
+}
+template <bool Q8, bool HALVES>
 void launch_append(const AppendArgs &a, unsigned rows, hipStream_t stream) {
-    const int lanes = a.head_dim <= 64 ? 8 : a.head_dim <= 128 ? 16 : 32;
-    const int units = a.heads + 2 * a.cache.kv_heads, per = kAppendThreads / lanes;
-    const dim3 grid(rows, (unsigned)((units + per - 1) / per)), block(kAppendThreads);
-    if (lanes == 8) hipLaunchKernelGGL((jl_kv_append_kernel<Q8, 8>), grid, block, 0, stream, a);
-    else if (lanes == 16) hipLaunchKernelGGL((jl_kv_append_kernel<Q8, 16>), grid, block, 0, stream, a);
-    else hipLaunchKernelGGL((jl_kv_append_kernel<Q8, 32>), grid, block, 0, stream, a);
+    if (a.head_dim <= 64) launch_append_lanes<Q8, 8, HALVES>(a, rows, stream);
+    else if (a.head_dim <= 128) launch_append_lanes<Q8, 16, HALVES>(a, rows, stream);
+    else launch_append_lanes<Q8, 32, HALVES>(a, rows, stream);
 }
 
 bool aligned(const void *p, int to) { return ((uintptr_t)p & (to - 1)) == 0; }
@@ -546,9 +563,11 @@ int jl_kv_append(jl_context *ctx, jl_kv_cache *cache, const float *q, int heads,
     a.ldq = ldq, a.ldk = ldk, a.ldv = ldv, a.ldq_out = ldq_out;
     a.positions = positions, a.slots = slots, a.frequencies = frequencies;
     a.q_norm = q_norm, a.k_norm = k_norm, a.eps = eps;
-    a.heads = q ? heads : 0, a.head_dim = dim, a.rotated = rotated, a.halves = rope_style == JL_ROPE_HALVES;
-    if (cache->type == JL_KV_Q8_0) launch_append<true>(a, (unsigned)rows, ctx->stream);
-    else launch_append<false>(a, (unsigned)rows, ctx->stream);
+    a.heads = q ? heads : 0, a.head_dim = dim, a.rotated = rotated;
+    const bool halves = rope_style == JL_ROPE_HALVES && rotated > 0;
+    const unsigned n = (unsigned)rows;
+    if (cache->type == JL_KV_Q8_0) halves ? launch_append<true, true>(a, n, ctx->stream) : launch_append<true, false>(a, n, ctx->stream);
+    else halves ? launch_append<false, true>(a, n, ctx->stream) : launch_append<false, false>(a, n, ctx->stream);
     JL_HIP(hipGetLastError());
     return JL_OK;
 }

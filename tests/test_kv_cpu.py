@@ -170,17 +170,18 @@ def test_cache_of_another_device(L, lib, memory, cache):
 
 def test_binding_checks_what_the_library_cannot():
     """Rows that leave their array, arrays too short for the rows, norms of another length."""
-    from jitllm_amd.attention import BlockTables, Rows
+    from jitllm_amd.attention import BlockTables, Rows, _place
 
     class Array:
         def __init__(self, size, itemsize=4):
             self.size, self.nbytes, self.ptr = size, size * itemsize, C.c_void_p(4096)
 
-    assert Rows(Array(100), 10, 4).ptr("x", 10, 6) == 4096 + 16
-    assert Rows(Array(100, 2), 10, 4).ptr("x", 10, 6) == 4096 + 8
+    assert _place("x", Rows(Array(100), 10, 4), 10, 6) == (4096 + 16, 10)
+    assert _place("x", Rows(Array(100, 2), 10, 4), 10, 6) == (4096 + 8, 10)
+    assert _place("x", Array(60), 10, 6) == (4096, 6) and _place("x", Rows(Array(0), 6), 0, 6) == (4096, 6)
     for rows, width, stride, offset in ((11, 6, 10, 4), (10, 7, 10, 4), (1, 11, 10, 0), (1, 4, 10, -1)):
         with pytest.raises(ValueError):
-            Rows(Array(100), stride, offset).ptr("x", rows, width)
+            _place("x", Rows(Array(100), stride, offset), rows, width)
     with pytest.raises(ValueError, match="no such arrays"):
         class Ctx:
             _lib = None
