@@ -103,6 +103,15 @@ __device__ __forceinline__ T load_at(const uint8_t *base, uint32_t offset) {
 __device__ __forceinline__ jl_half2v as_half2(uint32_t x) { return __builtin_bit_cast(jl_half2v, x); }
 __device__ __forceinline__ uint32_t as_u32(jl_half2v x) { return __builtin_bit_cast(uint32_t, x); }
 
+// Bytes 0 and 2 of a word, signed, as binary16.  A byte b of 0 ... 255 under 0x64 is the binary16 of 1024 + b, so with the
+// sign bit turned over (b = q + 128) a subtraction of 1152 leaves q, exactly.  One bit operation puts both in place; the
+// kernel over 8-bit blocks is bound by its vector instructions, and those that permute bytes take twice as long as bit
+// operations do (1.9 and 1.05 ns of a SIMD's time).
+__device__ __forceinline__ jl_half2v even_bytes(uint32_t x) {
+    const jl_half2v bias = {(_Float16)1152.f, (_Float16)1152.f};
+    return as_half2((x & 0x00ff00ffu) ^ 0x64806480u) - bias;
+}
+
 // A tile's k and v as they lie in memory.  Lane (g, m) = (lane / 16, lane % 16) has, of k, token m of each 16-token half,
 // and of v the tokens 4 g + i of each half at a few consecutive elements: head_dim is cut into pieces of 128, 64 and 32,
 // and m has 8, 4 or 2 values of a piece.
@@ -119,6 +128,7 @@ struct Raw<false, DIM> {
     uintx2 v2[kHalves][4];
     uint32_t v1[kHalves][4];
     __device__ static int element(int step, int g) { return 32 * step + 8 * g; }   // first of the eight of k step `step`
+    __device__ static constexpr int in_eight(int i) { return i; }                  // ... and their order
     __device__ void load_k(int half, const uint8_t *part, int in_page, int, int g, int m) {
 #pragma unroll
         for (int s = 0; s < kSteps; s++) k[half][s] = load_at<uintx4>(part, (in_page + m) * (2 * DIM) + 64 * s + 16 * g);
@@ -148,11 +158,10 @@ struct Raw<false, DIM> {
                 if constexpr (kThin) v1[h][i] = seen[h][i] ? v1[h][i] : 0;
             }
     }
-    // eight tokens (of both halves of 32) of the column that output block `block` takes of this lane
-    __device__ jl_half8 v_operand(int sub, int block) const {
-        uintx4 r;
+    // eight tokens (of both halves of 32) of the columns that output blocks `block` and `block` + 1 take of this lane
+    __device__ void v_operands(int sub, int block, jl_half8 (&v)[2]) const {
+        uintx4 r[2];
         const int word = block / 2;
-        const uint32_t pick = block % 2 ? 0x07060302u : 0x05040100u;
 #pragma unroll
         for (int pair = 0; pair < 4; pair++) {
             const int h = 2 * sub + pair / 2, i = pair % 2 * 2;
@@ -160,9 +169,9 @@ struct Raw<false, DIM> {
             if (word < 4 * kWide) a = v4[h][i][word / 4][word % 4], b = v4[h][i + 1][word / 4][word % 4];
             else if (word < 4 * kWide + 2 * kMid) a = v2[h][i][word % 2], b = v2[h][i + 1][word % 2];
             else a = v1[h][i], b = v1[h][i + 1];
-            r[pair] = __builtin_amdgcn_perm(b, a, pick);
+            r[0][pair] = __builtin_amdgcn_perm(b, a, 0x05040100u), r[1][pair] = __builtin_amdgcn_perm(b, a, 0x07060302u);
         }
-        return __builtin_bit_cast(jl_half8, r);
+        v[0] = __builtin_bit_cast(jl_half8, r[0]), v[1] = __builtin_bit_cast(jl_half8, r[1]);
     }
 };
 
@@ -183,6 +192,8 @@ struct Raw<true, DIM> {
     __device__ static int element(int step, int g) {
         return step < 2 * kPairs ? 64 * (step / 2) + 16 * g + 8 * (step % 2) : 64 * kPairs + 8 * g;
     }
+    // (0, 2), (1, 3), (4, 6), (5, 7): the pairs that one operation takes out of a word
+    __device__ static constexpr int in_eight(int i) { return i / 4 * 4 + i % 4 / 2 + i % 2 * 2; }
     __device__ void load_k(int half, const uint8_t *part, int in_page, int page_shift, int g, int m) {
         const uint32_t row = (in_page + m) * DIM, scales = ((uint32_t)DIM << page_shift) + 2 * (in_page + m);
 #pragma unroll
@@ -216,11 +227,8 @@ struct Raw<true, DIM> {
         if (step < 2 * kPairs) lo = k[half][step / 2][step % 2 * 2], hi = k[half][step / 2][step % 2 * 2 + 1], d = k_scale[half][step / 2];
         else lo = k_tail[half].x, hi = k_tail[half].y, d = k_scale[half][kPairs + kTail - 1];
         const jl_half2v dd = as_half2(d | d << 16);
-        jl_half2v a, b, c, e;
-        jl_bytes_to_half(lo, a, b);
-        jl_bytes_to_half(hi, c, e);
-        a *= dd, b *= dd, c *= dd, e *= dd;
-        return jl_half8{a.x, a.y, b.x, b.y, c.x, c.y, e.x, e.y};
+        return __builtin_bit_cast(jl_half8, uintx4{as_u32(even_bytes(lo) * dd), as_u32(even_bytes(lo >> 8) * dd),
+                                                   as_u32(even_bytes(hi) * dd), as_u32(even_bytes(hi >> 8) * dd)});
     }
     // (a byte times a scale of 0; the scale alone can be an infinity or NaN)
     __device__ void mask_v(const bool (&seen)[kHalves][4]) {
@@ -232,8 +240,9 @@ struct Raw<true, DIM> {
                 for (int c = 0; c < 2; c++)
                     v_scale[h][w][c] &= (seen[h][2 * c] ? 0xffffu : 0u) | (seen[h][2 * c + 1] ? 0xffff0000u : 0u);
     }
-    __device__ jl_half8 v_operand(int sub, int block) const {
-        uintx4 r;
+    // Operands of two neighbouring blocks: their columns' bytes of two tokens come into one word, and out of it as pairs.
+    __device__ void v_operands(int sub, int block, jl_half8 (&v)[2]) const {
+        uintx4 r[2];
         const int piece = block < 8 * kWide ? block / 8 : block < 8 * kWide + 4 * kMid ? kWide : kWide + kMid;
 #pragma unroll
         for (int pair = 0; pair < 4; pair++) {
@@ -242,13 +251,12 @@ struct Raw<true, DIM> {
             int byte;
             if (block < 8 * kWide) a = v2[h][i][block / 8][block % 8 / 4], b = v2[h][i + 1][block / 8][block % 8 / 4], byte = block % 4;
             else if (block < 8 * kWide + 4 * kMid) a = v1[h][i], b = v1[h][i + 1], byte = block % 4;
-            else a = v0[h][i], b = v0[h][i + 1], byte = block % 2;
-            // byte `byte` of both tokens under 0x64, as in jl_bytes_to_half
-            const uint32_t both = __builtin_amdgcn_perm(b, a, 0x0c040c00u + byte * 0x00010001u) ^ 0x64806480u;
-            const jl_half2v bias = {(_Float16)1152.f, (_Float16)1152.f};
-            r[pair] = as_u32((as_half2(both) - bias) * as_half2(v_scale[h][piece][i / 2]));
+            else a = v0[h][i], b = v0[h][i + 1], byte = 0;
+            const uint32_t both = __builtin_amdgcn_perm(b, a, byte == 0 ? 0x05040100u : 0x07060302u);
+            const jl_half2v d = as_half2(v_scale[h][piece][i / 2]);
+            r[0][pair] = as_u32(even_bytes(both) * d), r[1][pair] = as_u32(even_bytes(both >> 8) * d);
         }
-        return __builtin_bit_cast(jl_half8, r);
+        v[0] = __builtin_bit_cast(jl_half8, r[0]), v[1] = __builtin_bit_cast(jl_half8, r[1]);
     }
 };
 
@@ -518,7 +526,8 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
             for (int s = 0; s < kSteps; s++)
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    const float y = x[s][i / 4][i % 4] * to;
+                    const int e = Raw<Q8, DIM>::in_eight(i);
+                    const float y = x[s][e / 4][e % 4] * to;
                     q_hi[s][i] = (_Float16)y;
                     q_lo[s][i] = (_Float16)(y - (float)q_hi[s][i]);
                 }
@@ -536,22 +545,26 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
             loaded = more || (next.left > 0 && next_tile < next_last);
             const int load_tile = more ? t + kWaves : next_tile, load_head = more ? kv_head : kv_head_of(next.head);
             if (loaded) find_pages(more ? cur : next, load_tile);
+            // (the halves side by side: a product waits for the one before it of its own half only)
             floatx4 s[kHalves];
 #pragma unroll
-            for (int h = 0; h < kHalves; h++) {
-                s[h] = floatx4{0.f, 0.f, 0.f, 0.f};
+            for (int h = 0; h < kHalves; h++) s[h] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int i = 0; i < kSteps; i++) {
-                    const jl_half8 k = raw.k_operand(h, i);
-                    s[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q_lo[i], s[h], 0, 0, 0);
-                    s[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q_hi[i], s[h], 0, 0, 0);
+            for (int i = 0; i < kSteps; i++) {
+                jl_half8 k[kHalves];
+#pragma unroll
+                for (int h = 0; h < kHalves; h++) {
+                    k[h] = raw.k_operand(h, i);
+                    s[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[h], q_lo[i], s[h], 0, 0, 0);
                 }
+#pragma unroll
+                for (int h = 0; h < kHalves; h++) s[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[h], q_hi[i], s[h], 0, 0, 0);
             }
             if (loaded) issue(load_head, load_tile, false);   // k of the next tile goes out as soon as this one's is used
             const bool all_seen = t * kTile >= cur.first && t * kTile + kTile <= cur.end && here == (1u << kHalves) - 1;
             float x[4 * kHalves];
 #pragma unroll
-            for (int i = 0; i < 4 * kHalves; i++) x[i] = s[i / 4][i % 4] * undo;
+            for (int i = 0; i < 4 * kHalves; i++) x[i] = s[i / 4][i % 4];
             if (!all_seen) {
                 bool seen[kHalves][4];
 #pragma unroll
@@ -565,7 +578,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
             float most = x[0];
 #pragma unroll
             for (int i = 1; i < 4 * kHalves; i++) most = fmaxf(most, x[i]);
-            most = over_groups_max(most);
+            most = over_groups_max(most) * undo;
             // The maximum may fall behind by a factor of 2^8 before everything is brought to the new one: weights
             // stay far inside binary16, and after a row's first tiles this is rare.
             if (__any(most > top + 8.f)) {
@@ -581,7 +594,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
                 uintx4 hi, lo;
 #pragma unroll
                 for (int i = 0; i < 8; i += 2) {
-                    const float a = __builtin_amdgcn_exp2f(x[8 * sub + i] - top), b = __builtin_amdgcn_exp2f(x[8 * sub + i + 1] - top);
+                    const float a = __builtin_amdgcn_exp2f(fmaf(x[8 * sub + i], undo, -top)), b = __builtin_amdgcn_exp2f(fmaf(x[8 * sub + i + 1], undo, -top));
                     sum += a + b;
                     const auto two = __builtin_amdgcn_cvt_pkrtz(a, b);
                     hi[i / 2] = __builtin_bit_cast(uint32_t, two);
@@ -589,10 +602,13 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
                 }
                 const jl_half8 p_hi = __builtin_bit_cast(jl_half8, hi), p_lo = __builtin_bit_cast(jl_half8, lo);
 #pragma unroll
-                for (int b = 0; b < kBlocks; b++) {
-                    const jl_half8 v = raw.v_operand(sub, b);
-                    o[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p_lo, o[b], 0, 0, 0);
-                    o[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p_hi, o[b], 0, 0, 0);
+                for (int b = 0; b < kBlocks; b += 2) {
+                    jl_half8 v[2];
+                    raw.v_operands(sub, b, v);
+                    o[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[0], p_lo, o[b], 0, 0, 0);
+                    o[b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[1], p_lo, o[b + 1], 0, 0, 0);
+                    o[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[0], p_hi, o[b], 0, 0, 0);
+                    o[b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[1], p_hi, o[b + 1], 0, 0, 0);
                 }
             }
             if (loaded) issue(load_head, load_tile, true);
