@@ -11,6 +11,8 @@
 //                              TornadoTensor.java:17-101; TornadoVM's FloatArray / HalfFloatArray;
 //                              J/backend/tornado/workspace/TornadoWorkspace.java)
 //   GGUF                       J/format/GGUF.java:40-255, as far as a tensor's upload needs it
+//   PagedKvCache, BlockTables, PagedAttention, Rope
+//                              what lies between a layer's q|k|v and its output projection
 //
 // Where the reference adds a task to a TaskGraph these enqueue a kernel on the context's stream, so
 // the `graph` / `name` arguments of the reference disappear.  Error behaviour is the reference's: a
@@ -429,6 +431,169 @@ private:
 
     jl_context *ctx_;
     int batch_, math_;
+    DeviceBuffer workspace_;
+};
+
+// ---- key-value cache in pages, and the attention that reads it (jl_kv_*) -----------------------
+
+// int32 device array: positions, slots, block tables.
+class IntArray : public DeviceBuffer {
+public:
+    IntArray(const Context &context, std::size_t size) : DeviceBuffer(context, size * 4), size_(size) {}
+    IntArray(const Context &context, const std::vector<std::int32_t> &values) : IntArray(context, values.size()) { set(values); }
+    std::size_t size() const { return size_; }
+    std::int32_t *data() const { return static_cast<std::int32_t *>(ptr_); }
+    void set(const std::vector<std::int32_t> &values) const {
+        if (values.size() != size_) throw std::invalid_argument("values for an IntArray of another size");
+        if (size_) upload(values.data(), size_ * 4);
+    }
+    std::vector<std::int32_t> get() const {
+        std::vector<std::int32_t> out(size_);
+        if (size_) download(out.data(), size_ * 4);
+        return out;
+    }
+
+private:
+    std::size_t size_;
+};
+
+// Rows of a device array that lie `stride` elements apart, the first `offset` elements in: the q, k or v part of
+// the rows that a fused projection leaves side by side.
+template <typename T>
+struct Rows {
+    T *data;
+    std::size_t size;   // of the array
+    std::int64_t stride;
+    std::size_t offset;
+    Rows(const FloatArray &array, std::int64_t stride, std::size_t offset = 0)
+        : data(array.data()), size(array.size()), stride(stride), offset(offset) {}
+    Rows(const HalfFloatArray &array, std::int64_t stride, std::size_t offset = 0)
+        : data(array.data()), size(array.size()), stride(stride), offset(offset) {}
+    T *at(std::int64_t rows, std::int64_t width) const {
+        if (stride < width || (rows > 0 && offset + static_cast<std::size_t>((rows - 1) * stride + width) > size))
+            throw std::out_of_range("rows past the end of the device array");
+        return data + offset;
+    }
+};
+using FloatRows = Rows<float>;
+using HalfRows = Rows<std::uint16_t>;
+
+// A rotation: pair i of every head turns by position * frequencies[i] radians.
+class Rope {
+public:
+    Rope(const Context &context, const std::vector<double> &frequencies, jl_rope_style style = JL_ROPE_PAIRS)
+        : frequencies_(context, frequencies.size() * sizeof(double)), rotated_(2 * static_cast<int>(frequencies.size())), style_(style) {
+        frequencies_.upload(frequencies.data(), frequencies.size() * sizeof(double));
+    }
+    const double *frequencies() const { return static_cast<const double *>(frequencies_.ptr()); }
+    int rotated() const { return rotated_; }
+    jl_rope_style style() const { return style_; }
+
+private:
+    DeviceBuffer frequencies_;
+    int rotated_;
+    jl_rope_style style_;
+};
+
+// One layer's keys and values in pages (jl_kv_cache).
+class PagedKvCache {
+public:
+    PagedKvCache(const Context &context, jl_kv_type type, std::int64_t pages, int kvHeads, int headDim, int pageTokens)
+        : ctx_(context.handle()), kvHeads_(kvHeads), headDim_(headDim) {
+        check(jl_kv_cache_create(ctx_, type, pages, kvHeads, headDim, pageTokens, &handle_));
+    }
+    ~PagedKvCache() { jl_kv_cache_free(handle_); }
+    PagedKvCache(const PagedKvCache &) = delete;
+    PagedKvCache &operator=(const PagedKvCache &) = delete;
+    jl_kv_cache *handle() const { return handle_; }
+    int kvHeads() const { return kvHeads_; }
+    int headDim() const { return headDim_; }
+    // Turns q in place (or into qOut) and writes k and v to `slots`; q null: only k and v.
+    void append(const FloatRows &k, const FloatRows &v, const IntArray &positions, const IntArray &slots, std::int64_t rows,
+                const Rope *rope = nullptr, const FloatRows *q = nullptr, int heads = 0, const FloatRows *qOut = nullptr,
+                const FloatArray *qNorm = nullptr, const FloatArray *kNorm = nullptr, float eps = 0.f) const {
+        const std::int64_t width = static_cast<std::int64_t>(kvHeads_) * headDim_, qWidth = static_cast<std::int64_t>(heads) * headDim_;
+        if (!qOut) qOut = q;
+        need(positions.size(), rows), need(slots.size(), rows);
+        if (qNorm) need(qNorm->size(), headDim_);
+        if (kNorm) need(kNorm->size(), headDim_);
+        check(jl_kv_append(ctx_, handle_, q ? q->at(rows, qWidth) : nullptr, heads, q ? q->stride : 0, k.at(rows, width), k.stride,
+                           v.at(rows, width), v.stride, q ? qOut->at(rows, qWidth) : nullptr, q ? qOut->stride : 0, positions.data(),
+                           slots.data(), rows, rope ? rope->frequencies() : nullptr, rope ? rope->rotated() : 0,
+                           rope ? rope->style() : JL_ROPE_PAIRS, qNorm ? qNorm->data() : nullptr, kNorm ? kNorm->data() : nullptr, eps));
+    }
+    void read(const IntArray &slots, std::int64_t rows, const FloatArray &k, const FloatArray &v) const {
+        need(slots.size(), rows), need(k.size(), rows * kvHeads_ * headDim_), need(v.size(), rows * kvHeads_ * headDim_);
+        check(jl_kv_read(ctx_, handle_, slots.data(), rows, k.data(), v.data(), 0));
+    }
+
+private:
+    static void need(std::size_t size, std::int64_t count) {
+        if (count > 0 && size < static_cast<std::size_t>(count)) throw std::out_of_range("a device array shorter than its rows");
+    }
+    jl_context *ctx_;
+    jl_kv_cache *handle_ = nullptr;
+    int kvHeads_, headDim_;
+};
+
+// The pages of a batch's requests and the rows of a step (jl_kv_plan): no tokens and every page free at first.
+class BlockTables {
+public:
+    BlockTables(const Context &context, int requests, int blocksPerRequest, int pages, int pageTokens, int maxRows)
+        : table(context, static_cast<std::size_t>(requests) * blocksPerRequest), lengths(context, requests), rowStarts(context, requests + 1),
+          slots(context, maxRows), positions(context, maxRows), rowRequests(context, maxRows), pageRing(context, pages), freePages(context, 2),
+          ctx_(context.handle()), requests_(requests), blocks_(blocksPerRequest), pages_(pages), pageTokens_(pageTokens), maxRows_(maxRows) {
+        std::vector<std::int32_t> ring(pages);
+        for (int i = 0; i < pages; i++) ring[i] = i;
+        pageRing.set(ring);
+        freePages.set({0, pages});
+        table.set(std::vector<std::int32_t>(table.size(), -1));
+        lengths.set(std::vector<std::int32_t>(requests, 0));
+    }
+    // One step: new tokens of each request, negative where it has ended; lengths and free pages move on.
+    void plan(const IntArray &fresh) const {
+        if (fresh.size() < static_cast<std::size_t>(requests_)) throw std::out_of_range("fresh shorter than the requests");
+        check(jl_kv_plan(ctx_, lengths.data(), fresh.data(), requests_, pages_, pageTokens_, pageRing.data(), freePages.data(),
+                         freePages.data(), table.data(), blocks_, lengths.data(), rowStarts.data(), slots.data(), positions.data(),
+                         rowRequests.data(), maxRows_));
+    }
+    int requests() const { return requests_; }
+    int blocksPerRequest() const { return blocks_; }
+    const IntArray table, lengths, rowStarts, slots, positions, rowRequests, pageRing, freePages;
+
+private:
+    jl_context *ctx_;
+    int requests_, blocks_, pages_, pageTokens_, maxRows_;
+};
+
+// Attention of one new token a row over paged caches of one shape, with the workspace it joins in.
+class PagedAttention {
+public:
+    PagedAttention(const Context &context, int heads, int kvHeads, int headDim)
+        : ctx_(context.handle()), heads_(heads), kvHeads_(kvHeads), headDim_(headDim),
+          workspace_(context, jl_kv_attention_workspace_bytes(heads, kvHeads, headDim)) {
+        check(jl_kv_attention_workspace_init(ctx_, workspace_.ptr(), workspace_.bytes()));
+    }
+    void attend(const PagedKvCache &cache, const FloatRows &q, std::int64_t rows, const BlockTables &tables, const FloatRows &out,
+                float scale, std::int64_t window = 0) const {
+        run(cache, q, rows, tables, out.at(rows, static_cast<std::int64_t>(heads_) * headDim_), 0, out.stride, scale, window);
+    }
+    void attend(const PagedKvCache &cache, const FloatRows &q, std::int64_t rows, const BlockTables &tables, const HalfRows &out,
+                float scale, std::int64_t window = 0) const {
+        run(cache, q, rows, tables, out.at(rows, static_cast<std::int64_t>(heads_) * headDim_), 1, out.stride, scale, window);
+    }
+
+private:
+    void run(const PagedKvCache &cache, const FloatRows &q, std::int64_t rows, const BlockTables &tables, void *out, int half,
+             std::int64_t ldo, float scale, std::int64_t window) const {
+        if (cache.kvHeads() != kvHeads_ || cache.headDim() != headDim_) throw std::invalid_argument("a cache of another shape");
+        if (rows > 0 && tables.positions.size() < static_cast<std::size_t>(rows)) throw std::out_of_range("more rows than the step's");
+        check(jl_kv_attention(ctx_, cache.handle(), q.at(rows, static_cast<std::int64_t>(heads_) * headDim_), heads_, q.stride, rows,
+                              tables.positions.data(), tables.rowRequests.data(), tables.table.data(), tables.requests(),
+                              tables.blocksPerRequest(), scale, window, out, half, ldo, workspace_.ptr(), workspace_.bytes()));
+    }
+    jl_context *ctx_;
+    int heads_, kvHeads_, headDim_;
     DeviceBuffer workspace_;
 };
 

@@ -28,16 +28,18 @@
 namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / JL_WAVE;
-constexpr int kMostGroups = 1024;         // workgroups of a launch, and spans
+constexpr int kMostGroups = 512;          // workgroups of a launch, and spans: two on each of 256 compute units
 constexpr int kStart = 4;                 // what beginning a (row, head) pair takes, in tiles
-constexpr uint32_t kMostParts = 32;       // of a head
+// Parts of a head: 32 at most, up to 64 of 64 tiles and more (8 heads of 4000 tokens: 13.4 and 15.5 us; of 131072: 95.2
+// and 93.4).
+constexpr uint32_t kParts = 32, kMostParts = 64, kLargePart = 64;
 constexpr int kDeviceScope = 16;          // a buffer load's policy: sc1
 constexpr float kNone = -3.0e38f;         // the running maximum of nothing: finite, so that differences are numbers
 
+constexpr int kHalves = 2, kTile = 16 * kHalves;   // a wave's tile: tokens, in halves of 16
+
 template <bool Q8, int DIM>
 struct Shape {
-    // 16-token halves of a wave's tile: 64 tokens of 8-bit blocks are the registers, and the bytes in flight, of 32 of binary16
-    static constexpr int kHalves = Q8 && DIM <= 128 ? 4 : 2, kTile = 16 * kHalves;
     static constexpr int kPerUnit = DIM == 256 ? 1 : 2;   // workgroups that a compute unit holds at a time
     // Tiles that the whole chip reads (6 TB/s) in the time that a workgroup alone takes for one (half a microsecond).
     static constexpr int kTileBytes = Q8 ? 2 * kTile * (DIM + DIM / 16) : 2 * kTile * DIM * 2;
@@ -70,8 +72,7 @@ struct AttentionArgs {
 // The tokens [first, end) of its request that a row sees.
 struct Range {
     int first, end, request;
-    template <int TILE>
-    __device__ int tiles() const { return end > first ? (end + TILE - 1) / TILE - first / TILE : 0; }
+    __device__ int tiles() const { return end > first ? (end + kTile - 1) / kTile - first / kTile : 0; }
 };
 __device__ __forceinline__ Range range_of(const AttentionArgs &p, int row) {
     const int position = p.positions[row];
@@ -120,7 +121,6 @@ struct Raw;
 
 template <int DIM>
 struct Raw<false, DIM> {
-    static constexpr int kHalves = Shape<false, DIM>::kHalves;
     static constexpr int kSteps = DIM / 32;
     static constexpr int kWide = DIM / 128, kMid = DIM % 128 / 64, kThin = DIM % 64 / 32;
     uintx4 k[kHalves][kSteps];
@@ -158,13 +158,13 @@ struct Raw<false, DIM> {
                 if constexpr (kThin) v1[h][i] = seen[h][i] ? v1[h][i] : 0;
             }
     }
-    // eight tokens (of both halves of 32) of the columns that output blocks `block` and `block` + 1 take of this lane
-    __device__ void v_operands(int sub, int block, jl_half8 (&v)[2]) const {
+    // eight tokens of the columns that output blocks `block` and `block` + 1 take of this lane
+    __device__ void v_operands(int block, jl_half8 (&v)[2]) const {
         uintx4 r[2];
         const int word = block / 2;
 #pragma unroll
         for (int pair = 0; pair < 4; pair++) {
-            const int h = 2 * sub + pair / 2, i = pair % 2 * 2;
+            const int h = pair / 2, i = pair % 2 * 2;
             uint32_t a, b;
             if (word < 4 * kWide) a = v4[h][i][word / 4][word % 4], b = v4[h][i + 1][word / 4][word % 4];
             else if (word < 4 * kWide + 2 * kMid) a = v2[h][i][word % 2], b = v2[h][i + 1][word % 2];
@@ -177,7 +177,6 @@ struct Raw<false, DIM> {
 
 template <int DIM>
 struct Raw<true, DIM> {
-    static constexpr int kHalves = Shape<true, DIM>::kHalves;
     static constexpr int kSteps = DIM / 32, kPairs = DIM / 64, kTail = DIM % 64 / 32;
     static constexpr int kWide = DIM / 128, kMid = DIM % 128 / 64, kThin = DIM % 64 / 32;
     static constexpr int kPieces = kWide + kMid + kThin;
@@ -241,12 +240,12 @@ struct Raw<true, DIM> {
                     v_scale[h][w][c] &= (seen[h][2 * c] ? 0xffffu : 0u) | (seen[h][2 * c + 1] ? 0xffff0000u : 0u);
     }
     // Operands of two neighbouring blocks: their columns' bytes of two tokens come into one word, and out of it as pairs.
-    __device__ void v_operands(int sub, int block, jl_half8 (&v)[2]) const {
+    __device__ void v_operands(int block, jl_half8 (&v)[2]) const {
         uintx4 r[2];
         const int piece = block < 8 * kWide ? block / 8 : block < 8 * kWide + 4 * kMid ? kWide : kWide + kMid;
 #pragma unroll
         for (int pair = 0; pair < 4; pair++) {
-            const int h = 2 * sub + pair / 2, i = pair % 2 * 2;
+            const int h = pair / 2, i = pair % 2 * 2;
             uint32_t a, b;
             int byte;
             if (block < 8 * kWide) a = v2[h][i][block / 8][block % 8 / 4], b = v2[h][i + 1][block / 8][block % 8 / 4], byte = block % 4;
@@ -306,7 +305,6 @@ struct Cut {
 template <bool Q8, int DIM>
 __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_attention_kernel(AttentionArgs p) {
     constexpr int kSteps = DIM / 32, kBlocks = DIM / 16;
-    constexpr int kHalves = Shape<Q8, DIM>::kHalves, kTile = Shape<Q8, DIM>::kTile, kSubs = kHalves / 2;
     constexpr int kRound = DIM == 256 ? 128 : DIM;            // elements that are joined at a time: 64 KB of LDS at most
     constexpr int kStride = kRound + 4;                       // (four floats on: rows start on other banks)
     constexpr int kSlot = 16 * (DIM + 2);
@@ -330,14 +328,14 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
     // ---- this workgroup's share of the list: whole (row, head) pairs one after the other where all rows are short, else
     // an equal span of tiles.  (All tiles together are fewer than 2^32: jl_kv_attention.)
     load_window(0);
-    const uint32_t mine = units_of(in_lane.tiles<kTile>());
+    const uint32_t mine = units_of(in_lane.tiles());
     uint32_t all, through = mine;                             // tiles of all rows; of those up to this lane's (this thread's last)
     uint32_t longest = mine, own = mine;
     const int per = (p.rows + kThreads - 1) / kThreads;       // rows a thread, where a wave does not hold them all
     if (p.rows > JL_WAVE) {
         own = longest = 0;
         for (int r = tid * per; r < min((tid + 1) * per, p.rows); r++) {
-            const uint32_t n = units_of(range_of(p, r).tiles<kTile>());
+            const uint32_t n = units_of(range_of(p, r).tiles());
             own += n;
             longest = max(longest, n);
         }
@@ -365,17 +363,18 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
     // Pairs are not cut where a workgroup is done with its whole ones in the time that all take to read anyway, or in what
     // joining parts takes besides, ten tiles' worth.  (32 rows of 8 heads, 1000 tokens each: 27.8 us whole, 31.6 cut; 8 heads
     // of 1000 tokens: 20.2 whole, 10.2 cut; of 256 tokens: 9.1 and 9.7.)
-    const uint32_t most_units = longest * ((p.rows * heads + gridDim.x - 1) / gridDim.x);
-    const bool whole = (float)((int)most_units - kStart - 10) * Shape<Q8, DIM>::kTilesAtOnce <= (float)all * heads;
+    const float rounds = ceilf((float)p.rows * heads / gridDim.x);
+    const bool whole = ((float)longest * rounds - kStart - 10) * Shape<Q8, DIM>::kTilesAtOnce <= (float)all * heads;
     const uint32_t total = all * heads;
-    const uint32_t span = max((total + gridDim.x - 1) / gridDim.x, (longest + kMostParts - 1) / kMostParts);
+    const uint32_t least = max((longest + kMostParts - 1) / kMostParts, min((longest + kParts - 1) / kParts, kLargePart));
+    const uint32_t span = max((total + gridDim.x - 1) / gridDim.x, least);
     const uint32_t begin = whole ? 0 : span * blockIdx.x;
     if (p.rows > JL_WAVE) {
         const uint32_t from = begin / heads;
         if (!whole && begin < total && from >= through - own && from < through) {
             uint32_t before = through - own;
             int r = tid * per;
-            for (uint32_t n; before + (n = units_of(range_of(p, r).tiles<kTile>())) <= from; r++) before += n;
+            for (uint32_t n; before + (n = units_of(range_of(p, r).tiles())) <= from; r++) before += n;
             start_row = r, start_units = before;
         }
         __syncthreads();
@@ -384,7 +383,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
     // rows with nothing to read
     const int width = p.cache.kv_heads * p.group * DIM;
     for (int r = blockIdx.x; r < p.rows; r += gridDim.x) {
-        const int n = p.rows <= JL_WAVE ? __builtin_amdgcn_readlane(in_lane.tiles<kTile>(), r) : range_of(p, r).tiles<kTile>();
+        const int n = p.rows <= JL_WAVE ? __builtin_amdgcn_readlane(in_lane.tiles(), r) : range_of(p, r).tiles();
         if (n == 0)
             for (int c = 4 * tid; c < width; c += 4 * kThreads) store_out(p, r * p.ldo + c, floatx4{0.f, 0.f, 0.f, 0.f});
     }
@@ -421,7 +420,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
             next.first = __builtin_amdgcn_readlane(in_lane.first, at);
             next.end = __builtin_amdgcn_readlane(in_lane.end, at);
             next.request = __builtin_amdgcn_readlane(in_lane.request, at);
-            next.tiles = Range{next.first, next.end, 0}.tiles<kTile>();
+            next.tiles = Range{next.first, next.end, 0}.tiles();
             if (next.tiles > 0) break;
             if (whole) {
                 next.row += row_step, next.head += head_step;
@@ -444,8 +443,8 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
     // k and v of a tile go from memory to `raw`; `page` are the pages of its halves, and one behind the last token, or one
     // outside the cache, is -1
     Raw<Q8, DIM> raw;
-    bool loaded = false;
-    uint32_t paged = 0;           // bit h: half h of the tile in `raw` has a page of the cache
+    bool loaded = false;          // it has, or waits for, the wave's first tile of the coming piece
+    uint32_t paged = 0;           // bit h: half h of its tile has a page of the cache
     int page[kHalves];
     auto find_pages = [&](const Piece &c, int t) {
         // (scalar loads: vector loads come back in order, and these would wait for the tile that is under way)
@@ -475,6 +474,10 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
     const bool one_block = p.blocks_of_16 == 1;
     auto kv_head_of = [&](int head) { return one_block ? head : head / p.blocks_of_16; };
 
+    // Of two workgroups on a compute unit the one that came first has the right of way, and is done with an equal span in
+    // three quarters of the time (65 and 87 us); the other one then has the unit to itself and cannot fill it.  The later
+    // half of the launch goes first in three of four tiles: 97.4 -> 94.6 us over 64 ragged rows, 68.9 -> 65.9 over 8-bit blocks.
+    const bool second = 2 * blockIdx.x >= gridDim.x;
     Cut went_on, opened;
     went_on.parts = opened.parts = 0;
     for (complete(); next.left > 0;) {
@@ -492,12 +495,15 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
         // (a row's tiles begin with the one of its first token)
         const int list_tile = cur.first / kTile + cur.tile, last = list_tile + count, from_tile = list_tile + wave;
         const int next_list = next.left > 0 ? next.first / kTile + next.tile : 0, next_last = next_list + next.count, next_tile = next_list + wave;
-        if (!loaded && from_tile < last) {
-            find_pages(cur, from_tile);
-            issue(kv_head, from_tile, false);
-            issue(kv_head, from_tile, true);
+        const int next_head = next.left > 0 ? kv_head_of(next.head) : 0;
+        // a first tile that is not on its way yet; a wave that this piece has none for goes on to the next one's at once
+        const bool here = from_tile < last, there = !here && next.left > 0 && next_tile < next_last;
+        if (here ? !loaded : there) {
+            find_pages(here ? cur : next, here ? from_tile : next_tile);
+            issue(here ? kv_head : next_head, here ? from_tile : next_tile, false);
+            issue(here ? kv_head : next_head, here ? from_tile : next_tile, true);
         }
-        loaded = false;
+        loaded = there;
         const int q_head = kv_head * p.group + 16 * block_of_16, q_heads = min(p.group - 16 * block_of_16, 16);
 
         // ---- q, times a power of two that brings its largest value to 2^10 ... 2^11: both parts are then binary16
@@ -539,11 +545,15 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
         float top = kNone, sum = 0.f;
 
         for (int t = from_tile; t < last; t += kWaves) {
-            const uint32_t here = paged;
+            if (second) {
+                if (t / kWaves % 4 != 0) __builtin_amdgcn_s_setprio(1);
+                else __builtin_amdgcn_s_setprio(0);
+            }
+            const uint32_t with_page = paged;
             // what is loaded next: this piece's next tile of the wave, or the next piece's first
             const bool more = t + kWaves < last;
             loaded = more || (next.left > 0 && next_tile < next_last);
-            const int load_tile = more ? t + kWaves : next_tile, load_head = more ? kv_head : kv_head_of(next.head);
+            const int load_tile = more ? t + kWaves : next_tile, load_head = more ? kv_head : next_head;
             if (loaded) find_pages(more ? cur : next, load_tile);
             // (the halves side by side: a product waits for the one before it of its own half only)
             floatx4 s[kHalves];
@@ -560,24 +570,24 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
 #pragma unroll
                 for (int h = 0; h < kHalves; h++) s[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[h], q_hi[i], s[h], 0, 0, 0);
             }
-            if (loaded) issue(load_head, load_tile, false);   // k of the next tile goes out as soon as this one's is used
-            const bool all_seen = t * kTile >= cur.first && t * kTile + kTile <= cur.end && here == (1u << kHalves) - 1;
-            float x[4 * kHalves];
+            if (loaded) issue(load_head, load_tile, false);   // k goes out as soon as this tile's is used
+            const bool all_seen = t * kTile >= cur.first && t * kTile + kTile <= cur.end && with_page == (1u << kHalves) - 1;
+            float x[8];
 #pragma unroll
-            for (int i = 0; i < 4 * kHalves; i++) x[i] = s[i / 4][i % 4];
+            for (int i = 0; i < 8; i++) x[i] = s[i / 4][i % 4];
             if (!all_seen) {
                 bool seen[kHalves][4];
 #pragma unroll
-                for (int i = 0; i < 4 * kHalves; i++) {
+                for (int i = 0; i < 8; i++) {
                     const int token = t * kTile + 16 * (i / 4) + 4 * g + i % 4;
-                    seen[i / 4][i % 4] = token >= cur.first && token < cur.end && (here >> (i / 4) & 1);
+                    seen[i / 4][i % 4] = token >= cur.first && token < cur.end && (with_page >> (i / 4) & 1);
                     x[i] = seen[i / 4][i % 4] ? x[i] : -INFINITY;
                 }
                 raw.mask_v(seen);
             }
             float most = x[0];
 #pragma unroll
-            for (int i = 1; i < 4 * kHalves; i++) most = fmaxf(most, x[i]);
+            for (int i = 1; i < 8; i++) most = fmaxf(most, x[i]);
             most = over_groups_max(most) * undo;
             // The maximum may fall behind by a factor of 2^8 before everything is brought to the new one: weights
             // stay far inside binary16, and after a row's first tiles this is rare.
@@ -589,27 +599,24 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
 #pragma unroll
                 for (int b = 0; b < kBlocks; b++) o[b] *= keep;
             }
+            uintx4 hi, lo;
 #pragma unroll
-            for (int sub = 0; sub < kSubs; sub++) {
-                uintx4 hi, lo;
+            for (int i = 0; i < 8; i += 2) {
+                const float a = __builtin_amdgcn_exp2f(fmaf(x[i], undo, -top)), b = __builtin_amdgcn_exp2f(fmaf(x[i + 1], undo, -top));
+                sum += a + b;
+                const auto two = __builtin_amdgcn_cvt_pkrtz(a, b);
+                hi[i / 2] = __builtin_bit_cast(uint32_t, two);
+                lo[i / 2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a - (float)two[0], b - (float)two[1]));
+            }
+            const jl_half8 p_hi = __builtin_bit_cast(jl_half8, hi), p_lo = __builtin_bit_cast(jl_half8, lo);
 #pragma unroll
-                for (int i = 0; i < 8; i += 2) {
-                    const float a = __builtin_amdgcn_exp2f(fmaf(x[8 * sub + i], undo, -top)), b = __builtin_amdgcn_exp2f(fmaf(x[8 * sub + i + 1], undo, -top));
-                    sum += a + b;
-                    const auto two = __builtin_amdgcn_cvt_pkrtz(a, b);
-                    hi[i / 2] = __builtin_bit_cast(uint32_t, two);
-                    lo[i / 2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a - (float)two[0], b - (float)two[1]));
-                }
-                const jl_half8 p_hi = __builtin_bit_cast(jl_half8, hi), p_lo = __builtin_bit_cast(jl_half8, lo);
-#pragma unroll
-                for (int b = 0; b < kBlocks; b += 2) {
-                    jl_half8 v[2];
-                    raw.v_operands(sub, b, v);
-                    o[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[0], p_lo, o[b], 0, 0, 0);
-                    o[b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[1], p_lo, o[b + 1], 0, 0, 0);
-                    o[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[0], p_hi, o[b], 0, 0, 0);
-                    o[b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[1], p_hi, o[b + 1], 0, 0, 0);
-                }
+            for (int b = 0; b < kBlocks; b += 2) {
+                jl_half8 v[2];
+                raw.v_operands(b, v);
+                o[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[0], p_lo, o[b], 0, 0, 0);
+                o[b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[1], p_lo, o[b + 1], 0, 0, 0);
+                o[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[0], p_hi, o[b], 0, 0, 0);
+                o[b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[1], p_hi, o[b + 1], 0, 0, 0);
             }
             if (loaded) issue(load_head, load_tile, true);
         }

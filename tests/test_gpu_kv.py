@@ -651,3 +651,145 @@ def test_decode_steps_through_a_layer(ctx, q8, half):
                 assert np.abs(got[row] - want).max() <= (0.15 if q8 else 0.03) * size.max(), (step, r, row)
                 row += 1
     assert tables.lengths.get().tolist() == [25, 16, 37, 31]   # 20 + 5, 16, 33 + 4, 29 + 2
+
+
+# ---- graphs, streams, contexts -------------------------------------------------------------------
+
+@pytest.mark.parametrize("q8", [False, True])
+def test_a_captured_step_replayed_while_lengths_grow(ctx, q8):
+    """plan, append and attend recorded once; every replay after the program's own eager work (inputs uploaded, another
+    call through the same workspace, a wait), held to the same step made eagerly over a copy of the state."""
+    import bench
+    from jitllm_amd.attention import BlockTables, KvType, PagedAttention, PagedKvCache, Rope, Rows
+    hip = bench.Hip()
+    rng = np.random.default_rng(31)
+    requests, stride, page, pages, max_rows, heads, kv, dim = 5, 80, 16, 260, 8, 8, 2, 64
+    w = (heads + 2 * kv) * dim
+    rope = Rope.of_base(ctx, dim, 1e4)
+    attention = PagedAttention(ctx, max_rows, heads, kv, dim)
+
+    class Side:
+        def __init__(self):
+            self.tables = BlockTables(ctx, requests, stride, pages, page, max_rows)
+            self.cache = PagedKvCache(ctx, KvType.Q8_0 if q8 else KvType.F16, pages, kv, dim, page)
+            self.fresh, self.qkv = ints(ctx, np.zeros(requests)), ctx.float_array(max_rows * w, fill=0.0)
+            self.out = ctx.float_array(max_rows * heads * dim, fill=7.0)
+
+        def step(self):
+            t = self.tables
+            t.plan(self.fresh)
+            self.cache.append(Rows(self.qkv, w, heads * dim), Rows(self.qkv, w, (heads + kv) * dim), t.positions, t.slots, max_rows, rope=rope,
+                              q=Rows(self.qkv, w), heads=heads)
+            attention.attend(self.cache, Rows(self.qkv, w), max_rows, t.positions, t.table, self.out, requests=requests, rowRequests=t.rowRequests)
+
+    a, b = Side(), Side()
+    lengths = np.array([1100, 3, 0, 700, 16])                  # long enough to be cut, short, none, a page's end
+    order = rng.permutation(pages)
+    need = -(-lengths // page)
+    table = np.full((requests, stride), -1)
+    table[np.arange(stride) < need[:, None]] = order[:need.sum()]
+    raw = random_pool(rng, q8, pages, kv, dim, page)
+    raw_at = ctx.raw_buffer(raw.nbytes)
+    raw_at.upload(raw)
+    for side in (a, b):
+        side.tables.table.set(table), side.tables.lengths.set(lengths)
+        ring = np.full(pages, -1)
+        ring[:pages - need.sum()] = order[need.sum():]
+        side.tables.pageRing.set(ring), side.tables.freePages.set([0, pages - need.sum()])
+        from jitllm_amd import _lib as L
+        host = raw.copy()
+        L.check(ctx._lib.jl_upload(ctx.handle, ctx._lib.jl_kv_cache_memory(side.cache.handle), host.ctypes.data, host.nbytes))
+    say("captured step", q8)
+    a.fresh.set([0] * requests)
+    a.step()                                                   # warmed up: nothing new
+    ctx.sync()
+    exe = hip.capture(ctx.stream, a.step)
+    other = PagedKvCache(ctx, KvType.F16, 40, kv, dim, page, memory=raw_at if not q8 else None)
+    try:
+        for n, fresh in enumerate([[1, 1, 0, 1, 1], [1, 1, 2, 1, 1], [1, -1, 1, 1, 0], [1, 0, 1, 1, 5], [1, 3, 1, -1, 1], [1, 1, 1, 0, 1]]):
+            x = rng.standard_normal((max_rows, w)).astype(np.float32)
+            for side in (a, b):
+                side.fresh.set(fresh), side.qkv.set(x), side.out.init(7.0)
+            b.step()
+            q = ctx.float_array(heads * dim, fill=0.5)
+            attention.attend(other, q, 1, ints(ctx, [600]), ints(ctx, np.arange(40)), ctx.float_array(heads * dim), requests=1)
+            ctx.sync()
+            hip.launch(exe, ctx.stream)
+            ctx.sync()
+            assert np.array_equal(a.out.get().view(np.uint32), b.out.get().view(np.uint32)), n
+            for name in NAMES:
+                assert np.array_equal(getattr(a.tables, name).get(), getattr(b.tables, name).get()), (n, name)
+            rows = sum(max(f, 0) for f in fresh)
+            assert (a.out.get().reshape(max_rows, -1)[rows:] == 0).all()       # padding: nothing to read
+    finally:
+        hip.destroy_graph(exe)
+
+
+def test_two_contexts_at_once(ctx):
+    """Two streams, a workspace each, calls in flight side by side: each is what it is alone."""
+    from jitllm_amd.attention import KvType, PagedAttention, PagedKvCache
+    from jitllm_amd.runtime import Context
+    rng = np.random.default_rng(41)
+    lengths = np.array([6000, 5, 900, 2500])
+    table, pages = make_tables(rng, lengths, 16)
+    raw = random_pool(rng, False, pages, 4, 128, 16)
+    q = [rng.standard_normal((4, 16, 128)).astype(np.float32) for _ in range(2)]
+    say("two contexts")
+    with Context(0) as second:
+        sides = []
+        for c, x in ((ctx, q[0]), (second, q[1])):
+            memory = c.raw_buffer(raw.nbytes)
+            memory.upload(raw)
+            sides.append((c, PagedKvCache(c, KvType.F16, pages, 4, 128, 16, memory=memory), PagedAttention(c, 4, 16, 4, 128), c.from_numpy(x),
+                          c.float_array(4 * 16 * 128), ints(c, lengths - 1), ints(c, table)))
+        alone = []
+        for c, cache, attention, x, out, positions, t in sides:
+            attention.attend(cache, x, 4, positions, t, out, requests=4)
+            c.sync()
+            alone.append(out.get())
+        for _ in range(20):
+            for c, cache, attention, x, out, positions, t in sides:
+                for _ in range(3):
+                    attention.attend(cache, x, 4, positions, t, out, requests=4)
+            for side, want in zip(sides, alone):
+                side[0].sync()
+                assert np.array_equal(side[4].get(), want)
+        for side in sides:
+            side[1].free()
+        del sides, cache, attention, x, out, positions, t, memory
+    want = M.attend(M.decode_pool(raw, False, pages, 4, 128, 16), q[0], lengths - 1, None, table, 128 ** -0.5)
+    check_attend(alone[0].astype(np.float64).reshape(4, 16, 128), *want, lengths, 128)
+
+
+def test_one_workspace_for_calls_of_several_shapes(ctx):
+    """Layers of different heads share the workspace of the widest; what one call leaves in it is the next one's zero."""
+    from jitllm_amd.attention import PagedAttention
+    rng = np.random.default_rng(43)
+    wide = PagedAttention(ctx, 8, 64, 2, 256)
+    for lengths, heads, kv, dim, q8 in (([3000, 40], 64, 2, 256, False), ([2000], 8, 1, 64, False), ([5, 900, 1800], 12, 4, 128, True), ([4000], 6, 6, 96, False)) * 2:
+        table, pages = make_tables(rng, lengths, 32)
+        raw = random_pool(rng, q8, pages, kv, dim, 32)
+        cache = cache_of(ctx, q8, pages, kv, dim, 32, raw)
+        attention = PagedAttention(ctx, 8, heads, kv, dim)
+        assert attention.workspace.nbytes <= wide.workspace.nbytes
+        attention.workspace = wide.workspace
+        q = rng.standard_normal((len(lengths), heads, dim)).astype(np.float32)
+        say("shared workspace", lengths, heads, kv, dim, q8)
+        got = run_attend(ctx, cache, q, np.array(lengths) - 1, None, table, attention=attention)
+        want = M.attend(M.decode_pool(raw, q8, pages, kv, dim, 32), q, np.array(lengths) - 1, None, table, dim ** -0.5)
+        check_attend(got, *want, lengths, dim)
+
+
+def test_attend_thousands_of_short_rows(ctx):
+    rng = np.random.default_rng(44)
+    rows, page, dim = 5000, 16, 64
+    lengths = rng.integers(0, 4, rows)
+    lengths[4321] = 200
+    table, pages = make_tables(rng, lengths, page)
+    raw = random_pool(rng, False, pages, 1, dim, page)
+    cache = cache_of(ctx, False, pages, 1, dim, page, raw)
+    q = rng.standard_normal((rows, 2, dim)).astype(np.float32)
+    say("attend thousands of rows")
+    got = run_attend(ctx, cache, q, lengths - 1, None, table)
+    want = M.attend(M.decode_pool(raw, False, pages, 1, dim, page), q, lengths - 1, None, table, dim ** -0.5)
+    check_attend(got, *want, lengths, dim)

@@ -159,6 +159,18 @@ def test_attention_workspace(L, lib, ctx, memory, cache):
     assert lib.jl_kv_attention(ctx, cache, *[memory if v == "m" else v for v in args.values()]) == L.JL_OK   # no rows: nothing to do
 
 
+def test_attention_workspace_init_refusals(L, lib, ctx, memory):
+    assert lib.jl_kv_attention_workspace_init(None, memory, 1 << 20) == L.JL_ERR_INVALID
+    assert lib.jl_kv_attention_workspace_init(ctx, None, 1 << 20) == L.JL_ERR_INVALID
+    assert lib.jl_kv_attention_workspace_init(ctx, memory + 4, 1 << 20) == L.JL_ERR_INVALID and "aligned" in said(lib)
+    assert lib.jl_kv_attention_workspace_init(ctx, memory, 16) == L.JL_ERR_WORKSPACE
+
+
+def test_attention_of_more_work_than_a_call_lists(L, lib, ctx, memory, cache):
+    args = dict(ATTEND, rows=65535, requests=65535, table_stride=2**27)
+    assert lib.jl_kv_attention(ctx, cache, *[memory if v == "m" else v for v in args.values()]) == L.JL_ERR_INVALID and "in one call" in said(lib)
+
+
 def test_cache_of_another_device(L, lib, memory, cache):
     other = C.create_string_buffer(4096)
     other[0] = 1
