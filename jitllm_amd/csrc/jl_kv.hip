@@ -275,24 +275,37 @@ struct AppendArgs {
     int heads, head_dim, rotated;   // heads: 0 without q
 };
 
+// (cosine, sine) of a number of whole turns, in double precision: whole turns and quarters come off exactly, and the Taylor
+// series of what is left (an eighth of a turn at most, 0.79 radians) end where a term is below 2^-45.
+__device__ __forceinline__ double2 cos_sin_of_turns(double turns) {
+    const double part = turns - rint(turns), quarters = rint(4.0 * part);
+    const double x = (part - 0.25 * quarters) * 6.283185307179586477, y = x * x;
+    const double s = x * (1 + y * (-1.0 / 6 + y * (1.0 / 120 + y * (-1.0 / 5040 + y * (1.0 / 362880 + y * (-1.0 / 39916800 + y * (1.0 / 6227020800.0)))))));
+    const double c = 1 + y * (-0.5 + y * (1.0 / 24 + y * (-1.0 / 720 + y * (1.0 / 40320 + y * (-1.0 / 3628800 + y * (1.0 / 479001600.0))))));
+    const int n = (int)quarters & 3;
+    return make_double2(n == 0 ? c : n == 1 ? -s : n == 2 ? -c : s, n == 0 ? s : n == 1 ? c : n == 2 ? -s : -c);
+}
+
 // LANES consecutive lanes have a head, eight values each (those past head_dim / 8 idle); a workgroup has kAppendPer times
 // 256 / LANES of a token's q, k and v heads, and all their loads are on their way before anything else is done.
 // Bound: the bytes.  The angles' cosines and sines are worked out once per workgroup, in LDS, while the loads come in.
+// Sums and products between the loads and the one rounding at the end are in double precision, which the bytes hide: what
+// the cache keeps is the nearest it can to the rotated value, and a value beside a border of binary16 falls to the right
+// side.
 template <bool Q8, int LANES, bool HALVES>
 __global__ void __launch_bounds__(kAppendThreads) jl_kv_append_kernel(AppendArgs p) {
-    __shared__ float2 turn[128];    // (cos, sin) of the token's pairs
+    __shared__ double2 turn[128];   // (cos, sin) of the token's pairs
+    __shared__ float turned[Q8 && HALVES ? kAppendThreads / LANES : 1][Q8 && HALVES ? 8 * LANES : 4];
     const int row = blockIdx.x, tid = threadIdx.x;
     const int position = p.positions[row];
     if (position < 0) return;
     const int slot = p.slots[row];
     const int kv_heads = p.cache.kv_heads, units = p.heads + 2 * kv_heads;
     const int first_unit = blockIdx.y * (kAppendPer * (kAppendThreads / LANES)) + tid / LANES, chunk = tid % LANES;
-    const bool in_head = chunk < p.head_dim / 8;
-    // where the partners of this lane's values lie: half the turned part on, or back
-    const int half_chunks = p.rotated / 16;
-    const bool turns = 8 * chunk < p.rotated, first_half = chunk < half_chunks;
-    const int partner = !HALVES || !turns ? chunk : first_half ? chunk + half_chunks : chunk - half_chunks;
-    float4 own[kAppendPer][2], other[kAppendPer][2];
+    const bool in_head = chunk < p.head_dim / 8, turns = 8 * chunk < p.rotated;
+    // A lane's eight values are two fours: consecutive ones, or (halves) four and those they turn with.
+    const int at0 = HALVES && turns ? 4 * chunk : 8 * chunk, at1 = HALVES && turns ? p.rotated / 2 + 4 * chunk : 8 * chunk + 4;
+    float4 own[kAppendPer][2];
 #pragma unroll
     for (int j = 0; j < kAppendPer; j++) {
         const int unit = first_unit + j * (kAppendThreads / LANES);
@@ -300,18 +313,11 @@ __global__ void __launch_bounds__(kAppendThreads) jl_kv_append_kernel(AppendArgs
             const float *x = unit < p.heads              ? p.q + row * p.ldq + unit * p.head_dim
                              : unit < p.heads + kv_heads ? p.k + row * p.ldk + (unit - p.heads) * p.head_dim
                                                          : p.v + row * p.ldv + (unit - p.heads - kv_heads) * p.head_dim;
-            own[j][0] = *(const float4 *)(x + 8 * chunk), own[j][1] = *(const float4 *)(x + 8 * chunk + 4);
-            if (HALVES && unit < p.heads + kv_heads)
-                other[j][0] = *(const float4 *)(x + 8 * partner), other[j][1] = *(const float4 *)(x + 8 * partner + 4);
+            own[j][0] = *(const float4 *)(x + at0), own[j][1] = *(const float4 *)(x + at1);
         }
     }
-    for (int i = tid; i < p.rotated / 2; i += kAppendThreads) {
-        // whole turns are dropped in double precision; what is left needs 24 bits
-        const double turns_of = (double)position * p.frequencies[i] * 0.15915494309189533577;
-        float s, c;
-        sincospif(2.0f * (float)(turns_of - rint(turns_of)), &s, &c);
-        turn[i] = make_float2(c, s);
-    }
+    for (int i = tid; i < p.rotated / 2; i += kAppendThreads)
+        turn[i] = cos_sin_of_turns((double)position * p.frequencies[i] * 0.15915494309189533577);
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < kAppendPer; j++) {
@@ -319,46 +325,44 @@ __global__ void __launch_bounds__(kAppendThreads) jl_kv_append_kernel(AppendArgs
         if (unit >= units) return;                            // (a head's lanes together)
         const bool is_q = unit < p.heads, is_v = unit >= p.heads + kv_heads;
         const float *norm = is_q ? p.q_norm : is_v ? nullptr : p.k_norm;
-        float a[8], b[8];
+        float a[8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            a[i] = in_head ? (&own[j][i / 4].x)[i % 4] : 0.f;
-            if constexpr (HALVES) b[i] = in_head && !is_v ? (&other[j][i / 4].x)[i % 4] : 0.f;
-        }
-        if (norm) {
-            float ss = 0.f;
+        for (int i = 0; i < 8; i++) a[i] = in_head ? (&own[j][i / 4].x)[i % 4] : 0.f;
+        if (!is_v && (norm || p.rotated > 0)) {
+            double x[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) ss = fmaf(a[i], a[i], ss);
-            ss = jl_group_sum<LANES>(ss);
-            const float root = sqrtf(ss / (float)p.head_dim + p.eps);
+            for (int i = 0; i < 8; i++) x[i] = a[i];
+            if (norm) {
+                double ss = 0;
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                if (in_head) a[i] = a[i] / root * norm[8 * chunk + i];
-                if (HALVES && in_head) b[i] = b[i] / root * norm[8 * partner + i];
-            }
-        }
-        if (in_head && turns && !is_v) {
-            if constexpr (HALVES) {
+                for (int i = 0; i < 8; i++) ss = fma(x[i], x[i], ss);
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const float2 t = turn[8 * (first_half ? chunk : partner) + i];
-                    a[i] = first_half ? a[i] * t.x - b[i] * t.y : b[i] * t.y + a[i] * t.x;
-                }
-            } else {
+                for (int off = LANES / 2; off >= 1; off >>= 1) ss += __shfl_xor(ss, off, JL_WAVE);
+                const double scale = 1 / sqrt(ss / p.head_dim + p.eps);
+                if (in_head) {
+                    const float4 w[2] = {*(const float4 *)(norm + at0), *(const float4 *)(norm + at1)};
 #pragma unroll
-                for (int i = 0; i < 8; i += 2) {
-                    const float2 t = turn[4 * chunk + i / 2];
-                    const float even = a[i], odd = a[i + 1];
-                    a[i] = even * t.x - odd * t.y;
-                    a[i + 1] = even * t.y + odd * t.x;
+                    for (int i = 0; i < 8; i++) x[i] *= scale * (&w[i / 4].x)[i % 4];
                 }
             }
+            if (in_head && turns) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const double2 t = turn[4 * chunk + i];
+                    const int m = HALVES ? i : 2 * i, n = HALVES ? i + 4 : 2 * i + 1;
+                    const double first = x[m], second = x[n];
+                    x[m] = first * t.x - second * t.y;
+                    x[n] = first * t.y + second * t.x;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++) a[i] = (float)x[i];
         }
         if (is_q) {
-            float *out = p.q_out + row * p.ldq_out + unit * p.head_dim + 8 * chunk;
+            float *out = p.q_out + row * p.ldq_out + unit * p.head_dim;
             if (in_head) {
-                *(float4 *)out = make_float4(a[0], a[1], a[2], a[3]);
-                *(float4 *)(out + 4) = make_float4(a[4], a[5], a[6], a[7]);
+                *(float4 *)(out + at0) = make_float4(a[0], a[1], a[2], a[3]);
+                *(float4 *)(out + at1) = make_float4(a[4], a[5], a[6], a[7]);
             }
             continue;
         }
@@ -367,11 +371,27 @@ __global__ void __launch_bounds__(kAppendThreads) jl_kv_append_kernel(AppendArgs
         uint8_t *part = p.cache.k + (is_v ? p.cache.v_offset : 0) +
                         ((int64_t)page * kv_heads + (is_v ? unit - p.heads - kv_heads : unit - p.heads)) * p.cache.part_bytes;
         if constexpr (!Q8) {
-            jl_half8 h;
-#pragma unroll
-            for (int i = 0; i < 8; i++) h[i] = (_Float16)a[i];
-            if (in_head) *(jl_half8 *)(part + (token * p.head_dim + 8 * chunk) * 2) = h;
+            _Float16 *to = (_Float16 *)part + token * p.head_dim;
+            const jl_half4v low = {(_Float16)a[0], (_Float16)a[1], (_Float16)a[2], (_Float16)a[3]};
+            const jl_half4v high = {(_Float16)a[4], (_Float16)a[5], (_Float16)a[6], (_Float16)a[7]};
+            if (in_head) *(jl_half4v *)(to + at0) = low, *(jl_half4v *)(to + at1) = high;
         } else {
+            if constexpr (HALVES) {
+                // blocks are of consecutive values: through LDS, inside the wave
+                float *head = turned[tid / LANES];
+                if (in_head) {
+                    *(float4 *)(head + at0) = make_float4(a[0], a[1], a[2], a[3]);
+                    *(float4 *)(head + at1) = make_float4(a[4], a[5], a[6], a[7]);
+                }
+                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+                if (in_head) {
+                    const float4 low = *(const float4 *)(head + 8 * chunk), high = *(const float4 *)(head + 8 * chunk + 4);
+                    a[0] = low.x, a[1] = low.y, a[2] = low.z, a[3] = low.w, a[4] = high.x, a[5] = high.y, a[6] = high.z, a[7] = high.w;
+                }
+                __builtin_amdgcn_wave_barrier();
+            }
             float most = 0.f;
 #pragma unroll
             for (int i = 0; i < 8; i++) most = fmaxf(most, fabsf(a[i]));
