@@ -2,7 +2,8 @@
 //
 // Mathematics.  For a row and a head of k and v, S = K Q^T over tiles of 32 tokens and up to 16 query heads (the heads
 // that share k and v), P = 2^(S - m) with a running maximum m, O = O 2^(m_old - m) + V^T P^T, l the sum of P; the result
-// is O / l, and two parts (m, l, O) of a row join by the same rule.  scale * log2(e) is folded into q.
+// is O / l, and two parts (m, l, O) of a row join by the same rule.  scale * log2(e) is folded into q; P, and with it l
+// and O, are held 2^13 times as large, so that weights far below the largest keep their precision.
 //
 // Matrix instructions.  v_mfma_f32_16x16x32_f16 throughout, laid out so that nothing is exchanged between lanes but
 // the maximum: S comes out with a query head per lane (lane % 16) and the tokens 4 g ... 4 g + 3 of both 16-token
@@ -34,6 +35,9 @@ constexpr int kStart = 4;                 // what beginning a (row, head) pair t
 // and 93.4).
 constexpr uint32_t kParts = 32, kMostParts = 64, kLargePart = 64;
 constexpr int kDeviceScope = 16;          // a buffer load's policy: sc1
+// Weights are 2^kLift at the running maximum, which may fall behind by 2^kSlack: 2^15 at most, and what binary16 keeps of
+// one (2^-25 off, however small it is) is 2^-38 of the largest.
+constexpr float kSlack = 2, kLift = 13;
 constexpr float kNone = -3.0e38f;         // the running maximum of nothing: finite, so that differences are numbers
 
 constexpr int kHalves = 2, kTile = 16 * kHalves;   // a wave's tile: tokens, in halves of 16
@@ -46,6 +50,7 @@ struct Shape {
     static constexpr float kTilesAtOnce = 3.0e6f / kTileBytes;
 };
 
+typedef float floatx2 __attribute__((ext_vector_type(2)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
 typedef uint32_t uintx2 __attribute__((ext_vector_type(2)));
@@ -589,9 +594,9 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
 #pragma unroll
             for (int i = 1; i < 8; i++) most = fmaxf(most, x[i]);
             most = over_groups_max(most) * undo;
-            // The maximum may fall behind by a factor of 2^8 before everything is brought to the new one: weights
-            // stay far inside binary16, and after a row's first tiles this is rare.
-            if (__any(most > top + 8.f)) {
+            // The maximum may fall behind by a factor of 2^kSlack before everything is brought to the new one: after a
+            // row's first tiles this is rare.
+            if (__any(most > top + kSlack)) {
                 const float next_top = fmaxf(top, most);
                 const float keep = __builtin_amdgcn_exp2f(top - next_top);
                 top = next_top;
@@ -599,14 +604,15 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
 #pragma unroll
                 for (int b = 0; b < kBlocks; b++) o[b] *= keep;
             }
+            const float lift = kLift - top;
             uintx4 hi, lo;
 #pragma unroll
             for (int i = 0; i < 8; i += 2) {
-                const float a = __builtin_amdgcn_exp2f(fmaf(x[i], undo, -top)), b = __builtin_amdgcn_exp2f(fmaf(x[i + 1], undo, -top));
+                const float a = __builtin_amdgcn_exp2f(fmaf(x[i], undo, lift)), b = __builtin_amdgcn_exp2f(fmaf(x[i + 1], undo, lift));
                 sum += a + b;
-                const auto two = __builtin_amdgcn_cvt_pkrtz(a, b);
-                hi[i / 2] = __builtin_bit_cast(uint32_t, two);
-                lo[i / 2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a - (float)two[0], b - (float)two[1]));
+                const jl_half2v two = __builtin_convertvector(floatx2{a, b}, jl_half2v);
+                hi[i / 2] = as_u32(two);
+                lo[i / 2] = as_u32(__builtin_convertvector(floatx2{a - (float)two[0], b - (float)two[1]}, jl_half2v));
             }
             const jl_half8 p_hi = __builtin_bit_cast(jl_half8, hi), p_lo = __builtin_bit_cast(jl_half8, lo);
 #pragma unroll

@@ -541,6 +541,29 @@ def test_attend_large_and_extreme_scores(ctx):
     check_attend(got[:, [0, 3]], *(w[:1, [0, 3]] for w in want), [n], dim)
 
 
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("n,every", [(6000, 32), (900, 300)])
+def test_attend_weights_far_below_the_largest(ctx, q8, n, every):
+    """Tokens that take nearly all the weight and have values of zero (a sequence's first token is often one): the
+    result is what the others say, a millionth of the weight each.  Those keep their precision."""
+    rng = np.random.default_rng(n)
+    dim, page = 64, 16
+    table, pages = make_tables(rng, [n], page)
+    cache = cache_of(ctx, q8, pages, 1, dim, page, random_pool(rng, q8, pages, 1, dim, page))
+    k, v = 0.1 * rng.standard_normal((n, dim)), 1 + 0.5 * rng.random((n, dim))
+    k[::every], v[::every] = 0, 0
+    k[::every, 3] = 10
+    slots = table[0, np.arange(n) // page] * page + np.arange(n) % page
+    cache.append(ctx.from_numpy(k), ctx.from_numpy(v), ints(ctx, np.arange(n)), ints(ctx, slots), n)
+    ctx.sync()
+    q = rng.standard_normal((1, 4, dim)).astype(np.float32)
+    q[:, :, 3] = 8 * np.array([1.25, 1.375, 1.4, 1.5])         # scores of 12.5 ... 15: weights of 2^-18 ... 2^-22
+    say("attend weak", n, q8)
+    got = run_attend(ctx, cache, q, np.array([n - 1]), None, table)
+    want = M.attend(M.decode_pool(pool_bytes(cache), q8, pages, 1, dim, page), q, [n - 1], None, table, dim ** -0.5)
+    check_attend(got, *want, [n], dim)
+
+
 def test_attend_is_the_same_every_time_and_with_any_workspace(ctx):
     rng = np.random.default_rng(14)
     lengths = np.array([5000, 12, 800, 0, 3333])
