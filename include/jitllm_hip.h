@@ -518,6 +518,7 @@ typedef enum jl_rope_style { JL_ROPE_PAIRS = 0, JL_ROPE_HALVES = 1 } jl_rope_sty
  *               frequencies may be null.
  *   q_norm, k_norm    [head_dim] fp32 or null: heads are normalised first, x <- w * (x / sqrt(sum x^2
  *               / head_dim + eps)), as Qwen3's are
+ * Sums and products are in double precision and rounded once, to fp32; fewer than 2^24 rows.
  * A JL_KV_F16 element is the nearest binary16 (infinite where fp32 is beyond it).  A block of
  * JL_KV_Q8_0 has d = the binary16 nearest to max |x| / 127 (at most 65504) and bytes rint(x / d)
  * in -127 ... 127; 0 where d is 0 or x is NaN.
@@ -531,7 +532,7 @@ int jl_kv_append(jl_context *ctx, jl_kv_cache *cache, const float *q, int heads,
  * Decodes the k and v at `slots` ([rows]) to rows of kv_heads x head_dim values, binary16 (exact) or,
  * with out_f16 == 0, fp32: the parity probe, and the way out of the cache for a prefix that is kept
  * elsewhere.  Zeros where the slot is none of the cache's.  k_out and v_out 16-byte aligned; either
- * may be null.
+ * may be null.  Fewer than 2^35 values of each a call.
  */
 int jl_kv_read(jl_context *ctx, const jl_kv_cache *cache, const int32_t *slots, int64_t rows, void *k_out,
                void *v_out, int out_f16);
@@ -547,12 +548,14 @@ int jl_kv_read(jl_context *ctx, const jl_kv_cache *cache, const int32_t *slots, 
  *        each reads its own range.
  *   out  fp32, or with out_f16 binary16 (rounded once, as the projections of jl_gemm_xf16 take it);
  *        `ldo` of its values between rows; 16-byte aligned, ldo a multiple of 4 (fp32) or 8 (binary16)
+ *        and none of q's memory
  * A row with nothing to read -- position -1, a request outside the table -- is zeros.  A position past
  * the table's last token reads the tokens that the table holds.  A page outside the cache counts as
  * one whose tokens are all masked.  What lies in the pages at masked tokens (other requests' or
- * stale values, infinities, NaN) has no influence.  Scores, weights and sums are fp32 (q and the weights enter
- * the matrix instructions as two binary16 parts each, 22 bits), so results are those of an fp32
- * softmax.  The work is cut over the cache's length where rows are few or lengths differ, and
+ * stale values, infinities, NaN) has no influence; an infinity or NaN that a row does read may leave
+ * NaN.  Scores, weights and sums are fp32 (q and the weights enter the matrix instructions as two
+ * binary16 parts each, 22 bits and, of weights, 2^-38 of the largest), so results are those of an
+ * fp32 softmax.  The work is cut over the cache's length where rows are few or lengths differ, and
  * joined in a fixed order: the same call gives the same bits, whose last few may differ between
  * batches of other lengths.
  * workspace: jl_kv_attention_workspace_bytes of the largest call that uses it, 16-byte aligned, which

@@ -72,9 +72,9 @@ class Rows:
         self.array, self.stride, self.offset = array, stride, offset
 
 
-def _place(who: str, value, rows: int, width: int):
-    """(address, stride) of ``rows`` rows of ``width`` elements; raises where they are not the array's.  An
-    array in place of Rows: its rows lie behind one another."""
+def _place(who: str, value, rows: int, width: int, itemsize: int = 0):
+    """(address, stride) of ``rows`` rows of ``width`` elements; raises where they are not the array's, or its
+    elements not of ``itemsize`` bytes (0: of any).  An array in place of Rows: its rows lie behind one another."""
     if value.__class__ is Rows:
         array, stride, offset = value.array, value.stride, value.offset
     else:
@@ -82,8 +82,11 @@ def _place(who: str, value, rows: int, width: int):
     size = array.size
     if stride < width or offset < 0 or (rows > 0 and offset + (rows - 1) * stride + width > size):
         raise ValueError(f"{who}: {rows} rows of {width} elements, {stride} apart from {offset} on, in an array of {size}")
-    address = array.ptr.value or 0
-    return (address + offset * (array.nbytes // size) if offset else address), stride
+    if itemsize == 0:
+        itemsize = array.nbytes // max(size, 1)
+    elif array.nbytes != itemsize * size:
+        raise ValueError(f"{who}: an array of {size} elements in {array.nbytes} bytes, of {itemsize} each is taken")
+    return (array.ptr.value or 0) + itemsize * offset, stride
 
 
 def _ints(who: str, array, count: int) -> int:
@@ -162,17 +165,17 @@ class PagedKvCache:
         """Turns q and k (normalised first where ``qNorm`` / ``kNorm`` are given) and writes k and v to
         ``slots`` (jl_kv_append).  ``q`` is turned into ``qOut``, or in place without one."""
         width = self.kvHeads * self.headDim
-        k, ldk = _place("k", k, rows, width)
-        v, ldv = _place("v", v, rows, width)
+        k, ldk = _place("k", k, rows, width, 4)
+        v, ldv = _place("v", v, rows, width, 4)
         if q is None:
             q = ldq = out = ldOut = heads = 0
         else:
             width = heads * self.headDim
-            out, ldOut = _place("qOut", q if qOut is None else qOut, rows, width)
-            q, ldq = _place("q", q, rows, width)
+            out, ldOut = _place("qOut", q if qOut is None else qOut, rows, width, 4)
+            q, ldq = _place("q", q, rows, width, 4)
         for name, norm in (("qNorm", qNorm), ("kNorm", kNorm)) if qNorm is not None or kNorm is not None else ():
-            if norm is not None and norm.size != self.headDim:
-                raise ValueError(f"{name} has {norm.size} weights, a head {self.headDim} values")
+            if norm is not None and not norm.size == self.headDim == norm.nbytes // 4:
+                raise ValueError(f"{name} has {norm.size} weights in {norm.nbytes} bytes, a head {self.headDim} values")
         frequencies, rotated, style = rope._args if rope is not None else _NO_ROPE
         status = self._lib.jl_kv_append(
             self.ctx.handle, self.handle, q, heads, ldq, k, ldk, v, ldv, out, ldOut, _ints("positions", positions, rows),
@@ -254,21 +257,29 @@ class PagedAttention:
         L.check(self._lib.jl_kv_attention_workspace_init(ctx.handle, self.workspace.ptr, nbytes))
 
     def attend(self, cache: PagedKvCache, q, rows: int, positions, table, out, requests: int, rowRequests=None,
-               scale: float | None = None, window: int = 0) -> None:
+               scale: float | None = None, window: int = 0, blocksPerRequest: int | None = None) -> None:
         """``out[row] = softmax(scale * q[row] . k) v`` over the tokens up to ``positions[row]`` (the last
         ``window`` of them where that is positive) of request ``rowRequests[row]``, or of request ``row``.
-        ``scale``: 1 / sqrt(headDim) unless given.  ``out``: a FloatArray or a HalfFloatArray."""
+        ``scale``: 1 / sqrt(headDim) unless given.  ``out``: a FloatArray or a HalfFloatArray.  ``requests`` are
+        all of the table's rows, unless ``blocksPerRequest`` says how many entries a row has."""
         if cache.kvHeads != self.kvHeads or cache.headDim != self.headDim:
             raise ValueError(f"a cache of {cache.kvHeads} heads of {cache.headDim}, attention over {self.kvHeads} of {self.headDim}")
         width = self.width
         array = out.array if out.__class__ is Rows else out
         half = array.nbytes == 2 * array.size
-        q, ldq = _place("q", q, rows, width)
-        out, ldOut = _place("out", out, rows, width)
+        q, ldq = _place("q", q, rows, width, 4)
+        out, ldOut = _place("out", out, rows, width, 2 if half else 4)
+        entries = table.nbytes // 4
+        if blocksPerRequest is None:
+            blocksPerRequest = entries // requests if requests > 0 else 1
+            if requests > 0 and blocksPerRequest * requests != entries:
+                raise ValueError(f"a block table of {entries} entries for {requests} requests: blocksPerRequest?")
+        elif blocksPerRequest * requests > entries:
+            raise ValueError(f"{requests} x {blocksPerRequest} entries of a block table of {entries}")
         status = self._lib.jl_kv_attention(
             self.ctx.handle, cache.handle, q, self.heads, ldq, rows, _ints("positions", positions, rows),
             _ints("rowRequests", rowRequests, rows) if rowRequests is not None else None, table.ptr, requests,
-            table.nbytes // 4 // requests if requests > 0 else 1, self.scale if scale is None else scale, window, out, half, ldOut,
+            blocksPerRequest, self.scale if scale is None else scale, window, out, half, ldOut,
             self.workspace.ptr, self.workspace.nbytes)
         if status:
             L.check(status)

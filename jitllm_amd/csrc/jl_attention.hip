@@ -787,7 +787,7 @@ extern "C" {
 
 size_t jl_kv_attention_workspace_bytes(int heads, int kv_heads, int head_dim) {
     if (kv_heads <= 0 || heads <= 0 || heads % kv_heads || head_dim <= 0) return 0;
-    return kArrivedBytes + (size_t)2 * kMostGroups * 16 * (head_dim + 2) * sizeof(float);
+    return kArrivedBytes + (size_t)2 * kMostGroups * 16 * ((size_t)head_dim + 2) * sizeof(float);
 }
 
 int jl_kv_attention_workspace_init(jl_context *ctx, void *workspace, size_t workspace_bytes) {
@@ -819,7 +819,8 @@ int jl_kv_attention(jl_context *ctx, const jl_kv_cache *cache, const float *q, i
     const int64_t lists = rows * cache->kv_heads * ((heads / cache->kv_heads + 15) / 16);
     JL_REQUIRE(lists <= 0 || table_tokens / 32 + 2 + kStart <= (int64_t)(UINT32_MAX - 2 * kMostGroups) / lists,
                "jl_kv_attention: %lld rows of %d heads over %lld tokens in one call", (long long)rows, heads, (long long)table_tokens);
-    JL_REQUIRE(std::isfinite(scale), "jl_kv_attention: scale %g", (double)scale);
+    const float scale_of_powers = scale * 1.44269504088896340736f;   // weights are powers of two
+    JL_REQUIRE(std::isfinite(scale_of_powers), "jl_kv_attention: scale %g", (double)scale);
     JL_REQUIRE(window >= 0, "jl_kv_attention: window %lld", (long long)window);
     const int64_t width = (int64_t)heads * dim;
     JL_REQUIRE(ldq >= width && ldo >= width, "jl_kv_attention: rows closer together (%lld, %lld) than they are long (%lld)",
@@ -830,6 +831,7 @@ int jl_kv_attention(jl_context *ctx, const jl_kv_cache *cache, const float *q, i
     if (workspace_bytes < needed)
         return jl_fail(JL_ERR_WORKSPACE, "jl_kv_attention: workspace of %zu bytes, %zu needed", workspace_bytes, needed);
     if (rows == 0) return JL_OK;
+    JL_REQUIRE(out != q, "jl_kv_attention: out in place of q");
     const JlOnDevice on(ctx);
     JL_HIP(on.status);
     AttentionArgs a;
@@ -837,7 +839,7 @@ int jl_kv_attention(jl_context *ctx, const jl_kv_cache *cache, const float *q, i
     a.q = q, a.ldq = ldq, a.ldo = ldo;
     a.positions = positions, a.row_requests = row_requests, a.table = block_table;
     a.requests = (int)requests, a.table_stride = table_stride, a.table_tokens = (int)table_tokens;
-    a.scale = scale * 1.44269504088896340736f;
+    a.scale = scale_of_powers;
     a.window = window > INT32_MAX ? 0 : (int)window;   // one that reaches behind every position
     a.group = heads / cache->kv_heads;
     a.blocks_of_16 = (a.group + 15) / 16;

@@ -559,7 +559,8 @@ int jl_kv_append(jl_context *ctx, jl_kv_cache *cache, const float *q, int heads,
     const int dim = cache->head_dim;
     JL_REQUIRE(cache->ctx->device == ctx->device, "jl_kv_append: the cache lies on device %d, the context's is %d",
                cache->ctx->device, ctx->device);
-    JL_REQUIRE(rows >= 0 && rows <= INT32_MAX, "jl_kv_append: %lld rows", (long long)rows);
+    // (a launch has fewer than 2^32 threads along a side)
+    JL_REQUIRE(rows >= 0 && rows < (1ll << 32) / kAppendThreads, "jl_kv_append: %lld rows (fewer than 2^24)", (long long)rows);
     JL_REQUIRE(rotated >= 0 && rotated <= dim && rotated % 16 == 0, "jl_kv_append: %d values turned of heads of %d (a multiple of 16)",
                rotated, dim);
     JL_REQUIRE(rotated == 0 || frequencies, "jl_kv_append: null frequencies for %d turned values", rotated);
@@ -601,7 +602,8 @@ int jl_kv_read(jl_context *ctx, const jl_kv_cache *cache, const int32_t *slots, 
     JL_REQUIRE(aligned(k_out, 16) && aligned(v_out, 16), "jl_kv_read: k_out and v_out must be 16-byte aligned");
     if (rows == 0 || (!k_out && !v_out)) return JL_OK;
     const int64_t threads = rows * cache->kv_heads * (cache->head_dim / 8);
-    JL_REQUIRE(threads <= (int64_t)INT32_MAX * 256, "jl_kv_read: %lld rows", (long long)rows);
+    JL_REQUIRE(threads < (1ll << 32) - 256, "jl_kv_read: %lld rows of %d values in one call (fewer than 2^35 values in all)", (long long)rows,
+               cache->kv_heads * cache->head_dim);
     const JlOnDevice on(ctx);
     JL_HIP(on.status);
     const dim3 grid((unsigned)((threads + 255) / 256)), block(256);

@@ -171,6 +171,17 @@ def test_attention_of_more_work_than_a_call_lists(L, lib, ctx, memory, cache):
     assert lib.jl_kv_attention(ctx, cache, *[memory if v == "m" else v for v in args.values()]) == L.JL_ERR_INVALID and "in one call" in said(lib)
 
 
+def test_calls_past_a_launch(L, lib, ctx, memory, cache):
+    """More threads than a launch has along a side, an output over the queries, a scale that the powers of two lose."""
+    args = dict(APPEND, rows=2**24)
+    assert lib.jl_kv_append(ctx, cache, *[memory if v == "m" else v for v in args.values()]) == L.JL_ERR_INVALID and "2^24" in said(lib)
+    assert lib.jl_kv_read(ctx, cache, memory, 2**27, memory, memory, 1) == L.JL_ERR_INVALID and "2^35" in said(lib)
+    args = dict(ATTEND, rows=1)
+    assert lib.jl_kv_attention(ctx, cache, *[memory if v == "m" else v for v in args.values()]) == L.JL_ERR_INVALID and "in place" in said(lib)
+    args = dict(ATTEND, scale=3e38)
+    assert lib.jl_kv_attention(ctx, cache, *[memory if v == "m" else v for v in args.values()]) == L.JL_ERR_INVALID and "scale" in said(lib)
+
+
 def test_cache_of_another_device(L, lib, memory, cache):
     other = C.create_string_buffer(4096)
     other[0] = 1
@@ -201,6 +212,41 @@ def test_binding_checks_what_the_library_cannot():
         BlockTables(Ctx(), 4, 2, 6, 16, 3, arrays={**{k: Array(n) for k, n in sizes.items()}, "tabel": Array(8)})
     with pytest.raises(ValueError, match="slots"):
         BlockTables(Ctx(), 4, 2, 6, 16, 3, arrays={**{k: Array(n) for k, n in sizes.items()}, "slots": Array(2)})
+
+
+def test_binding_checks_of_elements_and_tables():
+    """binary16 where fp32 is taken, norms of it, a table whose rows' length the number of requests does not say."""
+    from jitllm_amd.attention import PagedAttention, PagedKvCache, Rows, _place
+
+    class Array:
+        def __init__(self, size, itemsize=4):
+            self.size, self.nbytes, self.ptr = size, size * itemsize, C.c_void_p(4096)
+
+    calls = []
+
+    class Lib:
+        def jl_kv_attention(self, *args):
+            calls.append(args)
+            return 0
+
+    class Ctx:
+        handle, _lib = None, Lib()
+
+    with pytest.raises(ValueError, match="q: .* 2048 bytes"):
+        _place("q", Rows(Array(1024, 2), 128), 8, 128, 4)
+    assert _place("out", Rows(Array(1024, 2), 128, 64), 7, 128, 2) == (4096 + 128, 128)
+    cache, attention = object.__new__(PagedKvCache), object.__new__(PagedAttention)
+    cache.ctx, cache._lib, cache.kvHeads, cache.headDim, cache.handle = Ctx(), Lib(), 2, 64, None
+    with pytest.raises(ValueError, match="kNorm"):
+        cache.append(Array(128), Array(128), Array(1), Array(1), 1, kNorm=Array(64, 2))
+    attention.ctx, attention._lib, attention.kvHeads, attention.headDim, attention.heads = Ctx(), Lib(), 2, 64, 4
+    attention.width, attention.scale, attention.workspace = 256, 0.125, Array(10)
+    for more, stride in ((dict(requests=8), 16), (dict(requests=3, blocksPerRequest=16), 16), (dict(requests=0), 1)):
+        attention.attend(cache, Array(512), 2, Array(2), Array(128), Array(512), **more)
+        assert calls[-1][9:11] == (more["requests"], stride)
+    for more in (dict(requests=3), dict(requests=9, blocksPerRequest=16)):
+        with pytest.raises(ValueError, match="block table"):
+            attention.attend(cache, Array(512), 2, Array(2), Array(128), Array(512), **more)
 
 
 def test_models_agree_with_each_other():
