@@ -494,7 +494,8 @@ void *jl_kv_cache_memory(const jl_kv_cache *cache);
  * Only the table's new entries and the ring's returned pages are written; lengths may be past and
  * free_out may be free_in, and with other arrays there the same call can be made again and leaves
  * the same.  At most 8192 requests, 2^17 rows, 2^31 - 1 table entries.  One launch, or two where
- * max_rows is large; the order of nothing depends on timing.
+ * max_rows is large and lengths are past or free_out is free_in; the order of nothing depends on
+ * timing.
  */
 int jl_kv_plan(jl_context *ctx, const int32_t *past, const int32_t *fresh, int64_t requests, int64_t pages,
                int page_tokens, int32_t *page_ring, const int32_t *free_in, int32_t *free_out, int32_t *block_table,

@@ -12,13 +12,19 @@ namespace {
 // ---- jl_kv_plan ----------------------------------------------------------------------------------
 
 constexpr int kPlanMaxRequests = 8192, kPlanMaxRows = 1 << 17;
-// Up to this many rows the requests' workgroup fills the rows' arrays itself; more are spread over a second launch.
-constexpr int kPlanRowsAtOnce = 4096;
+// Workgroups of a launch: one for each 512 rows, or 64 requests, begun, so that a step with prompts in it is one element of
+// its list a thread (64 requests, 512 rows: 5.6 us with one workgroup, 4.8 with two; 512, 8192 rows and pages short: 18.3,
+// 7.6 with 8, 5.1 with 17; 4096 and 65 536: 125, 14 with 64, 9.4 with 128).
+constexpr int kPlanRowsEach = 512, kPlanRequestsEach = 64, kPlanMostGroups = 128;
+// Where lengths are past or free_out is free_in, several workgroups need a second launch, for those two: one workgroup does
+// up to this many rows (512 requests that all decode: 3.9 us with one workgroup, 7.0 with two launches; 4096 of them in
+// 4096 rows 9.6 and 12.1, in 65 536 rows 17.4 and 12.3, with prompts 125 and 14).
+constexpr int kPlanRowsInPlace = 4096;
 
 struct PlanArgs {
     const int32_t *past, *fresh, *free_in;
     int32_t *ring, *free_out, *table, *lengths, *row_starts, *slots, *positions, *row_requests;
-    int requests, pages, page_shift, table_stride, max_rows;
+    int requests, pages, page_shift, table_stride, max_rows, parts;
 };
 
 // Inclusive sum over a wave's lanes: within rows of sixteen, then rows' last lanes handed on.
@@ -73,26 +79,59 @@ __device__ __forceinline__ int slot_in(const PlanArgs &p, int page, int position
     return (unsigned)page < (unsigned)p.pages ? (page << p.page_shift) + (position & ((1 << p.page_shift) - 1)) : -1;
 }
 
-// One workgroup, ITEMS consecutive requests a thread.  Sums over the requests give each its rows and pages; what a
-// request has many of -- rows of a prompt, pages of one that begins or ends -- is dealt to all threads alike, each
-// finding its request by bisection in LDS.  Latency: of the lengths' loads, two sums over the workgroup, and the loads
-// of page numbers that hang on them.
-template <int THREADS, int ITEMS, bool ROWS>
+// A thread's ITEMS consecutive elements of an array of n: four at a time where there are four (0 behind the last one).
+typedef int int4_of_ints __attribute__((ext_vector_type(4), aligned(4)));
+template <int ITEMS>
+__device__ __forceinline__ void load_items(const int32_t *from, int n, int (&to)[ITEMS]) {
+    constexpr int W = ITEMS % 4 == 0 ? 4 : 1;
+#pragma unroll
+    for (int j = 0; j < ITEMS; j += W) {
+        const int at = (int)threadIdx.x * ITEMS + j;
+        if constexpr (W == 4) {
+            if (at + 4 <= n) {
+                const int4_of_ints four = *(const int4_of_ints *)(from + at);
+#pragma unroll
+                for (int i = 0; i < 4; i++) to[j + i] = four[i];
+                continue;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < W; i++) to[j + i] = at + i < n ? from[at + i] : 0;
+    }
+}
+template <int ITEMS>
+__device__ __forceinline__ void store_items(int32_t *to, int n, const int (&from)[ITEMS]) {
+#pragma unroll
+    for (int j = 0; j < ITEMS; j++)
+        if ((int)threadIdx.x * ITEMS + j < n) to[(int)threadIdx.x * ITEMS + j] = from[j];
+}
+
+// What a launch writes: everything but lengths and free_out, those two, or all.
+constexpr int kPlanMoves = 1, kPlanLengths = 2;
+
+// ITEMS consecutive requests a thread.  Sums over the requests give each its rows and pages; what a request has many
+// of -- rows of a prompt, pages of one that begins or ends -- is dealt to all threads of all workgroups alike, each
+// finding its request by bisection in LDS.  Every workgroup takes the sums over all requests for itself: they come out
+// of the caches, and nobody waits for anybody.  Latency: of the lengths' loads, two sums over the workgroup, and the
+// loads of page numbers that hang on them.
+template <int THREADS, int ITEMS>
 __global__ void __launch_bounds__(THREADS) jl_kv_plan_kernel(PlanArgs p) {
     extern __shared__ int lds[];
     int *rows_through = lds, *taken_through = lds + p.requests, *back_through = lds + 2 * p.requests, *first_position = lds + 3 * p.requests;
     __shared__ int sums[3][THREADS / JL_WAVE], granted_pages, most_rows;
     const int tid = threadIdx.x, page = 1 << p.page_shift;
+    const bool moves = p.parts & kPlanMoves, its_lengths = p.parts & kPlanLengths;
+    // the workgroup that writes what this wave's requests have one of
+    const bool mine = min((unsigned)tid / JL_WAVE, gridDim.x - 1) == blockIdx.x;
     if (tid == 0) granted_pages = most_rows = 0;
     int head = p.free_in[0], count = p.free_in[1];
     if (head < 0 || head >= p.pages || count < 0 || count > p.pages) head = count = 0;
     const int table_tokens = (int)min((int64_t)p.table_stride << p.page_shift, (int64_t)INT_MAX);   // positions are int32
     int past[ITEMS], fresh[ITEMS], wanted[ITEMS], need[ITEMS], back[ITEMS];
+    load_items(p.past, p.requests, past), load_items(p.fresh, p.requests, fresh);
     int rows = 0;
 #pragma unroll
     for (int j = 0; j < ITEMS; j++) {
-        const int r = tid * ITEMS + j;
-        past[j] = r < p.requests ? p.past[r] : 0, fresh[j] = r < p.requests ? p.fresh[r] : 0;
         wanted[j] = min(max(fresh[j], 0), p.max_rows + 1);
         rows += wanted[j];
     }
@@ -113,6 +152,7 @@ __global__ void __launch_bounds__(THREADS) jl_kv_plan_kernel(PlanArgs p) {
     int asked = sum_before<THREADS>(needs, all_need, sums[1]);
     int returned = sum_before<THREADS>(backs, all_back, sums[2]);
     int granted_through = 0, widest = 0;
+    int first_row[ITEMS], first_at[ITEMS], first_page[ITEMS], lengths[ITEMS], starts[ITEMS];   // (row -1: none)
 #pragma unroll
     for (int j = 0; j < ITEMS; j++) {
         const int r = tid * ITEMS + j;
@@ -126,39 +166,43 @@ __global__ void __launch_bounds__(THREADS) jl_kv_plan_kernel(PlanArgs p) {
             taken_through[r] = granted ? asked : min(asked, count);      // (nothing behind the last one granted is taken)
             back_through[r] = returned;
             first_position[r] = granted ? past[j] : -1;
-            p.lengths[r] = fresh[j] < 0 ? 0 : granted ? past[j] + wanted[j] : past[j];
-            p.row_starts[r + 1] = min(row + wanted[j], p.max_rows);
-            if (wanted[j] > 0 && row < p.max_rows) {
-                // its first row; a second launch takes the position from here for the others
-                p.positions[row] = granted ? past[j] : -1;
-                if constexpr (ROWS) {
-                    const int b = past[j] >> p.page_shift;
-                    int of = -1;
-                    if (granted) of = b < had ? p.table[(int64_t)r * p.table_stride + b] : p.ring[wrapped((int64_t)head + asked - take + b - had, p.pages)];
-                    p.row_requests[row] = r;
-                    p.slots[row] = slot_in(p, of, past[j]);
-                }
-            }
+        }
+        lengths[j] = fresh[j] < 0 ? 0 : granted ? past[j] + wanted[j] : past[j];
+        starts[j] = min(row + wanted[j], p.max_rows);
+        // its first row (others are in the list below): the loads of their pages are under way together
+        first_row[j] = mine && moves && wanted[j] > 0 && row < p.max_rows ? row : -1;
+        first_at[j] = granted ? past[j] : -1, first_page[j] = -1;
+        if (first_row[j] >= 0 && granted) {
+            const int b = past[j] >> p.page_shift;
+            first_page[j] = b < had ? p.table[(int64_t)r * p.table_stride + b] : p.ring[wrapped((int64_t)head + asked - take + b - had, p.pages)];
         }
         row += wanted[j];
     }
-    if (tid == 0) p.row_starts[0] = 0;
     if (granted_through > 0) atomicMax(&granted_pages, granted_through);
     if (widest > 1) atomicMax(&most_rows, widest);
     __syncthreads();
     const int taken = granted_pages, put_back = min(all_back, p.pages - count);
+    if (its_lengths) {
+        if (mine) store_items(p.lengths, p.requests, lengths);
+        if (tid == 0 && blockIdx.x == 0) {
+            p.free_out[0] = wrapped((int64_t)head + taken, p.pages);
+            p.free_out[1] = count - taken + put_back;
+        }
+    }
+    if (!moves) return;
     // Everything that is moved is one list -- pages taken, pages returned, rows -- dealt to the threads: all searches run
     // together, and then all loads.
     const int most = power_above(p.requests), behind = wrapped((int64_t)head + count, p.pages);
-    const int used = min(all_rows, p.max_rows), rows_listed = ROWS && most_rows > 1 ? used : 0;
-    const int listed = taken + put_back + rows_listed;
+    const int used = min(all_rows, p.max_rows), rows_listed = most_rows > 1 ? used : 0;
+    const int listed = taken + put_back + rows_listed;             // (at most twice 2^27 pages and 2^17 rows)
+    const int threads = THREADS * gridDim.x, me = blockIdx.x * THREADS + tid;
     auto move = [&](auto batch, int base) {
         constexpr int K = decltype(batch)::value;
-        int kind[K], i[K], r[K], of[K], position[K];
+        int kind[K], i[K], r[K], of[K], position[K], into[K];
         const int *through[K];
 #pragma unroll
         for (int j = 0; j < K; j++) {
-            const int e = min(base + j * THREADS + tid, listed - 1);
+            const int e = min(base + j * threads + me, listed - 1);
             kind[j] = e < taken ? 0 : e < taken + put_back ? 1 : 2;
             i[j] = e - (kind[j] == 0 ? 0 : kind[j] == 1 ? taken : taken + put_back);
             through[j] = kind[j] == 0 ? taken_through : kind[j] == 1 ? back_through : rows_through;
@@ -166,18 +210,19 @@ __global__ void __launch_bounds__(THREADS) jl_kv_plan_kernel(PlanArgs p) {
         first_above(through, p.requests, most, i, r);
 #pragma unroll
         for (int j = 0; j < K; j++) {
-            const int into = i[j] - (r[j] > 0 ? through[j][r[j] - 1] : 0), first = first_position[r[j]];
+            const int first = first_position[r[j]];
             const int had = (int)(((int64_t)first + page - 1) >> p.page_shift);
             int32_t *row_of_table = p.table + (int64_t)r[j] * p.table_stride;
             const int32_t *from;
+            into[j] = i[j] - (r[j] > 0 ? through[j][r[j] - 1] : 0);
             if (kind[j] == 0) {
                 from = p.ring + wrapped((int64_t)head + i[j], p.pages);
-                position[j] = had + into;                     // the entry that it becomes
+                position[j] = had + into[j];                  // the entry that it becomes
             } else if (kind[j] == 1) {
-                from = row_of_table + into;
+                from = row_of_table + into[j];
                 position[j] = 0;
             } else {
-                position[j] = first < 0 ? -1 : first + into;
+                position[j] = first < 0 ? -1 : first + into[j];
                 const int b = max(position[j], 0) >> p.page_shift;
                 from = b < had ? row_of_table + b : p.ring + wrapped((int64_t)head + (r[j] > 0 ? taken_through[r[j] - 1] : 0) + b - had, p.pages);
             }
@@ -185,13 +230,13 @@ __global__ void __launch_bounds__(THREADS) jl_kv_plan_kernel(PlanArgs p) {
         }
 #pragma unroll
         for (int j = 0; j < K; j++) {
-            if (base + j * THREADS + tid >= listed) continue;
+            if (base + j * threads + me >= listed) continue;
             if (kind[j] == 0) {
                 p.table[(int64_t)r[j] * p.table_stride + position[j]] = of[j];
             } else if (kind[j] == 1) {
                 // (places that no page is taken from: together with those they are at most the ring's)
                 p.ring[wrapped((int64_t)behind + i[j], p.pages)] = of[j];
-            } else {
+            } else if (into[j] > 0) {
                 p.row_requests[i[j]] = r[j];
                 p.positions[i[j]] = position[j];
                 p.slots[i[j]] = slot_in(p, of[j], position[j]);
@@ -199,62 +244,42 @@ __global__ void __launch_bounds__(THREADS) jl_kv_plan_kernel(PlanArgs p) {
         }
     };
     int base = 0;
-    for (; listed - base > THREADS; base += 4 * THREADS) move(std::integral_constant<int, 4>{}, base);
+    for (; listed - base > threads; base += 4 * threads) move(std::integral_constant<int, 4>{}, base);
     if (listed > base) move(std::integral_constant<int, 1>{}, base);
-    if constexpr (ROWS)
-        for (int i = used + tid; i < p.max_rows; i += THREADS) p.slots[i] = p.positions[i] = p.row_requests[i] = -1;
-    if (tid == 0) {
-        p.free_out[0] = wrapped((int64_t)head + taken, p.pages);
-        p.free_out[1] = count - taken + put_back;
-    }
-}
-
-// The rows of many: request, position and slot of each, from what the first launch left (row_starts, the table, and the
-// position of every request's first row).
-__global__ void __launch_bounds__(256) jl_kv_plan_rows_kernel(PlanArgs p) {
-    extern __shared__ int lds[];
-    for (int r = threadIdx.x; r < p.requests; r += 256) lds[r] = p.row_starts[r + 1];
-    __syncthreads();
-    const int i = blockIdx.x * 256 + threadIdx.x;
-    if (i < p.max_rows) {
-        const int *const ends[1] = {lds};
-        const int mine[1] = {i};
-        int found[1];
-        first_above(ends, p.requests, power_above(p.requests), mine, found);
-        const int r = found[0];
-        int position = -1, slot = -1;
-        if (r < p.requests) {
-            // (the first row's thread writes the value that the others read)
-            const int start = r > 0 ? lds[r - 1] : 0, first = __hip_atomic_load(p.positions + start, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            if (first >= 0) {
-                position = first + i - start;
-                slot = slot_in(p, p.table[(int64_t)r * p.table_stride + (position >> p.page_shift)], position);
-            }
-        }
-        p.row_requests[i] = r < p.requests ? r : -1;
-        __hip_atomic_store(p.positions + i, position, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        p.slots[i] = slot;
+    for (int i = used + me; i < p.max_rows; i += threads) p.slots[i] = p.positions[i] = p.row_requests[i] = -1;
+    if (mine) store_items(p.row_starts + 1, p.requests, starts);
+    if (tid == 0 && blockIdx.x == 0) p.row_starts[0] = 0;
+#pragma unroll
+    for (int j = 0; j < ITEMS; j++) {
+        if (first_row[j] < 0) continue;
+        p.row_requests[first_row[j]] = tid * ITEMS + j;
+        p.positions[first_row[j]] = first_at[j];
+        p.slots[first_row[j]] = slot_in(p, first_page[j], first_at[j]);
     }
 }
 
 template <int THREADS, int ITEMS>
-int launch_plan(jl_context *ctx, const PlanArgs &p) {
+int launch_plan(jl_context *ctx, PlanArgs p) {
     const int lds = std::max(4 * p.requests * (int)sizeof(int), 16);
-    const bool rows = p.max_rows <= kPlanRowsAtOnce;
-    const void *kernel = rows ? (const void *)jl_kv_plan_kernel<THREADS, ITEMS, true> : (const void *)jl_kv_plan_kernel<THREADS, ITEMS, false>;
     if (lds > 60 * 1024) {
-        static jl_lds_limit_flags raised[2];
-        const int st = jl_raise_lds_limit(raised[rows], ctx->device, kernel, 4 * THREADS * ITEMS * (int)sizeof(int));
+        static jl_lds_limit_flags raised;
+        const int st = jl_raise_lds_limit(raised, ctx->device, (const void *)jl_kv_plan_kernel<THREADS, ITEMS>, 4 * THREADS * ITEMS * (int)sizeof(int));
         if (st != JL_OK) return st;
     }
-    if (rows) {
-        hipLaunchKernelGGL((jl_kv_plan_kernel<THREADS, ITEMS, true>), dim3(1), dim3(THREADS), lds, ctx->stream, p);
-    } else {
-        hipLaunchKernelGGL((jl_kv_plan_kernel<THREADS, ITEMS, false>), dim3(1), dim3(THREADS), lds, ctx->stream, p);
-        JL_HIP(hipGetLastError());
-        hipLaunchKernelGGL(jl_kv_plan_rows_kernel, dim3((unsigned)((p.max_rows + 255) / 256)), dim3(256), std::max(4 * p.requests, 16), ctx->stream, p);
-    }
+    const bool in_place = p.lengths == p.past || p.free_out == p.free_in;
+    const int groups = in_place && p.max_rows <= kPlanRowsInPlace
+                           ? 1
+                           : std::min(std::max(p.max_rows / kPlanRowsEach, (p.requests - 1) / kPlanRequestsEach) + 1, kPlanMostGroups);
+    // (several workgroups: none may write what another one has yet to read)
+    const bool two = in_place && groups > 1;
+    p.parts = two ? kPlanMoves : kPlanMoves | kPlanLengths;
+    hipLaunchKernelGGL((jl_kv_plan_kernel<THREADS, ITEMS>), dim3((unsigned)groups), dim3(THREADS), lds, ctx->stream, p);
     JL_HIP(hipGetLastError());
+    if (two) {
+        p.parts = kPlanLengths;
+        hipLaunchKernelGGL((jl_kv_plan_kernel<THREADS, ITEMS>), dim3(1), dim3(THREADS), lds, ctx->stream, p);
+        JL_HIP(hipGetLastError());
+    }
     return JL_OK;
 }
 

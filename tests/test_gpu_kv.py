@@ -155,11 +155,11 @@ def test_plan_of_no_requests(ctx):
     assert t.slots.get().tolist() == t.positions.get().tolist() == t.rowRequests.get().tolist() == [-1] * 6
 
 
-def test_plan_many_steps_lose_no_page(ctx):
+@pytest.mark.parametrize("requests,stride,page,pages,max_rows", [(40, 8, 16, 150, 400), (300, 8, 16, 1100, 5000)])
+def test_plan_many_steps_lose_no_page(ctx, requests, stride, page, pages, max_rows):
     """A server's life: requests begin, decode, wait, end; in place, step after step, against the sequential one."""
     from jitllm_amd.attention import BlockTables
     rng = np.random.default_rng(8)
-    requests, stride, page, pages, max_rows = 40, 8, 16, 150, 400
     t = BlockTables(ctx, requests, stride, pages, page, max_rows)
     state = {"lengths": np.zeros(requests, int), "table": np.full((requests, stride), -1), "pageRing": np.arange(pages), "freePages": np.array([0, pages])}
     for step in range(60):
