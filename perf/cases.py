@@ -3,8 +3,8 @@
 A pass is what a program runs between two of its own decisions: one projection, one token of a
 single-sequence decode, one token of every sequence of a batch, one chunk of a prompt.  It goes through
 the Python binding (``jitllm_amd.projections``) on a torch stream, eagerly, over weights that lie on the
-device as GGUF blocks; attention is not part of the framework, so what attention would hand to a
-layer's output projection is an input.  ``listed()`` names the cases, ``draw()`` gives more of the same
+device as GGUF blocks; attention is not part of these passes (perf/operators.py has it), so what it would
+hand to a layer's output projection is an input.  ``listed()`` names the cases, ``draw()`` gives more of the same
 ranges: the same four kinds of pass over model-like widths, row counts from 1 to 2048 and weight types
 as files hold them.
 
