@@ -469,6 +469,7 @@ int jl_kv_cache_create(jl_context *ctx, int kv_type, int64_t pages, int kv_heads
 /* The same over jl_kv_cache_bytes(...) bytes of device memory that the caller owns, 16-byte aligned. */
 int jl_kv_cache_wrap(jl_context *ctx, void *device_memory, int kv_type, int64_t pages, int kv_heads, int head_dim,
                      int page_tokens, jl_kv_cache **out);
+/* Before the context that it was made with is destroyed; other contexts of that device may use it too. */
 int jl_kv_cache_free(jl_kv_cache *cache);
 void *jl_kv_cache_memory(const jl_kv_cache *cache);
 
