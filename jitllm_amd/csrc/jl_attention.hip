@@ -20,9 +20,13 @@
 // launch's workgroups whatever the rows' lengths are; a workgroup's four waves take a span's tiles in turn and
 // join in LDS.  A head that a cut goes through leaves its parts in the workspace, and the workgroup that is done last
 // with it joins them, in their order whoever that is (nobody waits for anybody).
+//
+// Rows of one request (a prompt's, a draft's) go through its pages together where there are more rows than requests: 16
+// columns of the matrix instructions are the query heads of one row after the other, each with its own mask.
 #include <algorithm>
 #include <climits>
 #include <cmath>
+#include <type_traits>
 
 #include "jl_kv.h"
 
@@ -67,6 +71,7 @@ struct AttentionArgs {
     int window;           // 0: none
     int group;            // query heads to a head of k and v
     int blocks_of_16;     // ... in sixteens
+    int rows_each;        // of one request that go together: a power of two, at most 16 / group; 1: each alone
     int rows;
     void *out;
     bool out_f16;
@@ -76,16 +81,78 @@ struct AttentionArgs {
 
 // The tokens [first, end) of its request that a row sees.
 struct Range {
-    int first, end, request;
+    int first, end, request, members = 1;
     __device__ int tiles() const { return end > first ? (end + kTile - 1) / kTile - first / kTile : 0; }
 };
-__device__ __forceinline__ Range range_of(const AttentionArgs &p, int row) {
-    const int position = p.positions[row];
+__device__ __forceinline__ Range range_at(const AttentionArgs &p, int position, int request) {
     Range r;
-    r.request = p.row_requests ? p.row_requests[row] : row;
+    r.request = request;
     r.end = position >= 0 && r.request >= 0 && r.request < p.requests ? min(position, p.table_tokens - 1) + 1 : 0;
     r.first = p.window > 0 ? max(position - p.window + 1, 0) : 0;
     return r;
+}
+
+__device__ __forceinline__ Range range_of(const AttentionArgs &p, int row) {
+    return range_at(p, p.positions[row], p.row_requests ? p.row_requests[row] : row);
+}
+
+// Rows that go together (SHARED): a run of one request's among rows_each rows that begin at a multiple of it.  The first of
+// a run has what its members see, all together; the others have nothing.
+__device__ __forceinline__ void join_ranges(Range &r, const Range &next) {
+    if (next.end > next.first) {
+        const bool any = r.end > r.first;
+        r.first = any ? min(r.first, next.first) : next.first;
+        r.end = any ? max(r.end, next.end) : next.end;
+    }
+    r.members += next.members;
+}
+// Of the row in every lane; sixteen lanes' first one has a row at such a multiple.
+__device__ __forceinline__ Range run_in_lanes(const AttentionArgs &p, Range r, int row, int lane) {
+    const int request = row < p.rows ? r.request : INT_MIN, in_block = lane & (p.rows_each - 1);
+#define JL_ROW_SHL(X, N) __builtin_amdgcn_update_dpp(0, X, 0x100 + N, 0xF, 0xF, true)     // from N lanes on, of sixteen
+#define JL_JOIN_FROM(N)                                                                                                        \
+    if (N < p.rows_each) {                                                                                                     \
+        Range other{JL_ROW_SHL(r.first, N), JL_ROW_SHL(r.end, N), 0, JL_ROW_SHL(r.members, N)};                                \
+        const int its = JL_ROW_SHL(request, N);                                                                                \
+        if (r.members == N && in_block + N < p.rows_each && its == request) join_ranges(r, other);                             \
+    }
+    const int before = __builtin_amdgcn_update_dpp(0, request, 0x111, 0xF, 0xF, true);
+    JL_JOIN_FROM(1)
+    JL_JOIN_FROM(2)
+    JL_JOIN_FROM(4)
+    JL_JOIN_FROM(8)
+#undef JL_JOIN_FROM
+#undef JL_ROW_SHL
+    if ((in_block != 0 && before == request) || row >= p.rows) r.end = 0;
+    return r;
+}
+// Calls work(row, range) for the runs that begin at rows begin ... end - 1, in order, until it returns false; `begin` is at
+// such a multiple.
+template <bool SHARED, typename WORK>
+__device__ __forceinline__ void for_runs(const AttentionArgs &p, int begin, int end, WORK work) {
+    if constexpr (!SHARED) {
+        for (int r = begin; r < end; r++)
+            if (!work(r, range_of(p, r))) return;
+    } else {
+        Range run;
+        int first_row = -1;
+        for (int r = begin; r < end; r += 4) {
+            Range four[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) four[j] = range_of(p, min(r + j, p.rows - 1));
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                if (r + j >= end) break;
+                if (first_row >= 0 && ((r + j) & (p.rows_each - 1)) && four[j].request == run.request) {
+                    join_ranges(run, four[j]);
+                    continue;
+                }
+                if (first_row >= 0 && !work(first_row, run)) return;
+                first_row = r + j, run = four[j];
+            }
+        }
+        if (first_row >= 0) work(first_row, run);
+    }
 }
 
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
@@ -102,9 +169,11 @@ __device__ __forceinline__ void agent_store4(float *to, floatx4 v) {
 }
 // k and v pass once: loads that do not stay in the caches (512 MB in 16 KB pieces, nothing else done: 90 us with ordinary
 // loads, 80 with these).
-template <typename T>
+// Where rows of one request follow each other over the same pages, theirs stay.
+template <typename T, bool STAY>
 __device__ __forceinline__ T load_at(const uint8_t *base, uint32_t offset) {
-    return __builtin_nontemporal_load((const T *)(base + offset));
+    if constexpr (STAY) return *(const T *)(base + offset);
+    else return __builtin_nontemporal_load((const T *)(base + offset));
 }
 __device__ __forceinline__ jl_half2v as_half2(uint32_t x) { return __builtin_bit_cast(jl_half2v, x); }
 __device__ __forceinline__ uint32_t as_u32(jl_half2v x) { return __builtin_bit_cast(uint32_t, x); }
@@ -134,18 +203,20 @@ struct Raw<false, DIM> {
     uint32_t v1[kHalves][4];
     __device__ static int element(int step, int g) { return 32 * step + 8 * g; }   // first of the eight of k step `step`
     __device__ static constexpr int in_eight(int i) { return i; }                  // ... and their order
+    template <bool STAY>
     __device__ void load_k(int half, const uint8_t *part, int in_page, int, int g, int m) {
 #pragma unroll
-        for (int s = 0; s < kSteps; s++) k[half][s] = load_at<uintx4>(part, (in_page + m) * (2 * DIM) + 64 * s + 16 * g);
+        for (int s = 0; s < kSteps; s++) k[half][s] = load_at<uintx4, STAY>(part, (in_page + m) * (2 * DIM) + 64 * s + 16 * g);
     }
+    template <bool STAY>
     __device__ void load_v(int half, const uint8_t *part, int in_page, int, int g, int m) {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const uint32_t row = (in_page + 4 * g + i) * (2 * DIM);
 #pragma unroll
-            for (int w = 0; w < kWide; w++) v4[half][i][w] = load_at<uintx4>(part, row + 256 * w + 16 * m);
-            if constexpr (kMid) v2[half][i] = load_at<uintx2>(part, row + 256 * kWide + 8 * m);
-            if constexpr (kThin) v1[half][i] = load_at<uint32_t>(part, row + 256 * kWide + 128 * kMid + 4 * m);
+            for (int w = 0; w < kWide; w++) v4[half][i][w] = load_at<uintx4, STAY>(part, row + 256 * w + 16 * m);
+            if constexpr (kMid) v2[half][i] = load_at<uintx2, STAY>(part, row + 256 * kWide + 8 * m);
+            if constexpr (kThin) v1[half][i] = load_at<uint32_t, STAY>(part, row + 256 * kWide + 128 * kMid + 4 * m);
         }
     }
     __device__ jl_half8 k_operand(int half, int step) const { return __builtin_bit_cast(jl_half8, k[half][step]); }
@@ -198,32 +269,34 @@ struct Raw<true, DIM> {
     }
     // (0, 2), (1, 3), (4, 6), (5, 7): the pairs that one operation takes out of a word
     __device__ static constexpr int in_eight(int i) { return i / 4 * 4 + i % 4 / 2 + i % 2 * 2; }
+    template <bool STAY>
     __device__ void load_k(int half, const uint8_t *part, int in_page, int page_shift, int g, int m) {
         const uint32_t row = (in_page + m) * DIM, scales = ((uint32_t)DIM << page_shift) + 2 * (in_page + m);
 #pragma unroll
         for (int i = 0; i < kPairs; i++) {
-            k[half][i] = load_at<uintx4>(part, row + 64 * i + 16 * g);
-            k_scale[half][i] = load_at<uint16_t>(part, scales + ((2 * (2 * i + g / 2)) << page_shift));
+            k[half][i] = load_at<uintx4, STAY>(part, row + 64 * i + 16 * g);
+            k_scale[half][i] = load_at<uint16_t, STAY>(part, scales + ((2 * (2 * i + g / 2)) << page_shift));
         }
         if constexpr (kTail) {
-            k_tail[half] = load_at<uintx2>(part, row + 64 * kPairs + 8 * g);
-            k_scale[half][kPairs] = load_at<uint16_t>(part, scales + ((2 * 2 * kPairs) << page_shift));
+            k_tail[half] = load_at<uintx2, STAY>(part, row + 64 * kPairs + 8 * g);
+            k_scale[half][kPairs] = load_at<uint16_t, STAY>(part, scales + ((2 * 2 * kPairs) << page_shift));
         }
     }
+    template <bool STAY>
     __device__ void load_v(int half, const uint8_t *part, int in_page, int page_shift, int g, int m) {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const uint32_t row = (in_page + 4 * g + i) * DIM;
 #pragma unroll
-            for (int w = 0; w < kWide; w++) v2[half][i][w] = load_at<uintx2>(part, row + 128 * w + 8 * m);
-            if constexpr (kMid) v1[half][i] = load_at<uint32_t>(part, row + 128 * kWide + 4 * m);
-            if constexpr (kThin) v0[half][i] = load_at<uint16_t>(part, row + 128 * kWide + 64 * kMid + 2 * m);
+            for (int w = 0; w < kWide; w++) v2[half][i][w] = load_at<uintx2, STAY>(part, row + 128 * w + 8 * m);
+            if constexpr (kMid) v1[half][i] = load_at<uint32_t, STAY>(part, row + 128 * kWide + 4 * m);
+            if constexpr (kThin) v0[half][i] = load_at<uint16_t, STAY>(part, row + 128 * kWide + 64 * kMid + 2 * m);
         }
         const uint32_t scales = ((uint32_t)DIM << page_shift) + 2 * (in_page + 4 * g);
 #pragma unroll
-        for (int w = 0; w < kWide; w++) v_scale[half][w] = load_at<uintx2>(part, scales + ((2 * (4 * w + m / 4)) << page_shift));
-        if constexpr (kMid) v_scale[half][kWide] = load_at<uintx2>(part, scales + ((2 * (4 * kWide + m / 8)) << page_shift));
-        if constexpr (kThin) v_scale[half][kWide + kMid] = load_at<uintx2>(part, scales + ((2 * (4 * kWide + 2 * kMid)) << page_shift));
+        for (int w = 0; w < kWide; w++) v_scale[half][w] = load_at<uintx2, STAY>(part, scales + ((2 * (4 * w + m / 4)) << page_shift));
+        if constexpr (kMid) v_scale[half][kWide] = load_at<uintx2, STAY>(part, scales + ((2 * (4 * kWide + m / 8)) << page_shift));
+        if constexpr (kThin) v_scale[half][kWide + kMid] = load_at<uintx2, STAY>(part, scales + ((2 * (4 * kWide + 2 * kMid)) << page_shift));
     }
     __device__ jl_half8 k_operand(int half, int step) const {
         uint32_t lo, hi;
@@ -297,17 +370,18 @@ __device__ __forceinline__ uint32_t units_of(int tiles) { return tiles > 0 ? til
 // A piece of a workgroup's list: tiles tile ... tile + count - 1 of a row's head, and what the row sees.
 struct Piece {
     int row, head, tile, count, tiles;
-    int first, end, request;
+    int first, end, request, members;
     int unit;         // where the piece begins in its head
     uint32_t left;    // units of the span, this piece's included; 0: no such piece
 };
 
 // A head that the workgroup has one of several parts of: those of spans group ... group + parts - 1.
 struct Cut {
-    int row, kv_head, block_of_16, group, parts;
+    int row, members, kv_head, block_of_16, group, parts;
 };
 
-template <bool Q8, int DIM>
+// SHARED: rows of one request go through the tiles together, a (row, query head) a column.
+template <bool Q8, int DIM, bool SHARED>
 __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_attention_kernel(AttentionArgs p) {
     constexpr int kSteps = DIM / 32, kBlocks = DIM / 16;
     constexpr int kRound = DIM == 256 ? 128 : DIM;            // elements that are joined at a time: 64 KB of LDS at most
@@ -315,7 +389,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
     constexpr int kSlot = 16 * (DIM + 2);
     __shared__ float joined[kWaves][16][kStride];
     __shared__ float joined_max[kWaves][16], joined_sum[kWaves][16];
-    __shared__ uint32_t scan[kWaves], scan_longest[kWaves], start_units, arrived[2];
+    __shared__ uint32_t scan[kWaves], scan_longest[kWaves], scan_dealt[kWaves], start_units, arrived[2];
     __shared__ int start_row;
     const int tid = threadIdx.x, lane = tid % JL_WAVE, wave = uniform(tid / JL_WAVE);
     const int g = lane / 16, m = lane % 16;
@@ -325,9 +399,12 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
     // ---- the rows' ranges, 64 at a time in the lanes of every wave
     int window_row = 0;
     Range in_lane;
+    int own_tiles = 0;                                        // without those of rows that go with the lane's
     auto load_window = [&](int from) {
         window_row = from;
         in_lane = from + lane < p.rows ? range_of(p, from + lane) : Range{0, 0, 0};
+        own_tiles = in_lane.tiles();
+        if constexpr (SHARED) in_lane = run_in_lanes(p, in_lane, from + lane, lane);
     };
 
     // ---- this workgroup's share of the list: whole (row, head) pairs one after the other where all rows are short, else
@@ -335,15 +412,24 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
     load_window(0);
     const uint32_t mine = units_of(in_lane.tiles());
     uint32_t all, through = mine;                             // tiles of all rows; of those up to this lane's (this thread's last)
-    uint32_t longest = mine, own = mine;
-    const int per = (p.rows + kThreads - 1) / kThreads;       // rows a thread, where a wave does not hold them all
+    uint32_t longest = mine, own = mine, longest_dealt = mine;   // ... of what is dealt whole
+    int per = (p.rows + kThreads - 1) / kThreads;             // rows a thread, where a wave does not hold them all
+    if constexpr (SHARED) per = (per + p.rows_each - 1) & -p.rows_each;
+    if constexpr (SHARED)
+        for (int off = 1; off < p.rows_each; off <<= 1) longest_dealt += __shfl_xor(longest_dealt, off, JL_WAVE);
     if (p.rows > JL_WAVE) {
-        own = longest = 0;
-        for (int r = tid * per; r < min((tid + 1) * per, p.rows); r++) {
-            const uint32_t n = units_of(range_of(p, r).tiles());
+        uint32_t dealt = 0;
+        own = longest = longest_dealt = 0;
+        for_runs<SHARED>(p, tid * per, min((tid + 1) * per, p.rows), [&](int r, const Range &range) {
+            const uint32_t n = units_of(range.tiles());
             own += n;
             longest = max(longest, n);
-        }
+            if constexpr (SHARED) {
+                dealt = (r & (p.rows_each - 1)) ? dealt + n : n;
+                longest_dealt = max(longest_dealt, dealt);
+            }
+            return true;
+        });
         through = own;
     }
 #pragma unroll
@@ -352,24 +438,33 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
         if (lane >= off) through += other;
     }
 #pragma unroll
-    for (int off = JL_WAVE / 2; off; off >>= 1) longest = max(longest, (uint32_t)__shfl_xor(longest, off, JL_WAVE));
+    for (int off = JL_WAVE / 2; off; off >>= 1) {
+        longest = max(longest, (uint32_t)__shfl_xor(longest, off, JL_WAVE));
+        if constexpr (SHARED) longest_dealt = max(longest_dealt, (uint32_t)__shfl_xor(longest_dealt, off, JL_WAVE));
+    }
     all = __builtin_amdgcn_readlane(through, JL_WAVE - 1);
     if (p.rows > JL_WAVE) {
-        if (lane == 0) scan[wave] = all, scan_longest[wave] = longest;
+        if (lane == 0) scan[wave] = all, scan_longest[wave] = longest, scan_dealt[wave] = longest_dealt;
         __syncthreads();
         all = 0;
         for (int w = 0; w < kWaves; w++) {
             if (w < wave) through += scan[w];
             all += scan[w];
             longest = max(longest, scan_longest[w]);
+            if constexpr (SHARED) longest_dealt = max(longest_dealt, scan_dealt[w]);
         }
     }
-    all = uniform(all), longest = uniform(longest);
+    all = uniform(all), longest = uniform(longest), longest_dealt = uniform(longest_dealt);
     // Pairs are not cut where a workgroup is done with its whole ones in the time that all take to read anyway, or in what
     // joining parts takes besides, ten tiles' worth.  (32 rows of 8 heads, 1000 tokens each: 27.8 us whole, 31.6 cut; 8 heads
     // of 1000 tokens: 20.2 whole, 10.2 cut; of 256 tokens: 9.1 and 9.7.)
-    const float rounds = ceilf((float)p.rows * heads / gridDim.x);
-    const bool whole = ((float)longest * rounds - kStart - 10) * Shape<Q8, DIM>::kTilesAtOnce <= (float)all * heads;
+    // (Rows that go together: what is dealt whole is rows_each rows, whose runs come one after the other.)
+    const int each = SHARED ? p.rows_each : 1;
+    const float rounds = ceilf((float)((p.rows + each - 1) / each) * heads / gridDim.x);
+    // Rows that go together read from the caches: whole where that is at most twice an equal span (2048 tokens, 32 heads over 8
+    // of 64: 118 us whole, 203 cut).
+    const bool whole = SHARED ? ((float)longest_dealt * rounds - kStart - 10) * gridDim.x <= 2.f * (float)all * heads
+                              : ((float)longest * rounds - kStart - 10) * Shape<Q8, DIM>::kTilesAtOnce <= (float)all * heads;
     const uint32_t total = all * heads;
     const uint32_t least = max((longest + kMostParts - 1) / kMostParts, min((longest + kParts - 1) / kParts, kLargePart));
     const uint32_t span = max((total + gridDim.x - 1) / gridDim.x, least);
@@ -378,17 +473,23 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
         const uint32_t from = begin / heads;
         if (!whole && begin < total && from >= through - own && from < through) {
             uint32_t before = through - own;
-            int r = tid * per;
-            for (uint32_t n; before + (n = units_of(range_of(p, r).tiles())) <= from; r++) before += n;
-            start_row = r, start_units = before;
+            for_runs<SHARED>(p, tid * per, min((tid + 1) * per, p.rows), [&](int r, const Range &range) {
+                const uint32_t n = units_of(range.tiles());
+                if (before + n > from) {
+                    start_row = r, start_units = before;
+                    return false;
+                }
+                before += n;
+                return true;
+            });
         }
         __syncthreads();
     }
 
-    // rows with nothing to read
+    // rows with nothing to read (one that goes with others is zeros from them too)
     const int width = p.cache.kv_heads * p.group * DIM;
     for (int r = blockIdx.x; r < p.rows; r += gridDim.x) {
-        const int n = p.rows <= JL_WAVE ? __builtin_amdgcn_readlane(in_lane.tiles(), r) : range_of(p, r).tiles();
+        const int n = p.rows <= JL_WAVE ? __builtin_amdgcn_readlane(own_tiles, r) : range_of(p, r).tiles();
         if (n == 0)
             for (int c = 4 * tid; c < width; c += 4 * kThreads) store_out(p, r * p.ldo + c, floatx4{0.f, 0.f, 0.f, 0.f});
     }
@@ -396,7 +497,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
     const int row_step = gridDim.x / heads, head_step = gridDim.x % heads;    // from one whole pair of a workgroup to its next
     Piece next;
     if (whole) {
-        next.row = blockIdx.x / heads, next.head = blockIdx.x % heads, next.unit = 0;
+        next.row = blockIdx.x / heads * each, next.head = blockIdx.x % heads, next.unit = 0;
         next.left = 1;
     } else {
         if (begin >= total) return;
@@ -412,6 +513,14 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
         next.unit = -1;
         next.left = min(span, total - begin);
     }
+    auto next_whole = [&]() {
+        if ((next.row + 1) & (each - 1)) {
+            next.row++;
+        } else {
+            next.row = (next.row & -each) + row_step * each, next.head += head_step;
+            if (next.head >= heads) next.head -= heads, next.row += each;
+        }
+    };
     // Completes `next` from its row, head and tile, going on to the first row that has tiles.
     auto complete = [&]() {
         next.row = uniform(next.row), next.head = uniform(next.head), next.unit = uniform(next.unit), next.left = uniform(next.left);
@@ -420,19 +529,16 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
                 next.left = 0;
                 break;
             }
-            if (next.row < window_row || next.row >= window_row + JL_WAVE) load_window(next.row);
+            if (next.row < window_row || next.row >= window_row + JL_WAVE) load_window(SHARED ? next.row & -16 : next.row);
             const int at = uniform(next.row - window_row);
             next.first = __builtin_amdgcn_readlane(in_lane.first, at);
             next.end = __builtin_amdgcn_readlane(in_lane.end, at);
             next.request = __builtin_amdgcn_readlane(in_lane.request, at);
+            next.members = SHARED ? __builtin_amdgcn_readlane(in_lane.members, at) : 1;
             next.tiles = Range{next.first, next.end, 0}.tiles();
             if (next.tiles > 0) break;
-            if (whole) {
-                next.row += row_step, next.head += head_step;
-                if (next.head >= heads) next.head -= heads, next.row++;
-            } else {
-                next.row++;
-            }
+            if (whole) next_whole();
+            else next.row++;
         }
         if (next.unit < 0 && next.left > 0) {
             const int into = next.head, units = units_of(next.tiles);
@@ -461,7 +567,8 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
             page[h] = token < c.end ? table[token >> page_shift] : -1;
         }
     };
-    auto issue = [&](int kv_head, int t, bool values) {
+    auto issue_as = [&](auto stay, int kv_head, int t, bool values) {
+        constexpr bool STAY = decltype(stay)::value;
         if (values) paged = 0;
 #pragma unroll
         for (int h = 0; h < kHalves; h++) {
@@ -469,12 +576,16 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
             const uint8_t *part = p.cache.k + ((int64_t)(real ? page[h] : 0) * p.cache.kv_heads + kv_head) * p.cache.part_bytes;
             const int in_page = (t * kTile + 16 * h) & in_page_mask;
             if (values) {
-                raw.load_v(h, part + p.cache.v_offset, in_page, page_shift, g, m);
+                raw.template load_v<STAY>(h, part + p.cache.v_offset, in_page, page_shift, g, m);
                 paged |= real ? 1u << h : 0u;
             } else {
-                raw.load_k(h, part, in_page, page_shift, g, m);
+                raw.template load_k<STAY>(h, part, in_page, page_shift, g, m);
             }
         }
+    };
+    auto issue = [&](const Piece &c, int kv_head, int t, bool values) {
+        if (SHARED && c.members > 1) issue_as(std::true_type{}, kv_head, t, values);
+        else issue_as(std::false_type{}, kv_head, t, values);
     };
     const bool one_block = p.blocks_of_16 == 1;
     auto kv_head_of = [&](int head) { return one_block ? head : head / p.blocks_of_16; };
@@ -490,9 +601,8 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
         // the piece behind this one: the loads of its first tiles go out with this one's last
         next.left = whole ? 1 : next.left - min(next.left, units_of(cur.tiles) - cur.unit);
         next.unit = 0;
-        if (whole) next.row += row_step, next.head += head_step;
-        else next.head++;
-        if (next.head >= heads) next.head -= heads, next.row++;
+        if (whole) next_whole();
+        else if (++next.head >= heads) next.head -= heads, next.row++;
         complete();
         const int count = cur.count, row = cur.row;
         if (count == 0) continue;
@@ -505,11 +615,18 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
         const bool here = from_tile < last, there = !here && next.left > 0 && next_tile < next_last;
         if (here ? !loaded : there) {
             find_pages(here ? cur : next, here ? from_tile : next_tile);
-            issue(here ? kv_head : next_head, here ? from_tile : next_tile, false);
-            issue(here ? kv_head : next_head, here ? from_tile : next_tile, true);
+            issue(here ? cur : next, here ? kv_head : next_head, here ? from_tile : next_tile, false);
+            issue(here ? cur : next, here ? kv_head : next_head, here ? from_tile : next_tile, true);
         }
         loaded = there;
-        const int q_head = kv_head * p.group + 16 * block_of_16, q_heads = min(p.group - 16 * block_of_16, 16);
+        // columns: query heads of a row, or of one row after the other
+        const int q_head = kv_head * p.group + 16 * block_of_16, q_heads = SHARED ? cur.members * p.group : min(p.group - 16 * block_of_16, 16);
+        int row_of_lane = row, head_of_lane = m < q_heads ? m : 0;
+        int position = 0;
+        if constexpr (SHARED) {
+            row_of_lane += head_of_lane / p.group, head_of_lane %= p.group;
+            position = p.positions[row_of_lane];
+        }
 
         // ---- q, times a power of two that brings its largest value to 2^10 ... 2^11: both parts are then binary16
         // numbers of full precision however large or small the row is
@@ -517,7 +634,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
         float undo;
         {
             floatx4 x[kSteps][2];
-            const float *from = p.q + row * p.ldq + (q_head + (m < q_heads ? m : 0)) * DIM;
+            const float *from = p.q + row_of_lane * p.ldq + (q_head + head_of_lane) * DIM;
             float most = 0.f;
 #pragma unroll
             for (int s = 0; s < kSteps; s++)
@@ -542,6 +659,17 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
                     q_hi[s][i] = (_Float16)y;
                     q_lo[s][i] = (_Float16)(y - (float)q_hi[s][i]);
                 }
+        }
+
+        Range seen_here{cur.first, cur.end, 0}, seen_by_all = seen_here;      // what the lane's row sees, what all of them do
+        if constexpr (SHARED) {
+            seen_here = range_at(p, position, cur.request), seen_by_all = seen_here;
+#define JL_SEEN_FROM(N)                                                                                                        \
+    seen_by_all.first = max(seen_by_all.first, __builtin_amdgcn_update_dpp(0, seen_by_all.first, 0x120 + N, 0xF, 0xF, true));  \
+    seen_by_all.end = min(seen_by_all.end, __builtin_amdgcn_update_dpp(0, seen_by_all.end, 0x120 + N, 0xF, 0xF, true));
+            JL_SEEN_FROM(8) JL_SEEN_FROM(4) JL_SEEN_FROM(2) JL_SEEN_FROM(1)   // (round the sixteen lanes)
+#undef JL_SEEN_FROM
+            seen_by_all.first = uniform(seen_by_all.first), seen_by_all.end = uniform(seen_by_all.end);
         }
 
         floatx4 o[kBlocks];
@@ -575,8 +703,8 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
 #pragma unroll
                 for (int h = 0; h < kHalves; h++) s[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[h], q_hi[i], s[h], 0, 0, 0);
             }
-            if (loaded) issue(load_head, load_tile, false);   // k goes out as soon as this tile's is used
-            const bool all_seen = t * kTile >= cur.first && t * kTile + kTile <= cur.end && with_page == (1u << kHalves) - 1;
+            if (loaded) issue(more ? cur : next, load_head, load_tile, false);   // k goes out as soon as this tile's is used
+            const bool all_seen = t * kTile >= seen_by_all.first && t * kTile + kTile <= seen_by_all.end && with_page == (1u << kHalves) - 1;
             float x[8];
 #pragma unroll
             for (int i = 0; i < 8; i++) x[i] = s[i / 4][i % 4];
@@ -586,7 +714,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
                 for (int i = 0; i < 8; i++) {
                     const int token = t * kTile + 16 * (i / 4) + 4 * g + i % 4;
                     seen[i / 4][i % 4] = token >= cur.first && token < cur.end && (with_page >> (i / 4) & 1);
-                    x[i] = seen[i / 4][i % 4] ? x[i] : -INFINITY;
+                    x[i] = seen[i / 4][i % 4] && (!SHARED || (token >= seen_here.first && token < seen_here.end)) ? x[i] : -INFINITY;
                 }
                 raw.mask_v(seen);
             }
@@ -624,7 +752,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
                 o[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[0], p_hi, o[b], 0, 0, 0);
                 o[b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[1], p_hi, o[b + 1], 0, 0, 0);
             }
-            if (loaded) issue(load_head, load_tile, true);
+            if (loaded) issue(more ? cur : next, load_head, load_tile, true);
         }
 
         // ---- the four waves' parts into one
@@ -633,7 +761,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
         const bool opens = cur.tile == 0, closes = cur.tile + count == cur.tiles;
         float *slot = p.parts + (int64_t)(2 * blockIdx.x + (opens ? 1 : 0)) * kSlot;
         auto finish = [&](int h, int d, floatx4 v, float l) {
-            store_out(p, row * p.ldo + (int64_t)(q_head + h) * DIM + d, l == 0.f ? floatx4{0.f, 0.f, 0.f, 0.f} : v / l);
+            store_out(p, (SHARED ? (row + h / p.group) * p.ldo + (int64_t)(q_head + h % p.group) * DIM : row * p.ldo + (int64_t)(q_head + h) * DIM) + d, l == 0.f ? floatx4{0.f, 0.f, 0.f, 0.f} : v / l);
         };
 #pragma unroll
         for (int from = 0; from < DIM; from += kRound) {
@@ -667,7 +795,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
         if (!(opens && closes)) {
             const uint32_t head_begin = begin + min(span, total - begin) - cur.left - cur.unit;   // in the list of all units
             Cut &c = opens ? opened : went_on;
-            c.row = row, c.kv_head = kv_head, c.block_of_16 = block_of_16;
+            c.row = row, c.members = cur.members, c.kv_head = kv_head, c.block_of_16 = block_of_16;
             // the spans that have tiles of it: from the one of its first tile on
             c.group = (head_begin + kStart) / span, c.parts = (head_begin + kStart + cur.tiles - 1) / span - c.group + 1;
         }
@@ -693,7 +821,8 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
     for (int which = 0; which < 2; which++) {
         const Cut c = which ? opened : went_on;
         if (c.parts == 0 || arrived[which] != (uint32_t)c.parts) continue;
-        const int q_head = c.kv_head * p.group + 16 * c.block_of_16, q_heads = min(p.group - 16 * c.block_of_16, 16), parts = c.parts;
+        const int q_head = c.kv_head * p.group + 16 * c.block_of_16, parts = c.parts;
+        const int q_heads = SHARED ? c.members * p.group : min(p.group - 16 * c.block_of_16, 16);
         // (the parts were written past the second-level caches and are read past this XCD's own, which may hold an earlier
         // call's: buffer loads with the bit for that.  A fence would empty the cache for everybody: 40 us instead of 32 where
         // 256 heads are joined at once)
@@ -753,7 +882,9 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
                     const float keep = __builtin_amdgcn_exp2f(most - next_most), share = __builtin_amdgcn_exp2f(from[4] - next_most);
                     v = keep * v + share * *(const floatx4 *)from, l = keep * l + share * from[5], most = next_most;
                 }
-                store_out(p, c.row * p.ldo + (int64_t)q_head * DIM + 4 * at, l == 0.f ? floatx4{0.f, 0.f, 0.f, 0.f} : v / l);
+                const int64_t to = SHARED ? (c.row + h / p.group) * p.ldo + (int64_t)(q_head + h % p.group) * DIM + 4 * at - h * DIM
+                                          : c.row * p.ldo + (int64_t)q_head * DIM + 4 * at;
+                store_out(p, to, l == 0.f ? floatx4{0.f, 0.f, 0.f, 0.f} : v / l);
             }
         }
         __syncthreads();
@@ -763,7 +894,8 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
 template <bool Q8, int DIM>
 hipError_t launch(const AttentionArgs &a, int compute_units, hipStream_t stream) {
     const int groups = std::min(Shape<Q8, DIM>::kPerUnit * compute_units, kMostGroups);
-    hipLaunchKernelGGL((jl_kv_attention_kernel<Q8, DIM>), dim3((unsigned)groups), dim3(kThreads), 0, stream, a);
+    if (a.rows_each > 1) hipLaunchKernelGGL((jl_kv_attention_kernel<Q8, DIM, true>), dim3((unsigned)groups), dim3(kThreads), 0, stream, a);
+    else hipLaunchKernelGGL((jl_kv_attention_kernel<Q8, DIM, false>), dim3((unsigned)groups), dim3(kThreads), 0, stream, a);
     return hipGetLastError();
 }
 template <bool Q8>
@@ -843,6 +975,12 @@ int jl_kv_attention(jl_context *ctx, const jl_kv_cache *cache, const float *q, i
     a.window = window > INT32_MAX ? 0 : (int)window;   // one that reaches behind every position
     a.group = heads / cache->kv_heads;
     a.blocks_of_16 = (a.group + 15) / 16;
+    // More rows than requests: some are of one.  (32 heads over 8 of 128, one request, each row alone and together: a prompt of
+    // 2048 tokens 755 and 186 us, of 512 64 and 27; 4 rows after 30 000 tokens 79 and 43, after 1000 11.7 and 13.8.  32 heads
+    // over 32, 512 tokens: 225 and 31.)
+    a.rows_each = 1;
+    if (row_requests && rows > requests)
+        while (2 * a.rows_each * a.group <= 16) a.rows_each *= 2;
     a.rows = (int)rows;
     a.out = out, a.out_f16 = out_f16 != 0;
     a.arrived = (uint32_t *)workspace;

@@ -462,6 +462,40 @@ def test_attend_rows_of_one_request(ctx):
     assert (got[-4:] == 0).all()
 
 
+SHARED = [
+    # rows of each request in turn, the requests, heads, kv, dim, page, q8, window, half
+    ([(0, 0, 40)], 1, 8, 2, 64, 16, False, 0, False), ([(0, 0, 300)], 1, 4, 4, 128, 32, False, 0, False), ([(0, 0, 130)], 1, 14, 2, 64, 64, True, 33, False),
+    ([(r, 50 * r, 4) for r in range(20)], 20, 16, 4, 128, 16, True, 0, True), ([(r % 3, 7 * r, 1 + r % 5) for r in range(30)], 3, 6, 2, 96, 16, False, 0, False),
+    ([(1, 900, 33), (0, 0, 1), (2, 5, 70), (-1, 3, 5), (3, 3, 3), (1, 10, 2)], 3, 8, 8, 192, 16, False, 100, False), ([(0, 1000, 3)], 1, 16, 2, 256, 128, True, 0, False),
+    ([(0, 0, 600), (1, 30, 500)], 2, 5, 1, 64, 16, False, 0, False), ([(0, 500, 17)], 1, 9, 1, 128, 16, False, 0, False), ([(0, 2900, 2), (1, 0, 65)], 2, 24, 8, 256, 16, False, 0, True)]
+
+
+@pytest.mark.parametrize("runs,requests,heads,kv,dim,page,q8,window,half", SHARED)
+def test_attend_rows_that_share_requests(ctx, runs, requests, heads, kv, dim, page, q8, window, half):
+    """Runs of rows of one request (request, first position, rows), as prompts and drafts have them, of odd lengths and
+    beside other requests', some without a token; and the rows of a run in another order."""
+    say("attend shared", runs[:6], heads, kv, dim, page, q8, window, half)
+    rng = np.random.default_rng(len(runs) + dim + heads)
+    requests_of = np.concatenate([np.full(n, r) for r, _, n in runs])
+    positions = np.concatenate([np.arange(first, first + n) for _, first, n in runs])
+    most = np.ones(requests, int)
+    real = (requests_of >= 0) & (requests_of < requests)
+    np.maximum.at(most, requests_of[real], positions[real] + 1)
+    table, pages = make_tables(rng, most, page)
+    raw = random_pool(rng, q8, pages, kv, dim, page)
+    cache = cache_of(ctx, q8, pages, kv, dim, page, raw)
+    pool = M.decode_pool(raw, q8, pages, kv, dim, page)
+    positions[rng.random(len(positions)) < 0.05] = -1
+    for turn in range(2):
+        q = (2 * rng.standard_normal((len(positions), heads, dim))).astype(np.float32)
+        got = run_attend(ctx, cache, q, positions, requests_of, table, window=window, half=half, pad=8)
+        want = M.attend(pool, q, positions, requests_of, table, dim ** -0.5, window)
+        check_attend(got, *want, np.maximum(np.minimum(positions + 1, window or 1 << 30), 0), dim, half)
+        assert (got[~real | (positions < 0)] == 0).all()
+        positions = positions[::-1].copy()
+        requests_of, real = requests_of[::-1].copy(), real[::-1].copy()
+
+
 @pytest.mark.parametrize("q8", [False, True])
 def test_attend_masked_places_have_no_influence(ctx, q8):
     """NaN and infinities behind a row's last token, before its window, and in pages of others."""
