@@ -547,7 +547,7 @@ int jl_kv_read(jl_context *ctx, const jl_kv_cache *cache, const int32_t *slots, 
  *   q    fp32 rows of heads x head_dim values, ldq floats apart (16-byte aligned, ldq a multiple of 4)
  *   row_requests [rows]: the row of the block table that a row reads, or null: row i reads row i (and
  *        requests >= rows).  Rows of one request may stand beside each other (a prompt's, a draft's):
- *        each reads its own range.  Where there are more rows than requests, neighbours of one request
+ *        each reads its own range.  Where there are twice as many rows as requests, neighbours of one request
  *        go through its pages together, as many as make up to 16 query heads of one head of k and v; an
  *        infinity or NaN that one of them reads may then leave NaN in those beside it, too.
  *   out  fp32, or with out_f16 binary16 (rounded once, as the projections of jl_gemm_xf16 take it);

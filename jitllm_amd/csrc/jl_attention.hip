@@ -21,12 +21,11 @@
 // join in LDS.  A head that a cut goes through leaves its parts in the workspace, and the workgroup that is done last
 // with it joins them, in their order whoever that is (nobody waits for anybody).
 //
-// Rows of one request (a prompt's, a draft's) go through its pages together where there are more rows than requests: 16
-// columns of the matrix instructions are the query heads of one row after the other, each with its own mask.
+// Rows of one request (a prompt's, a draft's) go through its pages together where there are twice as many rows as
+// requests: 16 columns of the matrix instructions are the query heads of one row after the other, each with its own mask.
 #include <algorithm>
 #include <climits>
 #include <cmath>
-#include <type_traits>
 
 #include "jl_kv.h"
 
@@ -567,8 +566,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
             page[h] = token < c.end ? table[token >> page_shift] : -1;
         }
     };
-    auto issue_as = [&](auto stay, int kv_head, int t, bool values) {
-        constexpr bool STAY = decltype(stay)::value;
+    auto issue = [&](int kv_head, int t, bool values) {
         if (values) paged = 0;
 #pragma unroll
         for (int h = 0; h < kHalves; h++) {
@@ -576,16 +574,12 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
             const uint8_t *part = p.cache.k + ((int64_t)(real ? page[h] : 0) * p.cache.kv_heads + kv_head) * p.cache.part_bytes;
             const int in_page = (t * kTile + 16 * h) & in_page_mask;
             if (values) {
-                raw.template load_v<STAY>(h, part + p.cache.v_offset, in_page, page_shift, g, m);
+                raw.template load_v<SHARED>(h, part + p.cache.v_offset, in_page, page_shift, g, m);
                 paged |= real ? 1u << h : 0u;
             } else {
-                raw.template load_k<STAY>(h, part, in_page, page_shift, g, m);
+                raw.template load_k<SHARED>(h, part, in_page, page_shift, g, m);
             }
         }
-    };
-    auto issue = [&](const Piece &c, int kv_head, int t, bool values) {
-        if (SHARED && c.members > 1) issue_as(std::true_type{}, kv_head, t, values);
-        else issue_as(std::false_type{}, kv_head, t, values);
     };
     const bool one_block = p.blocks_of_16 == 1;
     auto kv_head_of = [&](int head) { return one_block ? head : head / p.blocks_of_16; };
@@ -615,8 +609,8 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
         const bool here = from_tile < last, there = !here && next.left > 0 && next_tile < next_last;
         if (here ? !loaded : there) {
             find_pages(here ? cur : next, here ? from_tile : next_tile);
-            issue(here ? cur : next, here ? kv_head : next_head, here ? from_tile : next_tile, false);
-            issue(here ? cur : next, here ? kv_head : next_head, here ? from_tile : next_tile, true);
+            issue(here ? kv_head : next_head, here ? from_tile : next_tile, false);
+            issue(here ? kv_head : next_head, here ? from_tile : next_tile, true);
         }
         loaded = there;
         // columns: query heads of a row, or of one row after the other
@@ -703,7 +697,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
 #pragma unroll
                 for (int h = 0; h < kHalves; h++) s[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[h], q_hi[i], s[h], 0, 0, 0);
             }
-            if (loaded) issue(more ? cur : next, load_head, load_tile, false);   // k goes out as soon as this tile's is used
+            if (loaded) issue(load_head, load_tile, false);   // k goes out as soon as this tile's is used
             const bool all_seen = t * kTile >= seen_by_all.first && t * kTile + kTile <= seen_by_all.end && with_page == (1u << kHalves) - 1;
             float x[8];
 #pragma unroll
@@ -752,7 +746,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
                 o[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[0], p_hi, o[b], 0, 0, 0);
                 o[b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[1], p_hi, o[b + 1], 0, 0, 0);
             }
-            if (loaded) issue(more ? cur : next, load_head, load_tile, true);
+            if (loaded) issue(load_head, load_tile, true);
         }
 
         // ---- the four waves' parts into one
@@ -975,11 +969,12 @@ int jl_kv_attention(jl_context *ctx, const jl_kv_cache *cache, const float *q, i
     a.window = window > INT32_MAX ? 0 : (int)window;   // one that reaches behind every position
     a.group = heads / cache->kv_heads;
     a.blocks_of_16 = (a.group + 15) / 16;
-    // More rows than requests: some are of one.  (32 heads over 8 of 128, one request, each row alone and together: a prompt of
-    // 2048 tokens 755 and 186 us, of 512 64 and 27; 4 rows after 30 000 tokens 79 and 43, after 1000 11.7 and 13.8.  32 heads
-    // over 32, 512 tokens: 225 and 31.)
+    // Twice as many rows as requests, or more: some are of one, unless they are padding.  (32 heads over 8 of 128, one request,
+    // each row alone and together: a prompt of 2048 tokens 755 and 186 us, of 512 64 and 27; 4 rows after 30 000 tokens 79 and
+    // 43, after 1000 11.7 and 13.8.  32 heads over 32, 512 tokens: 225 and 31.  64 rows of 64 requests of up to 8192 tokens
+    // padded to 512 rows: 118 and 124; to 72, which are too few: 104 and 117.)
     a.rows_each = 1;
-    if (row_requests && rows > requests)
+    if (row_requests && rows >= 2 * requests)
         while (2 * a.rows_each * a.group <= 16) a.rows_each *= 2;
     a.rows = (int)rows;
     a.out = out, a.out_f16 = out_f16 != 0;
