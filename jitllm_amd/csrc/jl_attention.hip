@@ -515,7 +515,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
         next.left = min(span, total - begin);
     }
     auto next_whole = [&]() {
-        if ((next.row + 1) & (each - 1)) {
+        if (((next.row + 1) & (each - 1)) && next.row + 1 < p.rows) {
             next.row++;
         } else {
             next.row = (next.row & -each) + row_step * each, next.head += head_step;

@@ -405,7 +405,7 @@ ATTENDS = [
     ([4096], 16, 4, 256, 16, True, 1024, False), ([700, 40, 90], 16, 4, 256, 64, False, 100, False), ([333, 1, 77], 9, 3, 96, 16, True, 0, False),
     ([1300, 64], 3, 3, 96, 128, False, 1, False), ([260, 511], 24, 2, 192, 256, False, 0, True), ([900, 5], 12, 2, 192, 16, True, 17, False),
     ([2000, 7], 71, 1, 64, 32, False, 0, False), ([129], 48, 1, 128, 16, True, 0, True), ([9000], 32, 8, 128, 64, False, 0, False),
-    ([5000, 1, 300], 8, 8, 64, 16, True, 0, False)]
+    ([5000, 1, 300], 8, 8, 64, 16, True, 0, False), ([3, 0, 20, 17], 1200, 600, 64, 16, False, 0, False), ([40, 3], 300, 300, 256, 16, True, 0, False)]
 
 
 @pytest.mark.parametrize("lengths,heads,kv,dim,page,q8,window,half", ATTENDS)
@@ -467,7 +467,9 @@ SHARED = [
     ([(0, 0, 40)], 1, 8, 2, 64, 16, False, 0, False), ([(0, 0, 300)], 1, 4, 4, 128, 32, False, 0, False), ([(0, 0, 130)], 1, 14, 2, 64, 64, True, 33, False),
     ([(r, 50 * r, 4) for r in range(20)], 20, 16, 4, 128, 16, True, 0, True), ([(r % 3, 7 * r, 1 + r % 5) for r in range(30)], 3, 6, 2, 96, 16, False, 0, False),
     ([(1, 900, 33), (0, 0, 1), (2, 5, 70), (-1, 3, 5), (3, 3, 3), (1, 10, 2)], 3, 8, 8, 192, 16, False, 100, False), ([(0, 1000, 3)], 1, 16, 2, 256, 128, True, 0, False),
-    ([(0, 0, 600), (1, 30, 500)], 2, 5, 1, 64, 16, False, 0, False), ([(0, 500, 17)], 1, 9, 1, 128, 16, False, 0, False), ([(0, 2900, 2), (1, 0, 65)], 2, 24, 8, 256, 16, False, 0, True)]
+    ([(0, 0, 600), (1, 30, 500)], 2, 5, 1, 64, 16, False, 0, False), ([(0, 500, 17)], 1, 9, 1, 128, 16, False, 0, False), ([(0, 2900, 2), (1, 0, 65)], 2, 24, 8, 256, 16, False, 0, True),
+    # more heads than workgroups, rows that fill no block
+    ([(0, 20, 3)], 1, 300, 300, 256, 16, False, 0, False), ([(0, 3, 5), (1, 7, 2)], 2, 600, 600, 64, 16, True, 0, False)]
 
 
 @pytest.mark.parametrize("runs,requests,heads,kv,dim,page,q8,window,half", SHARED)
