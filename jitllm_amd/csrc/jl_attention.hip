@@ -80,7 +80,8 @@ struct AttentionArgs {
     int rows_each;
 };
 
-// The tokens [first, end) of its request that a row sees.
+// The tokens [first, end) of its request that a row sees.  A row without a position or a request has [0, -1), which touches no
+// other's.
 struct Range {
     int first, end, request, members = 1;
     __device__ int tiles() const { return end > first ? (end + kTile - 1) / kTile - first / kTile : 0; }
@@ -88,7 +89,7 @@ struct Range {
 __device__ __forceinline__ Range range_at(const AttentionArgs &p, int position, int request) {
     Range r;
     r.request = request;
-    r.end = position >= 0 && r.request >= 0 && r.request < p.requests ? min(position, p.table_tokens - 1) + 1 : 0;
+    r.end = position >= 0 && r.request >= 0 && r.request < p.requests ? min(position, p.table_tokens - 1) + 1 : -1;
     r.first = p.window > 0 ? max(position - p.window + 1, 0) : 0;
     return r;
 }
@@ -97,34 +98,35 @@ __device__ __forceinline__ Range range_of(const AttentionArgs &p, int row) {
     return range_at(p, p.positions[row], p.row_requests ? p.row_requests[row] : row);
 }
 
-// Rows that go together (SHARED): a run of one request's among rows_each rows that begin at a multiple of it.  The first of
-// a run has what its members see, all together; the others have nothing.
+// Rows that go together (SHARED): a run among rows_each rows that begin at a multiple of it, of one request's, each of which
+// has tokens in common with the one before it or begins or ends where that one does: what they see together is then one
+// range, and no token between two windows is read.  The first of a run has the range of all; the others have nothing.
+__device__ __forceinline__ bool goes_on(const Range &before, const Range &r) {
+    return before.request == r.request && max(before.first, r.first) <= min(before.end, r.end);
+}
 __device__ __forceinline__ void join_ranges(Range &r, const Range &next) {
-    if (next.end > next.first) {
-        const bool any = r.end > r.first;
-        r.first = any ? min(r.first, next.first) : next.first;
-        r.end = any ? max(r.end, next.end) : next.end;
-    }
+    r.first = min(r.first, next.first), r.end = max(r.end, next.end);
     r.members += next.members;
 }
-// Of the row in every lane; sixteen lanes' first one has a row at such a multiple.
-__device__ __forceinline__ Range run_in_lanes(const AttentionArgs &p, Range r, int row, int lane) {
-    const int request = row < p.rows ? r.request : INT_MIN, in_block = lane & (p.rows_each - 1);
-#define JL_ROW_SHL(X, N) __builtin_amdgcn_update_dpp(0, X, 0x100 + N, 0xF, 0xF, true)     // from N lanes on, of sixteen
+// Of the row in every lane (one behind the last row has nothing); sixteen lanes' first one has a row at such a multiple.
+__device__ __forceinline__ Range run_in_lanes(const AttentionArgs &p, Range r, int lane) {
+    const int in_block = lane & (p.rows_each - 1);
+#define JL_ROW(X, CONTROL) __builtin_amdgcn_update_dpp(0, X, CONTROL, 0xF, 0xF, true)
+    const Range before{JL_ROW(r.first, 0x111), JL_ROW(r.end, 0x111), JL_ROW(r.request, 0x111)};   // of the lane before, of sixteen
+    const int goes = in_block != 0 && goes_on(before, r);
 #define JL_JOIN_FROM(N)                                                                                                        \
     if (N < p.rows_each) {                                                                                                     \
-        Range other{JL_ROW_SHL(r.first, N), JL_ROW_SHL(r.end, N), 0, JL_ROW_SHL(r.members, N)};                                \
-        const int its = JL_ROW_SHL(request, N);                                                                                \
-        if (r.members == N && in_block + N < p.rows_each && its == request) join_ranges(r, other);                             \
+        const Range other{JL_ROW(r.first, 0x100 + N), JL_ROW(r.end, 0x100 + N), 0, JL_ROW(r.members, 0x100 + N)};              \
+        const int its = JL_ROW(goes, 0x100 + N);                                                                               \
+        if (r.members == N && in_block + N < p.rows_each && its) join_ranges(r, other);                                        \
     }
-    const int before = __builtin_amdgcn_update_dpp(0, request, 0x111, 0xF, 0xF, true);
     JL_JOIN_FROM(1)
     JL_JOIN_FROM(2)
     JL_JOIN_FROM(4)
     JL_JOIN_FROM(8)
 #undef JL_JOIN_FROM
-#undef JL_ROW_SHL
-    if ((in_block != 0 && before == request) || row >= p.rows) r.end = 0;
+#undef JL_ROW
+    if (goes) r.end = 0;
     return r;
 }
 // Calls work(row, range) for the runs that begin at rows begin ... end - 1, in order, until it returns false; `begin` is at
@@ -135,7 +137,7 @@ __device__ __forceinline__ void for_runs(const AttentionArgs &p, int begin, int 
         for (int r = begin; r < end; r++)
             if (!work(r, range_of(p, r))) return;
     } else {
-        Range run;
+        Range run, before;
         int first_row = -1;
         for (int r = begin; r < end; r += 4) {
             Range four[4];
@@ -144,7 +146,9 @@ __device__ __forceinline__ void for_runs(const AttentionArgs &p, int begin, int 
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 if (r + j >= end) break;
-                if (first_row >= 0 && ((r + j) & (p.rows_each - 1)) && four[j].request == run.request) {
+                const bool goes = first_row >= 0 && ((r + j) & (p.rows_each - 1)) && goes_on(before, four[j]);
+                before = four[j];
+                if (goes) {
                     join_ranges(run, four[j]);
                     continue;
                 }
@@ -403,9 +407,9 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
     int own_tiles = 0;                                        // without those of rows that go with the lane's
     auto load_window = [&](int from) {
         window_row = from;
-        in_lane = from + lane < p.rows ? range_of(p, from + lane) : Range{0, 0, 0};
+        in_lane = from + lane < p.rows ? range_of(p, from + lane) : Range{0, -1, 0};
         own_tiles = in_lane.tiles();
-        if constexpr (SHARED) in_lane = run_in_lanes(p, in_lane, from + lane, lane);
+        if constexpr (SHARED) in_lane = run_in_lanes(p, in_lane, lane);
     };
 
     // ---- this workgroup's share of the list: whole (row, head) pairs one after the other where all rows are short, else

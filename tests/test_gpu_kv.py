@@ -852,3 +852,47 @@ def test_attend_thousands_of_short_rows(ctx):
     got = run_attend(ctx, cache, q, lengths - 1, None, table)
     want = M.attend(M.decode_pool(raw, False, pages, 1, dim, page), q, lengths - 1, None, table, dim ** -0.5)
     check_attend(got, *want, lengths, dim)
+
+
+# ---- rows of one request that go together: what none of them, or only some, may see ---------------
+
+def poisoned(raw, q8, pages, kv, dim, page, at, which, bad, element=None):
+    """The cache's bytes with `bad` in k (0) or v (1) at slots `at`: everywhere, or at one element (a block's scale)."""
+    dirty = raw.copy().reshape(2, pages, kv, -1)
+    for slot in np.atleast_1d(at):
+        if q8:
+            scales = dirty[..., page * dim:].view(np.float16).reshape(2, pages, kv, dim // 32, page)
+            scales[which, slot // page, :, slice(None) if element is None else element // 32, slot % page] = bad
+            dirty[..., page * dim:] = scales.reshape(2, pages, kv, -1).view(np.uint8)
+        else:
+            dirty.view(np.float16).reshape(2, pages, kv, page, dim)[which, slot // page, :, slot % page, slice(None) if element is None else element] = bad
+    return dirty.reshape(-1)
+
+
+GAPS = [
+    # positions of one request's rows, window, heads, kv, dim, page
+    ([10, 1000], 16, 8, 2, 128, 16), ([700, 5, 701, 3000], 40, 8, 4, 64, 32), ([900, 899, 100, 101, 400, 2, 1, 0], 7, 6, 3, 96, 64),
+    ([50, 2000, 50, 2000, 50], 33, 4, 1, 192, 16), ([31, 95, 159], 1, 4, 2, 256, 128), (list(range(100)) + list(range(3000, 3030)), 64, 4, 2, 64, 16)]
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("positions,window,heads,kv,dim,page", GAPS)
+def test_attend_shared_rows_with_a_gap_between_their_windows(ctx, positions, window, heads, kv, dim, page, q8):
+    """Rows of one request further apart than the window: what lies between is no row's, and has no influence."""
+    say("attend gap", positions[:8], window, heads, kv, dim, page, q8)
+    rng = np.random.default_rng(len(positions) + dim)
+    positions = np.array(positions)
+    rows, n = len(positions), int(positions.max()) + 1
+    table, pages = make_tables(rng, [n], page)
+    raw = random_pool(rng, q8, pages, kv, dim, page)
+    seen = np.zeros(pages * page, bool)
+    for i in positions:
+        j = np.arange(max(0, i - window + 1), i + 1)
+        seen[table[0, j // page] * page + j % page] = True
+    dirty = poisoned(raw, q8, pages, kv, dim, page, np.flatnonzero(~seen)[::2], 1, np.nan)
+    dirty = poisoned(dirty, q8, pages, kv, dim, page, np.flatnonzero(~seen)[1::2], 1, -np.inf)
+    dirty = poisoned(dirty, q8, pages, kv, dim, page, np.flatnonzero(~seen), 0, np.inf)
+    q = rng.standard_normal((rows, heads, dim)).astype(np.float32)
+    got = run_attend(ctx, cache_of(ctx, q8, pages, kv, dim, page, dirty), q, positions, np.zeros(rows, int), table, window=window)
+    want = M.attend(M.decode_pool(raw, q8, pages, kv, dim, page), q, positions, np.zeros(rows, int), table, dim ** -0.5, window)
+    check_attend(got, *want, np.minimum(positions + 1, window), dim)
