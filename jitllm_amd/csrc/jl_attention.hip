@@ -55,6 +55,7 @@ struct Shape {
 
 typedef float floatx2 __attribute__((ext_vector_type(2)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bfloat8 __attribute__((ext_vector_type(8)));
 typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
 typedef uint32_t uintx2 __attribute__((ext_vector_type(2)));
 
@@ -183,6 +184,11 @@ __device__ __forceinline__ T load_at(const uint8_t *base, uint32_t offset) {
 __device__ __forceinline__ jl_half2v as_half2(uint32_t x) { return __builtin_bit_cast(jl_half2v, x); }
 __device__ __forceinline__ uint32_t as_u32(jl_half2v x) { return __builtin_bit_cast(uint32_t, x); }
 
+// Halves of a word that are binary16 infinities or NaN, all their bits set.
+__device__ __forceinline__ uint32_t not_finite(uint32_t x) {
+    return ((x & 0x7c00u) == 0x7c00u ? 0xffffu : 0u) | ((x & 0x7c000000u) == 0x7c000000u ? 0xffff0000u : 0u);
+}
+
 // Bytes 0 and 2 of a word, signed, as binary16.  A byte b of 0 ... 255 under 0x64 is the binary16 of 1024 + b, so with the
 // sign bit turned over (b = q + 128) a subtraction of 1152 leaves q, exactly.  One bit operation puts both in place; the
 // kernel over 8-bit blocks is bound by its vector instructions, and those that permute bytes take twice as long as bit
@@ -237,6 +243,39 @@ struct Raw<false, DIM> {
                     for (int c = 0; c < 4; c++) v4[h][i][w][c] = seen[h][i] ? v4[h][i][w][c] : 0;
                 if constexpr (kMid) v2[h][i].x = seen[h][i] ? v2[h][i].x : 0, v2[h][i].y = seen[h][i] ? v2[h][i].y : 0;
                 if constexpr (kThin) v1[h][i] = seen[h][i] ? v1[h][i] : 0;
+            }
+    }
+    // whether any value is an infinity or NaN: nothing times it is no number
+    __device__ bool any_not_finite() const {
+        const jl_half2v nothing = {(_Float16)0.f, (_Float16)0.f};
+        jl_half2v sum = nothing;
+#pragma unroll
+        for (int h = 0; h < kHalves; h++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+#pragma unroll
+                for (int w = 0; w < kWide; w++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++) sum = __builtin_elementwise_fma(as_half2(v4[h][i][w][c]), nothing, sum);
+#pragma unroll
+                for (int c = 0; c < 2 * kMid; c++) sum = __builtin_elementwise_fma(as_half2(v2[h][i][c]), nothing, sum);
+                if constexpr (kThin) sum = __builtin_elementwise_fma(as_half2(v1[h][i]), nothing, sum);
+            }
+        return (as_u32(sum) & 0x7fff7fffu) != 0;
+    }
+    // those that are become 0
+    __device__ void drop_not_finite() {
+#pragma unroll
+        for (int h = 0; h < kHalves; h++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+#pragma unroll
+                for (int w = 0; w < kWide; w++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++) v4[h][i][w][c] &= ~not_finite(v4[h][i][w][c]);
+#pragma unroll
+                for (int c = 0; c < 2 * kMid; c++) v2[h][i][c] &= ~not_finite(v2[h][i][c]);
+                if constexpr (kThin) v1[h][i] &= ~not_finite(v1[h][i]);
             }
     }
     // eight tokens of the columns that output blocks `block` and `block` + 1 take of this lane
@@ -321,6 +360,42 @@ struct Raw<true, DIM> {
 #pragma unroll
                 for (int c = 0; c < 2; c++)
                     v_scale[h][w][c] &= (seen[h][2 * c] ? 0xffffu : 0u) | (seen[h][2 * c + 1] ? 0xffff0000u : 0u);
+    }
+    // whether any value may be an infinity or NaN: 128 times its scale is one
+    __device__ bool any_not_finite() const {
+        const jl_half2v nothing = {(_Float16)0.f, (_Float16)0.f}, most = {(_Float16)128.f, (_Float16)128.f};
+        jl_half2v sum = nothing;
+#pragma unroll
+        for (int h = 0; h < kHalves; h++)
+#pragma unroll
+            for (int w = 0; w < kPieces; w++)
+#pragma unroll
+                for (int c = 0; c < 2; c++) sum = __builtin_elementwise_fma(as_half2(v_scale[h][w][c]) * most, nothing, sum);
+        return (as_u32(sum) & 0x7fff7fffu) != 0;
+    }
+    // those that are become 0: bytes that a finite scale takes too far, and scales that are not finite
+    __device__ void drop_not_finite() {
+        auto drop = [](uint32_t x, uint32_t d) {
+            const uint32_t even = not_finite(as_u32(even_bytes(x) * as_half2(d))), odd = not_finite(as_u32(even_bytes(x >> 8) * as_half2(d)));
+            return x & ~((even & 0x00ff00ffu) | (odd & 0xff00ff00u));
+        };
+#pragma unroll
+        for (int h = 0; h < kHalves; h++) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                auto scale = [&](int piece) { return (v_scale[h][piece][i / 2] >> 16 * (i % 2) & 0xffffu) * 0x10001u; };
+#pragma unroll
+                for (int w = 0; w < kWide; w++)
+#pragma unroll
+                    for (int c = 0; c < 2; c++) v2[h][i][w][c] = drop(v2[h][i][w][c], scale(w));
+                if constexpr (kMid) v1[h][i] = drop(v1[h][i], scale(kWide));
+                if constexpr (kThin) v0[h][i] = (uint16_t)drop(v0[h][i], scale(kWide + kMid));
+            }
+#pragma unroll
+            for (int w = 0; w < kPieces; w++)
+#pragma unroll
+                for (int c = 0; c < 2; c++) v_scale[h][w][c] &= ~not_finite(v_scale[h][w][c]);
+        }
     }
     // Operands of two neighbouring blocks: their columns' bytes of two tokens come into one word, and out of it as pairs.
     __device__ void v_operands(int block, jl_half8 (&v)[2]) const {
@@ -717,6 +792,32 @@ __global__ void __launch_bounds__(kThreads, (Shape<Q8, DIM>::kPerUnit)) jl_kv_at
                     x[i] = seen[i / 4][i % 4] && (!SHARED || (token >= seen_here.first && token < seen_here.end)) ? x[i] : -INFINITY;
                 }
                 raw.mask_v(seen);
+                if constexpr (SHARED) {
+                    // An infinity or NaN that one row sees would reach one that does not, as nothing times it.  It is taken out
+                    // of v, and NaN goes to those that see it: in bfloat16, 2^127 in its place times 2^127 and -2^127 for each
+                    // such row, and zeros for all others.
+                    if (__any(raw.any_not_finite())) {
+                        uintx4 sees;
+#pragma unroll
+                        for (int i = 0; i < 8; i += 2) sees[i / 2] = (x[i] == -INFINITY ? 0u : 0x7f00u) | (x[i + 1] == -INFINITY ? 0u : 0x7f000000u);
+                        const bfloat8 plus = __builtin_bit_cast(bfloat8, sees), minus = __builtin_bit_cast(bfloat8, sees ^ 0x80008000u);
+#pragma unroll
+                        for (int b = 0; b < kBlocks; b += 2) {
+                            jl_half8 v[2];
+                            raw.v_operands(b, v);
+#pragma unroll
+                            for (int c = 0; c < 2; c++) {
+                                uintx4 its = __builtin_bit_cast(uintx4, v[c]);
+#pragma unroll
+                                for (int i = 0; i < 4; i++) its[i] = not_finite(its[i]) & 0x7f007f00u;
+                                const bfloat8 bad = __builtin_bit_cast(bfloat8, its);
+                                o[b + c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bad, plus, o[b + c], 0, 0, 0);
+                                o[b + c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bad, minus, o[b + c], 0, 0, 0);
+                            }
+                        }
+                        raw.drop_not_finite();
+                    }
+                }
             }
             float most = x[0];
 #pragma unroll

@@ -869,6 +869,14 @@ def poisoned(raw, q8, pages, kv, dim, page, at, which, bad, element=None):
     return dirty.reshape(-1)
 
 
+def check_where_finite(got, want, weight, reach, lengths, dim):
+    """check_attend where the definition says a number; no number where it says none."""
+    fine = np.isfinite(want)
+    assert not np.isfinite(got[~fine]).any()
+    zero = lambda y: np.where(fine, y, 0)                      # noqa: E731
+    check_attend(zero(got), zero(want), zero(weight), np.where(np.isfinite(reach), reach, 0), lengths, dim)
+
+
 GAPS = [
     # positions of one request's rows, window, heads, kv, dim, page
     ([10, 1000], 16, 8, 2, 128, 16), ([700, 5, 701, 3000], 40, 8, 4, 64, 32), ([900, 899, 100, 101, 400, 2, 1, 0], 7, 6, 3, 96, 64),
@@ -896,3 +904,57 @@ def test_attend_shared_rows_with_a_gap_between_their_windows(ctx, positions, win
     got = run_attend(ctx, cache_of(ctx, q8, pages, kv, dim, page, dirty), q, positions, np.zeros(rows, int), table, window=window)
     want = M.attend(M.decode_pool(raw, q8, pages, kv, dim, page), q, positions, np.zeros(rows, int), table, dim ** -0.5, window)
     check_attend(got, *want, np.minimum(positions + 1, window), dim)
+
+
+LATER = [
+    # first position, rows, window, heads, kv, dim, page, poisoned tokens, element of v (None: all)
+    (0, 40, 0, 8, 2, 128, 16, [17], None), (0, 40, 0, 8, 2, 128, 16, [5, 30], 77), (20, 64, 0, 4, 4, 64, 32, [50], 9), (0, 33, 9, 6, 3, 96, 64, [12], 70),
+    (0, 33, 0, 6, 2, 96, 16, [20], None), (1000, 5, 0, 8, 1, 192, 16, [1002], 150), (3000, 3, 100, 8, 2, 256, 128, [2901, 3001], 200), (6000, 4, 0, 4, 1, 64, 16, [6002], None),
+    (60, 10, 3, 16, 1, 256, 16, [64], None), (100, 16, 0, 1, 1, 128, 16, [107, 115], 0)]
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("bad", [np.inf, -np.inf, np.nan])
+@pytest.mark.parametrize("first,rows,window,heads,kv,dim,page,tokens,element", LATER)
+def test_attend_shared_rows_keep_to_their_own_tokens(ctx, first, rows, window, heads, kv, dim, page, tokens, element, bad, q8):
+    """An infinity or NaN in v at a token that some rows of a prompt see: those lose the columns that it stands in, the
+    others -- before it, or past a window behind it -- are what they are without it."""
+    say("attend later", first, rows, window, heads, kv, dim, page, tokens, element, bad, q8)
+    rng = np.random.default_rng(first + rows + dim)
+    positions, requests_of = np.arange(first, first + rows), np.zeros(rows, int)
+    table, pages = make_tables(rng, [first + rows], page)
+    raw = random_pool(rng, q8, pages, kv, dim, page)
+    at = [table[0, t // page] * page + t % page for t in tokens]
+    dirty = poisoned(raw, q8, pages, kv, dim, page, at, 1, bad, element)
+    q = rng.standard_normal((rows, heads, dim)).astype(np.float32)
+    clean, got = (run_attend(ctx, cache_of(ctx, q8, pages, kv, dim, page, r), q, positions, requests_of, table, window=window) for r in (raw, dirty))
+    pool = M.decode_pool(raw, q8, pages, kv, dim, page)
+    out, weight, reach = M.attend(pool, q, positions, requests_of, table, dim ** -0.5, window)
+    lost = np.zeros((rows, 1, dim), bool)
+    columns = slice(None) if element is None else slice(element // 32 * 32, element // 32 * 32 + 32) if q8 else element
+    for t in tokens:
+        sees = (positions >= t) & (positions < t + window if window else True)
+        lost[sees, :, columns] = True
+    lost = np.broadcast_to(lost, out.shape)
+    assert lost.any() and not np.isfinite(got[lost]).any()
+    assert np.array_equal(got[~lost], clean[~lost])
+    check_attend(np.where(lost, 0, got), np.where(lost, 0, out), np.where(lost, 0, weight), reach, np.minimum(positions + 1, window or 1 << 30), dim)
+
+
+def test_attend_shared_rows_over_8_bit_blocks_whose_values_overflow(ctx):
+    """Finite scales whose products with the bytes are infinite in binary16, and scales just below those."""
+    rng = np.random.default_rng(51)
+    heads, kv, dim, page, rows = 4, 2, 64, 16, 24
+    positions, requests_of = np.arange(rows), np.zeros(rows, int)
+    table, pages = make_tables(rng, [rows], page)
+    raw = random_pool(rng, True, pages, kv, dim, page)
+    at = [table[0, t // page] * page + t % page for t in (3, 13, 20)]
+    dirty = poisoned(poisoned(raw, True, pages, kv, dim, page, at[:1], 1, 500.0), True, pages, kv, dim, page, at[1:], 1, 5000.0)
+    q = rng.standard_normal((rows, heads, dim)).astype(np.float32)
+    say("attend 8-bit overflow")
+    got = run_attend(ctx, cache_of(ctx, True, pages, kv, dim, page, dirty), q, positions, requests_of, table)
+    pool = M.decode_pool(dirty, True, pages, kv, dim, page)
+    with np.errstate(invalid="ignore"):
+        want = M.attend(pool, q, positions, requests_of, table, dim ** -0.5)
+    assert np.isfinite(want[0][:13]).all() and not np.isfinite(want[0][13:]).all()
+    check_where_finite(got, *want, positions + 1, dim)
