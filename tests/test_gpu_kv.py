@@ -958,3 +958,173 @@ def test_attend_shared_rows_over_8_bit_blocks_whose_values_overflow(ctx):
         want = M.attend(pool, q, positions, requests_of, table, dim ** -0.5)
     assert np.isfinite(want[0][:13]).all() and not np.isfinite(want[0][13:]).all()
     check_where_finite(got, *want, positions + 1, dim)
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("window", [0, 50])
+def test_attend_shared_rows_over_bad_pages_and_past_the_table(ctx, window, q8):
+    """Pages outside the cache count as masked, positions past the table read what it holds, some rows are of no request."""
+    rng = np.random.default_rng(61)
+    dim, page, kv, heads = 96, 16, 2, 4
+    table, pages = make_tables(rng, [300, 70], page)
+    table[0, [0, 3, 17]], table[1, 1:3], table[0, 9:12] = -1, 2**31 - 1, pages
+    raw = random_pool(rng, q8, pages, kv, dim, page)
+    cache = cache_of(ctx, q8, pages, kv, dim, page, raw)
+    end = table.shape[1] * page
+    positions = np.concatenate([np.arange(30), np.arange(40, 60), np.arange(140, 200), [end - 1, end, end + 1, end + 40, end + 49, end + 50, 2**31 - 1],
+                                np.arange(10, 20), [3, -1, 4, 5, -2**31, 6]])
+    requests_of = np.concatenate([np.zeros(117, int), np.ones(10, int), [0, 0, 0, -1, 1, 2]])
+    q = rng.standard_normal((len(positions), heads, dim)).astype(np.float32)
+    say("attend shared bad pages", window, q8)
+    got = run_attend(ctx, cache, q, positions, requests_of, table, window=window)
+    want = M.attend(M.decode_pool(raw, q8, pages, kv, dim, page), q, positions, requests_of, table, dim ** -0.5, window)
+    check_attend(got, *want, np.clip(positions + 1, 0, end), dim)
+    assert (got[want[1].max((1, 2)) == 0] == 0).all()
+
+
+@pytest.mark.parametrize("q8", [False, True])
+def test_attend_shared_rows_of_extreme_queries(ctx, q8):
+    """Rows that go together, each with scores of another size: thousands apart, all equal, below binary16; one with an
+    infinity and one with NaN in a head, which are those heads' alone."""
+    rng = np.random.default_rng(62)
+    dim, page, kv, heads, rows, n = 64, 16, 2, 4, 24, 500
+    table, pages = make_tables(rng, [n], page)
+    raw = random_pool(rng, q8, pages, kv, dim, page)
+    positions, requests_of = np.arange(n - rows, n), np.zeros(rows, int)
+    q = rng.standard_normal((rows, heads, dim)).astype(np.float32)
+    q *= np.array([1, 3000, 0, 1e-9, 2.0 ** -140, 40], np.float32)[np.arange(rows) % 6, None, None]
+    q[7::6] *= np.exp(rng.uniform(-20, 5, (len(q[7::6]), heads, dim))).astype(np.float32)
+    cache = cache_of(ctx, q8, pages, kv, dim, page, raw)
+    say("attend shared extreme", q8)
+    got = run_attend(ctx, cache, q, positions, requests_of, table)
+    pool = M.decode_pool(raw, q8, pages, kv, dim, page)
+    out, weight, reach = M.attend(pool, q, positions, requests_of, table, dim ** -0.5)
+    # A weight is two binary16 parts of 2^13 times it, the second one off by 2^-25 however small the weight is: n tokens are
+    # off by n 2^-38 max |v| together, which is more than check_attend's share of sum p |v| where the token with nearly all
+    # of the weight has a v of 0 (an 8-bit block's often is).  Through that check's n + 64 half steps of 2^-24, 2^-14 max |v|
+    # more of sum p |v| stand for it.
+    want = out, weight + 2.0 ** -14 * np.abs(pool[1]).max(), reach
+    check_attend(got, *want, positions + 1, dim)
+    bad = q.copy()
+    bad[5, 1, 5], bad[18, 2, 7], bad[19, 2, 7] = np.inf, np.nan, -np.inf
+    lost = np.zeros((rows, heads), bool)
+    lost[[5, 18, 19], [1, 2, 2]] = True
+    got = run_attend(ctx, cache, bad, positions, requests_of, table)
+    assert np.isnan(got[lost]).all()
+    check_attend(np.where(lost[..., None], 0, got), *(np.where(lost[..., None] if w.ndim == 3 else lost, 0, w) for w in want), positions + 1, dim)
+
+
+def test_attend_shared_rows_are_the_same_every_time_and_with_any_workspace(ctx):
+    """Drafts and prompts, cut into parts and whole."""
+    rng = np.random.default_rng(63)
+    for rows, first, heads, kv, dim, q8 in ((4, 7000, 8, 2, 128, False), (3, 3000, 4, 4, 256, True), (90, 10, 6, 2, 64, False), (16, 2500, 1, 1, 64, True)):
+        table, pages = make_tables(rng, [first + rows], 16)
+        cache = cache_of(ctx, q8, pages, kv, dim, 16, random_pool(rng, q8, pages, kv, dim, 16))
+        q = rng.standard_normal((rows, heads, dim)).astype(np.float32)
+        say("attend shared repeats", rows, first, heads, kv, dim, q8)
+        runs = [run_attend(ctx, cache, q, np.arange(first, first + rows), np.zeros(rows, int), table, workspace=w) for w in (0, 0xff, 0x7f, None)]
+        for r in runs[1:]:
+            assert np.array_equal(r, runs[0])
+
+
+@pytest.mark.parametrize("q8", [False, True])
+def test_a_captured_step_whose_rows_go_together(ctx, q8):
+    """A step of up to 24 rows for 3 requests, recorded once: prompts, drafts, single tokens, padding; every replay after
+    eager work through the same workspace, against the same step made eagerly and against float64."""
+    import bench
+    from jitllm_amd.attention import BlockTables, KvType, PagedAttention, PagedKvCache, Rows
+    hip = bench.Hip()
+    rng = np.random.default_rng(64)
+    requests, stride, page, pages, max_rows, heads, kv, dim = 3, 12, 16, 30, 24, 4, 2, 64
+    w = (heads + 2 * kv) * dim
+    attention = PagedAttention(ctx, max_rows, heads, kv, dim)
+
+    class Side:
+        def __init__(self):
+            self.tables = BlockTables(ctx, requests, stride, pages, page, max_rows)
+            self.cache = PagedKvCache(ctx, KvType.Q8_0 if q8 else KvType.F16, pages, kv, dim, page, memory=ctx.raw_buffer(2 * pages * kv * M.part_bytes(q8, dim, page)))
+            self.cache.memory.upload(np.full(self.cache.nbytes, 0xff, np.uint8))           # NaN where nothing is written
+            self.fresh, self.qkv = ints(ctx, np.zeros(requests)), ctx.float_array(max_rows * w, fill=0.0)
+            self.out = ctx.float_array(max_rows * heads * dim, fill=7.0)
+
+        def step(self):
+            t = self.tables
+            t.plan(self.fresh)
+            self.cache.append(Rows(self.qkv, w, heads * dim), Rows(self.qkv, w, (heads + kv) * dim), t.positions, t.slots, max_rows)
+            attention.attend(self.cache, Rows(self.qkv, w), max_rows, t.positions, t.table, self.out, requests=requests, rowRequests=t.rowRequests)
+
+    a, b = Side(), Side()
+    say("captured step, rows together", q8)
+    a.fresh.set([0] * requests)
+    a.step()
+    ctx.sync()
+    exe = hip.capture(ctx.stream, a.step)
+    try:
+        for n, fresh in enumerate([[20, 3, 0], [1, 1, 1], [4, 4, 4], [1, -1, 9], [5, 0, 1], [24, 0, 0], [1, 17, 5], [0, 0, 0]]):
+            x = rng.standard_normal((max_rows, w)).astype(np.float32)
+            for side in (a, b):
+                side.fresh.set(fresh), side.qkv.set(x), side.out.init(7.0)
+            b.step()
+            ctx.sync()
+            hip.launch(exe, ctx.stream)
+            ctx.sync()
+            got = a.out.get().reshape(max_rows, heads, dim)
+            assert np.array_equal(got.view(np.uint32).reshape(-1), b.out.get().view(np.uint32)), n
+            positions, rows_of, table = (getattr(a.tables, k).get() for k in ("positions", "rowRequests", "table"))
+            want = M.attend(M.decode_pool(pool_bytes(a.cache), q8, pages, kv, dim, page), x[:, :heads * dim].reshape(max_rows, heads, dim), positions,
+                            rows_of, table.reshape(requests, stride), dim ** -0.5)
+            check_attend(got.astype(np.float64), *want, positions + 1, dim)
+            assert (got[positions < 0] == 0).all()
+    finally:
+        hip.destroy_graph(exe)
+
+
+def test_two_contexts_of_rows_that_go_together(ctx):
+    """A draft's rows on one stream, a prompt's on another, one cache: each is what it is alone."""
+    from jitllm_amd.attention import KvType, PagedAttention, PagedKvCache
+    from jitllm_amd.runtime import Context
+    rng = np.random.default_rng(65)
+    n = 6000
+    table, pages = make_tables(rng, [n], 16)
+    raw = random_pool(rng, False, pages, 4, 128, 16)
+    memory = ctx.raw_buffer(raw.nbytes)
+    memory.upload(raw)
+    cache = PagedKvCache(ctx, KvType.F16, pages, 4, 128, 16, memory=memory)
+    say("two contexts, rows together")
+    with Context(0) as second:
+        sides = []
+        for c, positions in ((ctx, np.arange(n - 4, n)), (second, np.arange(100))):
+            rows = len(positions)
+            q = rng.standard_normal((rows, 16, 128)).astype(np.float32)
+            sides.append((c, PagedAttention(c, rows, 16, 4, 128), c.from_numpy(q), c.float_array(rows * 16 * 128), ints(c, positions), ints(c, table),
+                          ints(c, np.zeros(rows)), rows, q, positions))
+        for _ in range(20):
+            for c, attention, x, out, positions, t, requests_of, rows, _, _ in sides:
+                for _ in range(3):
+                    attention.attend(cache, x, rows, positions, t, out, requests=1, rowRequests=requests_of)
+            for side in sides:
+                side[0].sync()
+        pool = M.decode_pool(raw, False, pages, 4, 128, 16)
+        for side in sides:
+            rows, q, positions = side[7:]
+            got = side[3].get().astype(np.float64).reshape(rows, 16, 128)
+            check_attend(got, *M.attend(pool, q, positions, np.zeros(rows, int), table, 128 ** -0.5), positions + 1, 128)
+            assert np.array_equal(got, run_attend(ctx, cache, q, positions, np.zeros(rows, int), table))
+        del sides, side, attention, x, out, t, requests_of, c
+
+
+def test_one_workspace_for_rows_together_and_alone(ctx):
+    from jitllm_amd.attention import PagedAttention
+    rng = np.random.default_rng(66)
+    shared = PagedAttention(ctx, 64, 32, 4, 256)
+    for rows, first, requests, heads, kv, dim, q8 in ((4, 3000, 1, 16, 4, 256, False), (2, 2500, 2, 8, 2, 128, True), (33, 0, 1, 8, 8, 64, True), (1, 4000, 1, 32, 4, 192, False)) * 2:
+        requests_of = np.arange(rows) % requests
+        positions = first + np.arange(rows) // requests
+        table, pages = make_tables(rng, positions + 1, 32, requests_of, requests)
+        raw = random_pool(rng, q8, pages, kv, dim, 32)
+        attention = PagedAttention(ctx, 64, heads, kv, dim)
+        attention.workspace = shared.workspace
+        q = rng.standard_normal((rows, heads, dim)).astype(np.float32)
+        say("one workspace, together and alone", rows, first, requests, heads, kv, dim, q8)
+        got = run_attend(ctx, cache_of(ctx, q8, pages, kv, dim, 32, raw), q, positions, requests_of, table, attention=attention)
+        check_attend(got, *M.attend(M.decode_pool(raw, q8, pages, kv, dim, 32), q, positions, requests_of, table, dim ** -0.5), positions + 1, dim)
