@@ -306,7 +306,7 @@ __device__ __forceinline__ double2 cos_sin_of_turns(double turns) {
     const double part = turns - rint(turns), quarters = rint(4.0 * part);
     const double x = (part - 0.25 * quarters) * 6.283185307179586477, y = x * x;
     const double s = x * (1 + y * (-1.0 / 6 + y * (1.0 / 120 + y * (-1.0 / 5040 + y * (1.0 / 362880 + y * (-1.0 / 39916800 + y * (1.0 / 6227020800.0)))))));
-    const double c = 1 + y * (-0.5 + y * (1.0 / 24 + y * (-1.0 / 720 + y * (1.0 / 40320 + y * (-1.0 / 3628800 + y * (1.0 / 479001600.0))))));
+    const double c = 1 + y * (-0.5 + y * (1.0 / 24 + y * (-1.0 / 720 + y * (1.0 / 40320 + y * (-1.0 / 3628800 + y * (1.0 / 479001600 + y * (-1.0 / 87178291200.0)))))));
     const int n = (int)quarters & 3;
     return make_double2(n == 0 ? c : n == 1 ? -s : n == 2 ? -c : s, n == 0 ? s : n == 1 ? c : n == 2 ? -s : -c);
 }

@@ -1128,3 +1128,76 @@ def test_one_workspace_for_rows_together_and_alone(ctx):
         say("one workspace, together and alone", rows, first, requests, heads, kv, dim, q8)
         got = run_attend(ctx, cache_of(ctx, q8, pages, kv, dim, 32, raw), q, positions, requests_of, table, attention=attention)
         check_attend(got, *M.attend(M.decode_pool(raw, q8, pages, kv, dim, 32), q, positions, requests_of, table, dim ** -0.5), positions + 1, dim)
+
+
+# ---- what the write promises of its precision ----------------------------------------------------
+
+def append_error(x, positions, freq, halves):
+    """What double precision leaves of heads [rows][heads][dim] that turned, next to their float64 form: the series of sine
+    and cosine end below 2^-45, an angle is rounded four times (product, turns, their fraction, radians) and the products
+    and sums, a norm's too, make no 2^-47 together, all of it of |a| + |b| of a pair (at most sqrt 2 times what the pair
+    has behind the turn as before it)."""
+    slack = np.abs(x) * 2.0 ** -47
+    pairs = len(freq)
+    first = np.arange(pairs) if halves else 2 * np.arange(pairs)
+    second = first + pairs if halves else first + 1
+    both = 2 ** 0.5 * (np.abs(x[..., first]) + np.abs(x[..., second])) * (2.0 ** -45 + 2.0 ** -47 + 4 * 2.0 ** -53 * np.abs(positions[:, None, None] * freq))
+    slack[..., first], slack[..., second] = both, both
+    return slack
+
+
+@pytest.mark.parametrize("halves", [False, True])
+def test_append_where_products_cancel(ctx, halves):
+    """a cos - b sin next to zero: the absolute error of the cosine and the sine, in every eighth of a turn."""
+    dim, page, rows = 64, 16, 33
+    pairs = dim // 2
+    freq = np.pi / 4 * (1 + np.linspace(-1e-9, 1e-9, pairs))
+    positions = np.arange(rows)
+    angle = positions.astype(np.longdouble)[:, None] * freq.astype(np.longdouble)
+    cos, sin = np.cos(angle), np.sin(angle)
+    a, b = np.ones((rows, pairs)), np.where(cos * sin > 0, 1.0, -1.0)        # near odd eighths |cos| = |sin|
+    x = np.zeros((rows, 3, dim), np.float32)
+    first = np.arange(pairs) if halves else 2 * np.arange(pairs)
+    second = first + pairs if halves else first + 1
+    x[:, 0, first], x[:, 0, second] = a, b
+    cache = cache_of(ctx, False, 3, 1, dim, page, np.zeros(2 * 3 * M.part_bytes(False, dim, page), np.uint8))
+    say("append cancel", halves)
+    got = run_append(ctx, cache, x, 1, 1, dim, positions, np.arange(rows), freq, halves, None, None, 0.0)[:, 0]
+    want = np.zeros((rows, dim), np.longdouble)
+    want[:, first], want[:, second] = a * cos - b * sin, a * sin + b * cos
+    slack = append_error(want[:, None].astype(np.float64), positions, freq, halves)[:, 0]
+    assert (np.abs(got - want) <= slack + ULP * np.abs(want)).all(), float(np.max(np.abs(got - want) - ULP * np.abs(want)))
+
+
+@pytest.mark.parametrize("rows,heads,kv,dim,page,q8,halves,turned,norm,context", [a for a in APPENDS if a[1]])
+def test_append_rounds_once(ctx, rows, heads, kv, dim, page, q8, halves, turned, norm, context):
+    """q is the fp32 value of the float64 form; k and v that, rounded to the cache's type.  (A neighbour where the error of
+    double precision reaches over a border: roundings are monotonic.)"""
+    say("append rounds", rows, heads, kv, dim, page, q8, halves, turned, norm, context)
+    rng = np.random.default_rng(rows * dim + page)
+    pages = rows // page + 1
+    x = rng.standard_normal((rows, heads + 2 * kv, dim)).astype(np.float32)
+    x[:, :, 3] *= 20
+    cache = cache_of(ctx, q8, pages, kv, dim, page, np.zeros(2 * pages * kv * M.part_bytes(q8, dim, page), np.uint8))
+    slots, positions = rng.permutation(pages * page)[:rows], rng.integers(0, context, rows)
+    freq = 500000.0 ** (-np.arange(0, turned, 2) / turned) if turned else np.zeros(0)
+    qn, kn = (1 + 0.1 * rng.standard_normal(dim).astype(np.float32) for _ in range(2)) if norm else (None, None)
+    eps = np.float32(1e-6)
+    got_q = run_append(ctx, cache, x, heads, kv, dim, positions, slots, freq, halves, qn, kn, eps)
+    ends = []
+    for part, w in ((x[:, :heads], qn), (x[:, heads:heads + kv], kn)):
+        y = M.rotate(part, positions, freq, halves, w, float(eps))
+        slack = append_error(y, positions, freq, halves) if turned or norm else 0
+        ends.append([(y + side * slack).astype(np.float32) for side in (-1, 1)])
+    assert ((ends[0][0] <= got_q) & (got_q <= ends[0][1])).all()
+    after = M.decode_pool(pool_bytes(cache), q8, pages, kv, dim, page)
+    kept = after[:, slots // page, :, slots % page]                                  # [rows][2][kv][dim]
+    for got, (low, high) in ((kept[:, 0], ends[1]), (kept[:, 1], [x[:, heads + kv:]] * 2)):
+        if not q8:
+            assert ((low.astype(np.float16) <= got) & (got <= high.astype(np.float16))).all()
+            continue
+        blocks = low.reshape(-1, 32)
+        sure = (blocks == high.reshape(-1, 32)).all(-1)                              # (fp32 division and rint, as the blocks are defined)
+        d = np.minimum(np.abs(blocks).max(-1, keepdims=True) / np.float32(127), np.float32(65504)).astype(np.float16).astype(np.float32)
+        want = (np.clip(np.rint(blocks / d), -127, 127) * d).astype(np.float16)
+        assert sure.mean() > 0.9 and np.array_equal(got.reshape(-1, 32)[sure], want[sure].astype(np.float64))
