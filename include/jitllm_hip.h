@@ -520,10 +520,11 @@ typedef enum jl_rope_style { JL_ROPE_PAIRS = 0, JL_ROPE_HALVES = 1 } jl_rope_sty
  *               frequencies may be null.
  *   q_norm, k_norm    [head_dim] fp32 or null: heads are normalised first, x <- w * (x / sqrt(sum x^2
  *               / head_dim + eps)), as Qwen3's are
- * Sums and products are in double precision and rounded once, to fp32; fewer than 2^24 rows.
- * A JL_KV_F16 element is the nearest binary16 (infinite where fp32 is beyond it).  A block of
- * JL_KV_Q8_0 has d = the binary16 nearest to max |x| / 127 (at most 65504) and bytes rint(x / d)
- * in -127 ... 127; 0 where d is 0 or x is NaN.
+ * Sums and products are in double precision and rounded to fp32, what q_out gets; the cache keeps
+ * what its type makes of that fp32 value.  A JL_KV_F16 element is the binary16 nearest to it (infinite
+ * where it is beyond binary16).  A block of JL_KV_Q8_0 has d = the binary16 nearest to max |x| / 127
+ * (at most 65504) and bytes rint(x / d) in -127 ... 127; 0 where d is 0 or x is NaN.
+ * Fewer than 2^24 rows, at most 65536 heads of q.
  */
 int jl_kv_append(jl_context *ctx, jl_kv_cache *cache, const float *q, int heads, int64_t ldq, const float *k,
                  int64_t ldk, const float *v, int64_t ldv, float *q_out, int64_t ldq_out, const int32_t *positions,
@@ -566,7 +567,10 @@ int jl_kv_read(jl_context *ctx, const jl_kv_cache *cache, const int32_t *slots, 
  * jl_kv_attention_workspace_init has been over once (on the stream, before the first call; every call
  * leaves it as it needs it).  Parts of rows that are cut are joined there.  Calls that may run at the
  * same time -- contexts, graphs on two streams -- need one each.
- * At most 65535 rows; heads a multiple of kv_heads.
+ * At most 65535 rows and 65536 heads, a multiple of kv_heads.  A call's tiles of 32 tokens are a 32-bit
+ * list: rows * kv_heads * ceil(heads / kv_heads / 16) * (table_stride * page_tokens / 32 + 6) stays below
+ * 2^32 - 1024 (8 heads of k and v: 65535 rows over a table of 261 900 tokens, 4096 rows over 4 million),
+ * counted by what the table's rows have room for, not by the lengths; others are refused.
  */
 size_t jl_kv_attention_workspace_bytes(int heads, int kv_heads, int head_dim);
 int jl_kv_attention_workspace_init(jl_context *ctx, void *workspace, size_t workspace_bytes);

@@ -244,7 +244,9 @@ class BlockTables:
 
 class PagedAttention:
     """Attention of one new token a row over paged caches of one shape, with the workspace it joins in
-    (jl_kv_attention).  One object for every layer; calls that may run at the same time need one each."""
+    (jl_kv_attention).  One object for every layer; calls that may run at the same time need one each.
+    ``maxRows`` is the caller's own note: the workspace is the same for any number of rows, and no call is
+    held to it (jl_kv_attention takes up to 65535)."""
 
     def __init__(self, ctx: Context, maxRows: int, heads: int, kvHeads: int, headDim: int):
         self.ctx, self._lib = ctx, ctx._lib

@@ -23,6 +23,8 @@
 //
 // Rows of one request (a prompt's, a draft's) go through its pages together where there are twice as many rows as
 // requests: 16 columns of the matrix instructions are the query heads of one row after the other, each with its own mask.
+// Only rows whose ranges touch do, so that no token is read that none of them sees, and in tiles that some of them do not
+// see all of, values of v that are not finite are kept from those.
 #include <algorithm>
 #include <climits>
 #include <cmath>
@@ -1077,9 +1079,9 @@ int jl_kv_attention(jl_context *ctx, const jl_kv_cache *cache, const float *q, i
     a.group = heads / cache->kv_heads;
     a.blocks_of_16 = (a.group + 15) / 16;
     // Twice as many rows as requests, or more: some are of one, unless they are padding.  (32 heads over 8 of 128, one request,
-    // each row alone and together: a prompt of 2048 tokens 755 and 186 us, of 512 64 and 27; 4 rows after 30 000 tokens 79 and
-    // 43, after 1000 11.7 and 13.8.  32 heads over 32, 512 tokens: 225 and 31.  64 rows of 64 requests of up to 8192 tokens
-    // padded to 512 rows: 118 and 124; to 72, which are too few: 104 and 117.)
+    // each row alone and together: a prompt of 2048 tokens 753 and 187 us, of 512 64 and 27; 4 rows after 30 000 tokens 79 and
+    // 44, after 1000 11.8 and 14.0.  32 heads over 32, 512 tokens: 224 and 32.  64 rows of 64 requests of up to 8192 tokens
+    // padded to 512 rows: 118 and 124; to 72, which are too few: 105 and 118.)
     a.rows_each = 1;
     if (row_requests && rows >= 2 * requests)
         while (2 * a.rows_each * a.group <= 16) a.rows_each *= 2;

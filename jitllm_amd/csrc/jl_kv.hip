@@ -314,9 +314,8 @@ __device__ __forceinline__ double2 cos_sin_of_turns(double turns) {
 // LANES consecutive lanes have a head, eight values each (those past head_dim / 8 idle); a workgroup has kAppendPer times
 // 256 / LANES of a token's q, k and v heads, and all their loads are on their way before anything else is done.
 // Bound: the bytes.  The angles' cosines and sines are worked out once per workgroup, in LDS, while the loads come in.
-// Sums and products between the loads and the one rounding at the end are in double precision, which the bytes hide: what
-// the cache keeps is the nearest it can to the rotated value, and a value beside a border of binary16 falls to the right
-// side.
+// Sums and products between the loads and the rounding to fp32 are in double precision, which the bytes hide; what the cache
+// keeps is rounded from that fp32 value.
 template <bool Q8, int LANES, bool HALVES>
 __global__ void __launch_bounds__(kAppendThreads) jl_kv_append_kernel(AppendArgs p) {
     __shared__ double2 turn[128];   // (cos, sin) of the token's pairs

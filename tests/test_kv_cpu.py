@@ -264,3 +264,18 @@ def test_models_agree_with_each_other():
     pool = rng.standard_normal((2, 3, 1, 16, 64))
     out, weight, _ = M.attend(pool, np.zeros((1, 2, 64)), [19], None, np.array([[2, 0]]), 1.0)
     assert np.allclose(out[0, 1], np.concatenate([pool[1, 2, 0], pool[1, 0, 0, :4]]).mean(0)) and (weight >= np.abs(out) - 1e-12).all()
+
+
+def test_limits_that_the_header_states(L, lib, ctx, memory, cache):
+    """One past each: heads of q, and the list of tiles, which goes by the table's room (2 heads of k and v, pages of 16)."""
+    at = lambda form, **change: [memory if v == "m" else v for v in dict(form, **change).values()]                # noqa: E731
+    wide = dict(heads=65538, ldq=65538 * 128)
+    assert lib.jl_kv_attention(ctx, cache, *at(ATTEND, **wide, ldo=65538 * 128)) == L.JL_ERR_INVALID and "65538 query heads" in said(lib)
+    assert lib.jl_kv_append(ctx, cache, *at(APPEND, **wide, ldq_out=65538 * 128)) == L.JL_ERR_INVALID and "65538 query heads" in said(lib)
+    rows = 65535
+    most = ((2 ** 32 - 1025) // (2 * rows) - 6) * 32 + 31       # tokens that are still listed
+    args = dict(rows=rows, requests=rows, table_stride=most // 16 + 1)
+    assert lib.jl_kv_attention(ctx, cache, *at(ATTEND, **args)) == L.JL_ERR_INVALID and "in one call" in said(lib)
+    # ... a list that fits comes to the next check
+    args["table_stride"] -= 1
+    assert lib.jl_kv_attention(ctx, cache, *at(ATTEND, **args, window=-1)) == L.JL_ERR_INVALID and "window" in said(lib)
