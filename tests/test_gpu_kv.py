@@ -1201,3 +1201,25 @@ def test_append_rounds_once(ctx, rows, heads, kv, dim, page, q8, halves, turned,
         d = np.minimum(np.abs(blocks).max(-1, keepdims=True) / np.float32(127), np.float32(65504)).astype(np.float16).astype(np.float32)
         want = (np.clip(np.rint(blocks / d), -127, 127) * d).astype(np.float16)
         assert sure.mean() > 0.9 and np.array_equal(got.reshape(-1, 32)[sure], want[sure].astype(np.float64))
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("bad", [np.inf, np.nan])
+def test_attend_shared_rows_over_keys_that_are_not_finite(ctx, bad, q8):
+    """... and in k: rows that see the token have no number, the others are what they are without it."""
+    rng = np.random.default_rng(67)
+    heads, kv, dim, page = 4, 2, 128, 16
+    for first, rows, window, token in ((0, 40, 0, 21), (0, 40, 6, 21), (2000, 7, 50, 2003), (2000, 7, 50, 1953)):
+        positions, requests_of = np.arange(first, first + rows), np.zeros(rows, int)
+        table, pages = make_tables(rng, [first + rows], page)
+        raw = random_pool(rng, q8, pages, kv, dim, page)
+        dirty = poisoned(raw, q8, pages, kv, dim, page, [table[0, token // page] * page + token % page], 0, bad)
+        q = rng.standard_normal((rows, heads, dim)).astype(np.float32)
+        say("attend keys", first, rows, window, token, bad, q8)
+        clean, got = (run_attend(ctx, cache_of(ctx, q8, pages, kv, dim, page, r), q, positions, requests_of, table, window=window) for r in (raw, dirty))
+        sees = (positions >= token) & (positions < token + window if window else True)
+        assert sees.any() and (~sees).any() and np.isnan(got[sees]).all()
+        # (the others' maximum may be brought forward with that of the rows beside them: the same but for rounding)
+        out, weight, reach = M.attend(M.decode_pool(raw, q8, pages, kv, dim, page), q, positions, requests_of, table, dim ** -0.5, window)
+        for r in (clean, got):
+            check_attend(r[~sees], out[~sees], weight[~sees], reach[~sees], np.minimum(positions + 1, window or 1 << 30)[~sees], dim)
