@@ -331,7 +331,7 @@ def _run_logprobs(s):
     if not own:
         return _plain_logprobs(s)
     s.probabilities.compute(s.m_logits, s.case["rows"], tokens=s.m_tokens, logprobs=s.m_logprobs, entropy=s.m_entropy, topTokens=s.m_top_tokens,
-                            topLogprobs=s.m_top_logprobs, scale=s.case["scale"], cap=s.case["cap"])
+                            topLogprobs=s.m_top_logprobs, tokensPerRow=s.case["tokens"], scale=s.case["scale"], cap=s.case["cap"])
     return {"logprobs": s.logprobs, "entropy": s.entropy, "top": s.top_tokens, "top_logprobs": s.top_logprobs}
 
 
