@@ -452,13 +452,18 @@ int jl_rms_apply_xf16(jl_context *ctx, float *X, const float *delta, const float
  *
  * Types.  JL_KV_F16: binary16.  JL_KV_Q8_0: blocks of 32 signed bytes with a binary16 scale d, as
  * GGUF's Q8_0, of 53 % of the bytes; an element stands for the binary16 nearest to d * byte.
+ * JL_KV_Q4_0: blocks of 32 numbers n of four bits, 0 ... 15, with a binary16 scale d of either sign, as
+ * GGUF's Q4_0, of 28 % of the bytes; an element stands for the binary16 nearest to d * (n - 8).
  *
  * Layout: [k, v][pages][kv_heads][part], where the part of one page and head is, for JL_KV_F16,
  * [page_tokens][head_dim] binary16, and for JL_KV_Q8_0 [page_tokens][head_dim] bytes followed by
- * [head_dim / 32][page_tokens] binary16 scales.  Heads of 64, 96, 128, 192 or 256 values (others:
+ * [head_dim / 32][page_tokens] binary16 scales; for JL_KV_Q4_0 page_tokens * head_dim / 2 bytes
+ * followed by the same scales.  Of keys, those bytes are [page_tokens][head_dim / 2], elements 2 b (low
+ * four bits) and 2 b + 1 in a token's byte b; of values, [page_tokens / 4][head_dim / 4][4][2], two bytes
+ * of four elements of each of four tokens, the earlier elements in the lower bits.  Heads of 64, 96, 128, 192 or 256 values (others:
  * JL_ERR_UNSUPPORTED); pages of 16, 32, 64, 128 or 256 tokens; at most 2^31 - 1 tokens in all.
  */
-typedef enum jl_kv_type { JL_KV_F16 = 1, JL_KV_Q8_0 = 8 } jl_kv_type;
+typedef enum jl_kv_type { JL_KV_F16 = 1, JL_KV_Q4_0 = 4, JL_KV_Q8_0 = 8 } jl_kv_type;
 typedef struct jl_kv_cache jl_kv_cache;
 
 /* Device bytes of such a cache; 0 where jl_kv_cache_create would refuse it. */
@@ -523,7 +528,9 @@ typedef enum jl_rope_style { JL_ROPE_PAIRS = 0, JL_ROPE_HALVES = 1 } jl_rope_sty
  * Sums and products are in double precision and rounded to fp32, what q_out gets; the cache keeps
  * what its type makes of that fp32 value.  A JL_KV_F16 element is the binary16 nearest to it (infinite
  * where it is beyond binary16).  A block of JL_KV_Q8_0 has d = the binary16 nearest to max |x| / 127
- * (at most 65504) and bytes rint(x / d) in -127 ... 127; 0 where d is 0 or x is NaN.
+ * (at most 65504) and bytes rint(x / d) in -127 ... 127; 0 where d is 0 or x is NaN.  A block of
+ * JL_KV_Q4_0 has d = the binary16 nearest to x_m / -8 (at most 65504 in magnitude), x_m the first of its
+ * values of largest magnitude, and n = 8 + rint(x / d) in 0 ... 15; 8 where d is 0 or x is NaN.
  * Fewer than 2^24 rows, at most 65536 heads of q.
  */
 int jl_kv_append(jl_context *ctx, jl_kv_cache *cache, const float *q, int heads, int64_t ldq, const float *k,
@@ -578,6 +585,25 @@ int jl_kv_attention(jl_context *ctx, const jl_kv_cache *cache, const float *q, i
                     const int32_t *positions, const int32_t *row_requests, const int32_t *block_table,
                     int64_t requests, int64_t table_stride, float scale, int64_t window, void *out, int out_f16,
                     int64_t ldo, void *workspace, size_t workspace_bytes);
+
+/*
+ * The same with other scores and masks.  The score of a row at `position` and a token j is
+ *   s = scale * q[row][h] . k_j
+ *   s = cap * tanh(s / cap)                     where cap > 0
+ *   s = s - slopes[h] * |position - j|          where slopes ([heads] fp32, finite, on the device) is not null
+ * and the row sees first <= j < end, with first as above -- the window's -- or first_tokens[row] where that
+ * is later, and end = position + 1 or, where end_tokens is not null, end_tokens[row]: documents packed into
+ * one request keep to themselves by first_tokens, a prefix that all of its rows see is an end_tokens of
+ * max(position + 1, prefix).  Both are [rows] int32 on the device or null; a row whose end is not behind its
+ * first is zeros, and so is one without a position, whatever they say.  The tokens up to end have been
+ * written (what lies in a page that was not would be read).
+ * cap 0 (none) or 1e-30 ... 1e30; a score stays within fp32.  tanh is within 2^-21 of its value.
+ */
+int jl_kv_attention_scored(jl_context *ctx, const jl_kv_cache *cache, const float *q, int heads, int64_t ldq, int64_t rows,
+                           const int32_t *positions, const int32_t *row_requests, const int32_t *block_table,
+                           int64_t requests, int64_t table_stride, float scale, int64_t window, float cap,
+                           const float *slopes, const int32_t *first_tokens, const int32_t *end_tokens, void *out,
+                           int out_f16, int64_t ldo, void *workspace, size_t workspace_bytes);
 
 /* ---- GGUF files: the caller either side of jl_weight_upload --------------------------------- */
 

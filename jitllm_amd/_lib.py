@@ -15,7 +15,7 @@ JL_OK = 0
 JL_ERR_INVALID, JL_ERR_UNSUPPORTED, JL_ERR_HIP, JL_ERR_OOM, JL_ERR_WORKSPACE = -1, -2, -3, -4, -5
 JL_STORE, JL_RESIDUAL, JL_SWIGLU = 0, 1, 2
 JL_MATH_DEFAULT, JL_MATH_F16, JL_MATH_INT8 = 0, 1, 2
-JL_KV_F16, JL_KV_Q8_0 = 1, 8
+JL_KV_F16, JL_KV_Q4_0, JL_KV_Q8_0 = 1, 4, 8
 JL_ROPE_PAIRS, JL_ROPE_HALVES = 0, 1
 ABI_VERSION = 1
 
@@ -83,6 +83,8 @@ SYMBOLS = {
     "jl_kv_attention_workspace_init": (C.c_int, [vp, vp, C.c_size_t]),
     "jl_kv_attention": (C.c_int, [vp, vp, vp, C.c_int, i64, i64, vp, vp, vp, i64, i64, C.c_float, i64, vp, C.c_int,
                                   i64, vp, C.c_size_t]),
+    "jl_kv_attention_scored": (C.c_int, [vp, vp, vp, C.c_int, i64, i64, vp, vp, vp, i64, i64, C.c_float, i64, C.c_float,
+                                         vp, vp, vp, vp, C.c_int, i64, vp, C.c_size_t]),
     "jl_gguf_open": (C.c_int, [C.c_char_p, C.POINTER(vp)]),
     "jl_gguf_close": (C.c_int, [vp]),
     "jl_gguf_version": (C.c_int, [vp]),

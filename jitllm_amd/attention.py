@@ -36,6 +36,7 @@ from .runtime import Context, DeviceBuffer, HalfFloatArray
 class KvType(enum.IntEnum):
     """What a cache keeps of an element (jl_kv_type)."""
     F16 = L.JL_KV_F16
+    Q4_0 = L.JL_KV_Q4_0
     Q8_0 = L.JL_KV_Q8_0
 
 
@@ -259,11 +260,17 @@ class PagedAttention:
         L.check(self._lib.jl_kv_attention_workspace_init(ctx.handle, self.workspace.ptr, nbytes))
 
     def attend(self, cache: PagedKvCache, q, rows: int, positions, table, out, requests: int, rowRequests=None,
-               scale: float | None = None, window: int = 0, blocksPerRequest: int | None = None) -> None:
+               scale: float | None = None, window: int = 0, blocksPerRequest: int | None = None, cap: float = 0.0,
+               slopes=None, firstTokens=None, endTokens=None) -> None:
         """``out[row] = softmax(scale * q[row] . k) v`` over the tokens up to ``positions[row]`` (the last
         ``window`` of them where that is positive) of request ``rowRequests[row]``, or of request ``row``.
         ``scale``: 1 / sqrt(headDim) unless given.  ``out``: a FloatArray or a HalfFloatArray.  ``requests`` are
-        all of the table's rows, unless ``blocksPerRequest`` says how many entries a row has."""
+        all of the table's rows, unless ``blocksPerRequest`` says how many entries a row has.
+
+        Scores s become ``cap * tanh(s / cap)`` where ``cap`` is positive, and are then lowered by
+        ``slopes[head] * |position - token|`` (heads fp32).  ``firstTokens`` [rows]: the first token that a row may
+        see, its document's; ``endTokens`` [rows]: one behind the last, in place of its own
+        position's (jl_kv_attention_scored)."""
         if cache.kvHeads != self.kvHeads or cache.headDim != self.headDim:
             raise ValueError(f"a cache of {cache.kvHeads} heads of {cache.headDim}, attention over {self.kvHeads} of {self.headDim}")
         width = self.width
@@ -278,10 +285,21 @@ class PagedAttention:
                 raise ValueError(f"a block table of {entries} entries for {requests} requests: blocksPerRequest?")
         elif blocksPerRequest * requests > entries:
             raise ValueError(f"{requests} x {blocksPerRequest} entries of a block table of {entries}")
-        status = self._lib.jl_kv_attention(
-            self.ctx.handle, cache.handle, q, self.heads, ldq, rows, _ints("positions", positions, rows),
-            _ints("rowRequests", rowRequests, rows) if rowRequests is not None else None, table.ptr, requests,
-            blocksPerRequest, self.scale if scale is None else scale, window, out, half, ldOut,
-            self.workspace.ptr, self.workspace.nbytes)
+        positions = _ints("positions", positions, rows)
+        rowRequests = _ints("rowRequests", rowRequests, rows) if rowRequests is not None else None
+        scale = self.scale if scale is None else scale
+        if cap == 0.0 and slopes is None and firstTokens is None and endTokens is None:
+            status = self._lib.jl_kv_attention(
+                self.ctx.handle, cache.handle, q, self.heads, ldq, rows, positions, rowRequests, table.ptr, requests,
+                blocksPerRequest, scale, window, out, half, ldOut, self.workspace.ptr, self.workspace.nbytes)
+        else:
+            if slopes is not None and not slopes.size == self.heads == slopes.nbytes // 4:
+                raise ValueError(f"{slopes.size} slopes in {slopes.nbytes} bytes for {self.heads} heads")
+            status = self._lib.jl_kv_attention_scored(
+                self.ctx.handle, cache.handle, q, self.heads, ldq, rows, positions, rowRequests, table.ptr, requests,
+                blocksPerRequest, scale, window, cap, slopes.ptr if slopes is not None else None,
+                _ints("firstTokens", firstTokens, rows) if firstTokens is not None else None,
+                _ints("endTokens", endTokens, rows) if endTokens is not None else None, out, half, ldOut,
+                self.workspace.ptr, self.workspace.nbytes)
         if status:
             L.check(status)

@@ -19,7 +19,7 @@ struct jl_kv_cache {
 // Bytes of one head's part of a page.
 static inline int64_t jl_kv_part_bytes(int type, int head_dim, int page_tokens) {
     const int64_t values = (int64_t)head_dim * page_tokens;
-    return type == JL_KV_F16 ? 2 * values : values + values / 16;
+    return type == JL_KV_F16 ? 2 * values : (type == JL_KV_Q8_0 ? values : values / 2) + values / 16;
 }
 
 // A cache by value, for kernels' arguments.
@@ -56,11 +56,32 @@ __device__ __forceinline__ void jl_bytes_to_half(uint32_t q, jl_half2v &lo, jl_h
     hi = __builtin_bit_cast(jl_half2v, __builtin_amdgcn_perm(0x64646464u, b, 0x04030402u)) - bias;
 }
 
-// Eight consecutive values, from element 8 * chunk of a token's, of the part of a page at `part`.
-template <bool Q8>
-__device__ __forceinline__ jl_half8 jl_kv_load8(const uint8_t *part, int page_shift, int head_dim, int token, int chunk) {
-    if constexpr (!Q8) {
+// Where in a part of JL_KV_Q4_0 the eight elements from 8 * chunk on of a token's lie: keys' in four consecutive bytes, values'
+// in two, and two more eight bytes on.
+__device__ __forceinline__ uint32_t jl_q4_key_at(int head_dim, int token, int chunk) { return token * (head_dim / 2) + 4 * chunk; }
+__device__ __forceinline__ uint32_t jl_q4_value_at(int head_dim, int token, int chunk) {
+    return token / 4 * (2 * head_dim) + 16 * chunk + 2 * (token % 4);
+}
+
+// Eight consecutive values, from element 8 * chunk of a token's, of the part of a page of keys or values at `part`.
+template <int TYPE>
+__device__ __forceinline__ jl_half8 jl_kv_load8(const uint8_t *part, bool values, int page_shift, int head_dim, int token, int chunk) {
+    if constexpr (TYPE == JL_KV_F16) {
         return *(const jl_half8 *)(part + ((int64_t)token * head_dim + 8 * chunk) * 2);
+    } else if constexpr (TYPE == JL_KV_Q4_0) {
+        uint32_t q;
+        if (values) {
+            const uint8_t *at = part + jl_q4_value_at(head_dim, token, chunk);
+            q = *(const uint16_t *)at | (uint32_t)*(const uint16_t *)(at + 8) << 16;
+        } else {
+            q = *(const uint32_t *)(part + jl_q4_key_at(head_dim, token, chunk));
+        }
+        const _Float16 *scales = (const _Float16 *)(part + ((int64_t)(head_dim / 2) << page_shift));
+        const _Float16 d = scales[((chunk >> 2) << page_shift) + token];
+        jl_half8 r;
+#pragma unroll
+        for (int i = 0; i < 8; i++) r[i] = (_Float16)(int)((q >> 4 * i & 15) - 8) * d;
+        return r;
     } else {
         const uint2 q = *(const uint2 *)(part + token * head_dim + 8 * chunk);
         const _Float16 *scales = (const _Float16 *)(part + ((int64_t)head_dim << page_shift));

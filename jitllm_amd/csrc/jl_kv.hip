@@ -316,10 +316,11 @@ __device__ __forceinline__ double2 cos_sin_of_turns(double turns) {
 // Bound: the bytes.  The angles' cosines and sines are worked out once per workgroup, in LDS, while the loads come in.
 // Sums and products between the loads and the rounding to fp32 are in double precision, which the bytes hide; what the cache
 // keeps is rounded from that fp32 value.
-template <bool Q8, int LANES, bool HALVES>
+template <int TYPE, int LANES, bool HALVES>
 __global__ void __launch_bounds__(kAppendThreads) jl_kv_append_kernel(AppendArgs p) {
     __shared__ double2 turn[128];   // (cos, sin) of the token's pairs
-    __shared__ float turned[Q8 && HALVES ? kAppendThreads / LANES : 1][Q8 && HALVES ? 8 * LANES : 4];
+    constexpr bool kBlocks = TYPE != JL_KV_F16;
+    __shared__ float turned[kBlocks && HALVES ? kAppendThreads / LANES : 1][kBlocks && HALVES ? 8 * LANES : 4];
     const int row = blockIdx.x, tid = threadIdx.x;
     const int position = p.positions[row];
     if (position < 0) return;
@@ -394,7 +395,7 @@ __global__ void __launch_bounds__(kAppendThreads) jl_kv_append_kernel(AppendArgs
         const int page = slot >> p.cache.page_shift, token = slot & ((1 << p.cache.page_shift) - 1);
         uint8_t *part = p.cache.k + (is_v ? p.cache.v_offset : 0) +
                         ((int64_t)page * kv_heads + (is_v ? unit - p.heads - kv_heads : unit - p.heads)) * p.cache.part_bytes;
-        if constexpr (!Q8) {
+        if constexpr (!kBlocks) {
             _Float16 *to = (_Float16 *)part + token * p.head_dim;
             const jl_half4v low = {(_Float16)a[0], (_Float16)a[1], (_Float16)a[2], (_Float16)a[3]};
             const jl_half4v high = {(_Float16)a[4], (_Float16)a[5], (_Float16)a[6], (_Float16)a[7]};
@@ -415,6 +416,39 @@ __global__ void __launch_bounds__(kAppendThreads) jl_kv_append_kernel(AppendArgs
                     a[0] = low.x, a[1] = low.y, a[2] = low.z, a[3] = low.w, a[4] = high.x, a[5] = high.y, a[6] = high.z, a[7] = high.w;
                 }
                 __builtin_amdgcn_wave_barrier();
+            }
+            if constexpr (TYPE == JL_KV_Q4_0) {
+                // the value of largest magnitude of the block, four lanes' values, the first of several; NaN is none
+                float largest = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; i++) largest = fabsf(a[i]) > fabsf(largest) ? a[i] : largest;
+#pragma unroll
+                for (int off = 1; off <= 2; off <<= 1) {
+                    const float other = __shfl_xor(largest, off, JL_WAVE);
+                    const bool takes = fabsf(other) > fabsf(largest) || (fabsf(other) == fabsf(largest) && (chunk & off));
+                    largest = takes ? other : largest;
+                }
+                const _Float16 d16 = (_Float16)fminf(fmaxf(largest * -0.125f, -65504.f), 65504.f);
+                const float d = (float)d16;
+                uint32_t word = 0;
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float y = d != 0.f && a[i] == a[i] ? fminf(fmaxf(rintf(a[i] / d), -8.f), 7.f) : 0.f;
+                    word |= (uint32_t)((int)y + 8) << 4 * i;
+                }
+                if (in_head) {
+                    if (is_v) {
+                        uint8_t *at = part + jl_q4_value_at(p.head_dim, token, chunk);
+                        *(uint16_t *)at = (uint16_t)word, *(uint16_t *)(at + 8) = (uint16_t)(word >> 16);
+                    } else {
+                        *(uint32_t *)(part + jl_q4_key_at(p.head_dim, token, chunk)) = word;
+                    }
+                    if (chunk % 4 == 0) {
+                        _Float16 *scales = (_Float16 *)(part + ((int64_t)(p.head_dim / 2) << p.cache.page_shift));
+                        scales[((chunk / 4) << p.cache.page_shift) + token] = d16;
+                    }
+                }
+                continue;
             }
             float most = 0.f;
 #pragma unroll
@@ -443,7 +477,7 @@ __global__ void __launch_bounds__(kAppendThreads) jl_kv_append_kernel(AppendArgs
 
 // ---- jl_kv_read ----------------------------------------------------------------------------------
 
-template <bool Q8, bool HALF>
+template <int TYPE, bool HALF>
 __global__ void __launch_bounds__(256) jl_kv_read_kernel(JlKvView cache, int head_dim, const int32_t *slots, int64_t rows,
                                                          void *k_out, void *v_out) {
     const int per_head = head_dim / 8, per_row = cache.kv_heads * per_head;
@@ -458,7 +492,7 @@ __global__ void __launch_bounds__(256) jl_kv_read_kernel(JlKvView cache, int hea
         void *out = which ? v_out : k_out;
         if (!out) continue;
         jl_half8 h = {0, 0, 0, 0, 0, 0, 0, 0};
-        if (slot >= 0 && page < cache.pages) h = jl_kv_load8<Q8>(part + (which ? cache.v_offset : 0), cache.page_shift, head_dim, token, chunk);
+        if (slot >= 0 && page < cache.pages) h = jl_kv_load8<TYPE>(part + (which ? cache.v_offset : 0), which, cache.page_shift, head_dim, token, chunk);
         if constexpr (HALF) {
             ((jl_half8 *)out)[at] = h;
         } else {
@@ -469,8 +503,8 @@ __global__ void __launch_bounds__(256) jl_kv_read_kernel(JlKvView cache, int hea
 }
 
 int cache_check(const char *who, int kv_type, int64_t pages, int kv_heads, int head_dim, int page_tokens) {
-    if (kv_type != JL_KV_F16 && kv_type != JL_KV_Q8_0)
-        return jl_fail(JL_ERR_UNSUPPORTED, "%s: no key-value cache of type %d (JL_KV_F16 or JL_KV_Q8_0)", who, kv_type);
+    if (kv_type != JL_KV_F16 && kv_type != JL_KV_Q8_0 && kv_type != JL_KV_Q4_0)
+        return jl_fail(JL_ERR_UNSUPPORTED, "%s: no key-value cache of type %d (JL_KV_F16, JL_KV_Q8_0 or JL_KV_Q4_0)", who, kv_type);
     if (head_dim != 64 && head_dim != 96 && head_dim != 128 && head_dim != 192 && head_dim != 256)
         return jl_fail(JL_ERR_UNSUPPORTED, "%s: no kernel for heads of %d values (64, 96, 128, 192 or 256)", who, head_dim);
     JL_REQUIRE(page_tokens == 16 || page_tokens == 32 || page_tokens == 64 || page_tokens == 128 || page_tokens == 256,
@@ -502,16 +536,16 @@ int cache_make(const char *who, jl_context *ctx, void *memory, int kv_type, int6
     return JL_OK;
 }
 
-template <bool Q8, int LANES, bool HALVES>
+template <int TYPE, int LANES, bool HALVES>
 void launch_append_lanes(const AppendArgs &a, unsigned rows, hipStream_t stream) {
     const int units = a.heads + 2 * a.cache.kv_heads, per = kAppendPer * (kAppendThreads / LANES);
-    hipLaunchKernelGGL((jl_kv_append_kernel<Q8, LANES, HALVES>), dim3(rows, (unsigned)((units + per - 1) / per)), dim3(kAppendThreads), 0, stream, a);
+    hipLaunchKernelGGL((jl_kv_append_kernel<TYPE, LANES, HALVES>), dim3(rows, (unsigned)((units + per - 1) / per)), dim3(kAppendThreads), 0, stream, a);
 }
-template <bool Q8, bool HALVES>
+template <int TYPE, bool HALVES>
 void launch_append(const AppendArgs &a, unsigned rows, hipStream_t stream) {
-    if (a.head_dim <= 64) launch_append_lanes<Q8, 8, HALVES>(a, rows, stream);
-    else if (a.head_dim <= 128) launch_append_lanes<Q8, 16, HALVES>(a, rows, stream);
-    else launch_append_lanes<Q8, 32, HALVES>(a, rows, stream);
+    if (a.head_dim <= 64) launch_append_lanes<TYPE, 8, HALVES>(a, rows, stream);
+    else if (a.head_dim <= 128) launch_append_lanes<TYPE, 16, HALVES>(a, rows, stream);
+    else launch_append_lanes<TYPE, 32, HALVES>(a, rows, stream);
 }
 
 bool aligned(const void *p, int to) { return ((uintptr_t)p & (to - 1)) == 0; }
@@ -611,8 +645,9 @@ int jl_kv_append(jl_context *ctx, jl_kv_cache *cache, const float *q, int heads,
     a.heads = q ? heads : 0, a.head_dim = dim, a.rotated = rotated;
     const bool halves = rope_style == JL_ROPE_HALVES && rotated > 0;
     const unsigned n = (unsigned)rows;
-    if (cache->type == JL_KV_Q8_0) halves ? launch_append<true, true>(a, n, ctx->stream) : launch_append<true, false>(a, n, ctx->stream);
-    else halves ? launch_append<false, true>(a, n, ctx->stream) : launch_append<false, false>(a, n, ctx->stream);
+    if (cache->type == JL_KV_Q8_0) halves ? launch_append<JL_KV_Q8_0, true>(a, n, ctx->stream) : launch_append<JL_KV_Q8_0, false>(a, n, ctx->stream);
+    else if (cache->type == JL_KV_Q4_0) halves ? launch_append<JL_KV_Q4_0, true>(a, n, ctx->stream) : launch_append<JL_KV_Q4_0, false>(a, n, ctx->stream);
+    else halves ? launch_append<JL_KV_F16, true>(a, n, ctx->stream) : launch_append<JL_KV_F16, false>(a, n, ctx->stream);
     JL_HIP(hipGetLastError());
     return JL_OK;
 }
@@ -633,13 +668,13 @@ int jl_kv_read(jl_context *ctx, const jl_kv_cache *cache, const int32_t *slots, 
     const dim3 grid((unsigned)((threads + 255) / 256)), block(256);
     const JlKvView c = jl_kv_view(cache);
     const int dim = cache->head_dim;
-    if (cache->type == JL_KV_Q8_0) {
-        if (out_f16) hipLaunchKernelGGL((jl_kv_read_kernel<true, true>), grid, block, 0, ctx->stream, c, dim, slots, rows, k_out, v_out);
-        else hipLaunchKernelGGL((jl_kv_read_kernel<true, false>), grid, block, 0, ctx->stream, c, dim, slots, rows, k_out, v_out);
-    } else {
-        if (out_f16) hipLaunchKernelGGL((jl_kv_read_kernel<false, true>), grid, block, 0, ctx->stream, c, dim, slots, rows, k_out, v_out);
-        else hipLaunchKernelGGL((jl_kv_read_kernel<false, false>), grid, block, 0, ctx->stream, c, dim, slots, rows, k_out, v_out);
-    }
+    auto launch = [&](auto type, auto half) {
+        hipLaunchKernelGGL((jl_kv_read_kernel<decltype(type)::value, decltype(half)::value>), grid, block, 0, ctx->stream, c, dim, slots, rows, k_out, v_out);
+    };
+    auto launch_type = [&](auto type) { out_f16 ? launch(type, std::true_type{}) : launch(type, std::false_type{}); };
+    if (cache->type == JL_KV_Q8_0) launch_type(std::integral_constant<int, JL_KV_Q8_0>{});
+    else if (cache->type == JL_KV_Q4_0) launch_type(std::integral_constant<int, JL_KV_Q4_0>{});
+    else launch_type(std::integral_constant<int, JL_KV_F16>{});
     JL_HIP(hipGetLastError());
     return JL_OK;
 }
