@@ -273,6 +273,30 @@ int jl_gemv_argmax(jl_context *ctx, const jl_weight *w, const float *x, const fl
 #define JL_ARGMAX_STATIC_MAX_VALUES ((int64_t)1 << 24)
 int jl_argmax_static(jl_context *ctx, const float *values, int64_t n, int32_t *index);
 
+/*
+ * What a server answers with beside the tokens: for each of `rows` rows of n logits, `row_stride` floats
+ * apart, with x = logit, or cap * tanh(logit / cap) where cap > 0, and p = softmax(scale * x),
+ *   logprobs [rows x tokens_per_row]   log p of the row's tokens[rows x tokens_per_row]; 0 for a token
+ *                                      outside 0 ... n - 1.  tokens_per_row 0: both may be null
+ *   entropy [rows]                     -sum p log p; may be null
+ *   top_tokens, top_logprobs [rows x top]  the tokens of the `top` largest logits, the largest first and of
+ *                                      equal ones the lowest, and log p of each.  top 0: both may be null
+ * in one pass over the logits.  A logit of -infinity is a token that is left out, with or without a cap: its
+ * log p is -infinity, and it adds nothing.  Where all are, all log p are -infinity and the entropy is 0.  A
+ * NaN is in no list (places that are left over have token -1 and -infinity) and makes its row's log p
+ * and entropy NaN, as +infinity without a cap does.
+ * scale: 1 / temperature, positive.  cap: 0 (none) or 1e-30 ... 1e30.  top: at most 64, and n.  At most
+ * 2^31 - 1 rows of 2^31 - 1 logits, 65536 tokens a row.  Sums are fp32; the same call gives the same bits.
+ * workspace: jl_logprobs_workspace_bytes of the largest n and top that use it, 16-byte aligned, which
+ * jl_logprobs_workspace_init has been over once (on the stream, before the first call; every call leaves it
+ * as it needs it).  Calls that may run at the same time need one each.
+ */
+size_t jl_logprobs_workspace_bytes(int64_t n, int top);
+int jl_logprobs_workspace_init(jl_context *ctx, void *workspace, size_t workspace_bytes);
+int jl_logprobs(jl_context *ctx, const float *logits, int64_t rows, int64_t n, int64_t row_stride, float scale, float cap,
+                const int32_t *tokens, int64_t tokens_per_row, float *logprobs, float *entropy, int top,
+                int32_t *top_tokens, float *top_logprobs, void *workspace, size_t workspace_bytes);
+
 /* ---- packed-activation ("dp4a") decode: faster, looser -------------------------------------- */
 /*
  * The reference's optional packed-integer decode path (QuantizedProjections.packed(),

@@ -59,6 +59,9 @@ SYMBOLS = {
     "jl_argmax_rows": (C.c_int, [vp, vp, i64, i64, i64, vp]),
     "jl_gemv_argmax": (C.c_int, [vp, vp, vp, vp, vp, C.c_float, vp, vp]),
     "jl_argmax_static": (C.c_int, [vp, vp, i64, vp]),
+    "jl_logprobs_workspace_bytes": (C.c_size_t, [i64, C.c_int]),
+    "jl_logprobs_workspace_init": (C.c_int, [vp, vp, C.c_size_t]),
+    "jl_logprobs": (C.c_int, [vp, vp, i64, i64, i64, C.c_float, C.c_float, vp, i64, vp, vp, C.c_int, vp, vp, vp, C.c_size_t]),
     "jl_quantize_q8": (C.c_int, [vp, vp, i64, vp, vp, vp]),
     "jl_rms_quantize_q8": (C.c_int, [vp, vp, vp, vp, i64, vp, vp, vp, vp]),
     "jl_gemv_q8": (C.c_int, [vp, vp, vp, vp, vp, vp, C.c_int]),

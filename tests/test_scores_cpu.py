@@ -60,6 +60,39 @@ def test_scored_of_nothing(L, lib, ctx, memory, cache):  # noqa: F811
     assert lib.jl_kv_attention_scored(None, cache, *args) == lib.jl_kv_attention_scored(ctx, None, *args) == L.JL_ERR_INVALID
 
 
+LOGPROBS = dict(logits="m", rows=0, n=100, row_stride=100, scale=1.0, cap=0.0, tokens="m", tokens_per_row=1, logprobs="m", entropy="m", top=5, top_tokens="m",
+                top_logprobs="m", workspace="m", workspace_bytes=1 << 40)
+
+
+@pytest.mark.parametrize("change,words", [
+    (dict(logits=None), "null"), (dict(workspace=None), "null"), (dict(rows=-1), "-1 rows"), (dict(rows=2**31), "rows"), (dict(n=0), "0 logits"),
+    (dict(n=2**31, row_stride=2**31), "2147483648 logits"), (dict(row_stride=99), "closer together"), (dict(scale=0.0), "scale 0"), (dict(scale=-1.0), "scale -1"),
+    (dict(scale=float("nan")), "scale nan"), (dict(scale=float("inf")), "scale inf"), (dict(scale=3e38), "scale"), (dict(scale=1e-40), "scale"),
+    (dict(cap=-2.0), "cap -2"), (dict(cap=float("nan")), "cap nan"), (dict(cap=1e31), "cap 1e+31"), (dict(tokens_per_row=-1), "-1 tokens"),
+    (dict(tokens_per_row=65537), "65537 tokens"), (dict(tokens=None), "null tokens"), (dict(logprobs=None), "null tokens"), (dict(top=-1), "-1 most"),
+    (dict(top=65), "65 most"), (dict(n=4, top=5), "5 most probable of 4"), (dict(top_tokens=None), "null top"), (dict(top_logprobs=None), "null top"),
+    (dict(logits="odd"), "aligned"), (dict(workspace="odd"), "aligned"), (dict(tokens="odd"), "aligned"), (dict(top_logprobs="odd"), "aligned")])
+def test_logprobs_refusals(L, lib, ctx, memory, change, words):  # noqa: F811
+    at = {"m": memory, "odd": memory + 2}
+    args = [at.get(v, v) if isinstance(v, str) else v for v in {**LOGPROBS, **change}.values()]
+    assert lib.jl_logprobs(ctx, *args) == L.JL_ERR_INVALID and words in said(lib), said(lib)
+
+
+def test_logprobs_workspace(L, lib, ctx, memory):  # noqa: F811
+    need = lib.jl_logprobs_workspace_bytes(100, 5)
+    assert 0 < need < 1 << 26
+    assert lib.jl_logprobs_workspace_bytes(0, 0) == lib.jl_logprobs_workspace_bytes(2**31, 0) == lib.jl_logprobs_workspace_bytes(9, -1) == 0
+    assert lib.jl_logprobs_workspace_bytes(100, 65) == 0
+    args = lambda **more: [memory if v == "m" else v for v in {**LOGPROBS, **more}.values()]      # noqa: E731
+    assert lib.jl_logprobs(ctx, *args(workspace_bytes=need - 1)) == L.JL_ERR_WORKSPACE
+    assert lib.jl_logprobs(ctx, *args(workspace_bytes=need)) == L.JL_OK                           # no rows: nothing to do
+    assert lib.jl_logprobs(ctx, *args(tokens_per_row=0, tokens=None, logprobs=None, entropy=None, top=0, top_tokens=None, top_logprobs=None)) == L.JL_OK
+    assert lib.jl_logprobs(None, *args()) == L.JL_ERR_INVALID
+    assert lib.jl_logprobs_workspace_init(None, memory, 1 << 20) == lib.jl_logprobs_workspace_init(ctx, None, 1 << 20) == L.JL_ERR_INVALID
+    assert lib.jl_logprobs_workspace_init(ctx, memory + 4, 1 << 20) == L.JL_ERR_INVALID
+    assert lib.jl_logprobs_workspace_init(ctx, memory, 8) == L.JL_ERR_WORKSPACE
+
+
 class Array:
     def __init__(self, size, itemsize=4):
         self.size, self.nbytes, self.ptr = size, size * itemsize, C.c_void_p(4096)
@@ -95,6 +128,31 @@ def test_binding_of_scored_attention(monkeypatch):
     for more in (dict(slopes=Array(5)), dict(slopes=Array(4, 2)), dict(firstTokens=Array(1)), dict(endTokens=Array(1))):
         with pytest.raises(ValueError):
             attend(**more)
+
+
+def test_binding_of_logprobs():
+    from jitllm_amd.logits import LogProbabilities
+    calls = []
+
+    class Lib:
+        def jl_logprobs(self, *args):
+            calls.append(args)
+            return 0
+
+    class Ctx:
+        handle, _lib = None, Lib()
+
+    p = object.__new__(LogProbabilities)
+    p.ctx, p._lib, p.vocab, p.top, p.workspace = Ctx(), Lib(), 100, 3, Array(10)
+    p.compute(Array(400), 4, tokens=Array(4), logprobs=Array(4), entropy=Array(4), topTokens=Array(12), topLogprobs=Array(12))
+    assert calls[-1][8] == 1 and calls[-1][11] == 3
+    p.compute(Array(400), 4)
+    assert calls[-1][8] == 0 and calls[-1][11] == 0
+    p.compute(Array(1), 0)
+    for more in (dict(tokens=Array(4)), dict(logprobs=Array(4)), dict(topTokens=Array(12)), dict(tokens=Array(3), logprobs=Array(4)), dict(entropy=Array(3)),
+                 dict(tokens=Array(4), logprobs=Array(4), tokensPerRow=2), dict(topTokens=Array(12), topLogprobs=Array(11)), dict(rowStride=99), dict(rowStride=101)):
+        with pytest.raises(ValueError):
+            p.compute(Array(400), 4, **more)
 
 
 def test_models_of_scores_agree_with_each_other():
