@@ -285,8 +285,8 @@ int jl_argmax_static(jl_context *ctx, const float *values, int64_t n, int32_t *i
  * log p is -infinity, and it adds nothing.  Where all are, all log p are -infinity and the entropy is 0.  A
  * NaN is in no list (places that are left over have token -1 and -infinity) and makes its row's log p
  * and entropy NaN, as +infinity without a cap does.
- * scale: 1 / temperature, positive.  cap: 0 (none) or 1e-30 ... 1e30.  top: at most 64, and n.  At most
- * 2^31 - 1 rows of 2^31 - 1 logits, 65536 tokens a row.  Sums are fp32; the same call gives the same bits.
+ * scale: 1 / temperature, positive.  cap: 0 (none) or 1e-30 ... 1e30.  top: at most 64, and n.  Fewer than
+ * 2^24 rows of at most 2^30 logits, 65536 tokens a row.  Sums are fp32; the same call gives the same bits.
  * workspace: jl_logprobs_workspace_bytes of the largest n and top that use it, 16-byte aligned, which
  * jl_logprobs_workspace_init has been over once (on the stream, before the first call; every call leaves it
  * as it needs it).  Calls that may run at the same time need one each.

@@ -1,7 +1,18 @@
 // jl_logprobs: log probabilities of given tokens, the entropy and the most probable tokens, of rows of logits.
 //
-// Mathematics.  x = l, or cap tanh(l / cap); m = max x; S = sum e^(scale (x - m)); T = sum e^(scale (x - m)) scale (x - m).
-// Then log p(t) = scale (x_t - m) - log S and the entropy is log S - T / S.  The list is by l, equal ones by their index.
+// Mathematics.  x = l, or cap tanh(l / cap); m = max x; with a = scale log2(e) (x - m), S = sum 2^a and T = sum 2^a a.  Then
+// log p(t) = scale (x_t - m) - log S and the entropy is log S - log(2) T / S.  Two parts (m, S, T) of a row join by bringing
+// both to the larger m: S by 2^d and T by (T + S d) 2^d, d = scale log2(e) (m - m').  The list is by l, equal ones by
+// their index: one 64-bit key that is larger for the one that comes first.
+//
+// Bound: the bytes of the logits, once.  A wave goes through its part in steps of 16 values a lane, the next step's on their
+// way; each lane has a running m, S and T.  For the list the wave keeps the 64 largest keys so far, sorted, one a lane: a
+// step none of whose values is larger than the last one that is wanted costs one comparison.  From others the larger ones are
+// gathered in LDS, and every 64 sorted and merged in.  The first step, and any that would gather more than 64, first sorts its lanes'
+// largest: of the top ones of those there are as many as are wanted, so that nothing smaller than the last of them is.
+//
+// Work.  A workgroup of four waves a row (one wave where rows are short); where rows are few each is cut into parts, and the workgroup that
+// is done last with a row joins them, in their order whoever that is (nobody waits for anybody).
 #include <algorithm>
 #include <cfloat>
 #include <climits>
@@ -14,15 +25,28 @@
 
 namespace {
 
-constexpr int kThreads = 256, kWaves = kThreads / JL_WAVE;
-constexpr int kMostTop = 64;
+constexpr int kMostTop = JL_WAVE;                 // a lane each
+constexpr int kEach = 4;                          // loads of four values a lane and step
+constexpr int kStepFours = kEach * JL_WAVE;       // fours of a wave's step
+constexpr int kMostParts = 32;                    // of a row; a wave of the last workgroup has kPartsEach of them
+constexpr int kPartsEach = kMostParts / 4;
+constexpr int kPartsRows = 512;                   // rows that are cut
+constexpr int kGroups = 512;                      // workgroups that a launch of few rows has, about
+constexpr int kShortRow = 2048;                   // logits of a row that one wave has
+constexpr int64_t kMostLogits = 1 << 30;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
+
+struct Part {
+    uint64_t keys[kMostTop];
+    float most, sum, weighted, unused;
+};
 
 struct LogprobsArgs {
     const float *logits;
     int64_t stride;
     int n;
-    float scale;
+    int parts, fours_each;        // parts of a row, and fours of a part: whole steps of a workgroup
+    float scale, power;           // power: scale log2(e)
     float cap, one_over_cap;      // 0: none
     const int32_t *tokens;
     int tokens_per_row;
@@ -30,6 +54,8 @@ struct LogprobsArgs {
     int top;
     int32_t *top_tokens;
     float *top_logprobs;
+    uint32_t *arrived;            // [kPartsRows], all 0 between calls
+    Part *part;                   // [rows * parts]
 };
 
 // A logit of -infinity is a token that is left out, and stays one.
@@ -43,72 +69,297 @@ __device__ __forceinline__ uint64_t key_of(float l, int at) {
     const uint32_t order = b & 0x80000000u ? ~b : b | 0x80000000u;
     return l == l ? (uint64_t)order << 32 | (uint32_t)~at : 0;
 }
+__device__ __forceinline__ float logit_of(uint64_t key) {
+    const uint32_t order = (uint32_t)(key >> 32);
+    return __uint_as_float(order & 0x80000000u ? order & 0x7fffffffu : ~order);
+}
 
-__global__ void __launch_bounds__(kThreads) jl_logprobs_kernel(LogprobsArgs p) {
-    __shared__ float part[3][kWaves];
-    __shared__ uint64_t best_of[kWaves];
-    const int tid = threadIdx.x, lane = tid % JL_WAVE, wave = tid / JL_WAVE;
-    const int64_t row = blockIdx.x;
-    const float *l = p.logits + row * p.stride;
-    float most = -FLT_MAX;
-    for (int i = tid; i < p.n; i += kThreads) most = fmaxf(most, capped(p, l[i]));
-    for (int off = JL_WAVE / 2; off; off >>= 1) most = fmaxf(most, __shfl_xor(most, off, JL_WAVE));
-    if (lane == 0) part[0][wave] = most;
-    __syncthreads();
-    for (int w = 0; w < kWaves; w++) most = fmaxf(most, part[0][w]);
-    float s = 0.f, t = 0.f;
-    for (int i = tid; i < p.n; i += kThreads) {
-        const float below = (capped(p, l[i]) - most) * (p.scale * kLog2e), a = below < -200.f ? -200.f : below;
-        const float e = __builtin_amdgcn_exp2f(a);
-        s += e, t += e * a;
+// The value of lane ^ N, by moves between lanes alone.
+template <int N>
+__device__ __forceinline__ uint32_t lane_xor(uint32_t x, int lane) {
+#define JL_MOVE(X, CONTROL) (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(X), CONTROL, 0xF, 0xF, true)
+    if constexpr (N == 1) return JL_MOVE(x, 0xB1);                        // quad_perm 1 0 3 2
+    if constexpr (N == 2) return JL_MOVE(x, 0x4E);                        // quad_perm 2 3 0 1
+    if constexpr (N == 4) return JL_MOVE(JL_MOVE(x, 0x141), 0x1B);        // row_half_mirror (^ 7), quad_perm 3 2 1 0 (^ 3)
+    if constexpr (N == 8) return JL_MOVE(x, 0x128);                       // row_ror 8
+#undef JL_MOVE
+    if constexpr (N == 16) {
+        const auto f = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+        return lane & 16 ? f[0] : f[1];
     }
-    for (int off = JL_WAVE / 2; off; off >>= 1) s += __shfl_xor(s, off, JL_WAVE), t += __shfl_xor(t, off, JL_WAVE);
-    if (lane == 0) part[1][wave] = s, part[2][wave] = t;
-    __syncthreads();
-    s = t = 0.f;
-    for (int w = 0; w < kWaves; w++) s += part[1][w], t += part[2][w];
-    const float log_sum = logf(s);
-    auto logprob = [&](float logit) { return s == 0.f ? -INFINITY : (capped(p, logit) - most) * p.scale - log_sum; };
-    if (tid == 0 && p.entropy) p.entropy[row] = s == 0.f ? 0.f : log_sum - t / s * kLn2;
-    for (int i = tid; i < p.tokens_per_row; i += kThreads) {
+    if constexpr (N == 32) {
+        const auto f = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+        return lane & 32 ? f[0] : f[1];
+    }
+    return x;
+}
+template <int N>
+__device__ __forceinline__ uint64_t lane_xor(uint64_t x, int lane) {
+    return (uint64_t)lane_xor<N>((uint32_t)(x >> 32), lane) << 32 | lane_xor<N>((uint32_t)x, lane);
+}
+template <int N>
+__device__ __forceinline__ float lane_xor(float x, int lane) { return __uint_as_float(lane_xor<N>(__float_as_uint(x), lane)); }
+
+// One step of a sorting network: of the pair (lane, lane ^ N) this lane keeps the larger key where `larger`.
+template <int N>
+__device__ __forceinline__ uint64_t keep_of_pair(uint64_t own, bool larger, int lane) {
+    const uint64_t other = lane_xor<N>(own, lane);
+    return (other > own) == larger ? other : own;
+}
+// A sequence that rises and then falls, or the other way round, into a falling one.
+template <int FROM = 32>
+__device__ __forceinline__ uint64_t bitonic_to_falling(uint64_t key, bool falling, int lane) {
+    key = keep_of_pair<FROM>(key, ((lane & FROM) == 0) == falling, lane);
+    if constexpr (FROM > 1) return bitonic_to_falling<FROM / 2>(key, falling, lane);
+    else return key;
+}
+// Sorted over the wave's lanes, rising.
+__device__ __forceinline__ uint64_t sorted_rising(uint64_t key, int lane) {
+    key = bitonic_to_falling<1>(key, (lane & 2) == 0, lane);
+    key = bitonic_to_falling<2>(key, (lane & 4) == 0, lane);
+    key = bitonic_to_falling<4>(key, (lane & 8) == 0, lane);
+    key = bitonic_to_falling<8>(key, (lane & 16) == 0, lane);
+    key = bitonic_to_falling<16>(key, (lane & 32) == 0, lane);
+    return bitonic_to_falling<32>(key, false, lane);
+}
+// The 64 largest of a falling and a rising sequence of 64, falling.
+__device__ __forceinline__ uint64_t merged(uint64_t falling, uint64_t rising, int lane) {
+    return bitonic_to_falling(falling > rising ? falling : rising, true, lane);
+}
+__device__ __forceinline__ uint64_t key_of_lane(uint64_t key, int lane) {   // (`lane` the same in all)
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(key >> 32), lane) << 32 |
+           (uint32_t)__builtin_amdgcn_readlane((int)key, lane);
+}
+
+// What of a difference of two values times the power: 0 where 2^it is, so that it times that is no NaN (NaN stays).
+__device__ __forceinline__ float exponent_of(float below) { return below < -200.f ? -200.f : below; }
+
+__device__ __forceinline__ void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+struct Sums {
+    float most = -FLT_MAX, sum = 0.f, weighted = 0.f;
+    __device__ __forceinline__ void bring_to(float other_most, float power) {
+        const float d = exponent_of((most - other_most) * power), share = __builtin_amdgcn_exp2f(d);
+        weighted = fmaf(sum, d, weighted) * share;
+        sum *= share;
+        most = other_most;
+    }
+    __device__ __forceinline__ void join(Sums other, float power) {
+        const float top = fmaxf(most, other.most);
+        bring_to(top, power), other.bring_to(top, power);
+        sum += other.sum, weighted += other.weighted;
+    }
+    template <int N>
+    __device__ __forceinline__ Sums of_lane_xor(int lane) const {
+        Sums s;
+        s.most = lane_xor<N>(most, lane), s.sum = lane_xor<N>(sum, lane), s.weighted = lane_xor<N>(weighted, lane);
+        return s;
+    }
+    // over the wave, in every lane
+    __device__ __forceinline__ void join_lanes(float power, int lane) {
+        join(of_lane_xor<1>(lane), power), join(of_lane_xor<2>(lane), power), join(of_lane_xor<4>(lane), power);
+        join(of_lane_xor<8>(lane), power), join(of_lane_xor<16>(lane), power), join(of_lane_xor<32>(lane), power);
+    }
+};
+
+template <int WAVES, bool TOP>
+__global__ void __launch_bounds__(WAVES * JL_WAVE) jl_logprobs_kernel(LogprobsArgs p) {
+    __shared__ uint64_t gathered[WAVES][TOP ? 2 * JL_WAVE : 1];
+    __shared__ uint64_t lists[WAVES][TOP ? JL_WAVE : 1];
+    __shared__ float sums_of[WAVES][3];
+    __shared__ uint32_t arrived;
+    const int tid = threadIdx.x, lane = tid % JL_WAVE, wave = __builtin_amdgcn_readfirstlane(tid / JL_WAVE);
+    const int64_t row = blockIdx.x / p.parts;
+    const int part = blockIdx.x % p.parts;
+    const float *l = p.logits + row * p.stride;
+    const int off = (int)((uintptr_t)l / 4 % 4);              // fours lie on 16-byte boundaries: the first begins this many before the row
+    const int fours = (p.n + off + 3) / 4, end = min((part + 1) * p.fours_each, fours);
+
+    uint64_t list = 0, gate = 0;                              // falling over the lanes; the last that is wanted
+    float gate_logit = -INFINITY;                             // ... as a logit, where the list is full
+    int count = 0;                                            // keys in `gathered`
+    Sums own;
+
+    auto load = [&](int four, float (&x)[4 * kEach]) {
+        const bool whole = 4 * four - off >= 0 && 4 * (four + kStepFours) - off <= p.n;
+#pragma unroll
+        for (int j = 0; j < kEach; j++) {
+            const int first = 4 * (four + j * JL_WAVE + lane) - off;
+            if (whole) {
+                const float4 v = *(const float4 *)(l + first);
+                x[4 * j] = v.x, x[4 * j + 1] = v.y, x[4 * j + 2] = v.z, x[4 * j + 3] = v.w;
+            } else {
+#pragma unroll
+                for (int c = 0; c < 4; c++) x[4 * j + c] = (unsigned)(first + c) < (unsigned)p.n ? l[first + c] : -INFINITY;
+            }
+        }
+    };
+    auto flush = [&]() {
+        // (between lanes of one wave, whose LDS accesses come in order)
+        wave_fence();
+        const uint64_t key = lane < count ? gathered[wave][lane] : 0, rest = gathered[wave][JL_WAVE + lane];
+        wave_fence();
+        gathered[wave][lane] = rest;
+        wave_fence();
+        count = max(count - JL_WAVE, 0);
+        list = merged(list, sorted_rising(key, lane), lane);
+        gate = key_of_lane(list, p.top - 1);
+        gate_logit = gate ? logit_of(gate) : -INFINITY;
+    };
+    auto gather = [&](int four, const float (&x)[4 * kEach]) {
+        auto key_at = [&](int i) {
+            const int at = 4 * (four + i / 4 * JL_WAVE + lane) - off + i % 4;
+            return (unsigned)at < (unsigned)p.n ? key_of(x[i], at) : 0;
+        };
+        uint64_t least = gate;                                // keys above it are gathered
+        uint64_t largest = 0;
+        int passing = 0;
+#pragma unroll
+        for (int i = 0; i < 4 * kEach; i++) {
+            const uint64_t key = key_at(i);
+            largest = key > largest ? key : largest;
+            passing += __popcll(__ballot(key > gate));
+        }
+        if (passing > JL_WAVE) {
+            const uint64_t last = key_of_lane(sorted_rising(largest, lane), JL_WAVE - p.top);   // one that is wanted itself
+            least = last > least ? last - 1 : least;
+        }
+#pragma unroll
+        for (int i = 0; i < 4 * kEach; i++) {
+            const uint64_t key = key_at(i);
+            const bool wanted = key > least && key > gate;
+            const uint64_t mask = __ballot(wanted);
+            if (mask == 0) continue;
+            if (wanted) gathered[wave][count + __popcll(mask & ((1ull << lane) - 1))] = key;
+            count += __popcll(mask);
+            if (count >= JL_WAVE) flush();
+        }
+        // the gate follows at once where the list is not full: all that is behind it would pass
+        if (gate == 0 && count > 0) flush();
+    };
+
+    float x[4 * kEach];
+    int four = part * p.fours_each + wave * kStepFours;
+    if (four < end) load(four, x);
+    while (four < end) {
+        float next[4 * kEach];
+        const int next_four = four + WAVES * kStepFours;
+        if (next_four < end) load(next_four, next);
+        float most = x[0];
+#pragma unroll
+        for (int i = 1; i < 4 * kEach; i++) most = fmaxf(most, x[i]);
+        if constexpr (TOP)
+            if (gate == 0 || __any(most > gate_logit)) gather(four, x);
+        own.bring_to(fmaxf(own.most, capped(p, most)), p.power);
+#pragma unroll
+        for (int i = 0; i < 4 * kEach; i++) {
+            const float a = exponent_of((capped(p, x[i]) - own.most) * p.power), e = __builtin_amdgcn_exp2f(a);
+            own.sum += e;
+            own.weighted = fmaf(e, a, own.weighted);
+        }
+#pragma unroll
+        for (int i = 0; i < 4 * kEach; i++) x[i] = next[i];
+        four = next_four;
+    }
+    if constexpr (TOP)
+        while (count > 0) flush();
+    own.join_lanes(p.power, lane);
+
+    // the waves' parts into the first one's
+    auto join_waves = [&]() {
+        if constexpr (WAVES > 1) {
+            if (lane == 0) sums_of[wave][0] = own.most, sums_of[wave][1] = own.sum, sums_of[wave][2] = own.weighted;
+            if constexpr (TOP) lists[wave][lane] = list;
+            __syncthreads();
+            if (wave == 0)
+                for (int w = 1; w < WAVES; w++) own.join(Sums{sums_of[w][0], sums_of[w][1], sums_of[w][2]}, p.power);
+            if constexpr (TOP) {
+#pragma unroll
+                for (int apart = 1; apart < WAVES; apart *= 2) {
+                    if (wave % (2 * apart) == 0) {
+                        list = merged(list, lists[wave + apart][JL_WAVE - 1 - lane], lane);
+                        lists[wave][lane] = list;
+                    }
+                    __syncthreads();
+                }
+            }
+        }
+    };
+    join_waves();
+    if (p.parts > 1) {
+        if (wave == 0) {
+            Part *to = p.part + row * p.parts + part;
+            if constexpr (TOP) __hip_atomic_store(&to->keys[lane], list, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (lane < 3) __hip_atomic_store(&to->most + lane, lane == 0 ? own.most : lane == 1 ? own.sum : own.weighted, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's stores have arrived
+            if (lane == 0) {
+                const uint32_t before = __hip_atomic_fetch_add(p.arrived + row, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1;
+                if (before == (uint32_t)p.parts) __hip_atomic_store(p.arrived + row, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                arrived = before;
+            }
+        }
+        __syncthreads();
+        if (arrived != (uint32_t)p.parts) return;
+        const Part *from = p.part + row * p.parts;
+        uint64_t keys[kPartsEach];
+        Sums sums[kPartsEach];
+#pragma unroll
+        for (int j = 0; j < kPartsEach; j++) {
+            const int at = min(wave + j * WAVES, p.parts - 1);
+            if constexpr (TOP) keys[j] = __hip_atomic_load(&from[at].keys[j == 0 ? lane : JL_WAVE - 1 - lane], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            sums[j].most = __hip_atomic_load(&from[at].most, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            sums[j].sum = __hip_atomic_load(&from[at].sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            sums[j].weighted = __hip_atomic_load(&from[at].weighted, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        own = Sums(), list = 0;
+#pragma unroll
+        for (int j = 0; j < kPartsEach; j++) {
+            if (wave + j * WAVES >= p.parts) break;
+            own.join(sums[j], p.power);
+            if constexpr (TOP) list = j == 0 ? keys[j] : merged(list, keys[j], lane);
+        }
+        join_waves();
+    }
+    if (wave != 0) return;
+
+    const float log_sum = logf(own.sum);
+    auto logprob = [&](float logit) { return own.sum == 0.f ? -INFINITY : (capped(p, logit) - own.most) * p.scale - log_sum; };
+    if (lane == 0 && p.entropy) p.entropy[row] = own.sum == 0.f ? 0.f : log_sum - own.weighted / own.sum * kLn2;
+    for (int i = lane; i < p.tokens_per_row; i += JL_WAVE) {
         const int token = p.tokens[row * p.tokens_per_row + i];
         p.logprobs[row * p.tokens_per_row + i] = (unsigned)token < (unsigned)p.n ? logprob(l[token]) : 0.f;
     }
-    uint64_t before = UINT64_MAX;
-    for (int k = 0; k < p.top; k++) {
-        uint64_t best = 0;
-        for (int i = tid; i < p.n; i += kThreads) {
-            const uint64_t key = key_of(l[i], i);
-            if (key < before && key > best) best = key;
-        }
-        for (int off = JL_WAVE / 2; off; off >>= 1) {
-            const uint64_t other = __shfl_xor((unsigned long long)best, off, JL_WAVE);
-            best = other > best ? other : best;
-        }
-        __syncthreads();
-        if (lane == 0) best_of[wave] = best;
-        __syncthreads();
-        for (int w = 0; w < kWaves; w++) best = best_of[w] > best ? best_of[w] : best;
-        before = best;
-        if (tid == 0) {
-            const int at = (int)~(uint32_t)best;
-            p.top_tokens[row * p.top + k] = best ? at : -1;
-            p.top_logprobs[row * p.top + k] = best ? logprob(l[at]) : -INFINITY;
+    if constexpr (TOP) {
+        if (lane < p.top) {
+            p.top_tokens[row * p.top + lane] = list ? (int)~(uint32_t)list : -1;
+            p.top_logprobs[row * p.top + lane] = list ? logprob(logit_of(list)) : -INFINITY;
         }
     }
 }
 
-constexpr size_t kArrivedBytes = 16;
+constexpr size_t kArrivedBytes = kPartsRows * sizeof(uint32_t);
+constexpr size_t kWorkspaceBytes = kArrivedBytes + (size_t)kGroups * sizeof(Part);
 
 bool aligned(const void *p, int to) { return ((uintptr_t)p & (to - 1)) == 0; }
+
+template <int WAVES>
+void launch(const LogprobsArgs &a, int64_t rows, hipStream_t stream) {
+    const dim3 grid((unsigned)(rows * a.parts)), block(WAVES * JL_WAVE);
+    if (a.top > 0) hipLaunchKernelGGL((jl_logprobs_kernel<WAVES, true>), grid, block, 0, stream, a);
+    else hipLaunchKernelGGL((jl_logprobs_kernel<WAVES, false>), grid, block, 0, stream, a);
+}
 
 }  // namespace
 
 extern "C" {
 
 size_t jl_logprobs_workspace_bytes(int64_t n, int top) {
-    if (n <= 0 || n > INT32_MAX || top < 0 || top > kMostTop) return 0;
-    return kArrivedBytes;
+    if (n <= 0 || n > kMostLogits || top < 0 || top > kMostTop) return 0;
+    return kWorkspaceBytes;
 }
 
 int jl_logprobs_workspace_init(jl_context *ctx, void *workspace, size_t workspace_bytes) {
@@ -125,8 +376,9 @@ int jl_logprobs(jl_context *ctx, const float *logits, int64_t rows, int64_t n, i
                 const int32_t *tokens, int64_t tokens_per_row, float *logprobs, float *entropy, int top,
                 int32_t *top_tokens, float *top_logprobs, void *workspace, size_t workspace_bytes) {
     JL_REQUIRE(ctx && logits && workspace, "jl_logprobs: null argument");
-    JL_REQUIRE(rows >= 0 && rows <= INT32_MAX, "jl_logprobs: %lld rows", (long long)rows);
-    JL_REQUIRE(n > 0 && n <= INT32_MAX, "jl_logprobs: rows of %lld logits", (long long)n);
+    // (a launch has fewer than 2^32 threads along a side)
+    JL_REQUIRE(rows >= 0 && rows < 1 << 24, "jl_logprobs: %lld rows (fewer than 2^24)", (long long)rows);
+    JL_REQUIRE(n > 0 && n <= kMostLogits, "jl_logprobs: rows of %lld logits (1 ... 2^30)", (long long)n);
     JL_REQUIRE(row_stride >= n, "jl_logprobs: rows closer together (%lld) than they are long (%lld)", (long long)row_stride, (long long)n);
     JL_REQUIRE(std::isfinite(scale * kLog2e) && scale * kLog2e >= FLT_MIN, "jl_logprobs: scale %g (positive and finite)", (double)scale);
     JL_REQUIRE(cap == 0.f || (cap >= 1e-30f && cap <= 1e30f), "jl_logprobs: cap %g (0, or 1e-30 ... 1e30)", (double)cap);
@@ -148,7 +400,13 @@ int jl_logprobs(jl_context *ctx, const float *logits, int64_t rows, int64_t n, i
     a.scale = scale, a.cap = cap, a.one_over_cap = cap > 0.f ? 1.f / cap : 0.f;
     a.tokens = tokens, a.tokens_per_row = (int)tokens_per_row, a.logprobs = logprobs, a.entropy = entropy;
     a.top = top, a.top_tokens = top_tokens, a.top_logprobs = top_logprobs;
-    hipLaunchKernelGGL(jl_logprobs_kernel, dim3((unsigned)rows), dim3(kThreads), 0, ctx->stream, a);
+    a.power = scale * kLog2e;
+    a.arrived = (uint32_t *)workspace, a.part = (Part *)((uint8_t *)workspace + kArrivedBytes);
+    const int waves = n <= kShortRow ? 1 : 4;
+    const int64_t steps = ((n + 3 + 3) / 4 + waves * kStepFours - 1) / (waves * kStepFours);   // of a workgroup, in a row that begins between two fours
+    a.parts = waves == 1 ? 1 : (int)std::max<int64_t>(std::min<int64_t>({steps, kMostParts, kGroups / rows}), 1);
+    a.fours_each = (int)((steps + a.parts - 1) / a.parts) * waves * kStepFours;
+    waves == 1 ? launch<1>(a, rows, ctx->stream) : launch<4>(a, rows, ctx->stream);
     JL_HIP(hipGetLastError());
     return JL_OK;
 }
