@@ -919,8 +919,16 @@ __global__ void __launch_bounds__(kThreads, (Shape<TYPE, DIM>::kPerUnit)) jl_kv_
 #pragma unroll
                 for (int i = 0; i < 8; i++) x[i] *= undo;
                 if (p.cap > 0.f) {
+                    float most = 0.f;
 #pragma unroll
-                    for (int i = 0; i < 8; i++) x[i] = p.cap * jl_tanh(x[i] * p.one_over_cap);
+                    for (int i = 0; i < 8; i++) x[i] *= p.one_over_cap, most = fmaxf(most, fabsf(x[i]));
+                    if (__any(!(most <= kTanhNear))) {
+#pragma unroll
+                        for (int i = 0; i < 8; i++) x[i] = p.cap * jl_tanh(x[i]);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 8; i++) x[i] = p.cap * jl_tanh_near(x[i]);
+                    }
                 }
                 if (p.slopes) {
                     const int from = t * kTile + 4 * g - position;

@@ -6,13 +6,13 @@
 // their index: one 64-bit key that is larger for the one that comes first.
 //
 // Bound: the bytes of the logits, once.  A wave goes through its part in steps of 16 values a lane, the next step's on their
-// way; each lane has a running m, S and T.  For the list the wave keeps the 64 largest keys so far, sorted, one a lane: a
-// step none of whose values is larger than the last one that is wanted costs one comparison.  From others the larger ones are
-// gathered in LDS, and every 64 sorted and merged in.  The first step, and any that would gather more than 64, first sorts its lanes'
-// largest: of the top ones of those there are as many as are wanted, so that nothing smaller than the last of them is.
+// way; each lane has a running m, S and T.  For the list the wave keeps its largest keys so far, sorted, one a lane: a step
+// none of whose values reaches the last one that is wanted costs one comparison.  From others those that do are gathered
+// in LDS, and every 64 sorted and merged in.  The first step, and any that would gather more than 64, sorts its lanes'
+// largest first: of the top ones of those there are as many as are wanted, so that nothing below the last of them is.
 //
-// Work.  A workgroup of four waves a row (one wave where rows are short); where rows are few each is cut into parts, and the workgroup that
-// is done last with a row joins them, in their order whoever that is (nobody waits for anybody).
+// Work.  A workgroup of four waves a row (one wave where rows are short); where rows are few each is cut into parts, and the
+// workgroup that is done last with a row joins them, in their order whoever that is (nobody waits for anybody).
 #include <algorithm>
 #include <cfloat>
 #include <climits>
@@ -28,8 +28,7 @@ namespace {
 constexpr int kMostTop = JL_WAVE;                 // a lane each
 constexpr int kEach = 4;                          // loads of four values a lane and step
 constexpr int kStepFours = kEach * JL_WAVE;       // fours of a wave's step
-constexpr int kMostParts = 32;                    // of a row; a wave of the last workgroup has kPartsEach of them
-constexpr int kPartsEach = kMostParts / 4;
+constexpr int kMostParts = 32;                    // of a row
 constexpr int kPartsRows = 512;                   // rows that are cut
 constexpr int kGroups = 512;                      // workgroups that a launch of few rows has, about
 constexpr int kShortRow = 2048;                   // logits of a row that one wave has
@@ -63,16 +62,13 @@ __device__ __forceinline__ float capped(const LogprobsArgs &p, float l) {
     return p.cap > 0.f && l != -INFINITY ? p.cap * jl_tanh(l * p.one_over_cap) : l;
 }
 
-// Larger logits are larger numbers, and of equal ones the earlier is; NaN is 0 and in no list.
-__device__ __forceinline__ uint64_t key_of(float l, int at) {
-    const uint32_t b = __float_as_uint(l + 0.f);              // (-0 is 0)
-    const uint32_t order = b & 0x80000000u ? ~b : b | 0x80000000u;
-    return l == l ? (uint64_t)order << 32 | (uint32_t)~at : 0;
+// Larger logits are larger numbers (-0 is 0, NaN a 0), and back; in the key, of equal ones the earlier is the larger.
+__device__ __forceinline__ uint32_t order_of(float l) {
+    const uint32_t b = __float_as_uint(l + 0.f);
+    return l == l ? (b & 0x80000000u ? ~b : b | 0x80000000u) : 0;
 }
-__device__ __forceinline__ float logit_of(uint64_t key) {
-    const uint32_t order = (uint32_t)(key >> 32);
-    return __uint_as_float(order & 0x80000000u ? order & 0x7fffffffu : ~order);
-}
+__device__ __forceinline__ float logit_of(uint32_t order) { return __uint_as_float(order & 0x80000000u ? order & 0x7fffffffu : ~order); }
+__device__ __forceinline__ uint64_t key_of(float l, uint32_t at) { return (uint64_t)order_of(l) << 32 | ~at; }
 
 // The value of lane ^ N, by moves between lanes alone.
 template <int N>
@@ -101,38 +97,47 @@ template <int N>
 __device__ __forceinline__ float lane_xor(float x, int lane) { return __uint_as_float(lane_xor<N>(__float_as_uint(x), lane)); }
 
 // One step of a sorting network: of the pair (lane, lane ^ N) this lane keeps the larger key where `larger`.
-template <int N>
-__device__ __forceinline__ uint64_t keep_of_pair(uint64_t own, bool larger, int lane) {
-    const uint64_t other = lane_xor<N>(own, lane);
+template <int N, typename KEY>
+__device__ __forceinline__ KEY keep_of_pair(KEY own, bool larger, int lane) {
+    const KEY other = lane_xor<N>(own, lane);
     return (other > own) == larger ? other : own;
 }
-// A sequence that rises and then falls, or the other way round, into a falling one.
-template <int FROM = 32>
-__device__ __forceinline__ uint64_t bitonic_to_falling(uint64_t key, bool falling, int lane) {
+// A sequence over 2 FROM lanes that rises and then falls, or the other way round, into a falling (or rising) one.
+template <int FROM, typename KEY>
+__device__ __forceinline__ KEY bitonic_sorted(KEY key, bool falling, int lane) {
     key = keep_of_pair<FROM>(key, ((lane & FROM) == 0) == falling, lane);
-    if constexpr (FROM > 1) return bitonic_to_falling<FROM / 2>(key, falling, lane);
+    if constexpr (FROM > 1) return bitonic_sorted<FROM / 2>(key, falling, lane);
     else return key;
 }
-// Sorted over the wave's lanes, rising.
-__device__ __forceinline__ uint64_t sorted_rising(uint64_t key, int lane) {
-    key = bitonic_to_falling<1>(key, (lane & 2) == 0, lane);
-    key = bitonic_to_falling<2>(key, (lane & 4) == 0, lane);
-    key = bitonic_to_falling<4>(key, (lane & 8) == 0, lane);
-    key = bitonic_to_falling<8>(key, (lane & 16) == 0, lane);
-    key = bitonic_to_falling<16>(key, (lane & 32) == 0, lane);
-    return bitonic_to_falling<32>(key, false, lane);
+// Every W lanes sorted.
+template <int W, typename KEY>
+__device__ __forceinline__ KEY sorted(KEY key, bool falling, int lane) {
+    if constexpr (W > 2) key = sorted<W / 2>(key, (lane & (W / 2)) == 0, lane);
+    return bitonic_sorted<W / 2>(key, falling, lane);
 }
-// The 64 largest of a falling and a rising sequence of 64, falling.
+// The W largest of a wave whose W lanes each are sorted, falling and rising in turn: falling (or rising) in every W lanes.
+template <int W>
+__device__ __forceinline__ uint64_t largest_of(uint64_t key, bool falling, int lane) {
+    if constexpr (W <= 16) {
+        const uint64_t other = lane_xor<16>(key, lane);
+        key = bitonic_sorted<W / 2>(other > key ? other : key, (lane & 32) == 0, lane);
+    }
+    if constexpr (W <= 32) {
+        const uint64_t other = lane_xor<32>(key, lane);
+        key = bitonic_sorted<W / 2>(other > key ? other : key, falling, lane);
+    }
+    return key;
+}
+template <int W>
+__device__ __forceinline__ bool falls(int lane) { return W == JL_WAVE || (lane & W) == 0; }   // in turn
+// The W largest of a falling and a rising sequence of W, falling.
+template <int W>
 __device__ __forceinline__ uint64_t merged(uint64_t falling, uint64_t rising, int lane) {
-    return bitonic_to_falling(falling > rising ? falling : rising, true, lane);
-}
-__device__ __forceinline__ uint64_t key_of_lane(uint64_t key, int lane) {   // (`lane` the same in all)
-    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(key >> 32), lane) << 32 |
-           (uint32_t)__builtin_amdgcn_readlane((int)key, lane);
+    return bitonic_sorted<W / 2>(falling > rising ? falling : rising, true, lane);
 }
 
-// What of a difference of two values times the power: 0 where 2^it is, so that it times that is no NaN (NaN stays).
-__device__ __forceinline__ float exponent_of(float below) { return below < -200.f ? -200.f : below; }
+// 2^it is 0, and 0 times it no NaN, as 0 times -infinity is.
+constexpr float kFar = -200.f;
 
 __device__ __forceinline__ void wave_fence() {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -143,8 +148,8 @@ __device__ __forceinline__ void wave_fence() {
 struct Sums {
     float most = -FLT_MAX, sum = 0.f, weighted = 0.f;
     __device__ __forceinline__ void bring_to(float other_most, float power) {
-        const float d = exponent_of((most - other_most) * power), share = __builtin_amdgcn_exp2f(d);
-        weighted = fmaf(sum, d, weighted) * share;
+        const float d = (most - other_most) * power, share = __builtin_amdgcn_exp2f(d);
+        weighted = fmaf(sum, fmaxf(d, kFar), weighted) * share;
         sum *= share;
         most = other_most;
     }
@@ -166,10 +171,13 @@ struct Sums {
     }
 };
 
-template <int WAVES, bool TOP>
+// W: keys that the list has room for, 16, 32 or 64; 0: there is none.
+template <int WAVES, int W>
 __global__ void __launch_bounds__(WAVES * JL_WAVE) jl_logprobs_kernel(LogprobsArgs p) {
-    __shared__ uint64_t gathered[WAVES][TOP ? 2 * JL_WAVE : 1];
-    __shared__ uint64_t lists[WAVES][TOP ? JL_WAVE : 1];
+    constexpr bool TOP = W > 0;
+    constexpr int kWide = TOP ? W : JL_WAVE, kLists = JL_WAVE / kWide;   // lists that a register holds
+    __shared__ uint2 gathered[WAVES][TOP ? 5 * JL_WAVE : 1];             // value, place
+    __shared__ uint64_t lists[WAVES * kWide];
     __shared__ float sums_of[WAVES][3];
     __shared__ uint32_t arrived;
     const int tid = threadIdx.x, lane = tid % JL_WAVE, wave = __builtin_amdgcn_readfirstlane(tid / JL_WAVE);
@@ -179,13 +187,15 @@ __global__ void __launch_bounds__(WAVES * JL_WAVE) jl_logprobs_kernel(LogprobsAr
     const int off = (int)((uintptr_t)l / 4 % 4);              // fours lie on 16-byte boundaries: the first begins this many before the row
     const int fours = (p.n + off + 3) / 4, end = min((part + 1) * p.fours_each, fours);
 
-    uint64_t list = 0, gate = 0;                              // falling over the lanes; the last that is wanted
-    float gate_logit = -INFINITY;                             // ... as a logit, where the list is full
-    int count = 0;                                            // keys in `gathered`
+    uint64_t list = 0;                                        // falling over the first W lanes
+    bool full = false;                                        // it has as many keys as are wanted
+    float bar = 0.f;                                          // then: the least value that is larger than its last
+    int count = 0;                                            // values in `gathered`
     Sums own;
 
+    auto is_whole = [&](int four) { return 4 * four - off >= 0 && 4 * (four + kStepFours) - off <= p.n; };
     auto load = [&](int four, float (&x)[4 * kEach]) {
-        const bool whole = 4 * four - off >= 0 && 4 * (four + kStepFours) - off <= p.n;
+        const bool whole = is_whole(four);
 #pragma unroll
         for (int j = 0; j < kEach; j++) {
             const int first = 4 * (four + j * JL_WAVE + lane) - off;
@@ -198,48 +208,52 @@ __global__ void __launch_bounds__(WAVES * JL_WAVE) jl_logprobs_kernel(LogprobsAr
             }
         }
     };
+    // up to 64 of what is gathered, the last ones, into the list
     auto flush = [&]() {
-        // (between lanes of one wave, whose LDS accesses come in order)
         wave_fence();
-        const uint64_t key = lane < count ? gathered[wave][lane] : 0, rest = gathered[wave][JL_WAVE + lane];
-        wave_fence();
-        gathered[wave][lane] = rest;
-        wave_fence();
-        count = max(count - JL_WAVE, 0);
-        list = merged(list, sorted_rising(key, lane), lane);
-        gate = key_of_lane(list, p.top - 1);
-        gate_logit = gate ? logit_of(gate) : -INFINITY;
+        const int taken = min(count, JL_WAVE);
+        count -= taken;
+        const uint2 value = gathered[wave][count + min(lane, taken - 1)];
+        uint64_t key = lane < taken ? key_of(__uint_as_float(value.x), value.y) : 0;
+        if (taken <= kWide) key = sorted<kWide>(key, false, lane);
+        else key = largest_of<kWide>(sorted<kWide>(key, kLists > 1 && falls<kWide>(lane), lane), false, lane);
+        list = merged<kWide>(list, key, lane);
+        const uint32_t last = __builtin_amdgcn_readlane((int)(list >> 32), p.top - 1);
+        full = last != 0;
+        bar = logit_of(last + 1);                             // (behind infinity: NaN, which nothing reaches)
     };
-    auto gather = [&](int four, const float (&x)[4 * kEach]) {
-        auto key_at = [&](int i) {
-            const int at = 4 * (four + i / 4 * JL_WAVE + lane) - off + i % 4;
-            return (unsigned)at < (unsigned)p.n ? key_of(x[i], at) : 0;
-        };
-        uint64_t least = gate;                                // keys above it are gathered
-        uint64_t largest = 0;
+    auto gather = [&](int four, const float (&x)[4 * kEach], float most) {
+        const bool whole = is_whole(four);
         int passing = 0;
+        if (full) {
 #pragma unroll
-        for (int i = 0; i < 4 * kEach; i++) {
-            const uint64_t key = key_at(i);
-            largest = key > largest ? key : largest;
-            passing += __popcll(__ballot(key > gate));
+            for (int i = 0; i < 4 * kEach; i++) passing += __popcll(__ballot(x[i] >= bar));
         }
-        if (passing > JL_WAVE) {
-            const uint64_t last = key_of_lane(sorted_rising(largest, lane), JL_WAVE - p.top);   // one that is wanted itself
-            least = last > least ? last - 1 : least;
+        float least = bar;
+        if (!full || passing > JL_WAVE) {
+            // (one that is wanted itself; without one, where NaN are many, any)
+            const uint32_t last = __builtin_amdgcn_readlane((int)sorted<JL_WAVE>(order_of(most), false, lane), JL_WAVE - p.top);
+            const float of_lanes = last ? logit_of(last) : -INFINITY;
+            least = full ? fmaxf(bar, of_lanes) : of_lanes;
         }
 #pragma unroll
-        for (int i = 0; i < 4 * kEach; i++) {
-            const uint64_t key = key_at(i);
-            const bool wanted = key > least && key > gate;
-            const uint64_t mask = __ballot(wanted);
-            if (mask == 0) continue;
-            if (wanted) gathered[wave][count + __popcll(mask & ((1ull << lane) - 1))] = key;
-            count += __popcll(mask);
-            if (count >= JL_WAVE) flush();
+        for (int j = 0; j < kEach; j++) {
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                const uint32_t at = 4 * (four + j * JL_WAVE + lane) - off + c;
+                const bool wanted = x[4 * j + c] >= least && (whole || at < (uint32_t)p.n);
+                const uint64_t mask = __ballot(wanted);
+                if (mask == 0) continue;
+                if (wanted) gathered[wave][count + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0))] = make_uint2(__float_as_uint(x[4 * j + c]), at);
+                count += __popcll(mask);
+            }
+            if (count >= JL_WAVE) {
+                while (count >= JL_WAVE) flush();
+                if (full) least = fmaxf(least, bar);          // (what comes next lies behind)
+            }
         }
-        // the gate follows at once where the list is not full: all that is behind it would pass
-        if (gate == 0 && count > 0) flush();
+        // (at once where the list is not full: all that is behind it would pass)
+        while (!full && count > 0) flush();
     };
 
     float x[4 * kEach];
@@ -253,13 +267,24 @@ __global__ void __launch_bounds__(WAVES * JL_WAVE) jl_logprobs_kernel(LogprobsAr
 #pragma unroll
         for (int i = 1; i < 4 * kEach; i++) most = fmaxf(most, x[i]);
         if constexpr (TOP)
-            if (gate == 0 || __any(most > gate_logit)) gather(four, x);
+            if (!full || __any(most >= bar)) gather(four, x, most);
         own.bring_to(fmaxf(own.most, capped(p, most)), p.power);
+        float least = x[0];
+#pragma unroll
+        for (int i = 1; i < 4 * kEach; i++) least = fminf(least, x[i]);
+        // (all of a step's where tanh's series ends: one form)
+        if (p.cap > 0.f && !__any(fmaxf(most, -least) * p.one_over_cap > kTanhNear)) {
+#pragma unroll
+            for (int i = 0; i < 4 * kEach; i++) x[i] = p.cap * jl_tanh_near(x[i] * p.one_over_cap);
+        } else if (p.cap > 0.f) {
+#pragma unroll
+            for (int i = 0; i < 4 * kEach; i++) x[i] = capped(p, x[i]);
+        }
 #pragma unroll
         for (int i = 0; i < 4 * kEach; i++) {
-            const float a = exponent_of((capped(p, x[i]) - own.most) * p.power), e = __builtin_amdgcn_exp2f(a);
+            const float a = (x[i] - own.most) * p.power, e = __builtin_amdgcn_exp2f(a);
             own.sum += e;
-            own.weighted = fmaf(e, a, own.weighted);
+            own.weighted = fmaf(e, fmaxf(a, kFar), own.weighted);
         }
 #pragma unroll
         for (int i = 0; i < 4 * kEach; i++) x[i] = next[i];
@@ -269,23 +294,27 @@ __global__ void __launch_bounds__(WAVES * JL_WAVE) jl_logprobs_kernel(LogprobsAr
         while (count > 0) flush();
     own.join_lanes(p.power, lane);
 
+    // the lists that `from` says where they lie, `lists_left` of them, into `list`: kLists at a time, falling and rising in turn
+    auto join_lists = [&](int lists_there, auto key_at) {
+        list = 0;
+#pragma unroll
+        for (int j = 0; j < (kMostParts / WAVES + kLists - 1) / kLists; j++) {
+            const int first = j * kLists, which = first + lane / kWide;
+            if (first >= lists_there) break;
+            const uint64_t key = which < lists_there ? key_at(which, j, falls<kWide>(lane) && kLists > 1 ? lane % kWide : kWide - 1 - lane % kWide) : 0;
+            list = merged<kWide>(list, largest_of<kWide>(key, false, lane), lane);
+        }
+    };
     // the waves' parts into the first one's
     auto join_waves = [&]() {
         if constexpr (WAVES > 1) {
             if (lane == 0) sums_of[wave][0] = own.most, sums_of[wave][1] = own.sum, sums_of[wave][2] = own.weighted;
-            if constexpr (TOP) lists[wave][lane] = list;
+            if constexpr (TOP)
+                if (lane < kWide) lists[wave * kWide + lane] = list;
             __syncthreads();
-            if (wave == 0)
+            if (wave == 0) {
                 for (int w = 1; w < WAVES; w++) own.join(Sums{sums_of[w][0], sums_of[w][1], sums_of[w][2]}, p.power);
-            if constexpr (TOP) {
-#pragma unroll
-                for (int apart = 1; apart < WAVES; apart *= 2) {
-                    if (wave % (2 * apart) == 0) {
-                        list = merged(list, lists[wave + apart][JL_WAVE - 1 - lane], lane);
-                        lists[wave][lane] = list;
-                    }
-                    __syncthreads();
-                }
+                if constexpr (TOP) join_lists(WAVES, [&](int which, int, int i) { return lists[which * kWide + i]; });
             }
         }
     };
@@ -293,7 +322,8 @@ __global__ void __launch_bounds__(WAVES * JL_WAVE) jl_logprobs_kernel(LogprobsAr
     if (p.parts > 1) {
         if (wave == 0) {
             Part *to = p.part + row * p.parts + part;
-            if constexpr (TOP) __hip_atomic_store(&to->keys[lane], list, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if constexpr (TOP)
+                if (lane < kWide) __hip_atomic_store(&to->keys[lane], list, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             if (lane < 3) __hip_atomic_store(&to->most + lane, lane == 0 ? own.most : lane == 1 ? own.sum : own.weighted, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's stores have arrived
             if (lane == 0) {
@@ -304,24 +334,26 @@ __global__ void __launch_bounds__(WAVES * JL_WAVE) jl_logprobs_kernel(LogprobsAr
         }
         __syncthreads();
         if (arrived != (uint32_t)p.parts) return;
+        // a wave has the parts from `first` on; a lane the sums of one
         const Part *from = p.part + row * p.parts;
-        uint64_t keys[kPartsEach];
-        Sums sums[kPartsEach];
+        const int each = (p.parts + WAVES - 1) / WAVES, first = wave * each, mine = max(min(each, p.parts - first), 0);
+        constexpr int kLoads = (kMostParts / WAVES + kLists - 1) / kLists;
+        uint64_t keys[kLoads];
+        if constexpr (TOP) {
 #pragma unroll
-        for (int j = 0; j < kPartsEach; j++) {
-            const int at = min(wave + j * WAVES, p.parts - 1);
-            if constexpr (TOP) keys[j] = __hip_atomic_load(&from[at].keys[j == 0 ? lane : JL_WAVE - 1 - lane], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            sums[j].most = __hip_atomic_load(&from[at].most, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            sums[j].sum = __hip_atomic_load(&from[at].sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            sums[j].weighted = __hip_atomic_load(&from[at].weighted, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            for (int j = 0; j < kLoads; j++) {
+                const int which = j * kLists + lane / kWide, i = falls<kWide>(lane) && kLists > 1 ? lane % kWide : kWide - 1 - lane % kWide;
+                keys[j] = which < mine ? __hip_atomic_load(&from[first + which].keys[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
+            }
         }
-        own = Sums(), list = 0;
-#pragma unroll
-        for (int j = 0; j < kPartsEach; j++) {
-            if (wave + j * WAVES >= p.parts) break;
-            own.join(sums[j], p.power);
-            if constexpr (TOP) list = j == 0 ? keys[j] : merged(list, keys[j], lane);
+        own = Sums();
+        if (lane < mine) {
+            own.most = __hip_atomic_load(&from[first + lane].most, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            own.sum = __hip_atomic_load(&from[first + lane].sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            own.weighted = __hip_atomic_load(&from[first + lane].weighted, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
+        if constexpr (TOP) join_lists(mine, [&](int, int j, int) { return keys[j]; });
+        own.join_lanes(p.power, lane);
         join_waves();
     }
     if (wave != 0) return;
@@ -335,8 +367,9 @@ __global__ void __launch_bounds__(WAVES * JL_WAVE) jl_logprobs_kernel(LogprobsAr
     }
     if constexpr (TOP) {
         if (lane < p.top) {
-            p.top_tokens[row * p.top + lane] = list ? (int)~(uint32_t)list : -1;
-            p.top_logprobs[row * p.top + lane] = list ? logprob(logit_of(list)) : -INFINITY;
+            const bool is = list >> 32 != 0;
+            p.top_tokens[row * p.top + lane] = is ? (int)~(uint32_t)list : -1;
+            p.top_logprobs[row * p.top + lane] = is ? logprob(logit_of((uint32_t)(list >> 32))) : -INFINITY;
         }
     }
 }
@@ -349,8 +382,10 @@ bool aligned(const void *p, int to) { return ((uintptr_t)p & (to - 1)) == 0; }
 template <int WAVES>
 void launch(const LogprobsArgs &a, int64_t rows, hipStream_t stream) {
     const dim3 grid((unsigned)(rows * a.parts)), block(WAVES * JL_WAVE);
-    if (a.top > 0) hipLaunchKernelGGL((jl_logprobs_kernel<WAVES, true>), grid, block, 0, stream, a);
-    else hipLaunchKernelGGL((jl_logprobs_kernel<WAVES, false>), grid, block, 0, stream, a);
+    if (a.top > 32) hipLaunchKernelGGL((jl_logprobs_kernel<WAVES, 64>), grid, block, 0, stream, a);
+    else if (a.top > 16) hipLaunchKernelGGL((jl_logprobs_kernel<WAVES, 32>), grid, block, 0, stream, a);
+    else if (a.top > 0) hipLaunchKernelGGL((jl_logprobs_kernel<WAVES, 16>), grid, block, 0, stream, a);
+    else hipLaunchKernelGGL((jl_logprobs_kernel<WAVES, 0>), grid, block, 0, stream, a);
 }
 
 }  // namespace
