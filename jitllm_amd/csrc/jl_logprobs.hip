@@ -30,7 +30,9 @@ constexpr int kEach = 4;                          // loads of four values a lane
 constexpr int kStepFours = kEach * JL_WAVE;       // fours of a wave's step
 constexpr int kMostParts = 32;                    // of a row
 constexpr int kPartsRows = 512;                   // rows that are cut
-constexpr int kGroups = 512;                      // workgroups that a launch of few rows has, about
+// Workgroups that a launch of few rows has, about (256 rows of 128256, five alternatives: 66 us with 512, 44 with 1024, 50 with
+// 2048; 64 of 151936, twenty: 25.7, 24.4 and 35.5).
+constexpr int kGroups = 1024;
 constexpr int kShortRow = 2048;                   // logits of a row that one wave has
 constexpr int64_t kMostLogits = 1 << 30;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
