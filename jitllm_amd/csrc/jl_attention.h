@@ -34,10 +34,18 @@ struct JlScoredArgs : JlAttentionArgs {
     float cap, one_over_cap;                     // of scores that are powers of two; 0: none
     const float *slopes;                         // [heads], or null
     const int32_t *first_tokens, *end_tokens;    // [rows], or null
+    // Blocks of this many rows, a multiple of rows_each, that jl_kv_attention_prompt_kernel has taken: what it says, and what the
+    // other kernel reads (null: there was no such launch).
+    int taken_rows;
+    uint8_t *taken_out;
+    const uint8_t *taken;
 };
 template <typename ARGS>
 inline constexpr bool kScored = std::is_same_v<ARGS, JlScoredArgs>;
 
+hipError_t jl_launch_attention_prompt_f16(const JlScoredArgs &a, int head_dim, int device, hipStream_t stream);
+hipError_t jl_launch_attention_prompt_q8(const JlScoredArgs &a, int head_dim, int device, hipStream_t stream);
+hipError_t jl_launch_attention_prompt_q4(const JlScoredArgs &a, int head_dim, int device, hipStream_t stream);
 hipError_t jl_launch_attention_f16(const JlAttentionArgs &a, int head_dim, int compute_units, hipStream_t stream);
 hipError_t jl_launch_attention_q8(const JlAttentionArgs &a, int head_dim, int compute_units, hipStream_t stream);
 hipError_t jl_launch_attention_q4(const JlAttentionArgs &a, int head_dim, int compute_units, hipStream_t stream);

@@ -2,12 +2,16 @@
 #include <algorithm>
 #include <climits>
 #include <cmath>
+#include <cstdlib>
 
 #include "jl_attention.h"
 
 namespace {
 
 constexpr size_t kArrivedBytes = kAttentionMostGroups * sizeof(uint32_t);
+constexpr size_t kTakenBytes = 32768;             // a byte for each block of rows, two rows at least
+// (Row block, head of k and v) pairs from which rows go in blocks.
+constexpr int64_t kPromptGroups = 128;
 
 bool aligned(const void *p, int to) { return ((uintptr_t)p & (to - 1)) == 0; }
 
@@ -72,10 +76,23 @@ int attention(const char *who, jl_context *ctx, const jl_kv_cache *cache, const 
     a.out = out, a.out_f16 = out_f16 != 0;
     a.arrived = (uint32_t *)workspace;
     a.parts = (float *)((uint8_t *)workspace + kArrivedBytes);
+    // Blocks of rows, where they are many: 64 columns to a workgroup, a (row, query head) each.
+    a.taken_rows = 64 / a.group & -a.rows_each, a.taken = nullptr, a.taken_out = nullptr;
+    const bool prompts = row_requests && rows >= 2 * requests && (shaping || cache->type == JL_KV_Q4_0) && a.taken_rows > 1 &&
+                         rows / a.taken_rows * cache->kv_heads >= (getenv("P1") ? atoi(getenv("P1")) : kPromptGroups);
+    if (prompts) a.taken_out = (uint8_t *)workspace + needed - kTakenBytes;
+    const Shaping nothing{0.f, nullptr, nullptr, nullptr};
+    if (prompts && !shaping) shaping = &nothing;
     JlAttentionArgs &plain = a;
     if (shaping) {
         a.cap = shaping->cap * 1.44269504088896340736f, a.one_over_cap = shaping->cap > 0.f ? 1.f / a.cap : 0.f;
         a.slopes = shaping->slopes, a.first_tokens = shaping->first_tokens, a.end_tokens = shaping->end_tokens;
+        if (prompts) {
+            JL_HIP((cache->type == JL_KV_Q8_0   ? jl_launch_attention_prompt_q8
+                    : cache->type == JL_KV_Q4_0 ? jl_launch_attention_prompt_q4
+                                                : jl_launch_attention_prompt_f16)(a, dim, ctx->device, ctx->stream));
+            a.taken = a.taken_out;
+        }
         JL_HIP((cache->type == JL_KV_Q8_0   ? jl_launch_attention_scored_q8
                 : cache->type == JL_KV_Q4_0 ? jl_launch_attention_scored_q4
                                             : jl_launch_attention_scored_f16)(a, dim, ctx->compute_units, ctx->stream));
@@ -93,7 +110,7 @@ extern "C" {
 
 size_t jl_kv_attention_workspace_bytes(int heads, int kv_heads, int head_dim) {
     if (kv_heads <= 0 || heads <= 0 || heads % kv_heads || head_dim <= 0) return 0;
-    return kArrivedBytes + (size_t)2 * kAttentionMostGroups * 16 * ((size_t)head_dim + 2) * sizeof(float);
+    return kArrivedBytes + (size_t)2 * kAttentionMostGroups * 16 * ((size_t)head_dim + 2) * sizeof(float) + kTakenBytes;
 }
 
 int jl_kv_attention_workspace_init(jl_context *ctx, void *workspace, size_t workspace_bytes) {

@@ -78,15 +78,30 @@ __device__ __forceinline__ Range range_at(const ARGS &p, int row, int position, 
     r.end = position >= 0 && r.request >= 0 && r.request < p.requests ? min(position, p.table_tokens - 1) + 1 : -1;
     r.first = p.window > 0 ? max(position - p.window + 1, 0) : 0;
     if constexpr (kScored<ARGS>) {
-        if (p.end_tokens && r.end >= 0) r.end = min(p.end_tokens[row], p.table_tokens);
-        if (p.first_tokens) r.first = max(r.first, p.first_tokens[row]);
+        // (whatever the position is: the loads go out together)
+        const int end = p.end_tokens ? p.end_tokens[row] : INT_MAX, first = p.first_tokens ? p.first_tokens[row] : 0;
+        if (p.end_tokens && r.end >= 0) r.end = min(end, p.table_tokens);
+        r.first = max(r.first, first);
         if (r.end <= r.first) r.first = 0, r.end = -1;
     }
     return r;
 }
+// Where the other kernel has taken blocks of rows, the rest is numbered through: row i is row i % taken_rows of block
+// blocks[i / taken_rows].  More blocks than the list holds: every row is looked at, and a taken one has nothing to read and nothing
+// to write.
+constexpr int kBlocksLeft = 1024, kTaken = -2;
+template <typename ARGS>
+__device__ __forceinline__ int row_at(const ARGS &p, int i, const uint16_t *blocks) {
+    if constexpr (kScored<ARGS>)
+        if (blocks) return blocks[i / p.taken_rows] * p.taken_rows + i % p.taken_rows;
+    return i;
+}
 
 template <typename ARGS>
-__device__ __forceinline__ Range range_of(const ARGS &p, int row) {
+__device__ __forceinline__ Range range_of(const ARGS &p, int i, const uint16_t *blocks) {
+    const int row = row_at(p, i, blocks);
+    if constexpr (kScored<ARGS>)
+        if (row >= p.rows || (p.taken && !blocks && p.taken[row / p.taken_rows])) return Range{0, kTaken, -1};
     return range_at(p, row, p.positions[row], p.row_requests ? p.row_requests[row] : row);
 }
 
@@ -125,17 +140,17 @@ __device__ __forceinline__ Range run_in_lanes(const ARGS &p, Range r, int lane) 
 // Calls work(row, range) for the runs that begin at rows begin ... end - 1, in order, until it returns false; `begin` is at
 // such a multiple.
 template <bool SHARED, typename ARGS, typename WORK>
-__device__ __forceinline__ void for_runs(const ARGS &p, int begin, int end, WORK work) {
+__device__ __forceinline__ void for_runs(const ARGS &p, int rows, const uint16_t *blocks, int begin, int end, WORK work) {
     if constexpr (!SHARED) {
         for (int r = begin; r < end; r++)
-            if (!work(r, range_of(p, r))) return;
+            if (!work(r, range_of(p, r, blocks))) return;
     } else {
         Range run, before;
         int first_row = -1;
         for (int r = begin; r < end; r += 4) {
             Range four[4];
 #pragma unroll
-            for (int j = 0; j < 4; j++) four[j] = range_of(p, min(r + j, p.rows - 1));
+            for (int j = 0; j < 4; j++) four[j] = range_of(p, min(r + j, rows - 1), blocks);
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 if (r + j >= end) break;
@@ -193,17 +208,17 @@ __device__ __forceinline__ jl_half2v even_bytes(uint32_t x) {
 // A tile's k and v as they lie in memory.  Lane (g, m) = (lane / 16, lane % 16) has, of k, token m of each 16-token half,
 // and of v the tokens 4 g + i of each half at a few consecutive elements: head_dim is cut into pieces of 128, 64 and 32,
 // and m has 8, 4 or 2 values of a piece.
-template <int TYPE, int DIM>
+template <int TYPE, int DIM, int H = kHalves>
 struct Raw;
 
-template <int DIM>
-struct Raw<JL_KV_F16, DIM> {
+template <int DIM, int H>
+struct Raw<JL_KV_F16, DIM, H> {
     static constexpr int kSteps = DIM / 32;
     static constexpr int kWide = DIM / 128, kMid = DIM % 128 / 64, kThin = DIM % 64 / 32;
-    uintx4 k[kHalves][kSteps];
-    uintx4 v4[kHalves][4][kWide ? kWide : 1];
-    uintx2 v2[kHalves][4];
-    uint32_t v1[kHalves][4];
+    uintx4 k[H][kSteps];
+    uintx4 v4[H][4][kWide ? kWide : 1];
+    uintx2 v2[H][4];
+    uint32_t v1[H][4];
     __device__ static int element(int step, int g) { return 32 * step + 8 * g; }   // first of the eight of k step `step`
     __device__ static constexpr int in_eight(int i) { return i; }                  // ... and their order
     template <bool STAY>
@@ -224,9 +239,9 @@ struct Raw<JL_KV_F16, DIM> {
     }
     __device__ jl_half8 k_operand(int half, int step) const { return __builtin_bit_cast(jl_half8, k[half][step]); }
     // masked tokens' values are nothing, whatever lies there
-    __device__ void mask_v(const bool (&seen)[kHalves][4]) {
+    __device__ void mask_v(const bool (&seen)[H][4]) {
 #pragma unroll
-        for (int h = 0; h < kHalves; h++)
+        for (int h = 0; h < H; h++)
 #pragma unroll
             for (int i = 0; i < 4; i++) {
 #pragma unroll
@@ -242,7 +257,7 @@ struct Raw<JL_KV_F16, DIM> {
         const jl_half2v nothing = {(_Float16)0.f, (_Float16)0.f};
         jl_half2v sum = nothing;
 #pragma unroll
-        for (int h = 0; h < kHalves; h++)
+        for (int h = 0; h < H; h++)
 #pragma unroll
             for (int i = 0; i < 4; i++) {
 #pragma unroll
@@ -258,7 +273,7 @@ struct Raw<JL_KV_F16, DIM> {
     // those that are become 0
     __device__ void drop_not_finite() {
 #pragma unroll
-        for (int h = 0; h < kHalves; h++)
+        for (int h = 0; h < H; h++)
 #pragma unroll
             for (int i = 0; i < 4; i++) {
 #pragma unroll
@@ -270,12 +285,11 @@ struct Raw<JL_KV_F16, DIM> {
                 if constexpr (kThin) v1[h][i] &= ~not_finite(v1[h][i]);
             }
     }
-    // eight tokens of the columns that output blocks `block` and `block` + 1 take of this lane
-    __device__ void v_operands(int block, jl_half8 (&v)[2]) const {
-        uintx4 r[2];
+    // the tokens, in pairs, of the columns that output blocks `block` and `block` + 1 take of this lane
+    __device__ void v_pairs(int block, uint32_t (&r)[2][2 * H]) const {
         const int word = block / 2;
 #pragma unroll
-        for (int pair = 0; pair < 4; pair++) {
+        for (int pair = 0; pair < 2 * H; pair++) {
             const int h = pair / 2, i = pair % 2 * 2;
             uint32_t a, b;
             if (word < 4 * kWide) a = v4[h][i][word / 4][word % 4], b = v4[h][i + 1][word / 4][word % 4];
@@ -283,22 +297,21 @@ struct Raw<JL_KV_F16, DIM> {
             else a = v1[h][i], b = v1[h][i + 1];
             r[0][pair] = __builtin_amdgcn_perm(b, a, 0x05040100u), r[1][pair] = __builtin_amdgcn_perm(b, a, 0x07060302u);
         }
-        v[0] = __builtin_bit_cast(jl_half8, r[0]), v[1] = __builtin_bit_cast(jl_half8, r[1]);
     }
 };
 
-template <int DIM>
-struct Raw<JL_KV_Q8_0, DIM> {
+template <int DIM, int H>
+struct Raw<JL_KV_Q8_0, DIM, H> {
     static constexpr int kSteps = DIM / 32, kPairs = DIM / 64, kTail = DIM % 64 / 32;
     static constexpr int kWide = DIM / 128, kMid = DIM % 128 / 64, kThin = DIM % 64 / 32;
     static constexpr int kPieces = kWide + kMid + kThin;
-    uintx4 k[kHalves][kPairs];
-    uintx2 k_tail[kHalves];
-    uint16_t k_scale[kHalves][kPairs + kTail];
-    uintx2 v2[kHalves][4][kWide ? kWide : 1];
-    uint32_t v1[kHalves][4];
-    uint16_t v0[kHalves][4];
-    uintx2 v_scale[kHalves][kPieces];
+    uintx4 k[H][kPairs];
+    uintx2 k_tail[H];
+    uint16_t k_scale[H][kPairs + kTail];
+    uintx2 v2[H][4][kWide ? kWide : 1];
+    uint32_t v1[H][4];
+    uint16_t v0[H][4];
+    uintx2 v_scale[H][kPieces];
     // (16 consecutive bytes serve two steps: a lane's loads stay 16 bytes wide)
     __device__ static int element(int step, int g) {
         return step < 2 * kPairs ? 64 * (step / 2) + 16 * g + 8 * (step % 2) : 64 * kPairs + 8 * g;
@@ -344,9 +357,9 @@ struct Raw<JL_KV_Q8_0, DIM> {
                                                    as_u32(even_bytes(hi) * dd), as_u32(even_bytes(hi >> 8) * dd)});
     }
     // (a byte times a scale of 0; the scale alone can be an infinity or NaN)
-    __device__ void mask_v(const bool (&seen)[kHalves][4]) {
+    __device__ void mask_v(const bool (&seen)[H][4]) {
 #pragma unroll
-        for (int h = 0; h < kHalves; h++)
+        for (int h = 0; h < H; h++)
 #pragma unroll
             for (int w = 0; w < kPieces; w++)
 #pragma unroll
@@ -358,7 +371,7 @@ struct Raw<JL_KV_Q8_0, DIM> {
         const jl_half2v nothing = {(_Float16)0.f, (_Float16)0.f}, most = {(_Float16)128.f, (_Float16)128.f};
         jl_half2v sum = nothing;
 #pragma unroll
-        for (int h = 0; h < kHalves; h++)
+        for (int h = 0; h < H; h++)
 #pragma unroll
             for (int w = 0; w < kPieces; w++)
 #pragma unroll
@@ -372,7 +385,7 @@ struct Raw<JL_KV_Q8_0, DIM> {
             return x & ~((even & 0x00ff00ffu) | (odd & 0xff00ff00u));
         };
 #pragma unroll
-        for (int h = 0; h < kHalves; h++) {
+        for (int h = 0; h < H; h++) {
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 auto scale = [&](int piece) { return (v_scale[h][piece][i / 2] >> 16 * (i % 2) & 0xffffu) * 0x10001u; };
@@ -390,11 +403,10 @@ struct Raw<JL_KV_Q8_0, DIM> {
         }
     }
     // Operands of two neighbouring blocks: their columns' bytes of two tokens come into one word, and out of it as pairs.
-    __device__ void v_operands(int block, jl_half8 (&v)[2]) const {
-        uintx4 r[2];
+    __device__ void v_pairs(int block, uint32_t (&r)[2][2 * H]) const {
         const int piece = block < 8 * kWide ? block / 8 : block < 8 * kWide + 4 * kMid ? kWide : kWide + kMid;
 #pragma unroll
-        for (int pair = 0; pair < 4; pair++) {
+        for (int pair = 0; pair < 2 * H; pair++) {
             const int h = pair / 2, i = pair % 2 * 2;
             uint32_t a, b;
             int byte;
@@ -405,7 +417,6 @@ struct Raw<JL_KV_Q8_0, DIM> {
             const jl_half2v d = as_half2(v_scale[h][piece][i / 2]);
             r[0][pair] = as_u32(even_bytes(both) * d), r[1][pair] = as_u32(even_bytes(both >> 8) * d);
         }
-        v[0] = __builtin_bit_cast(jl_half8, r[0]), v[1] = __builtin_bit_cast(jl_half8, r[1]);
     }
 };
 
@@ -421,20 +432,20 @@ __device__ __forceinline__ jl_half2v next_fours(uint32_t x) {
     return __builtin_elementwise_fma(as_half2((x & 0x00f000f0u) | 0x64006400u), part, bias);
 }
 
-template <int DIM>
-struct Raw<JL_KV_Q4_0, DIM> {
+template <int DIM, int H>
+struct Raw<JL_KV_Q4_0, DIM, H> {
     static constexpr int kSteps = DIM / 32;
     static constexpr int kWide = DIM / 128, kMid = DIM % 128 / 64, kThin = DIM % 64 / 32;
     static constexpr int kPieces = kWide + kMid + kThin;
     // of k, a lane has 32, 16 or 8 consecutive elements of a piece; of v as for the other types, four tokens beside each other
-    uintx4 k4[kHalves][kWide ? kWide : 1];
-    uintx2 k2[kHalves];
-    uint32_t k1[kHalves];
-    uint16_t k_scale[kHalves][kPieces];
-    uintx4 v4[kHalves][kWide ? kWide : 1];
-    uintx2 v2[kHalves], v1[kHalves];
+    uintx4 k4[H][kWide ? kWide : 1];
+    uintx2 k2[H];
+    uint32_t k1[H];
+    uint16_t k_scale[H][kPieces];
+    uintx4 v4[H][kWide ? kWide : 1];
+    uintx2 v2[H], v1[H];
     int v1_shift;
-    uintx2 v_scale[kHalves][kPieces];
+    uintx2 v_scale[H][kPieces];
     __device__ static int element(int step, int g) {
         if (step < 4 * kWide) return 128 * (step / 4) + 32 * g + 8 * (step % 4);
         if (step < 4 * kWide + 2 * kMid) return 128 * kWide + 16 * g + 8 * (step - 4 * kWide);
@@ -483,9 +494,9 @@ struct Raw<JL_KV_Q4_0, DIM> {
                                                    as_u32(low_fours(x >> 8) * dd), as_u32(next_fours(x >> 8) * dd)});
     }
     // (four bits times a scale of 0; the scale alone can be an infinity or NaN)
-    __device__ void mask_v(const bool (&seen)[kHalves][4]) {
+    __device__ void mask_v(const bool (&seen)[H][4]) {
 #pragma unroll
-        for (int h = 0; h < kHalves; h++)
+        for (int h = 0; h < H; h++)
 #pragma unroll
             for (int w = 0; w < kPieces; w++)
 #pragma unroll
@@ -497,7 +508,7 @@ struct Raw<JL_KV_Q4_0, DIM> {
         const jl_half2v nothing = {(_Float16)0.f, (_Float16)0.f}, most = {(_Float16)8.f, (_Float16)8.f};
         jl_half2v sum = nothing;
 #pragma unroll
-        for (int h = 0; h < kHalves; h++)
+        for (int h = 0; h < H; h++)
 #pragma unroll
             for (int w = 0; w < kPieces; w++)
 #pragma unroll
@@ -514,7 +525,7 @@ struct Raw<JL_KV_Q4_0, DIM> {
             return (x & ~bad) | (bad & 0x88888888u);
         };
 #pragma unroll
-        for (int h = 0; h < kHalves; h++) {
+        for (int h = 0; h < H; h++) {
 #pragma unroll
             for (int c = 0; c < 2; c++) {
 #pragma unroll
@@ -531,11 +542,10 @@ struct Raw<JL_KV_Q4_0, DIM> {
                 for (int c = 0; c < 2; c++) v_scale[h][w][c] &= ~not_finite(v_scale[h][w][c]);
         }
     }
-    __device__ void v_operands(int block, jl_half8 (&v)[2]) const {
-        uintx4 r[2];
+    __device__ void v_pairs(int block, uint32_t (&r)[2][2 * H]) const {
         const int piece = block < 8 * kWide ? block / 8 : block < 8 * kWide + 4 * kMid ? kWide : kWide + kMid;
 #pragma unroll
-        for (int pair = 0; pair < 4; pair++) {
+        for (int pair = 0; pair < 2 * H; pair++) {
             const int h = pair / 2, c = pair % 2;
             uint32_t x;
             if (block < 8 * kWide) x = v4[h][block / 8][block % 8 / 4 * 2 + c] >> block % 4 * 4;
@@ -544,9 +554,17 @@ struct Raw<JL_KV_Q4_0, DIM> {
             const jl_half2v d = as_half2(v_scale[h][piece][c]);
             r[0][pair] = as_u32(low_fours(x) * d), r[1][pair] = as_u32(next_fours(x) * d);
         }
-        v[0] = __builtin_bit_cast(jl_half8, r[0]), v[1] = __builtin_bit_cast(jl_half8, r[1]);
     }
 };
+
+// Eight tokens of two output blocks' columns.
+template <int TYPE, int DIM>
+__device__ __forceinline__ void v_operands(const Raw<TYPE, DIM> &raw, int block, jl_half8 (&v)[2]) {
+    uint32_t r[2][4];
+    raw.v_pairs(block, r);
+#pragma unroll
+    for (int i = 0; i < 2; i++) v[i] = __builtin_bit_cast(jl_half8, uintx4{r[i][0], r[i][1], r[i][2], r[i][3]});
+}
 
 // The output element that row 4 g + i of output block `block` is: 8, 4 or 2 consecutive blocks are consecutive elements.
 template <int DIM>
@@ -573,6 +591,60 @@ __device__ __forceinline__ float over_groups_sum(float x) {
 __device__ __forceinline__ void store_out(const JlAttentionArgs &p, int64_t at, const floatx4 v) {
     if (p.out_f16) *(jl_half4v *)((_Float16 *)p.out + at) = jl_half4v{(_Float16)v.x, (_Float16)v.y, (_Float16)v.z, (_Float16)v.w};
     else *(floatx4 *)((float *)p.out + at) = v;
+}
+
+// q, times a power of two that brings its largest value to 2^10 ... 2^11: both parts are then binary16 numbers of full
+// precision however large or small the row is.
+template <int TYPE, int DIM>
+__device__ __forceinline__ void split_q(const floatx4 (&x)[DIM / 32][2], float most, jl_half8 (&q_hi)[DIM / 32], jl_half8 (&q_lo)[DIM / 32], float &undo) {
+    int exponent = (int)((__float_as_uint(most) >> 23) & 255) - 127;
+    if (exponent < -100 || exponent == 128) exponent = 10;                  // zeros and the like, infinities, NaN
+    const float to = __uint_as_float((uint32_t)(10 - exponent + 127) << 23);
+    undo = __uint_as_float((uint32_t)(exponent - 10 + 127) << 23);
+#pragma unroll
+    for (int s = 0; s < DIM / 32; s++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int e = Raw<TYPE, DIM>::in_eight(i);
+            const float y = x[s][e / 4][e % 4] * to;
+            q_hi[s][i] = (_Float16)y;
+            q_lo[s][i] = (_Float16)(y - (float)q_hi[s][i]);
+        }
+}
+
+// A lane's eight scores of a tile, in powers of two: capped, and lowered by distance; `from` is the first one's token less the
+// row's position.
+__device__ __forceinline__ void shape_scores(const JlScoredArgs &p, float (&x)[8], float slope, int from) {
+    if (p.cap > 0.f) {
+        float most = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] *= p.one_over_cap, most = fmaxf(most, fabsf(x[i]));
+        if (__any(!(most <= kTanhNear))) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = p.cap * jl_tanh(x[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = p.cap * jl_tanh_near(x[i]);
+        }
+    }
+    if (p.slopes) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = fmaf(-slope, (float)abs(from + 16 * (i / 4) + i % 4), x[i]);
+    }
+}
+
+// 2^(x unit + lift) of eight scores, as two binary16 parts; added to the lane's sum.
+__device__ __forceinline__ void weights_of(const float (&x)[8], float unit, float lift, float &sum, jl_half8 &p_hi, jl_half8 &p_lo) {
+    uintx4 hi, lo;
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+        const float a = __builtin_amdgcn_exp2f(fmaf(x[i], unit, lift)), b = __builtin_amdgcn_exp2f(fmaf(x[i + 1], unit, lift));
+        sum += a + b;
+        const jl_half2v two = __builtin_convertvector(floatx2{a, b}, jl_half2v);
+        hi[i / 2] = as_u32(two);
+        lo[i / 2] = as_u32(__builtin_convertvector(floatx2{a - (float)two[0], b - (float)two[1]}, jl_half2v));
+    }
+    p_hi = __builtin_bit_cast(jl_half8, hi), p_lo = __builtin_bit_cast(jl_half8, lo);
 }
 
 // Units of a head in the list of all work: its tiles, and what beginning it takes.
@@ -605,6 +677,38 @@ __global__ void __launch_bounds__(kThreads, (Shape<TYPE, DIM>::kPerUnit)) jl_kv_
     const int tid = threadIdx.x, lane = tid % JL_WAVE, wave = uniform(tid / JL_WAVE);
     const int g = lane / 16, m = lane % 16;
     const int heads = p.cache.kv_heads * p.blocks_of_16;      // of a row's list
+    int rows = p.rows;
+    const uint16_t *blocks = nullptr;
+    if constexpr (kScored<ARGS>) {
+        __shared__ uint16_t blocks_left[kBlocksLeft];
+        __shared__ int left_of[kWaves];
+        if (p.taken) {
+            const int all = (rows + p.taken_rows - 1) / p.taken_rows, each = (all + kThreads - 1) / kThreads;
+            int own_left = 0;
+            for (int i = tid * each; i < min((tid + 1) * each, all); i++) own_left += p.taken[i] ? 0 : 1;
+            int through = own_left;
+#pragma unroll
+            for (int off = 1; off < JL_WAVE; off <<= 1) {
+                const int other = __shfl_up(through, off, JL_WAVE);
+                if (lane >= off) through += other;
+            }
+            if (lane == JL_WAVE - 1) left_of[wave] = through;
+            __syncthreads();
+            int left = 0;
+            for (int w = 0; w < kWaves; w++) {
+                if (w < wave) through += left_of[w];
+                left += left_of[w];
+            }
+            if (left == 0) return;
+            if (left <= kBlocksLeft) {
+                int at = through - own_left;
+                for (int i = tid * each; i < min((tid + 1) * each, all); i++)
+                    if (!p.taken[i]) blocks_left[at++] = (uint16_t)i;
+                blocks = blocks_left, rows = uniform(left * p.taken_rows);
+                __syncthreads();
+            }
+        }
+    }
     const int page_shift = p.cache.page_shift, in_page_mask = (1 << page_shift) - 1;
 
     // ---- the rows' ranges, 64 at a time in the lanes of every wave
@@ -613,8 +717,8 @@ __global__ void __launch_bounds__(kThreads, (Shape<TYPE, DIM>::kPerUnit)) jl_kv_
     int own_tiles = 0;                                        // without those of rows that go with the lane's
     auto load_window = [&](int from) {
         window_row = from;
-        in_lane = from + lane < p.rows ? range_of(p, from + lane) : Range{0, -1, 0};
-        own_tiles = in_lane.tiles();
+        in_lane = from + lane < rows ? range_of(p, from + lane, blocks) : Range{0, -1, 0};
+        own_tiles = kScored<ARGS> && in_lane.end == kTaken ? -1 : in_lane.tiles();
         if constexpr (SHARED) in_lane = run_in_lanes(p, in_lane, lane);
     };
 
@@ -624,14 +728,14 @@ __global__ void __launch_bounds__(kThreads, (Shape<TYPE, DIM>::kPerUnit)) jl_kv_
     const uint32_t mine = units_of(in_lane.tiles());
     uint32_t all, through = mine;                             // tiles of all rows; of those up to this lane's (this thread's last)
     uint32_t longest = mine, own = mine, longest_dealt = mine;   // ... of what is dealt whole
-    int per = (p.rows + kThreads - 1) / kThreads;             // rows a thread, where a wave does not hold them all
+    int per = (rows + kThreads - 1) / kThreads;             // rows a thread, where a wave does not hold them all
     if constexpr (SHARED) per = (per + p.rows_each - 1) & -p.rows_each;
     if constexpr (SHARED)
         for (int off = 1; off < p.rows_each; off <<= 1) longest_dealt += __shfl_xor(longest_dealt, off, JL_WAVE);
-    if (p.rows > JL_WAVE) {
+    if (rows > JL_WAVE) {
         uint32_t dealt = 0;
         own = longest = longest_dealt = 0;
-        for_runs<SHARED>(p, tid * per, min((tid + 1) * per, p.rows), [&](int r, const Range &range) {
+        for_runs<SHARED>(p, rows, blocks, tid * per, min((tid + 1) * per, rows), [&](int r, const Range &range) {
             const uint32_t n = units_of(range.tiles());
             own += n;
             longest = max(longest, n);
@@ -654,7 +758,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<TYPE, DIM>::kPerUnit)) jl_kv_
         if constexpr (SHARED) longest_dealt = max(longest_dealt, (uint32_t)__shfl_xor(longest_dealt, off, JL_WAVE));
     }
     all = __builtin_amdgcn_readlane(through, JL_WAVE - 1);
-    if (p.rows > JL_WAVE) {
+    if (rows > JL_WAVE) {
         if (lane == 0) scan[wave] = all, scan_longest[wave] = longest, scan_dealt[wave] = longest_dealt;
         __syncthreads();
         all = 0;
@@ -671,7 +775,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<TYPE, DIM>::kPerUnit)) jl_kv_
     // of 1000 tokens: 20.2 whole, 10.2 cut; of 256 tokens: 9.1 and 9.7.)
     // (Rows that go together: what is dealt whole is rows_each rows, whose runs come one after the other.)
     const int each = SHARED ? p.rows_each : 1;
-    const float rounds = ceilf((float)((p.rows + each - 1) / each) * heads / gridDim.x);
+    const float rounds = ceilf((float)((rows + each - 1) / each) * heads / gridDim.x);
     // Rows that go together read from the caches: whole where that is at most twice an equal span (2048 tokens, 32 heads over 8
     // of 64: 118 us whole, 203 cut).
     const bool whole = SHARED ? ((float)longest_dealt * rounds - kStart - 10) * gridDim.x <= 2.f * (float)all * heads
@@ -680,11 +784,11 @@ __global__ void __launch_bounds__(kThreads, (Shape<TYPE, DIM>::kPerUnit)) jl_kv_
     const uint32_t least = max((longest + kMostParts - 1) / kMostParts, min((longest + kParts - 1) / kParts, kLargePart));
     const uint32_t span = max((total + gridDim.x - 1) / gridDim.x, least);
     const uint32_t begin = whole ? 0 : span * blockIdx.x;
-    if (p.rows > JL_WAVE) {
+    if (rows > JL_WAVE) {
         const uint32_t from = begin / heads;
         if (!whole && begin < total && from >= through - own && from < through) {
             uint32_t before = through - own;
-            for_runs<SHARED>(p, tid * per, min((tid + 1) * per, p.rows), [&](int r, const Range &range) {
+            for_runs<SHARED>(p, rows, blocks, tid * per, min((tid + 1) * per, rows), [&](int r, const Range &range) {
                 const uint32_t n = units_of(range.tiles());
                 if (before + n > from) {
                     start_row = r, start_units = before;
@@ -699,10 +803,16 @@ __global__ void __launch_bounds__(kThreads, (Shape<TYPE, DIM>::kPerUnit)) jl_kv_
 
     // rows with nothing to read (one that goes with others is zeros from them too)
     const int width = p.cache.kv_heads * p.group * DIM;
-    for (int r = blockIdx.x; r < p.rows; r += gridDim.x) {
-        const int n = p.rows <= JL_WAVE ? __builtin_amdgcn_readlane(own_tiles, r) : range_of(p, r).tiles();
+    for (int r = blockIdx.x; r < rows; r += gridDim.x) {
+        int n;
+        if (rows <= JL_WAVE) {
+            n = __builtin_amdgcn_readlane(own_tiles, r);
+        } else {
+            const Range range = range_of(p, r, blocks);
+            n = kScored<ARGS> && range.end == kTaken ? -1 : range.tiles();
+        }
         if (n == 0)
-            for (int c = 4 * tid; c < width; c += 4 * kThreads) store_out(p, r * p.ldo + c, floatx4{0.f, 0.f, 0.f, 0.f});
+            for (int c = 4 * tid; c < width; c += 4 * kThreads) store_out(p, row_at(p, r, blocks) * p.ldo + c, floatx4{0.f, 0.f, 0.f, 0.f});
     }
 
     const int row_step = gridDim.x / heads, head_step = gridDim.x % heads;    // from one whole pair of a workgroup to its next
@@ -714,7 +824,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<TYPE, DIM>::kPerUnit)) jl_kv_
         if (begin >= total) return;
         const uint32_t from = begin / heads;
         uint32_t before;
-        if (p.rows <= JL_WAVE) {
+        if (rows <= JL_WAVE) {
             next.row = __popcll(__ballot(through <= from));
             before = next.row == 0 ? 0 : __builtin_amdgcn_readlane(through, uniform(next.row - 1));
         } else {
@@ -725,7 +835,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<TYPE, DIM>::kPerUnit)) jl_kv_
         next.left = min(span, total - begin);
     }
     auto next_whole = [&]() {
-        if (((next.row + 1) & (each - 1)) && next.row + 1 < p.rows) {
+        if (((next.row + 1) & (each - 1)) && next.row + 1 < rows) {
             next.row++;
         } else {
             next.row = (next.row & -each) + row_step * each, next.head += head_step;
@@ -736,7 +846,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<TYPE, DIM>::kPerUnit)) jl_kv_
     auto complete = [&]() {
         next.row = uniform(next.row), next.head = uniform(next.head), next.unit = uniform(next.unit), next.left = uniform(next.left);
         while (next.left > 0) {
-            if (next.row >= p.rows) {
+            if (next.row >= rows) {
                 next.left = 0;
                 break;
             }
@@ -810,7 +920,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<TYPE, DIM>::kPerUnit)) jl_kv_
         if (whole) next_whole();
         else if (++next.head >= heads) next.head -= heads, next.row++;
         complete();
-        const int count = cur.count, row = cur.row;
+        const int count = cur.count, row = kScored<ARGS> ? uniform(row_at(p, cur.row, blocks)) : cur.row;
         if (count == 0) continue;
         const int kv_head = kv_head_of(cur.head), block_of_16 = cur.head - kv_head * p.blocks_of_16;
         // (a row's tiles begin with the one of its first token)
@@ -835,8 +945,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<TYPE, DIM>::kPerUnit)) jl_kv_
         if constexpr (kScored<ARGS>)
             if (p.slopes) slope = 1.44269504088896340736f * p.slopes[q_head + head_of_lane];
 
-        // ---- q, times a power of two that brings its largest value to 2^10 ... 2^11: both parts are then binary16
-        // numbers of full precision however large or small the row is
+        // ---- q
         jl_half8 q_hi[kSteps], q_lo[kSteps];
         float undo;
         {
@@ -852,20 +961,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<TYPE, DIM>::kPerUnit)) jl_kv_
 #pragma unroll
                     for (int i = 0; i < 4; i++) most = fmaxf(most, fabsf(x[s][c][i]));
                 }
-            most = over_groups_max(most);
-            int exponent = (int)((__float_as_uint(most) >> 23) & 255) - 127;
-            if (exponent < -100 || exponent == 128) exponent = 10;                  // zeros and the like, infinities, NaN
-            const float to = __uint_as_float((uint32_t)(10 - exponent + 127) << 23);
-            undo = __uint_as_float((uint32_t)(exponent - 10 + 127) << 23);
-#pragma unroll
-            for (int s = 0; s < kSteps; s++)
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const int e = Raw<TYPE, DIM>::in_eight(i);
-                    const float y = x[s][e / 4][e % 4] * to;
-                    q_hi[s][i] = (_Float16)y;
-                    q_lo[s][i] = (_Float16)(y - (float)q_hi[s][i]);
-                }
+            split_q<TYPE, DIM>(x, over_groups_max(most), q_hi, q_lo, undo);
         }
 
         Range seen_here{cur.first, cur.end, 0}, seen_by_all = seen_here;      // what the lane's row sees, what all of them do
@@ -918,23 +1014,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<TYPE, DIM>::kPerUnit)) jl_kv_
             if constexpr (kScored<ARGS>) {
 #pragma unroll
                 for (int i = 0; i < 8; i++) x[i] *= undo;
-                if (p.cap > 0.f) {
-                    float most = 0.f;
-#pragma unroll
-                    for (int i = 0; i < 8; i++) x[i] *= p.one_over_cap, most = fmaxf(most, fabsf(x[i]));
-                    if (__any(!(most <= kTanhNear))) {
-#pragma unroll
-                        for (int i = 0; i < 8; i++) x[i] = p.cap * jl_tanh(x[i]);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 8; i++) x[i] = p.cap * jl_tanh_near(x[i]);
-                    }
-                }
-                if (p.slopes) {
-                    const int from = t * kTile + 4 * g - position;
-#pragma unroll
-                    for (int i = 0; i < 8; i++) x[i] = fmaf(-slope, (float)abs(from + 16 * (i / 4) + i % 4), x[i]);
-                }
+                shape_scores(p, x, slope, t * kTile + 4 * g - position);
             }
             const float unit = kScored<ARGS> ? 1.f : undo;    // of a score, in powers of two
             if (!all_seen) {
@@ -958,7 +1038,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<TYPE, DIM>::kPerUnit)) jl_kv_
 #pragma unroll
                         for (int b = 0; b < kBlocks; b += 2) {
                             jl_half8 v[2];
-                            raw.v_operands(b, v);
+                            v_operands(raw, b, v);
 #pragma unroll
                             for (int c = 0; c < 2; c++) {
                                 uintx4 its = __builtin_bit_cast(uintx4, v[c]);
@@ -987,21 +1067,12 @@ __global__ void __launch_bounds__(kThreads, (Shape<TYPE, DIM>::kPerUnit)) jl_kv_
 #pragma unroll
                 for (int b = 0; b < kBlocks; b++) o[b] *= keep;
             }
-            const float lift = kLift - top;
-            uintx4 hi, lo;
-#pragma unroll
-            for (int i = 0; i < 8; i += 2) {
-                const float a = __builtin_amdgcn_exp2f(fmaf(x[i], unit, lift)), b = __builtin_amdgcn_exp2f(fmaf(x[i + 1], unit, lift));
-                sum += a + b;
-                const jl_half2v two = __builtin_convertvector(floatx2{a, b}, jl_half2v);
-                hi[i / 2] = as_u32(two);
-                lo[i / 2] = as_u32(__builtin_convertvector(floatx2{a - (float)two[0], b - (float)two[1]}, jl_half2v));
-            }
-            const jl_half8 p_hi = __builtin_bit_cast(jl_half8, hi), p_lo = __builtin_bit_cast(jl_half8, lo);
+            jl_half8 p_hi, p_lo;
+            weights_of(x, unit, kLift - top, sum, p_hi, p_lo);
 #pragma unroll
             for (int b = 0; b < kBlocks; b += 2) {
                 jl_half8 v[2];
-                raw.v_operands(b, v);
+                v_operands(raw, b, v);
                 o[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[0], p_lo, o[b], 0, 0, 0);
                 o[b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[1], p_lo, o[b + 1], 0, 0, 0);
                 o[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[0], p_hi, o[b], 0, 0, 0);

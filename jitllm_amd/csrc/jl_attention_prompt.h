@@ -1,0 +1,323 @@
+// The kernel of attention over pages for blocks of rows of few requests: a prompt's.
+//
+// Mathematics and layouts are those of jl_attention_kernel.h.  There the waves of a workgroup share 16 columns, a (row,
+// query head) each, and take the tokens in turn: every 16 columns read all tokens.  Here a workgroup has 64 columns, 16 a
+// wave, that go through the same tokens.  Two tiles of 32 tokens at a time, each wave loads a half of one, decodes it, turns v
+// as the second product wants it, and leaves the matrix instructions' operands in LDS, as they are; all waves then
+// take both tiles from there, while the next two are on their way to registers and on to the other buffer.  What a tile costs to load and decode is paid once for 64
+// columns.
+//
+// Bound: the matrix instructions, four for a 16 x 16 x 32 piece (q and P are two binary16 parts each), and, as much, the
+// powers and conversions of P.
+//
+// Work.  A workgroup has a block of rows beside each other and a head of k and v.  Rows of one request whose
+// ranges touch go together, one run after the other.  A block with a run that is long and has few rows is left, whole, to the
+// other kernel, which cuts long ranges among workgroups; `taken` says to it which are not.
+#pragma once
+
+#include "jl_attention_kernel.h"
+
+namespace {
+
+constexpr int kLongRun = 32;                      // tiles of a run that has to have a quarter of the block's rows
+constexpr int kTilesAtATime = kWaves / kHalves;
+
+template <int DIM>
+struct PromptShape {
+    static constexpr int kFragments = DIM / 16 + DIM / 16;                 // of a tile, 1 KB each: k's, v's
+    static constexpr int kBufferBytes = kTilesAtATime * kFragments * 1024, kLdsBytes = 2 * kBufferBytes;
+    static constexpr int kPerUnit = DIM <= 128 ? 2 : 1;
+};
+
+// over the sixteen lanes of a row of lanes, and over all, in all of them
+__device__ __forceinline__ int over_16_min(int x) {
+#define JL_MIN_FROM(N) x = min(x, __builtin_amdgcn_update_dpp(0, x, 0x120 + N, 0xF, 0xF, true));
+    JL_MIN_FROM(8) JL_MIN_FROM(4) JL_MIN_FROM(2) JL_MIN_FROM(1)
+#undef JL_MIN_FROM
+    return x;
+}
+__device__ __forceinline__ int over_lanes_min(int x) {
+    x = over_16_min(x);
+    const auto f = __builtin_amdgcn_permlane32_swap((uint32_t)x, (uint32_t)x, false, false);
+    x = min((int)f[0], (int)f[1]);
+    const auto h = __builtin_amdgcn_permlane16_swap((uint32_t)x, (uint32_t)x, false, false);
+    return min((int)h[0], (int)h[1]);
+}
+
+template <int TYPE, int DIM>
+__global__ void __launch_bounds__(kThreads, PromptShape<DIM>::kPerUnit) jl_kv_attention_prompt_kernel(JlScoredArgs p) {
+    constexpr int kSteps = DIM / 32, kBlocks = DIM / 16, kFragments = PromptShape<DIM>::kFragments;
+    extern __shared__ __align__(16) uint8_t fragments[];       // [2][kTilesAtATime][kFragments][64 lanes][16 bytes]
+    __shared__ int half_info[2][kWaves];
+    const int tid = threadIdx.x, lane = tid % JL_WAVE, wave = uniform(tid / JL_WAVE);
+    const int g = lane / 16, m = lane % 16;
+    const int kv_heads = p.cache.kv_heads, kv_head = blockIdx.x % kv_heads;
+    const int block = gridDim.x / kv_heads - 1 - blockIdx.x / kv_heads;    // (the last rows first: a prompt's longest)
+    const int row0 = block * p.taken_rows, rows = min(p.taken_rows, p.rows - row0);
+    const int page_shift = p.cache.page_shift, in_page_mask = (1 << page_shift) - 1;
+
+    // ---- the rows' ranges, one a lane, and the runs that they make; rows without tokens make runs of their own
+    Range in_lane{0, -1, -1};
+    int position_in_lane;
+    {
+        const int row = row0 + min(lane, rows - 1);
+        position_in_lane = p.positions[row];
+        const Range r = range_at(p, row, position_in_lane, p.row_requests[row]);
+        if (lane < rows && r.end > r.first) in_lane = r;
+    }
+    const Range before{__shfl_up(in_lane.first, 1, JL_WAVE), __shfl_up(in_lane.end, 1, JL_WAVE), __shfl_up(in_lane.request, 1, JL_WAVE)};
+    const bool goes = lane > 0 && (in_lane.request < 0 ? before.request < 0 : goes_on(before, in_lane));
+    const uint64_t starts = __ballot(lane < rows && !goes);
+    auto run_end = [&](int from) {                            // of the run that begins at row `from`
+        const uint64_t behind = from < JL_WAVE - 1 ? starts >> (from + 1) : 0;
+        return behind ? from + 1 + (int)__builtin_ctzll(behind) : rows;
+    };
+    auto run_range = [&](int from, int to) {
+        const bool is = lane >= from && lane < to;
+        return Range{uniform(over_lanes_min(is ? in_lane.first : INT_MAX)), uniform(-over_lanes_min(is ? -in_lane.end : INT_MAX)),
+                     __builtin_amdgcn_readlane(in_lane.request, from)};
+    };
+    bool some = false, takes = true;
+    for (int from = 0, to; from < rows; from = to) {
+        to = run_end(from);
+        const int tiles = run_range(from, to).tiles();
+        some |= tiles > 0;
+        takes &= tiles <= kLongRun || 4 * (to - from) >= p.taken_rows;
+    }
+    takes &= some;
+    if (kv_head == 0 && tid == 0) p.taken_out[block] = takes;
+    if (!takes) return;
+
+    Raw<TYPE, DIM, 1> raw;
+    for (int from = 0, to; from < rows; from = to) {
+        to = run_end(from);
+        const int columns = (to - from) * p.group;
+        const Range run = run_range(from, to);
+        const int tile_begin = run.first / kTile, tile_end = run.end > run.first ? (run.end + kTile - 1) / kTile : tile_begin;
+
+        // a half of a tile of this wave's: its page, and the loads
+        const int its_tile = wave / kHalves, its_half = wave % kHalves;
+        bool paged = false;
+        auto issue = [&](int t) {
+            typedef const __attribute__((address_space(4))) int32_t constant_int;
+            constant_int *table = (constant_int *)(uintptr_t)(p.table + run.request * p.table_stride);
+            const int token = t * kTile + 16 * its_half;
+            const int page = token < run.end ? table[token >> page_shift] : -1;
+            paged = (unsigned)page < (unsigned)p.cache.pages;
+            const uint8_t *part = p.cache.k + ((int64_t)(paged ? page : 0) * kv_heads + kv_head) * p.cache.part_bytes;
+            raw.template load_k<true>(0, part, token & in_page_mask, page_shift, g, m);
+            raw.template load_v<true>(0, part + p.cache.v_offset, token & in_page_mask, page_shift, g, m);
+        };
+        auto issue_if = [&](int t) {
+            paged = false;
+            if (t < tile_end) issue(t);
+        };
+        // what was loaded, into a buffer; a half behind the last tile, or with no page, as tokens that nobody sees
+        auto stage = [&](int t, int buffer) {
+            const int token0 = t * kTile + 16 * its_half;
+            if (token0 < run.first || token0 + 16 > run.end || !paged) {
+                bool seen[1][4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) seen[0][i] = token0 + 4 * g + i >= run.first && token0 + 4 * g + i < run.end && paged;
+                raw.mask_v(seen);
+            }
+            const bool bad = __any(raw.any_not_finite());
+            if (lane == 0) half_info[buffer][wave] = (paged ? 1 : 0) | (bad ? 2 : 0);
+            uint8_t *to_fragment = fragments + buffer * PromptShape<DIM>::kBufferBytes + its_tile * (kFragments * 1024) + lane * 16;
+#pragma unroll
+            for (int s = 0; s < kSteps; s++) *(jl_half8 *)(to_fragment + (its_half * kSteps + s) * 1024) = raw.k_operand(0, s);
+#pragma unroll
+            for (int b = 0; b < kBlocks; b += 2) {
+                uint32_t v[2][2];
+                raw.v_pairs(b, v);
+#pragma unroll
+                for (int c = 0; c < 2; c++) *(uintx2 *)(to_fragment + (kBlocks + b + c) * 1024 + 8 * its_half) = uintx2{v[c][0], v[c][1]};
+            }
+        };
+        issue_if(tile_begin + its_tile);
+
+        // ---- this wave's columns: the query heads of one row after the other; lanes past the last one double it
+        const bool works = wave * 16 < columns;
+        const int column = min(wave * 16 + m, columns - 1), in_run = column / p.group;
+        const int row = row0 + from + in_run, head = kv_head * p.group + column - in_run * p.group;
+        const int position = __shfl(position_in_lane, from + in_run, JL_WAVE);
+        const int first_seen = __shfl(in_lane.first, from + in_run, JL_WAVE), end_seen = __shfl(in_lane.end, from + in_run, JL_WAVE);
+        // of all columns, and of any
+        const int all_first = uniform(-over_16_min(-first_seen)), all_end = uniform(over_16_min(end_seen));
+        const int any_first = uniform(over_16_min(first_seen)), any_end = uniform(-over_16_min(-end_seen));
+        const float slope = p.slopes ? 1.44269504088896340736f * p.slopes[head] : 0.f;
+        float undo = 0.f, top = kNone, sum = 0.f;
+        jl_half8 q_hi[kSteps], q_lo[kSteps];
+        floatx4 o[kBlocks];
+#pragma unroll
+        for (int b = 0; b < kBlocks; b++) o[b] = floatx4{0.f, 0.f, 0.f, 0.f};
+        if (works) {
+            const float *x_from = p.q + row * p.ldq + (int64_t)head * DIM;
+            floatx4 x[kSteps][2];
+            float most = 0.f;
+#pragma unroll
+            for (int s = 0; s < kSteps; s++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    x[s][e] = *(const floatx4 *)(x_from + Raw<TYPE, DIM>::element(s, g) + 4 * e);
+                    x[s][e] *= p.scale;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) most = fmaxf(most, fabsf(x[s][e][i]));
+                }
+            split_q<TYPE, DIM>(x, over_groups_max(most), q_hi, q_lo, undo);
+        }
+
+        __syncthreads();                                      // (all have read what the run before left)
+        stage(tile_begin + its_tile, 0);
+        issue_if(tile_begin + kTilesAtATime + its_tile);
+        for (int base = tile_begin, buffer = 0; base < tile_end; base += kTilesAtATime, buffer ^= 1) {
+            __syncthreads();                                  // (this buffer is written, and the other one read, by all)
+            if (works && base * kTile < any_end && (base + kTilesAtATime) * kTile > any_first) {
+                const uint8_t *fragment = fragments + buffer * PromptShape<DIM>::kBufferBytes + lane * 16;
+                auto operand = [&](int tile, int at) { return *(const jl_half8 *)(fragment + (tile * kFragments + at) * 1024); };
+                int info = 0, some_info = 0;                  // bit i: half i has a page; whether one has values that are not finite
+#pragma unroll
+                for (int i = 0; i < kWaves; i++) {
+                    const int its = uniform(half_info[buffer][i]);
+                    info |= (its & 1) << i, some_info |= its & 2;
+                }
+                floatx4 s[kTilesAtATime][kHalves];
+#pragma unroll
+                for (int t = 0; t < kTilesAtATime; t++)
+#pragma unroll
+                    for (int h = 0; h < kHalves; h++) s[t][h] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < kSteps; i++) {
+                    jl_half8 k[kTilesAtATime][kHalves];
+#pragma unroll
+                    for (int t = 0; t < kTilesAtATime; t++)
+#pragma unroll
+                        for (int h = 0; h < kHalves; h++) {
+                            k[t][h] = operand(t, h * kSteps + i);
+                            s[t][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[t][h], q_lo[i], s[t][h], 0, 0, 0);
+                        }
+#pragma unroll
+                    for (int t = 0; t < kTilesAtATime; t++)
+#pragma unroll
+                        for (int h = 0; h < kHalves; h++) s[t][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[t][h], q_hi[i], s[t][h], 0, 0, 0);
+                }
+                const bool all_seen = base * kTile >= all_first && (base + kTilesAtATime) * kTile <= all_end && info == (1 << kWaves) - 1;
+                float x[kTilesAtATime][8];
+                float most = -INFINITY;
+#pragma unroll
+                for (int t = 0; t < kTilesAtATime; t++) {
+                    const int token0 = (base + t) * kTile + 4 * g;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) x[t][i] = s[t][i / 4][i % 4] * undo;
+                    shape_scores(p, x[t], slope, token0 - position);
+                    if (!all_seen) {
+#pragma unroll
+                        for (int i = 0; i < 8; i++) {
+                            const int token = token0 + 16 * (i / 4) + i % 4;
+                            x[t][i] = token >= first_seen && token < end_seen && (info >> (t * kHalves + i / 4) & 1) ? x[t][i] : -INFINITY;
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; i++) most = fmaxf(most, x[t][i]);
+                }
+                most = over_groups_max(most);
+                if (__any(most > top + kSlack)) {
+                    const float next_top = fmaxf(top, most);
+                    const float keep = __builtin_amdgcn_exp2f(top - next_top);
+                    top = next_top;
+                    sum *= keep;
+#pragma unroll
+                    for (int b = 0; b < kBlocks; b++) o[b] *= keep;
+                }
+                jl_half8 p_hi[kTilesAtATime], p_lo[kTilesAtATime];
+#pragma unroll
+                for (int t = 0; t < kTilesAtATime; t++) weights_of(x[t], 1.f, kLift - top, sum, p_hi[t], p_lo[t]);
+                if (some_info) {
+                    // an infinity or NaN among the values: NaN to the columns that see it, nothing to the others (see there)
+#pragma unroll
+                    for (int t = 0; t < kTilesAtATime; t++) {
+                        uintx4 sees;
+#pragma unroll
+                        for (int i = 0; i < 8; i += 2) sees[i / 2] = (x[t][i] == -INFINITY ? 0u : 0x7f00u) | (x[t][i + 1] == -INFINITY ? 0u : 0x7f000000u);
+                        const bfloat8 plus = __builtin_bit_cast(bfloat8, sees), minus = __builtin_bit_cast(bfloat8, sees ^ 0x80008000u);
+#pragma unroll
+                        for (int b = 0; b < kBlocks; b++) {
+                            uintx4 v = __builtin_bit_cast(uintx4, operand(t, kBlocks + b)), its;
+#pragma unroll
+                            for (int i = 0; i < 4; i++) {
+                                const uint32_t bits = not_finite(v[i]);
+                                its[i] = bits & 0x7f007f00u, v[i] &= ~bits;
+                            }
+                            const jl_half8 rest = __builtin_bit_cast(jl_half8, v);
+                            o[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bfloat8, its), plus, o[b], 0, 0, 0);
+                            o[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bfloat8, its), minus, o[b], 0, 0, 0);
+                            o[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(rest, p_lo[t], o[b], 0, 0, 0);
+                            o[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(rest, p_hi[t], o[b], 0, 0, 0);
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int t = 0; t < kTilesAtATime; t++)
+#pragma unroll
+                        for (int b = 0; b < kBlocks; b += 2) {
+                            jl_half8 v[2];
+#pragma unroll
+                            for (int c = 0; c < 2; c++) {
+                                v[c] = operand(t, kBlocks + b + c);
+                                o[b + c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[c], p_lo[t], o[b + c], 0, 0, 0);
+                            }
+#pragma unroll
+                            for (int c = 0; c < 2; c++) o[b + c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[c], p_hi[t], o[b + c], 0, 0, 0);
+                        }
+                }
+            }
+            if (base + kTilesAtATime < tile_end) {
+                stage(base + kTilesAtATime + its_tile, buffer ^ 1);
+                issue_if(base + 2 * kTilesAtATime + its_tile);
+            }
+        }
+        if (!works) continue;
+        const float l = over_groups_sum(sum);
+        if (wave * 16 + m >= columns) continue;
+        const int64_t at = row * p.ldo + (int64_t)head * DIM;
+        auto put = [&](int element, floatx4 v) { store_out(p, at + element, l == 0.f ? floatx4{0.f, 0.f, 0.f, 0.f} : v / l); };
+        constexpr int wide = DIM / 128, mid = DIM % 128 / 64, thin = DIM % 64 / 32;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+#pragma unroll
+            for (int b = 0; b < 8 * wide; b += 4) put(128 * (b / 8) + 8 * (4 * g + i) + b % 8, floatx4{o[b][i], o[b + 1][i], o[b + 2][i], o[b + 3][i]});
+            if constexpr (mid) {
+                constexpr int b = 8 * wide;
+                put(128 * wide + 4 * (4 * g + i), floatx4{o[b][i], o[b + 1][i], o[b + 2][i], o[b + 3][i]});
+            }
+            if constexpr (thin) {
+                constexpr int b = 8 * wide + 4 * mid;
+                if (i % 2 == 0) put(128 * wide + 64 * mid + 2 * (4 * g + i), floatx4{o[b][i], o[b + 1][i], o[b][i + 1], o[b + 1][i + 1]});
+            }
+        }
+    }
+}
+
+template <int TYPE, int DIM>
+hipError_t launch_prompt(const JlScoredArgs &a, int device, hipStream_t stream) {
+    constexpr int lds = PromptShape<DIM>::kLdsBytes;
+    if (lds > 60 * 1024) {
+        static jl_lds_limit_flags raised;
+        if (jl_raise_lds_limit(raised, device, (const void *)jl_kv_attention_prompt_kernel<TYPE, DIM>, lds) != JL_OK) return hipErrorInvalidValue;
+    }
+    const unsigned groups = (unsigned)((a.rows + a.taken_rows - 1) / a.taken_rows) * a.cache.kv_heads;
+    hipLaunchKernelGGL((jl_kv_attention_prompt_kernel<TYPE, DIM>), dim3(groups), dim3(kThreads), lds, stream, a);
+    return hipGetLastError();
+}
+template <int TYPE>
+hipError_t launch_prompt_dim(const JlScoredArgs &a, int head_dim, int device, hipStream_t stream) {
+    switch (head_dim) {
+        case 64: return launch_prompt<TYPE, 64>(a, device, stream);
+        case 96: return launch_prompt<TYPE, 96>(a, device, stream);
+        case 128: return launch_prompt<TYPE, 128>(a, device, stream);
+        case 192: return launch_prompt<TYPE, 192>(a, device, stream);
+        default: return launch_prompt<TYPE, 256>(a, device, stream);
+    }
+}
+
+}  // namespace
