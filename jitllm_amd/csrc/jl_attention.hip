@@ -2,7 +2,6 @@
 #include <algorithm>
 #include <climits>
 #include <cmath>
-#include <cstdlib>
 
 #include "jl_attention.h"
 
@@ -10,8 +9,11 @@ namespace {
 
 constexpr size_t kArrivedBytes = kAttentionMostGroups * sizeof(uint32_t);
 constexpr size_t kTakenBytes = 32768;             // a byte for each block of rows, two rows at least
-// (Row block, head of k and v) pairs from which rows go in blocks.
-constexpr int64_t kPromptGroups = 128;
+// (Row block, head of k and v) pairs to a compute unit from which rows go in blocks: each is a workgroup's, whole, and the other
+// kernel cuts what it has among all.  (4-bit cache, 8 query heads over 4 of 128: 700 rows of one request, 88 pairs: 25.5 us in
+// blocks, 21.6 without; 1400, 176 pairs: 44.0 and 52.5; 4 requests of 175 ... 700, 220 pairs: 28.9 and 39.9.  32 over 8, after
+// 30 000 tokens: 128 rows, 64 pairs: 727 and 308; 512, 256 pairs, binary16: 750 and 1062.)
+constexpr float kPromptShare = 0.625f;
 
 bool aligned(const void *p, int to) { return ((uintptr_t)p & (to - 1)) == 0; }
 
@@ -79,7 +81,7 @@ int attention(const char *who, jl_context *ctx, const jl_kv_cache *cache, const 
     // Blocks of rows, where they are many: 64 columns to a workgroup, a (row, query head) each.
     a.taken_rows = 64 / a.group & -a.rows_each, a.taken = nullptr, a.taken_out = nullptr;
     const bool prompts = row_requests && rows >= 2 * requests && (shaping || cache->type == JL_KV_Q4_0) && a.taken_rows > 1 &&
-                         rows / a.taken_rows * cache->kv_heads >= (getenv("P1") ? atoi(getenv("P1")) : kPromptGroups);
+                         rows / a.taken_rows * cache->kv_heads >= ctx->compute_units * kPromptShare;
     if (prompts) a.taken_out = (uint8_t *)workspace + needed - kTakenBytes;
     const Shaping nothing{0.f, nullptr, nullptr, nullptr};
     if (prompts && !shaping) shaping = &nothing;

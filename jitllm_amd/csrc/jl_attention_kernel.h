@@ -423,13 +423,14 @@ struct Raw<JL_KV_Q8_0, DIM, H> {
 // Blocks of 32 values of four bits.  A word has eight elements of a token's keys, or four elements of two tokens' values, so
 // that one bit operation takes a pair out of it: 0x64 over four bits n is the binary16 of 1024 + n, or, where they are the
 // next four, of 1024 + 16 n; a subtraction, or a product and a sum that need no rounding, leave n - 8.
-__device__ __forceinline__ jl_half2v low_fours(uint32_t x) {
+// (`over` is 0x64006400, in a register, so that the and and the or are one instruction.)
+__device__ __forceinline__ jl_half2v low_fours(uint32_t x, uint32_t over) {
     const jl_half2v bias = {(_Float16)1032.f, (_Float16)1032.f};
-    return as_half2((x & 0x000f000fu) | 0x64006400u) - bias;
+    return as_half2((x & 0x000f000fu) | over) - bias;
 }
-__device__ __forceinline__ jl_half2v next_fours(uint32_t x) {
+__device__ __forceinline__ jl_half2v next_fours(uint32_t x, uint32_t over) {
     const jl_half2v part = {(_Float16)0.0625f, (_Float16)0.0625f}, bias = {(_Float16)-72.f, (_Float16)-72.f};
-    return __builtin_elementwise_fma(as_half2((x & 0x00f000f0u) | 0x64006400u), part, bias);
+    return __builtin_elementwise_fma(as_half2((x & 0x00f000f0u) | over), part, bias);
 }
 
 template <int DIM, int H>
@@ -445,7 +446,9 @@ struct Raw<JL_KV_Q4_0, DIM, H> {
     uintx4 v4[H][kWide ? kWide : 1];
     uintx2 v2[H], v1[H];
     int v1_shift;
+    uint32_t over;
     uintx2 v_scale[H][kPieces];
+    __device__ Raw() : over(0x64006400u) { asm("" : "+v"(over)); }
     __device__ static int element(int step, int g) {
         if (step < 4 * kWide) return 128 * (step / 4) + 32 * g + 8 * (step % 4);
         if (step < 4 * kWide + 2 * kMid) return 128 * kWide + 16 * g + 8 * (step - 4 * kWide);
@@ -490,8 +493,8 @@ struct Raw<JL_KV_Q4_0, DIM, H> {
         else if (step < 4 * kWide + 2 * kMid) x = k2[half][step % 2], d = k_scale[half][kMid ? kWide : 0];
         else x = k1[half], d = k_scale[half][kPieces - 1];
         const jl_half2v dd = as_half2(d | d << 16);
-        return __builtin_bit_cast(jl_half8, uintx4{as_u32(low_fours(x) * dd), as_u32(next_fours(x) * dd),
-                                                   as_u32(low_fours(x >> 8) * dd), as_u32(next_fours(x >> 8) * dd)});
+        return __builtin_bit_cast(jl_half8, uintx4{as_u32(low_fours(x, over) * dd), as_u32(next_fours(x, over) * dd),
+                                                   as_u32(low_fours(x >> 8, over) * dd), as_u32(next_fours(x >> 8, over) * dd)});
     }
     // (four bits times a scale of 0; the scale alone can be an infinity or NaN)
     __device__ void mask_v(const bool (&seen)[H][4]) {
@@ -518,10 +521,10 @@ struct Raw<JL_KV_Q4_0, DIM, H> {
     // those that are become 0, which four bits hold as 8: multiples that a finite scale takes too far, and scales that are not
     // finite
     __device__ void drop_not_finite() {
-        auto drop = [](uint32_t x, uint32_t scale) {
+        auto drop = [this](uint32_t x, uint32_t scale) {
             const jl_half2v d = as_half2(scale);
-            const uint32_t bad = (not_finite(as_u32(low_fours(x) * d)) & 0x000f000fu) | (not_finite(as_u32(next_fours(x) * d)) & 0x00f000f0u) |
-                                 (not_finite(as_u32(low_fours(x >> 8) * d)) & 0x0f000f00u) | (not_finite(as_u32(next_fours(x >> 8) * d)) & 0xf000f000u);
+            const uint32_t bad = (not_finite(as_u32(low_fours(x, over) * d)) & 0x000f000fu) | (not_finite(as_u32(next_fours(x, over) * d)) & 0x00f000f0u) |
+                                 (not_finite(as_u32(low_fours(x >> 8, over) * d)) & 0x0f000f00u) | (not_finite(as_u32(next_fours(x >> 8, over) * d)) & 0xf000f000u);
             return (x & ~bad) | (bad & 0x88888888u);
         };
 #pragma unroll
@@ -552,7 +555,7 @@ struct Raw<JL_KV_Q4_0, DIM, H> {
             else if (block < 8 * kWide + 4 * kMid) x = v2[h][c] >> block % 4 * 4;
             else x = v1[h][c] >> v1_shift;
             const jl_half2v d = as_half2(v_scale[h][piece][c]);
-            r[0][pair] = as_u32(low_fours(x) * d), r[1][pair] = as_u32(next_fours(x) * d);
+            r[0][pair] = as_u32(low_fours(x, over) * d), r[1][pair] = as_u32(next_fours(x, over) * d);
         }
     }
 };
@@ -612,20 +615,24 @@ __device__ __forceinline__ void split_q(const floatx4 (&x)[DIM / 32][2], float m
         }
 }
 
-// A lane's eight scores of a tile, in powers of two: capped, and lowered by distance; `from` is the first one's token less the
-// row's position.
-__device__ __forceinline__ void shape_scores(const JlScoredArgs &p, float (&x)[8], float slope, int from) {
+// A lane's eight scores of a tile, times `undo` in powers of two: capped, and lowered by distance; `from` is the first one's
+// token less the row's position.
+__device__ __forceinline__ void shape_scores(const JlScoredArgs &p, float (&x)[8], float undo, float slope, int from) {
     if (p.cap > 0.f) {
+        const float to = undo * p.one_over_cap;
         float most = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; i++) x[i] *= p.one_over_cap, most = fmaxf(most, fabsf(x[i]));
-        if (__any(!(most <= kTanhNear))) {
+        for (int i = 0; i < 8; i++) x[i] *= to, most = fmaxf(most, fabsf(x[i]));
+        if (__any(!(most <= kTanhMiddle))) {
 #pragma unroll
             for (int i = 0; i < 8; i++) x[i] = p.cap * jl_tanh(x[i]);
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = p.cap * jl_tanh_near(x[i]);
+            for (int i = 0; i < 8; i++) x[i] = p.cap * jl_tanh_middle(x[i]);
         }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] *= undo;
     }
     if (p.slopes) {
 #pragma unroll
@@ -1012,9 +1019,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<TYPE, DIM>::kPerUnit)) jl_kv_
 #pragma unroll
             for (int i = 0; i < 8; i++) x[i] = s[i / 4][i % 4];
             if constexpr (kScored<ARGS>) {
-#pragma unroll
-                for (int i = 0; i < 8; i++) x[i] *= undo;
-                shape_scores(p, x, slope, t * kTile + 4 * g - position);
+                shape_scores(p, x, undo, slope, t * kTile + 4 * g - position);
             }
             const float unit = kScored<ARGS> ? 1.f : undo;    // of a score, in powers of two
             if (!all_seen) {

@@ -4,7 +4,7 @@
 // query head) each, and take the tokens in turn: every 16 columns read all tokens.  Here a workgroup has 64 columns, 16 a
 // wave, that go through the same tokens.  Two tiles of 32 tokens at a time, each wave loads a half of one, decodes it, turns v
 // as the second product wants it, and leaves the matrix instructions' operands in LDS, as they are; all waves then
-// take both tiles from there, while the next two are on their way to registers and on to the other buffer.  What a tile costs to load and decode is paid once for 64
+// take both tiles from there, while the next two go on to the other buffer and two more are on their way.  What a tile costs to load and decode is paid once for 64
 // columns.
 //
 // Bound: the matrix instructions, four for a 16 x 16 x 32 piece (q and P are two binary16 parts each), and, as much, the
@@ -88,7 +88,7 @@ __global__ void __launch_bounds__(kThreads, PromptShape<DIM>::kPerUnit) jl_kv_at
     if (kv_head == 0 && tid == 0) p.taken_out[block] = takes;
     if (!takes) return;
 
-    Raw<TYPE, DIM, 1> raw;
+    Raw<TYPE, DIM, 1> raw[2];                                 // two tiles' and the next two's
     for (int from = 0, to; from < rows; from = to) {
         to = run_end(from);
         const int columns = (to - from) * p.group;
@@ -97,44 +97,47 @@ __global__ void __launch_bounds__(kThreads, PromptShape<DIM>::kPerUnit) jl_kv_at
 
         // a half of a tile of this wave's: its page, and the loads
         const int its_tile = wave / kHalves, its_half = wave % kHalves;
-        bool paged = false;
-        auto issue = [&](int t) {
+        bool paged[2];
+        auto issue = [&](auto which, int t) {
+            constexpr int W = decltype(which)::value;
+            paged[W] = false;
+            if (t >= tile_end) return;
             typedef const __attribute__((address_space(4))) int32_t constant_int;
             constant_int *table = (constant_int *)(uintptr_t)(p.table + run.request * p.table_stride);
             const int token = t * kTile + 16 * its_half;
             const int page = token < run.end ? table[token >> page_shift] : -1;
-            paged = (unsigned)page < (unsigned)p.cache.pages;
-            const uint8_t *part = p.cache.k + ((int64_t)(paged ? page : 0) * kv_heads + kv_head) * p.cache.part_bytes;
-            raw.template load_k<true>(0, part, token & in_page_mask, page_shift, g, m);
-            raw.template load_v<true>(0, part + p.cache.v_offset, token & in_page_mask, page_shift, g, m);
-        };
-        auto issue_if = [&](int t) {
-            paged = false;
-            if (t < tile_end) issue(t);
+            paged[W] = (unsigned)page < (unsigned)p.cache.pages;
+            const uint8_t *part = p.cache.k + ((int64_t)(paged[W] ? page : 0) * kv_heads + kv_head) * p.cache.part_bytes;
+            raw[W].template load_k<true>(0, part, token & in_page_mask, page_shift, g, m);
+            raw[W].template load_v<true>(0, part + p.cache.v_offset, token & in_page_mask, page_shift, g, m);
         };
         // what was loaded, into a buffer; a half behind the last tile, or with no page, as tokens that nobody sees
-        auto stage = [&](int t, int buffer) {
+        auto stage = [&](auto which, int t) {
+            constexpr int W = decltype(which)::value;
             const int token0 = t * kTile + 16 * its_half;
-            if (token0 < run.first || token0 + 16 > run.end || !paged) {
+            if (token0 < run.first || token0 + 16 > run.end || !paged[W]) {
                 bool seen[1][4];
 #pragma unroll
-                for (int i = 0; i < 4; i++) seen[0][i] = token0 + 4 * g + i >= run.first && token0 + 4 * g + i < run.end && paged;
-                raw.mask_v(seen);
+                for (int i = 0; i < 4; i++) seen[0][i] = token0 + 4 * g + i >= run.first && token0 + 4 * g + i < run.end && paged[W];
+                raw[W].mask_v(seen);
             }
-            const bool bad = __any(raw.any_not_finite());
-            if (lane == 0) half_info[buffer][wave] = (paged ? 1 : 0) | (bad ? 2 : 0);
-            uint8_t *to_fragment = fragments + buffer * PromptShape<DIM>::kBufferBytes + its_tile * (kFragments * 1024) + lane * 16;
+            const bool bad = __any(raw[W].any_not_finite());
+            if (lane == 0) half_info[W][wave] = (paged[W] ? 1 : 0) | (bad ? 2 : 0);
+            uint8_t *to_fragment = fragments + W * PromptShape<DIM>::kBufferBytes + its_tile * (kFragments * 1024) + lane * 16;
 #pragma unroll
-            for (int s = 0; s < kSteps; s++) *(jl_half8 *)(to_fragment + (its_half * kSteps + s) * 1024) = raw.k_operand(0, s);
+            for (int s = 0; s < kSteps; s++) *(jl_half8 *)(to_fragment + (its_half * kSteps + s) * 1024) = raw[W].k_operand(0, s);
 #pragma unroll
             for (int b = 0; b < kBlocks; b += 2) {
                 uint32_t v[2][2];
-                raw.v_pairs(b, v);
+                raw[W].v_pairs(b, v);
 #pragma unroll
                 for (int c = 0; c < 2; c++) *(uintx2 *)(to_fragment + (kBlocks + b + c) * 1024 + 8 * its_half) = uintx2{v[c][0], v[c][1]};
             }
         };
-        issue_if(tile_begin + its_tile);
+        const std::integral_constant<int, 0> even{};
+        const std::integral_constant<int, 1> odd{};
+        issue(even, tile_begin + its_tile);
+        issue(odd, tile_begin + kTilesAtATime + its_tile);
 
         // ---- this wave's columns: the query heads of one row after the other; lanes past the last one double it
         const bool works = wave * 16 < columns;
@@ -168,59 +171,99 @@ __global__ void __launch_bounds__(kThreads, PromptShape<DIM>::kPerUnit) jl_kv_at
         }
 
         __syncthreads();                                      // (all have read what the run before left)
-        stage(tile_begin + its_tile, 0);
-        issue_if(tile_begin + kTilesAtATime + its_tile);
-        for (int base = tile_begin, buffer = 0; base < tile_end; base += kTilesAtATime, buffer ^= 1) {
+        stage(even, tile_begin + its_tile);
+        issue(even, tile_begin + 2 * kTilesAtATime + its_tile);
+        auto step = [&](auto which, auto other, int base) {
+            constexpr int buffer = decltype(which)::value;
             __syncthreads();                                  // (this buffer is written, and the other one read, by all)
-            if (works && base * kTile < any_end && (base + kTilesAtATime) * kTile > any_first) {
-                const uint8_t *fragment = fragments + buffer * PromptShape<DIM>::kBufferBytes + lane * 16;
-                auto operand = [&](int tile, int at) { return *(const jl_half8 *)(fragment + (tile * kFragments + at) * 1024); };
-                int info = 0, some_info = 0;                  // bit i: half i has a page; whether one has values that are not finite
+            const uint8_t *fragment = fragments + buffer * PromptShape<DIM>::kBufferBytes + lane * 16;
+            auto operand = [&](int i) { return *(const jl_half8 *)(fragment + (i / (2 * kBlocks) * kFragments + i % (2 * kBlocks)) * 1024); };
+            int info = 0, bad = 0;                            // bit i: half i has a page; one has values that are not finite
 #pragma unroll
-                for (int i = 0; i < kWaves; i++) {
-                    const int its = uniform(half_info[buffer][i]);
-                    info |= (its & 1) << i, some_info |= its & 2;
-                }
-                floatx4 s[kTilesAtATime][kHalves];
+            for (int i = 0; i < kWaves; i++) {
+                const int its = uniform(half_info[buffer][i]);
+                info |= (its & 1) << i, bad |= its & 2;
+            }
+            const bool reads = works && base * kTile < any_end && (base + kTilesAtATime) * kTile > any_first;
+            auto sees = [&](int i) {                          // token i of the lane's sixteen
+                const int token = base * kTile + i / 4 * 16 + 4 * g + i % 4;
+                return token >= first_seen && token < end_seen && (info >> i / 4 & 1);
+            };
+            if (bad) {
+                // An infinity or NaN among the values: NaN to the columns that see it (2^127 in its place times 2^127, and times
+                // -2^127), and 0 where it lay.
+                if (reads) {
+#pragma unroll 1
+                    for (int t = 0; t < kTilesAtATime; t++) {
+                        uintx4 plus;
 #pragma unroll
-                for (int t = 0; t < kTilesAtATime; t++)
+                        for (int i = 0; i < 8; i += 2) plus[i / 2] = (sees(8 * t + i) ? 0x7f00u : 0u) | (sees(8 * t + i + 1) ? 0x7f000000u : 0u);
+                        const bfloat8 both[2] = {__builtin_bit_cast(bfloat8, plus), __builtin_bit_cast(bfloat8, plus ^ 0x80008000u)};
 #pragma unroll
-                    for (int h = 0; h < kHalves; h++) s[t][h] = floatx4{0.f, 0.f, 0.f, 0.f};
+                        for (int b = 0; b < kBlocks; b++) {
+                            uintx4 its = __builtin_bit_cast(uintx4, operand(2 * kBlocks * t + kBlocks + b));
 #pragma unroll
-                for (int i = 0; i < kSteps; i++) {
-                    jl_half8 k[kTilesAtATime][kHalves];
+                            for (int i = 0; i < 4; i++) its[i] = not_finite(its[i]) & 0x7f007f00u;
 #pragma unroll
-                    for (int t = 0; t < kTilesAtATime; t++)
-#pragma unroll
-                        for (int h = 0; h < kHalves; h++) {
-                            k[t][h] = operand(t, h * kSteps + i);
-                            s[t][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[t][h], q_lo[i], s[t][h], 0, 0, 0);
+                            for (int i = 0; i < 2; i++) o[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bfloat8, its), both[i], o[b], 0, 0, 0);
                         }
-#pragma unroll
-                    for (int t = 0; t < kTilesAtATime; t++)
-#pragma unroll
-                        for (int h = 0; h < kHalves; h++) s[t][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[t][h], q_hi[i], s[t][h], 0, 0, 0);
+                    }
                 }
+                __syncthreads();
+                uint8_t *own_half = fragments + buffer * PromptShape<DIM>::kBufferBytes + its_tile * (kFragments * 1024) + lane * 16 + 8 * its_half;
+#pragma unroll 1
+                for (int b = 0; b < kBlocks; b++) {
+                    uintx2 *at = (uintx2 *)(own_half + (kBlocks + b) * 1024);
+                    const uintx2 v = *at;
+                    *at = uintx2{v.x & ~not_finite(v.x), v.y & ~not_finite(v.y)};
+                }
+                __syncthreads();
+            }
+            if (reads) {
+                // (operands come from LDS a step ahead of the matrix instructions that take them, the values' first ones before
+                // the weights are worked out)
+                constexpr int kAtOnce = kTilesAtATime * kHalves;
+                floatx4 s[kAtOnce];
+                jl_half8 k[2][kAtOnce];
+                auto key_operand = [&](int step, int i) { return operand(2 * kBlocks * (i / kHalves) + i % kHalves * kSteps + step); };
+#pragma unroll
+                for (int i = 0; i < kAtOnce; i++) s[i] = floatx4{0.f, 0.f, 0.f, 0.f}, k[0][i] = key_operand(0, i);
+#pragma unroll
+                for (int step = 0; step < kSteps; step++) {
+                    if (step + 1 < kSteps) {
+#pragma unroll
+                        for (int i = 0; i < kAtOnce; i++) k[(step + 1) % 2][i] = key_operand(step + 1, i);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int i = 0; i < kAtOnce; i++) s[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[step % 2][i], q_lo[step], s[i], 0, 0, 0);
+#pragma unroll
+                    for (int i = 0; i < kAtOnce; i++) s[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[step % 2][i], q_hi[step], s[i], 0, 0, 0);
+                }
+                constexpr int kAhead = 4;
+                jl_half8 v[2][kAhead];
+                auto value_operand = [&](int i) { return operand(i / kBlocks * 2 * kBlocks + kBlocks + i % kBlocks); };
+#pragma unroll
+                for (int i = 0; i < kAhead; i++) v[0][i] = value_operand(i);
+                __builtin_amdgcn_sched_barrier(0);
                 const bool all_seen = base * kTile >= all_first && (base + kTilesAtATime) * kTile <= all_end && info == (1 << kWaves) - 1;
+                const bool shaped = p.cap > 0.f || p.slopes;
+                const float unit = shaped ? 1.f : undo;       // of a score, in powers of two
                 float x[kTilesAtATime][8];
                 float most = -INFINITY;
 #pragma unroll
                 for (int t = 0; t < kTilesAtATime; t++) {
-                    const int token0 = (base + t) * kTile + 4 * g;
 #pragma unroll
-                    for (int i = 0; i < 8; i++) x[t][i] = s[t][i / 4][i % 4] * undo;
-                    shape_scores(p, x[t], slope, token0 - position);
+                    for (int i = 0; i < 8; i++) x[t][i] = s[t * kHalves + i / 4][i % 4];
+                    if (shaped) shape_scores(p, x[t], undo, slope, (base + t) * kTile + 4 * g - position);
                     if (!all_seen) {
 #pragma unroll
-                        for (int i = 0; i < 8; i++) {
-                            const int token = token0 + 16 * (i / 4) + i % 4;
-                            x[t][i] = token >= first_seen && token < end_seen && (info >> (t * kHalves + i / 4) & 1) ? x[t][i] : -INFINITY;
-                        }
+                        for (int i = 0; i < 8; i++) x[t][i] = sees(8 * t + i) ? x[t][i] : -INFINITY;
                     }
 #pragma unroll
                     for (int i = 0; i < 8; i++) most = fmaxf(most, x[t][i]);
                 }
-                most = over_groups_max(most);
+                most = over_groups_max(most) * unit;
                 if (__any(most > top + kSlack)) {
                     const float next_top = fmaxf(top, most);
                     const float keep = __builtin_amdgcn_exp2f(top - next_top);
@@ -231,50 +274,39 @@ __global__ void __launch_bounds__(kThreads, PromptShape<DIM>::kPerUnit) jl_kv_at
                 }
                 jl_half8 p_hi[kTilesAtATime], p_lo[kTilesAtATime];
 #pragma unroll
-                for (int t = 0; t < kTilesAtATime; t++) weights_of(x[t], 1.f, kLift - top, sum, p_hi[t], p_lo[t]);
-                if (some_info) {
-                    // an infinity or NaN among the values: NaN to the columns that see it, nothing to the others (see there)
+                for (int t = 0; t < kTilesAtATime; t++) weights_of(x[t], unit, kLift - top, sum, p_hi[t], p_lo[t]);
+                constexpr int kValues = kTilesAtATime * kBlocks;
 #pragma unroll
-                    for (int t = 0; t < kTilesAtATime; t++) {
-                        uintx4 sees;
+                for (int from = 0; from < kValues; from += kAhead) {
+                    const int now = from / kAhead % 2;
+                    if (from + kAhead < kValues) {
 #pragma unroll
-                        for (int i = 0; i < 8; i += 2) sees[i / 2] = (x[t][i] == -INFINITY ? 0u : 0x7f00u) | (x[t][i + 1] == -INFINITY ? 0u : 0x7f000000u);
-                        const bfloat8 plus = __builtin_bit_cast(bfloat8, sees), minus = __builtin_bit_cast(bfloat8, sees ^ 0x80008000u);
-#pragma unroll
-                        for (int b = 0; b < kBlocks; b++) {
-                            uintx4 v = __builtin_bit_cast(uintx4, operand(t, kBlocks + b)), its;
-#pragma unroll
-                            for (int i = 0; i < 4; i++) {
-                                const uint32_t bits = not_finite(v[i]);
-                                its[i] = bits & 0x7f007f00u, v[i] &= ~bits;
-                            }
-                            const jl_half8 rest = __builtin_bit_cast(jl_half8, v);
-                            o[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bfloat8, its), plus, o[b], 0, 0, 0);
-                            o[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bfloat8, its), minus, o[b], 0, 0, 0);
-                            o[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(rest, p_lo[t], o[b], 0, 0, 0);
-                            o[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(rest, p_hi[t], o[b], 0, 0, 0);
-                        }
+                        for (int i = 0; i < kAhead; i++)
+                            if (from + kAhead + i < kValues) v[1 - now][i] = value_operand(from + kAhead + i);
                     }
-                } else {
+                    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int t = 0; t < kTilesAtATime; t++)
+                    for (int i = 0; i < kAhead; i++)
+                        if (from + i < kValues) {
+                            const int b = (from + i) % kBlocks, its = (from + i) / kBlocks;
+                            o[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[now][i], p_lo[its], o[b], 0, 0, 0);
+                        }
 #pragma unroll
-                        for (int b = 0; b < kBlocks; b += 2) {
-                            jl_half8 v[2];
-#pragma unroll
-                            for (int c = 0; c < 2; c++) {
-                                v[c] = operand(t, kBlocks + b + c);
-                                o[b + c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[c], p_lo[t], o[b + c], 0, 0, 0);
-                            }
-#pragma unroll
-                            for (int c = 0; c < 2; c++) o[b + c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[c], p_hi[t], o[b + c], 0, 0, 0);
+                    for (int i = 0; i < kAhead; i++)
+                        if (from + i < kValues) {
+                            const int b = (from + i) % kBlocks, its = (from + i) / kBlocks;
+                            o[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[now][i], p_hi[its], o[b], 0, 0, 0);
                         }
                 }
             }
             if (base + kTilesAtATime < tile_end) {
-                stage(base + kTilesAtATime + its_tile, buffer ^ 1);
-                issue_if(base + 2 * kTilesAtATime + its_tile);
+                stage(other, base + kTilesAtATime + its_tile);
+                issue(other, base + 3 * kTilesAtATime + its_tile);
             }
+        };
+        for (int base = tile_begin; base < tile_end; base += 2 * kTilesAtATime) {
+            step(even, odd, base);
+            if (base + kTilesAtATime < tile_end) step(odd, even, base + kTilesAtATime);
         }
         if (!works) continue;
         const float l = over_groups_sum(sum);

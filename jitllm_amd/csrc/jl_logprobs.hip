@@ -274,10 +274,10 @@ __global__ void __launch_bounds__(WAVES * JL_WAVE) jl_logprobs_kernel(LogprobsAr
         float least = x[0];
 #pragma unroll
         for (int i = 1; i < 4 * kEach; i++) least = fminf(least, x[i]);
-        // (all of a step's where tanh's series ends: one form)
-        if (p.cap > 0.f && !__any(fmaxf(most, -least) * p.one_over_cap > kTanhNear)) {
+        // (one form of tanh where all of a step's are within its reach)
+        if (p.cap > 0.f && !__any(!(fmaxf(most, -least) * p.one_over_cap <= kTanhMiddle))) {
 #pragma unroll
-            for (int i = 0; i < 4 * kEach; i++) x[i] = p.cap * jl_tanh_near(x[i] * p.one_over_cap);
+            for (int i = 0; i < 4 * kEach; i++) x[i] = p.cap * jl_tanh_middle(x[i] * p.one_over_cap);
         } else if (p.cap > 0.f) {
 #pragma unroll
             for (int i = 0; i < 4 * kEach; i++) x[i] = capped(p, x[i]);

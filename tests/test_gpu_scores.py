@@ -265,6 +265,54 @@ def test_attend_scored(ctx, runs, requests, heads, kv, dim, page, kind, window, 
         first, end = (None if x is None else x[::-1].copy() for x in (first, end))
 
 
+PROMPTS = [
+    # enough rows that they go in blocks: of one request, of several of odd lengths, beside rows that decode over long and short
+    # contexts, beside rows of nothing
+    ([(0, 0, 1400)], 1, 8, 2, 64, 16, "q4", 0, False, 0.0, False, False, 0), ([(0, 0, 500), (1, 900, 333), (2, 3, 70)], 3, 12, 4, 96, 16, "f16", 0, True, 20.0, True, True, 0),
+    ([(0, 0, 300)] + [(1 + r, 1000 + 13 * r, 1) for r in range(40)] + [(41, 40, 35)], 42, 32, 8, 128, 32, "q8", 0, False, 30.0, False, False, 100),
+    ([(0, 0, 300)] + [(1 + r, 1000 + 13 * r, 1) for r in range(40)] + [(-1, 5, 30)], 41, 32, 8, 64, 64, "q4", 0, False, 0.0, False, False, 0),
+    ([(r, 11 * r, 9) for r in range(60)], 60, 16, 8, 64, 16, "f16", 0, False, 0.0, True, False, 0), ([(0, 50, 620)], 1, 7, 7, 128, 16, "q4", 200, True, 5.0, False, False, 0),
+    ([(0, 0, 330), (1, 700, 90)], 2, 14, 7, 192, 16, "q8", 0, False, 0.0, False, True, 0), ([(0, 0, 130), (1, 0, 75)], 2, 48, 16, 256, 32, "f16", 64, False, 50.0, False, False, 40),
+    ([(0, 0, 90)], 1, 96, 4, 256, 16, "q4", 0, False, 0.0, True, False, 60), ([(0, 10, 1300), (-1, 0, 2400), (1, 0, 400)], 2, 32, 1, 64, 16, "f16", 30, False, 0.0, True, False, 0)]
+
+
+@pytest.mark.parametrize("runs,requests,heads,kv,dim,page,kind,window,half,cap,slopes,documents,prefix", PROMPTS)
+def test_attend_prompts(ctx, runs, requests, heads, kv, dim, page, kind, window, half, cap, slopes, documents, prefix):
+    test_attend_scored(ctx, runs, requests, heads, kv, dim, page, kind, window, half, cap, slopes, documents, prefix)
+
+
+@pytest.mark.parametrize("kind", S.KINDS)
+def test_attend_prompts_of_values_that_are_not_finite(ctx, kind):
+    """Infinities, NaN and, in four bits, a scale that takes its multiples past binary16, at tokens that some rows of a block
+    see: those may get NaN, the others are what they are without; and pages outside the cache."""
+    rng = np.random.default_rng(21)
+    heads, kv, dim, page, rows = 4, 4, 64, 16, 3000
+    table, pages = K.make_tables(rng, [rows], page)
+    table[0, 7], table[0, 100] = -1, pages
+    raw = S.random_pool(rng, kind, pages, kv, dim, page)
+    bad_tokens = [37, 640, 1001, 2999]
+    dirty = raw.reshape(2, pages, kv, -1).copy()
+    for t, bad in zip(bad_tokens, (np.inf, np.nan, 30000 if kind == "q4" else -np.inf, np.nan)):
+        p, o = table[0, t // page], t % page
+        if kind == "f16":
+            dirty.view(np.float16).reshape(2, pages, kv, page, dim)[1, p, :, o, 5::7] = bad
+        else:
+            codes = page * dim // (1 if kind == "q8" else 2)
+            scales = dirty[..., codes:].view(np.float16).reshape(2, pages, kv, dim // 32, page)
+            scales[1, p, :, 1, o] = np.float16(bad)
+            dirty[..., codes:] = scales.view(np.uint8).reshape(2, pages, kv, -1)
+    cache = cache_of(ctx, kind, pages, kv, dim, page, dirty.reshape(-1))
+    q = rng.standard_normal((rows, heads, dim)).astype(np.float32)
+    positions, of = np.arange(rows), np.zeros(rows, int)
+    say("attend prompts not finite", kind)
+    window = 20
+    got = run(ctx, cache, q, positions, of, table, window, cap=20.0)
+    hit = np.array([any(i - window < t <= i for t in bad_tokens) for i in range(rows)])
+    want, bound = S.attend(S.decode_pool(raw, kind, pages, kv, dim, page), q, positions, of, table, dim ** -0.5, window, 20.0)
+    check(got[~hit], want[~hit], bound[~hit])
+    assert hit.sum() == 3 * window + 1 and not np.isfinite(got[hit]).all()
+
+
 @pytest.mark.parametrize("rows_together", [False, True])
 def test_attend_scored_ranges_that_leave_nothing(ctx, rows_together):
     """Ends before their beginnings, behind the table's last token, below 0; documents that begin behind the row."""
