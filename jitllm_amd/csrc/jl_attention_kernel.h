@@ -674,6 +674,10 @@ struct Cut {
 template <int TYPE, int DIM, bool SHARED, typename ARGS>
 __global__ void __launch_bounds__(kThreads, (Shape<TYPE, DIM>::kPerUnit)) jl_kv_attention_kernel(ARGS p) {
     constexpr int kSteps = DIM / 32, kBlocks = DIM / 16;
+    // Loads go out whether there is a next tile or not: where one path has none, the wait for k in front of a tile is made for
+    // that path, and waits for v too, which went out last (131072 tokens in 4-bit blocks: 53.3 -> 49.8 us).  Those of the other types
+    // are large enough that all of memory's rate goes to them either way.
+    constexpr bool EAGER = !SHARED && TYPE == JL_KV_Q4_0;
     constexpr int kRound = DIM == 256 ? 128 : DIM;            // elements that are joined at a time: 64 KB of LDS at most
     constexpr int kStride = kRound + 4;                       // (four floats on: rows start on other banks)
     constexpr int kSlot = 16 * (DIM + 2);
@@ -996,8 +1000,10 @@ __global__ void __launch_bounds__(kThreads, (Shape<TYPE, DIM>::kPerUnit)) jl_kv_
             // what is loaded next: this piece's next tile of the wave, or the next piece's first
             const bool more = t + kWaves < last;
             loaded = more || (next.left > 0 && next_tile < next_last);
-            const int load_tile = more ? t + kWaves : next_tile, load_head = more ? kv_head : next_head;
-            if (loaded) find_pages(more ? cur : next, load_tile);
+            // (EAGER: this tile's again where there is none)
+            const bool own_piece = more || (EAGER && !loaded);
+            const int load_tile = more ? t + kWaves : own_piece ? t : next_tile, load_head = own_piece ? kv_head : next_head;
+            if (EAGER || loaded) find_pages(own_piece ? cur : next, load_tile);
             // (the halves side by side: a product waits for the one before it of its own half only)
             floatx4 s[kHalves];
 #pragma unroll
@@ -1013,7 +1019,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<TYPE, DIM>::kPerUnit)) jl_kv_
 #pragma unroll
                 for (int h = 0; h < kHalves; h++) s[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[h], q_hi[i], s[h], 0, 0, 0);
             }
-            if (loaded) issue(load_head, load_tile, false);   // k goes out as soon as this tile's is used
+            if (EAGER || loaded) issue(load_head, load_tile, false);   // k goes out as soon as this tile's is used
             const bool all_seen = t * kTile >= seen_by_all.first && t * kTile + kTile <= seen_by_all.end && with_page == (1u << kHalves) - 1;
             float x[8];
 #pragma unroll
@@ -1083,7 +1089,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<TYPE, DIM>::kPerUnit)) jl_kv_
                 o[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[0], p_hi, o[b], 0, 0, 0);
                 o[b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[1], p_hi, o[b + 1], 0, 0, 0);
             }
-            if (loaded) issue(load_head, load_tile, true);
+            if (EAGER || loaded) issue(load_head, load_tile, true);
         }
 
         // ---- the four waves' parts into one
