@@ -13,6 +13,7 @@
 //   GGUF                       J/format/GGUF.java:40-255, as far as a tensor's upload needs it
 //   PagedKvCache, BlockTables, PagedAttention, Rope
 //                              what lies between a layer's q|k|v and its output projection
+//   LogProbabilities           what is answered with beside the tokens, behind the vocabulary projection
 //
 // Where the reference adds a task to a TaskGraph these enqueue a kernel on the context's stream, so
 // the `graph` / `name` arguments of the reference disappear.  Error behaviour is the reference's: a
@@ -566,6 +567,13 @@ private:
     int requests_, blocks_, pages_, pageTokens_, maxRows_;
 };
 
+// What attention makes of its scores and sees, as jl_kv_attention_scored does; what is left as it is here changes nothing.
+struct Scores {
+    float cap = 0.f;
+    const FloatArray *slopes = nullptr;                            // of each head
+    const IntArray *firstTokens = nullptr, *endTokens = nullptr;   // of each row
+};
+
 // Attention of one new token a row over paged caches of one shape, with the workspace it joins in.
 class PagedAttention {
 public:
@@ -582,8 +590,29 @@ public:
                 float scale, std::int64_t window = 0) const {
         run(cache, q, rows, tables, out.at(rows, static_cast<std::int64_t>(heads_) * headDim_), 1, out.stride, scale, window);
     }
+    void attend(const PagedKvCache &cache, const FloatRows &q, std::int64_t rows, const BlockTables &tables, const FloatRows &out,
+                float scale, std::int64_t window, const Scores &scores) const {
+        run(cache, q, rows, tables, out.at(rows, static_cast<std::int64_t>(heads_) * headDim_), 0, out.stride, scale, window, scores);
+    }
+    void attend(const PagedKvCache &cache, const FloatRows &q, std::int64_t rows, const BlockTables &tables, const HalfRows &out,
+                float scale, std::int64_t window, const Scores &scores) const {
+        run(cache, q, rows, tables, out.at(rows, static_cast<std::int64_t>(heads_) * headDim_), 1, out.stride, scale, window, scores);
+    }
 
 private:
+    void run(const PagedKvCache &cache, const FloatRows &q, std::int64_t rows, const BlockTables &tables, void *out, int half,
+             std::int64_t ldo, float scale, std::int64_t window, const Scores &scores) const {
+        if (cache.kvHeads() != kvHeads_ || cache.headDim() != headDim_) throw std::invalid_argument("a cache of another shape");
+        if (scores.slopes && scores.slopes->size() != static_cast<std::size_t>(heads_)) throw std::invalid_argument("slopes for other heads");
+        for (const IntArray *a : {&tables.positions, scores.firstTokens, scores.endTokens})
+            if (a && rows > 0 && a->size() < static_cast<std::size_t>(rows)) throw std::out_of_range("a device array shorter than its rows");
+        check(jl_kv_attention_scored(ctx_, cache.handle(), q.at(rows, static_cast<std::int64_t>(heads_) * headDim_), heads_, q.stride, rows,
+                                     tables.positions.data(), tables.rowRequests.data(), tables.table.data(), tables.requests(),
+                                     tables.blocksPerRequest(), scale, window, scores.cap, scores.slopes ? scores.slopes->data() : nullptr,
+                                     scores.firstTokens ? scores.firstTokens->data() : nullptr,
+                                     scores.endTokens ? scores.endTokens->data() : nullptr, out, half, ldo, workspace_.ptr(),
+                                     workspace_.bytes()));
+    }
     void run(const PagedKvCache &cache, const FloatRows &q, std::int64_t rows, const BlockTables &tables, void *out, int half,
              std::int64_t ldo, float scale, std::int64_t window) const {
         if (cache.kvHeads() != kvHeads_ || cache.headDim() != headDim_) throw std::invalid_argument("a cache of another shape");
@@ -594,6 +623,47 @@ private:
     }
     jl_context *ctx_;
     int heads_, kvHeads_, headDim_;
+    DeviceBuffer workspace_;
+};
+
+// ---- log probabilities of the answer (jl_logprobs) ---------------------------------------------
+
+// Over rows of `vocab` logits, with the workspace that a call's workgroups join in.  Calls that may run at the same
+// time need one each.  top: how many of the most probable tokens a call lists.
+class LogProbabilities {
+public:
+    LogProbabilities(const Context &context, std::int64_t vocab, int top = 0)
+        : ctx_(context.handle()), vocab_(vocab), top_(top), workspace_(context, sizeOf(vocab, top)) {
+        check(jl_logprobs_workspace_init(ctx_, workspace_.ptr(), workspace_.bytes()));
+    }
+    // What is null is not computed.  tokens and logprobs: tokensPerRow of each row; entropy: one; the list: `top`.
+    void compute(const FloatRows &logits, std::int64_t rows, const IntArray *tokens, const FloatArray *logprobs,
+                 const FloatArray *entropy = nullptr, const IntArray *topTokens = nullptr, const FloatArray *topLogprobs = nullptr,
+                 std::int64_t tokensPerRow = 1, float scale = 1.f, float cap = 0.f) const {
+        if (!tokens != !logprobs || !topTokens != !topLogprobs) throw std::invalid_argument("one of two arrays that go together");
+        const std::int64_t per = tokens ? tokensPerRow : 0;
+        const int top = topTokens ? top_ : 0;
+        if (tokens) need(tokens->size(), rows * per), need(logprobs->size(), rows * per);
+        if (entropy) need(entropy->size(), rows);
+        if (topTokens) need(topTokens->size(), rows * top), need(topLogprobs->size(), rows * top);
+        check(jl_logprobs(ctx_, logits.at(rows, vocab_), rows, vocab_, logits.stride, scale, cap, tokens ? tokens->data() : nullptr, per,
+                          logprobs ? logprobs->data() : nullptr, entropy ? entropy->data() : nullptr, top,
+                          topTokens ? topTokens->data() : nullptr, topLogprobs ? topLogprobs->data() : nullptr, workspace_.ptr(),
+                          workspace_.bytes()));
+    }
+
+private:
+    static std::size_t sizeOf(std::int64_t vocab, int top) {
+        const std::size_t bytes = top <= vocab ? jl_logprobs_workspace_bytes(vocab, top) : 0;
+        if (!bytes) throw std::invalid_argument("no such vocabulary, or a list of more than 64 or of more than it has");
+        return bytes;
+    }
+    static void need(std::size_t size, std::int64_t count) {
+        if (count > 0 && size < static_cast<std::size_t>(count)) throw std::out_of_range("a device array shorter than its rows");
+    }
+    jl_context *ctx_;
+    std::int64_t vocab_;
+    int top_;
     DeviceBuffer workspace_;
 };
 
