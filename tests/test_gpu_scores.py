@@ -481,3 +481,31 @@ def test_fours_past_32_bit_offsets(ctx):
         pool[which, :, :, :8] = kept.reshape(5, 8, kv, dim).transpose(0, 2, 1, 3)
     check(out, *S.attend(pool, x[7::8, :heads], np.full(5, 7), None, np.arange(5).reshape(5, 1), dim ** -0.5, cap=30.0))
     cache.free()
+
+
+@pytest.mark.parametrize("rows", [9, 340])
+@pytest.mark.parametrize("kind", S.KINDS)
+def test_scored_rows_of_extreme_queries(ctx, kind, rows):
+    """Rows that go together, few and a prompt's block, each with scores of another size: thousands apart, all equal, below
+    binary16; one with an infinity and one with NaN in a head, which are those heads' alone."""
+    rng = np.random.default_rng(rows)
+    dim, page, kv, heads, n = 64, 16, 16, 32, 400
+    table, pages = K.make_tables(rng, [n], page)
+    raw = S.random_pool(rng, kind, pages, kv, dim, page)
+    positions, of = np.arange(n - rows, n), np.zeros(rows, int)
+    q = rng.standard_normal((rows, heads, dim)).astype(np.float32)
+    q *= np.array([1, 300, 0, 1e-9, 2.0 ** -140, 40], np.float32)[np.arange(rows) % 6, None, None]
+    q[7::6] *= np.exp(rng.uniform(-20, 5, (len(q[7::6]), heads, dim))).astype(np.float32)
+    cache = cache_of(ctx, kind, pages, kv, dim, page, raw)
+    pool = S.decode_pool(raw, kind, pages, kv, dim, page)
+    slopes = (2.0 ** (-8 * np.arange(1, heads + 1) / heads)).astype(np.float32)
+    for cap, m in ((0.0, slopes), (30.0, None), (5.0, slopes)):
+        say("attend scored extreme", kind, rows, cap)
+        clean = run(ctx, cache, q, positions, of, table, cap=cap, slopes=m, window=150)
+        check(clean, *S.attend(pool, q, positions, of, table, dim ** -0.5, 150, cap, m))
+        bad = q.copy()
+        bad[rows // 2, 5, 3], bad[rows // 3, 30, 60] = np.inf, np.nan
+        got = run(ctx, cache, bad, positions, of, table, cap=cap, slopes=m, window=150)
+        lost = np.zeros(got.shape[:2], bool)
+        lost[rows // 2, 5] = lost[rows // 3, 30] = True
+        assert np.array_equal(got[~lost], clean[~lost]) and not np.isfinite(got[rows // 3, 30]).any()
