@@ -23,6 +23,10 @@
 #include "jl_kv.h"
 #include "jl_math.h"
 
+// A product and a sum become one rounding where fmaf says so, and nowhere else: what a call leaves is the same whatever else it is
+// asked for, which is another kernel.
+#pragma clang fp contract(off)
+
 namespace {
 
 constexpr int kMostTop = JL_WAVE;                 // a lane each
@@ -49,6 +53,12 @@ struct LogprobsArgs {
     int parts, fours_each;        // parts of a row, and fours of a part: whole steps of a workgroup
     float scale, power;           // power: scale log2(e)
     float cap, one_over_cap;      // 0: none
+    // The quotient of jl_tanh_middle for logits of at most cap_middle, in powers of the logit's square: l (1 + ...) / (1 + ...) is
+    // the capped logit, with no product in front and none behind.
+    float cap_middle, over[3], under[3];
+    // ... and Lambert's fraction up to 9, which is off by 6.2e-8 of the value at 1, for those of at most cap_near (2048 rows of
+    // 32000, capped: as products around the longer one 69 us, as powers of the square 68, the shorter one 62).
+    float cap_near, near_over[2], near_under[2];
     const int32_t *tokens;
     int tokens_per_row;
     float *logprobs, *entropy;
@@ -174,8 +184,11 @@ struct Sums {
 };
 
 // W: keys that the list has room for, 16, 32 or 64; 0: there is none.
-template <int WAVES, int W>
-__global__ void __launch_bounds__(WAVES * JL_WAVE) jl_logprobs_kernel(LogprobsArgs p) {
+// CUT: rows are.  Where they are not there are many, and registers for eight waves a SIMD bring the workgroups of 2048 rows onto
+// the card at once (2048 rows of 32000, five alternatives: 76 -> 63 us, twenty: 80 -> 69; none, with nothing left of the
+// parts: 52 -> 49); where they are, that gains nothing and costs a few spilled registers (64 rows of 151936, twenty: 24.3 and 26.3).
+template <int WAVES, int W, bool CUT>
+__global__ void __launch_bounds__(WAVES * JL_WAVE, (WAVES > 1 && !CUT ? 8 : 1)) jl_logprobs_kernel(LogprobsArgs p) {
     constexpr bool TOP = W > 0;
     constexpr int kWide = TOP ? W : JL_WAVE, kLists = JL_WAVE / kWide;   // lists that a register holds
     __shared__ uint2 gathered[WAVES][TOP ? 5 * JL_WAVE : 1];             // value, place
@@ -183,8 +196,8 @@ __global__ void __launch_bounds__(WAVES * JL_WAVE) jl_logprobs_kernel(LogprobsAr
     __shared__ float sums_of[WAVES][3];
     __shared__ uint32_t arrived;
     const int tid = threadIdx.x, lane = tid % JL_WAVE, wave = __builtin_amdgcn_readfirstlane(tid / JL_WAVE);
-    const int64_t row = blockIdx.x / p.parts;
-    const int part = blockIdx.x % p.parts;
+    const int64_t row = CUT ? blockIdx.x / p.parts : blockIdx.x;
+    const int part = CUT ? blockIdx.x % p.parts : 0;
     const float *l = p.logits + row * p.stride;
     const int off = (int)((uintptr_t)l / 4 % 4);              // fours lie on 16-byte boundaries: the first begins this many before the row
     const int fours = (p.n + off + 3) / 4, end = min((part + 1) * p.fours_each, fours);
@@ -275,9 +288,23 @@ __global__ void __launch_bounds__(WAVES * JL_WAVE) jl_logprobs_kernel(LogprobsAr
 #pragma unroll
         for (int i = 1; i < 4 * kEach; i++) least = fminf(least, x[i]);
         // (one form of tanh where all of a step's are within its reach)
-        if (p.cap > 0.f && !__any(!(fmaxf(most, -least) * p.one_over_cap <= kTanhMiddle))) {
+        const float size = fmaxf(most, -least);
+        if (p.cap > 0.f && !__any(!(size <= p.cap_near))) {
 #pragma unroll
-            for (int i = 0; i < 4 * kEach; i++) x[i] = p.cap * jl_tanh_middle(x[i] * p.one_over_cap);
+            for (int i = 0; i < 4 * kEach; i++) {
+                const float z = x[i] * x[i];
+                const float over = fmaf(z, fmaf(z, p.near_over[1], p.near_over[0]), 1.f);
+                const float under = fmaf(z, fmaf(z, p.near_under[1], p.near_under[0]), 1.f);
+                x[i] *= over * __builtin_amdgcn_rcpf(under);
+            }
+        } else if (p.cap > 0.f && !__any(!(size <= p.cap_middle))) {
+#pragma unroll
+            for (int i = 0; i < 4 * kEach; i++) {
+                const float z = x[i] * x[i];
+                const float over = fmaf(z, fmaf(z, fmaf(z, p.over[2], p.over[1]), p.over[0]), 1.f);
+                const float under = fmaf(z, fmaf(z, fmaf(z, p.under[2], p.under[1]), p.under[0]), 1.f);
+                x[i] *= over * __builtin_amdgcn_rcpf(under);
+            }
         } else if (p.cap > 0.f) {
 #pragma unroll
             for (int i = 0; i < 4 * kEach; i++) x[i] = capped(p, x[i]);
@@ -321,7 +348,7 @@ __global__ void __launch_bounds__(WAVES * JL_WAVE) jl_logprobs_kernel(LogprobsAr
         }
     };
     join_waves();
-    if (p.parts > 1) {
+    if constexpr (CUT) {
         if (wave == 0) {
             Part *to = p.part + row * p.parts + part;
             if constexpr (TOP)
@@ -361,8 +388,8 @@ __global__ void __launch_bounds__(WAVES * JL_WAVE) jl_logprobs_kernel(LogprobsAr
     if (wave != 0) return;
 
     const float log_sum = logf(own.sum);
-    auto logprob = [&](float logit) { return own.sum == 0.f ? -INFINITY : (capped(p, logit) - own.most) * p.scale - log_sum; };
-    if (lane == 0 && p.entropy) p.entropy[row] = own.sum == 0.f ? 0.f : log_sum - own.weighted / own.sum * kLn2;
+    auto logprob = [&](float logit) { return own.sum == 0.f ? -INFINITY : fmaf(capped(p, logit) - own.most, p.scale, -log_sum); };
+    if (lane == 0 && p.entropy) p.entropy[row] = own.sum == 0.f ? 0.f : fmaf(own.weighted / own.sum, -kLn2, log_sum);
     for (int i = lane; i < p.tokens_per_row; i += JL_WAVE) {
         const int token = p.tokens[row * p.tokens_per_row + i];
         p.logprobs[row * p.tokens_per_row + i] = (unsigned)token < (unsigned)p.n ? logprob(l[token]) : 0.f;
@@ -381,13 +408,13 @@ constexpr size_t kWorkspaceBytes = kArrivedBytes + (size_t)kGroups * sizeof(Part
 
 bool aligned(const void *p, int to) { return ((uintptr_t)p & (to - 1)) == 0; }
 
-template <int WAVES>
+template <int WAVES, bool CUT>
 void launch(const LogprobsArgs &a, int64_t rows, hipStream_t stream) {
     const dim3 grid((unsigned)(rows * a.parts)), block(WAVES * JL_WAVE);
-    if (a.top > 32) hipLaunchKernelGGL((jl_logprobs_kernel<WAVES, 64>), grid, block, 0, stream, a);
-    else if (a.top > 16) hipLaunchKernelGGL((jl_logprobs_kernel<WAVES, 32>), grid, block, 0, stream, a);
-    else if (a.top > 0) hipLaunchKernelGGL((jl_logprobs_kernel<WAVES, 16>), grid, block, 0, stream, a);
-    else hipLaunchKernelGGL((jl_logprobs_kernel<WAVES, 0>), grid, block, 0, stream, a);
+    if (a.top > 32) hipLaunchKernelGGL((jl_logprobs_kernel<WAVES, 64, CUT>), grid, block, 0, stream, a);
+    else if (a.top > 16) hipLaunchKernelGGL((jl_logprobs_kernel<WAVES, 32, CUT>), grid, block, 0, stream, a);
+    else if (a.top > 0) hipLaunchKernelGGL((jl_logprobs_kernel<WAVES, 16, CUT>), grid, block, 0, stream, a);
+    else hipLaunchKernelGGL((jl_logprobs_kernel<WAVES, 0, CUT>), grid, block, 0, stream, a);
 }
 
 }  // namespace
@@ -435,6 +462,14 @@ int jl_logprobs(jl_context *ctx, const float *logits, int64_t rows, int64_t n, i
     LogprobsArgs a;
     a.logits = logits, a.stride = row_stride, a.n = (int)n;
     a.scale = scale, a.cap = cap, a.one_over_cap = cap > 0.f ? 1.f / cap : 0.f;
+    // (of a cap whose sixth power is a number and whose square's products are: else each logit on its own)
+    const double y = cap >= 1e-5f && cap <= 1e5f ? 1. / ((double)cap * cap) : 0.;
+    a.cap_middle = y > 0. ? kTanhMiddle * cap : 0.f;
+    a.over[0] = (float)(17325. / 135135. * y), a.over[1] = (float)(378. / 135135. * y * y), a.over[2] = (float)(y * y * y / 135135.);
+    a.under[0] = (float)(62370. / 135135. * y), a.under[1] = (float)(3150. / 135135. * y * y), a.under[2] = (float)(28. / 135135. * y * y * y);
+    a.cap_near = y > 0. ? cap : 0.f;
+    a.near_over[0] = (float)(105. / 945. * y), a.near_over[1] = (float)(y * y / 945.);
+    a.near_under[0] = (float)(420. / 945. * y), a.near_under[1] = (float)(15. / 945. * y * y);
     a.tokens = tokens, a.tokens_per_row = (int)tokens_per_row, a.logprobs = logprobs, a.entropy = entropy;
     a.top = top, a.top_tokens = top_tokens, a.top_logprobs = top_logprobs;
     a.power = scale * kLog2e;
@@ -443,7 +478,7 @@ int jl_logprobs(jl_context *ctx, const float *logits, int64_t rows, int64_t n, i
     const int64_t steps = ((n + 3 + 3) / 4 + waves * kStepFours - 1) / (waves * kStepFours);   // of a workgroup, in a row that begins between two fours
     a.parts = waves == 1 ? 1 : (int)std::max<int64_t>(std::min<int64_t>({steps, kMostParts, kGroups / rows}), 1);
     a.fours_each = (int)((steps + a.parts - 1) / a.parts) * waves * kStepFours;
-    waves == 1 ? launch<1>(a, rows, ctx->stream) : launch<4>(a, rows, ctx->stream);
+    waves == 1 ? launch<1, false>(a, rows, ctx->stream) : a.parts == 1 ? launch<4, false>(a, rows, ctx->stream) : launch<4, true>(a, rows, ctx->stream);
     JL_HIP(hipGetLastError());
     return JL_OK;
 }
