@@ -203,3 +203,19 @@ def test_logprobs_of_no_rows(ctx):
     one = LogProbabilities(ctx, 4, 100, 3)
     one.compute(ctx.float_array(100), 0, topTokens=ints(ctx, []), topLogprobs=ctx.float_array(1))
     ctx.sync()
+
+
+@pytest.mark.parametrize("rows", [3, 1030])
+@pytest.mark.parametrize("cap", [1e-30, 1e-6, 1e-4, 0.7, 30.0, 5e4, 1e6, 1e30])
+def test_logprobs_of_logits_around_a_cap(ctx, rows, cap):
+    """Logits of rows that are cut and that are not, within the cap, a few times as large, beyond; caps whose powers are no numbers."""
+    rng = np.random.default_rng(8)
+    n = 6000
+    reach = np.array([0.02, 0.99, 2.4, 7, 1000])[np.arange(rows) % 5, None]
+    top = min(cap, 1e30)
+    logits = (np.clip(rng.standard_normal((rows, n)) / 3, -1, 1) * reach * top).astype(np.float32)
+    logits[1::5, 100] = np.float32(top)
+    scale = float(np.float32(8 / cap)) if 1e-8 < cap < 1e8 else 1.0
+    say("logprobs around a cap", rows, cap)
+    tokens = rng.integers(0, n, (rows, 1))
+    check(logits, tokens, run(ctx, logits, tokens, 5, scale, cap), 5, scale, cap)
