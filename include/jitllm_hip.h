@@ -581,7 +581,7 @@ int jl_kv_read(jl_context *ctx, const jl_kv_cache *cache, const int32_t *slots, 
  *        requests >= rows).  Rows of one request may stand beside each other (a prompt's, a draft's):
  *        each reads its own range.  Where there are twice as many rows as requests, neighbours of one request
  *        whose ranges touch go through its pages together, as many as make up to 16 query heads of one head
- *        of k and v; each is what its own tokens make it, whatever the others read.
+ *        of k and v (up to 64 where rows are many, over 4-bit blocks and in jl_kv_attention_scored); each is what its own tokens make it, whatever the others read.
  *   out  fp32, or with out_f16 binary16 (rounded once, as the projections of jl_gemm_xf16 take it);
  *        `ldo` of its values between rows; 16-byte aligned, ldo a multiple of 4 (fp32) or 8 (binary16)
  *        and none of q's memory
