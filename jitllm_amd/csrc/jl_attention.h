@@ -43,9 +43,9 @@ struct JlScoredArgs : JlAttentionArgs {
 template <typename ARGS>
 inline constexpr bool kScored = std::is_same_v<ARGS, JlScoredArgs>;
 
-hipError_t jl_launch_attention_prompt_f16(const JlScoredArgs &a, int head_dim, int device, hipStream_t stream);
-hipError_t jl_launch_attention_prompt_q8(const JlScoredArgs &a, int head_dim, int device, hipStream_t stream);
-hipError_t jl_launch_attention_prompt_q4(const JlScoredArgs &a, int head_dim, int device, hipStream_t stream);
+hipError_t jl_launch_attention_prompt_f16(const JlScoredArgs &a, int head_dim, int compute_units, int device, hipStream_t stream);
+hipError_t jl_launch_attention_prompt_q8(const JlScoredArgs &a, int head_dim, int compute_units, int device, hipStream_t stream);
+hipError_t jl_launch_attention_prompt_q4(const JlScoredArgs &a, int head_dim, int compute_units, int device, hipStream_t stream);
 hipError_t jl_launch_attention_f16(const JlAttentionArgs &a, int head_dim, int compute_units, hipStream_t stream);
 hipError_t jl_launch_attention_q8(const JlAttentionArgs &a, int head_dim, int compute_units, hipStream_t stream);
 hipError_t jl_launch_attention_q4(const JlAttentionArgs &a, int head_dim, int compute_units, hipStream_t stream);

@@ -10,9 +10,9 @@ namespace {
 constexpr size_t kArrivedBytes = kAttentionMostGroups * sizeof(uint32_t);
 constexpr size_t kTakenBytes = 32768;             // a byte for each block of rows, two rows at least
 // (Row block, head of k and v) pairs to a compute unit from which rows go in blocks: each is a workgroup's, whole, and the other
-// kernel cuts what it has among all.  (4-bit cache, 8 query heads over 4 of 128: 700 rows of one request, 88 pairs: 25.5 us in
-// blocks, 21.6 without; 1400, 176 pairs: 44.0 and 52.5; 4 requests of 175 ... 700, 220 pairs: 28.9 and 39.9.  32 over 8, after
-// 30 000 tokens: 128 rows, 64 pairs: 727 and 308; 512, 256 pairs, binary16: 750 and 1062.)
+// kernel cuts what it has among all.  (4-bit cache, 8 query heads over 4 of 128: 700 rows of one request, 88 pairs: 22.7 us in
+// blocks, 21.0 without; 1400, 176 pairs: 34.6 and 52.5; 4 requests of 175 ... 700, 220 pairs: 27.1 and 39.9.  32 over 8: 256 rows
+// after 4000 tokens, 128 pairs: 83 and 70; 512 after 30 000, 256 pairs, binary16: 570 and 1062.)
 constexpr float kPromptShare = 0.625f;
 
 bool aligned(const void *p, int to) { return ((uintptr_t)p & (to - 1)) == 0; }
@@ -92,7 +92,7 @@ int attention(const char *who, jl_context *ctx, const jl_kv_cache *cache, const 
         if (prompts) {
             JL_HIP((cache->type == JL_KV_Q8_0   ? jl_launch_attention_prompt_q8
                     : cache->type == JL_KV_Q4_0 ? jl_launch_attention_prompt_q4
-                                                : jl_launch_attention_prompt_f16)(a, dim, ctx->device, ctx->stream));
+                                                : jl_launch_attention_prompt_f16)(a, dim, ctx->compute_units, ctx->device, ctx->stream));
             a.taken = a.taken_out;
         }
         JL_HIP((cache->type == JL_KV_Q8_0   ? jl_launch_attention_scored_q8

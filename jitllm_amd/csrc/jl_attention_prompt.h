@@ -4,8 +4,8 @@
 // query head) each, and take the tokens in turn: every 16 columns read all tokens.  Here a workgroup has 64 columns, 16 a
 // wave, that go through the same tokens.  Two tiles of 32 tokens at a time, each wave loads a half of one, decodes it, turns v
 // as the second product wants it, and leaves the matrix instructions' operands in LDS, as they are; all waves then
-// take both tiles from there, while the next two go on to the other buffer and two more are on their way.  What a tile costs to load and decode is paid once for 64
-// columns.
+// take both tiles from there, while the next two go on to the other buffer and two more are on their way.  What a tile costs to
+// load and decode is paid once for 64 columns.
 //
 // Bound: the matrix instructions, four for a 16 x 16 x 32 piece (q and P are two binary16 parts each), and, as much, the
 // powers and conversions of P.
@@ -20,13 +20,18 @@
 namespace {
 
 constexpr int kLongRun = 32;                      // tiles of a run that has to have a quarter of the block's rows
-constexpr int kTilesAtATime = kWaves / kHalves;
+constexpr int kColumnWaves = 4, kTilesAtATime = 2;   // waves beside each other, and the tiles that one takes at a time
 
-template <int DIM>
+// WAVES: four, or eight, the second four of which take every other two tiles, and are joined with the first through LDS: where there are
+// no more workgroups than compute units, each of which would have one wave a SIMD (4-bit cache, 8 query heads over 4 of 128: 1400
+// rows of a prompt, 176 workgroups, 44.0 -> 34.6 us; 4 prompts of 175 ... 700 with a cap and a prefix, 220, 42.3 -> 37.6; 512 rows after
+// 30 000 tokens, 32 over 8, binary16, 256: 750 -> 570).  Their LDS holds up to 128 values a head.
+template <int DIM, int WAVES>
 struct PromptShape {
     static constexpr int kFragments = DIM / 16 + DIM / 16;                 // of a tile, 1 KB each: k's, v's
-    static constexpr int kBufferBytes = kTilesAtATime * kFragments * 1024, kLdsBytes = 2 * kBufferBytes;
-    static constexpr int kPerUnit = DIM <= 128 ? 2 : 1;
+    static constexpr int kTilesStaged = WAVES / kHalves;                   // a half by each wave
+    static constexpr int kBufferBytes = kTilesStaged * kFragments * 1024, kLdsBytes = 2 * kBufferBytes;
+    static constexpr int kWavesASimd = DIM <= 128 ? 2 : 1;
 };
 
 // over the sixteen lanes of a row of lanes, and over all, in all of them
@@ -44,12 +49,15 @@ __device__ __forceinline__ int over_lanes_min(int x) {
     return min((int)h[0], (int)h[1]);
 }
 
-template <int TYPE, int DIM>
-__global__ void __launch_bounds__(kThreads, PromptShape<DIM>::kPerUnit) jl_kv_attention_prompt_kernel(JlScoredArgs p) {
-    constexpr int kSteps = DIM / 32, kBlocks = DIM / 16, kFragments = PromptShape<DIM>::kFragments;
-    extern __shared__ __align__(16) uint8_t fragments[];       // [2][kTilesAtATime][kFragments][64 lanes][16 bytes]
-    __shared__ int half_info[2][kWaves];
+template <int TYPE, int DIM, int WAVES>
+__global__ void __launch_bounds__(WAVES * JL_WAVE, (PromptShape<DIM, WAVES>::kWavesASimd)) jl_kv_attention_prompt_kernel(JlScoredArgs p) {
+    typedef PromptShape<DIM, WAVES> Its;
+    constexpr int kSteps = DIM / 32, kBlocks = DIM / 16, kFragments = Its::kFragments, kTilesStaged = Its::kTilesStaged;
+    extern __shared__ __align__(16) uint8_t fragments[];       // [2][kTilesStaged][kFragments][64 lanes][16 bytes]
+    __shared__ int half_info[2][WAVES];
     const int tid = threadIdx.x, lane = tid % JL_WAVE, wave = uniform(tid / JL_WAVE);
+    const int column_wave = WAVES > kColumnWaves ? wave % kColumnWaves : wave;
+    const int own_tiles = WAVES > kColumnWaves ? wave / kColumnWaves * kTilesAtATime : 0;   // of those that are staged
     const int g = lane / 16, m = lane % 16;
     const int kv_heads = p.cache.kv_heads, kv_head = blockIdx.x % kv_heads;
     const int block = gridDim.x / kv_heads - 1 - blockIdx.x / kv_heads;    // (the last rows first: a prompt's longest)
@@ -114,7 +122,7 @@ __global__ void __launch_bounds__(kThreads, PromptShape<DIM>::kPerUnit) jl_kv_at
         // what was loaded, into a buffer; a half behind the last tile, or with no page, as tokens that nobody sees
         auto stage = [&](auto which, int t) {
             constexpr int W = decltype(which)::value;
-            const int token0 = t * kTile + 16 * its_half;
+            const int token0 = min(t, tile_end) * kTile + 16 * its_half;
             if (token0 < run.first || token0 + 16 > run.end || !paged[W]) {
                 bool seen[1][4];
 #pragma unroll
@@ -123,7 +131,7 @@ __global__ void __launch_bounds__(kThreads, PromptShape<DIM>::kPerUnit) jl_kv_at
             }
             const bool bad = __any(raw[W].any_not_finite());
             if (lane == 0) half_info[W][wave] = (paged[W] ? 1 : 0) | (bad ? 2 : 0);
-            uint8_t *to_fragment = fragments + W * PromptShape<DIM>::kBufferBytes + its_tile * (kFragments * 1024) + lane * 16;
+            uint8_t *to_fragment = fragments + W * Its::kBufferBytes + its_tile * (kFragments * 1024) + lane * 16;
 #pragma unroll
             for (int s = 0; s < kSteps; s++) *(jl_half8 *)(to_fragment + (its_half * kSteps + s) * 1024) = raw[W].k_operand(0, s);
 #pragma unroll
@@ -137,11 +145,11 @@ __global__ void __launch_bounds__(kThreads, PromptShape<DIM>::kPerUnit) jl_kv_at
         const std::integral_constant<int, 0> even{};
         const std::integral_constant<int, 1> odd{};
         issue(even, tile_begin + its_tile);
-        issue(odd, tile_begin + kTilesAtATime + its_tile);
+        issue(odd, tile_begin + kTilesStaged + its_tile);
 
         // ---- this wave's columns: the query heads of one row after the other; lanes past the last one double it
-        const bool works = wave * 16 < columns;
-        const int column = min(wave * 16 + m, columns - 1), in_run = column / p.group;
+        const bool works = column_wave * 16 < columns;
+        const int column = min(column_wave * 16 + m, columns - 1), in_run = column / p.group;
         const int row = row0 + from + in_run, head = kv_head * p.group + column - in_run * p.group;
         const int position = __shfl(position_in_lane, from + in_run, JL_WAVE);
         const int first_seen = __shfl(in_lane.first, from + in_run, JL_WAVE), end_seen = __shfl(in_lane.end, from + in_run, JL_WAVE);
@@ -172,18 +180,19 @@ __global__ void __launch_bounds__(kThreads, PromptShape<DIM>::kPerUnit) jl_kv_at
 
         __syncthreads();                                      // (all have read what the run before left)
         stage(even, tile_begin + its_tile);
-        issue(even, tile_begin + 2 * kTilesAtATime + its_tile);
-        auto step = [&](auto which, auto other, int base) {
+        issue(even, tile_begin + 2 * kTilesStaged + its_tile);
+        auto step = [&](auto which, auto other, int staged) {
+            const int base = staged + own_tiles;              // this wave's two
             constexpr int buffer = decltype(which)::value;
             __syncthreads();                                  // (this buffer is written, and the other one read, by all)
-            const uint8_t *fragment = fragments + buffer * PromptShape<DIM>::kBufferBytes + lane * 16;
+            const uint8_t *fragment = fragments + buffer * Its::kBufferBytes + own_tiles * (kFragments * 1024) + lane * 16;
             auto operand = [&](int i) { return *(const jl_half8 *)(fragment + (i / (2 * kBlocks) * kFragments + i % (2 * kBlocks)) * 1024); };
             int info = 0, bad = 0;                            // bit i: half i has a page; one has values that are not finite
 #pragma unroll
-            for (int i = 0; i < kWaves; i++) {
-                const int its = uniform(half_info[buffer][i]);
-                info |= (its & 1) << i, bad |= its & 2;
-            }
+            for (int i = 0; i < WAVES; i++) bad |= half_info[buffer][i];
+            bad = uniform(bad) & 2;
+#pragma unroll
+            for (int i = 0; i < kTilesAtATime * kHalves; i++) info |= (uniform(half_info[buffer][own_tiles * kHalves + i]) & 1) << i;
             const bool reads = works && base * kTile < any_end && (base + kTilesAtATime) * kTile > any_first;
             auto sees = [&](int i) {                          // token i of the lane's sixteen
                 const int token = base * kTile + i / 4 * 16 + 4 * g + i % 4;
@@ -210,7 +219,7 @@ __global__ void __launch_bounds__(kThreads, PromptShape<DIM>::kPerUnit) jl_kv_at
                     }
                 }
                 __syncthreads();
-                uint8_t *own_half = fragments + buffer * PromptShape<DIM>::kBufferBytes + its_tile * (kFragments * 1024) + lane * 16 + 8 * its_half;
+                uint8_t *own_half = fragments + buffer * Its::kBufferBytes + its_tile * (kFragments * 1024) + lane * 16 + 8 * its_half;
 #pragma unroll 1
                 for (int b = 0; b < kBlocks; b++) {
                     uintx2 *at = (uintx2 *)(own_half + (kBlocks + b) * 1024);
@@ -246,7 +255,7 @@ __global__ void __launch_bounds__(kThreads, PromptShape<DIM>::kPerUnit) jl_kv_at
 #pragma unroll
                 for (int i = 0; i < kAhead; i++) v[0][i] = value_operand(i);
                 __builtin_amdgcn_sched_barrier(0);
-                const bool all_seen = base * kTile >= all_first && (base + kTilesAtATime) * kTile <= all_end && info == (1 << kWaves) - 1;
+                const bool all_seen = base * kTile >= all_first && (base + kTilesAtATime) * kTile <= all_end && info == (1 << kTilesAtATime * kHalves) - 1;
                 const bool shaped = p.cap > 0.f || p.slopes;
                 const float unit = shaped ? 1.f : undo;       // of a score, in powers of two
                 float x[kTilesAtATime][8];
@@ -299,18 +308,41 @@ __global__ void __launch_bounds__(kThreads, PromptShape<DIM>::kPerUnit) jl_kv_at
                         }
                 }
             }
-            if (base + kTilesAtATime < tile_end) {
-                stage(other, base + kTilesAtATime + its_tile);
-                issue(other, base + 3 * kTilesAtATime + its_tile);
+            if (staged + kTilesStaged < tile_end) {
+                stage(other, staged + kTilesStaged + its_tile);
+                issue(other, staged + 3 * kTilesStaged + its_tile);
             }
         };
-        for (int base = tile_begin; base < tile_end; base += 2 * kTilesAtATime) {
+        for (int base = tile_begin; base < tile_end; base += 2 * kTilesStaged) {
             step(even, odd, base);
-            if (base + kTilesAtATime < tile_end) step(odd, even, base + kTilesAtATime);
+            if (base + kTilesStaged < tile_end) step(odd, even, base + kTilesStaged);
+        }
+        if constexpr (WAVES > kColumnWaves) {
+            // the second four waves' parts, through LDS, to the first ones
+            float *joined = (float *)fragments + column_wave * ((4 * kBlocks + 2) * JL_WAVE) + lane;
+            __syncthreads();
+            if (own_tiles > 0 && works) {
+#pragma unroll
+                for (int b = 0; b < kBlocks; b++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) joined[(4 * b + i) * JL_WAVE] = o[b][i];
+                joined[4 * kBlocks * JL_WAVE] = top, joined[(4 * kBlocks + 1) * JL_WAVE] = sum;
+            }
+            __syncthreads();
+            if (own_tiles > 0) continue;
+            if (works) {
+                const float its_top = joined[4 * kBlocks * JL_WAVE], most = fmaxf(top, its_top);
+                const float keep = __builtin_amdgcn_exp2f(top - most), share = __builtin_amdgcn_exp2f(its_top - most);
+                sum = keep * sum + share * joined[(4 * kBlocks + 1) * JL_WAVE];
+#pragma unroll
+                for (int b = 0; b < kBlocks; b++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) o[b][i] = keep * o[b][i] + share * joined[(4 * b + i) * JL_WAVE];
+            }
         }
         if (!works) continue;
         const float l = over_groups_sum(sum);
-        if (wave * 16 + m >= columns) continue;
+        if (column_wave * 16 + m >= columns) continue;
         const int64_t at = row * p.ldo + (int64_t)head * DIM;
         auto put = [&](int element, floatx4 v) { store_out(p, at + element, l == 0.f ? floatx4{0.f, 0.f, 0.f, 0.f} : v / l); };
         constexpr int wide = DIM / 128, mid = DIM % 128 / 64, thin = DIM % 64 / 32;
@@ -330,25 +362,31 @@ __global__ void __launch_bounds__(kThreads, PromptShape<DIM>::kPerUnit) jl_kv_at
     }
 }
 
-template <int TYPE, int DIM>
-hipError_t launch_prompt(const JlScoredArgs &a, int device, hipStream_t stream) {
-    constexpr int lds = PromptShape<DIM>::kLdsBytes;
+template <int TYPE, int DIM, int WAVES>
+hipError_t launch_prompt_waves(const JlScoredArgs &a, unsigned groups, int device, hipStream_t stream) {
+    constexpr int lds = PromptShape<DIM, WAVES>::kLdsBytes;
     if (lds > 60 * 1024) {
         static jl_lds_limit_flags raised;
-        if (jl_raise_lds_limit(raised, device, (const void *)jl_kv_attention_prompt_kernel<TYPE, DIM>, lds) != JL_OK) return hipErrorInvalidValue;
+        if (jl_raise_lds_limit(raised, device, (const void *)jl_kv_attention_prompt_kernel<TYPE, DIM, WAVES>, lds) != JL_OK) return hipErrorInvalidValue;
     }
-    const unsigned groups = (unsigned)((a.rows + a.taken_rows - 1) / a.taken_rows) * a.cache.kv_heads;
-    hipLaunchKernelGGL((jl_kv_attention_prompt_kernel<TYPE, DIM>), dim3(groups), dim3(kThreads), lds, stream, a);
+    hipLaunchKernelGGL((jl_kv_attention_prompt_kernel<TYPE, DIM, WAVES>), dim3(groups), dim3(WAVES * JL_WAVE), lds, stream, a);
     return hipGetLastError();
 }
+template <int TYPE, int DIM>
+hipError_t launch_prompt(const JlScoredArgs &a, int compute_units, int device, hipStream_t stream) {
+    const unsigned groups = (unsigned)((a.rows + a.taken_rows - 1) / a.taken_rows) * a.cache.kv_heads;
+    if constexpr (DIM <= 128)
+        if (groups <= (unsigned)compute_units) return launch_prompt_waves<TYPE, DIM, 8>(a, groups, device, stream);
+    return launch_prompt_waves<TYPE, DIM, 4>(a, groups, device, stream);
+}
 template <int TYPE>
-hipError_t launch_prompt_dim(const JlScoredArgs &a, int head_dim, int device, hipStream_t stream) {
+hipError_t launch_prompt_dim(const JlScoredArgs &a, int head_dim, int compute_units, int device, hipStream_t stream) {
     switch (head_dim) {
-        case 64: return launch_prompt<TYPE, 64>(a, device, stream);
-        case 96: return launch_prompt<TYPE, 96>(a, device, stream);
-        case 128: return launch_prompt<TYPE, 128>(a, device, stream);
-        case 192: return launch_prompt<TYPE, 192>(a, device, stream);
-        default: return launch_prompt<TYPE, 256>(a, device, stream);
+        case 64: return launch_prompt<TYPE, 64>(a, compute_units, device, stream);
+        case 96: return launch_prompt<TYPE, 96>(a, compute_units, device, stream);
+        case 128: return launch_prompt<TYPE, 128>(a, compute_units, device, stream);
+        case 192: return launch_prompt<TYPE, 192>(a, compute_units, device, stream);
+        default: return launch_prompt<TYPE, 256>(a, compute_units, device, stream);
     }
 }
 

@@ -273,7 +273,12 @@ PROMPTS = [
     ([(0, 0, 300)] + [(1 + r, 1000 + 13 * r, 1) for r in range(40)] + [(-1, 5, 30)], 41, 32, 8, 64, 64, "q4", 0, False, 0.0, False, False, 0),
     ([(r, 11 * r, 9) for r in range(60)], 60, 16, 8, 64, 16, "f16", 0, False, 0.0, True, False, 0), ([(0, 50, 620)], 1, 7, 7, 128, 16, "q4", 200, True, 5.0, False, False, 0),
     ([(0, 0, 330), (1, 700, 90)], 2, 14, 7, 192, 16, "q8", 0, False, 0.0, False, True, 0), ([(0, 0, 130), (1, 0, 75)], 2, 48, 16, 256, 32, "f16", 64, False, 50.0, False, False, 40),
-    ([(0, 0, 90)], 1, 96, 4, 256, 16, "q4", 0, False, 0.0, True, False, 60), ([(0, 10, 1300), (-1, 0, 2400), (1, 0, 400)], 2, 32, 1, 64, 16, "f16", 30, False, 0.0, True, False, 0)]
+    ([(0, 0, 90)], 1, 96, 4, 256, 16, "q4", 0, False, 0.0, True, False, 60), ([(0, 10, 1300), (-1, 0, 2400), (1, 0, 400)], 2, 32, 1, 64, 16, "f16", 30, False, 0.0, True, False, 0),
+    # ... and enough that there are several workgroups to a compute unit
+    ([(0, 0, 500), (1, 300, 250)], 2, 32, 8, 128, 16, "q4", 0, False, 30.0, False, False, 64), ([(0, 0, 300), (1, 700, 333), (2, 3, 70)], 3, 24, 8, 96, 16, "q8", 100, True, 20.0, True, True, 0),
+    ([(0, 0, 1100)], 1, 16, 8, 64, 32, "q8", 0, False, 0.0, False, False, 0), ([(0, 50, 520), (-1, 5, 30), (1, 0, 90)], 2, 28, 7, 128, 16, "f16", 0, False, 8.0, True, False, 0),
+    ([(0, 0, 300), (1, 60, 120)], 2, 48, 12, 96, 16, "f16", 70, False, 0.0, False, True, 0), ([(0, 0, 600)], 1, 32, 16, 96, 64, "q4", 0, True, 0.0, False, False, 0),
+    ([(0, 9, 600), (1, 0, 50)], 2, 32, 16, 64, 16, "q4", 0, False, 50.0, True, False, 0), ([(0, 0, 560)], 1, 32, 8, 128, 128, "q8", 0, False, 0.0, True, False, 30)]
 
 
 @pytest.mark.parametrize("runs,requests,heads,kv,dim,page,kind,window,half,cap,slopes,documents,prefix", PROMPTS)
@@ -281,12 +286,12 @@ def test_attend_prompts(ctx, runs, requests, heads, kv, dim, page, kind, window,
     test_attend_scored(ctx, runs, requests, heads, kv, dim, page, kind, window, half, cap, slopes, documents, prefix)
 
 
-@pytest.mark.parametrize("kind", S.KINDS)
-def test_attend_prompts_of_values_that_are_not_finite(ctx, kind):
+@pytest.mark.parametrize("kind,kv", [(kind, kv) for kv in (4, 8) for kind in S.KINDS])
+def test_attend_prompts_of_values_that_are_not_finite(ctx, kind, kv):
     """Infinities, NaN and, in four bits, a scale that takes its multiples past binary16, at tokens that some rows of a block
     see: those may get NaN, the others are what they are without; and pages outside the cache."""
     rng = np.random.default_rng(21)
-    heads, kv, dim, page, rows = 4, 4, 64, 16, 3000
+    heads, dim, page, rows = kv, 64, 16, 3000
     table, pages = K.make_tables(rng, [rows], page)
     table[0, 7], table[0, 100] = -1, pages
     raw = S.random_pool(rng, kind, pages, kv, dim, page)
@@ -304,7 +309,7 @@ def test_attend_prompts_of_values_that_are_not_finite(ctx, kind):
     cache = cache_of(ctx, kind, pages, kv, dim, page, dirty.reshape(-1))
     q = rng.standard_normal((rows, heads, dim)).astype(np.float32)
     positions, of = np.arange(rows), np.zeros(rows, int)
-    say("attend prompts not finite", kind)
+    say("attend prompts not finite", kind, kv)
     window = 20
     got = run(ctx, cache, q, positions, of, table, window, cap=20.0)
     hit = np.array([any(i - window < t <= i for t in bad_tokens) for i in range(rows)])
