@@ -136,10 +136,10 @@ __global__ void __launch_bounds__(WAVES * JL_WAVE, (PromptShape<DIM, WAVES>::kWa
             for (int s = 0; s < kSteps; s++) *(jl_half8 *)(to_fragment + (its_half * kSteps + s) * 1024) = raw[W].k_operand(0, s);
 #pragma unroll
             for (int b = 0; b < kBlocks; b += 2) {
-                uint32_t v[2][2];
+                uintx2 v[2];
                 raw[W].v_pairs(b, v);
 #pragma unroll
-                for (int c = 0; c < 2; c++) *(uintx2 *)(to_fragment + (kBlocks + b + c) * 1024 + 8 * its_half) = uintx2{v[c][0], v[c][1]};
+                for (int c = 0; c < 2; c++) *(uintx2 *)(to_fragment + (kBlocks + b + c) * 1024 + 8 * its_half) = v[c];
             }
         };
         const std::integral_constant<int, 0> even{};
@@ -175,7 +175,8 @@ __global__ void __launch_bounds__(WAVES * JL_WAVE, (PromptShape<DIM, WAVES>::kWa
 #pragma unroll
                     for (int i = 0; i < 4; i++) most = fmaxf(most, fabsf(x[s][e][i]));
                 }
-            split_q<TYPE, DIM>(x, over_groups_max(most), q_hi, q_lo, undo);
+            most = over_groups_max(most);
+            JL_SPLIT_Q(TYPE, DIM, x, most, q_hi, q_lo, undo);
         }
 
         __syncthreads();                                      // (all have read what the run before left)
