@@ -20,12 +20,16 @@
 namespace {
 
 constexpr int kLongRun = 32;                      // tiles of a run that has to have a quarter of the block's rows
+constexpr int kLongPrompt = 2000;                 // rows a request
 constexpr int kColumnWaves = 4, kTilesAtATime = 2;   // waves beside each other, and the tiles that one takes at a time
 
 // WAVES: four, or eight, the second four of which take every other two tiles, and are joined with the first through LDS: where there are
 // no more workgroups than compute units, each of which would have one wave a SIMD (4-bit cache, 8 query heads over 4 of 128: 1400
 // rows of a prompt, 176 workgroups, 44.0 -> 34.6 us; 4 prompts of 175 ... 700 with a cap and a prefix, 220, 42.3 -> 37.6; 512 rows after
-// 30 000 tokens, 32 over 8, binary16, 256: 750 -> 570).  Their LDS holds up to 128 values a head.
+// 30 000 tokens, 32 over 8, binary16, 256: 750 -> 570); and up to twice as many of prompts of kLongPrompt rows or more, the last of whose
+// blocks would else go on alone (8 heads over 4 of 128, 2400 rows, 300: 73 -> 57; 4096, 512: 115 -> 97; 16 over 8 of 64, 2000 rows,
+// 504: 46 -> 42; but 900 rows of 32 over 8, 456: 34.5 and 36.1, 8 prompts of 512, 512: 29.9 and 36.1, 3200 with a window of 300, 400: 26.4
+// and 33.6).  Their LDS holds up to 128 values a head.
 template <int DIM, int WAVES>
 struct PromptShape {
     static constexpr int kFragments = DIM / 16 + DIM / 16;                 // of a tile, 1 KB each: k's, v's
@@ -376,8 +380,9 @@ hipError_t launch_prompt_waves(const JlScoredArgs &a, unsigned groups, int devic
 template <int TYPE, int DIM>
 hipError_t launch_prompt(const JlScoredArgs &a, int compute_units, int device, hipStream_t stream) {
     const unsigned groups = (unsigned)((a.rows + a.taken_rows - 1) / a.taken_rows) * a.cache.kv_heads;
+    const bool long_runs = a.window == 0 && !a.first_tokens && kLongPrompt * (int64_t)a.requests <= a.rows;
     if constexpr (DIM <= 128)
-        if (groups <= (unsigned)compute_units) return launch_prompt_waves<TYPE, DIM, 8>(a, groups, device, stream);
+        if (groups <= (unsigned)compute_units * (long_runs ? 2 : 1)) return launch_prompt_waves<TYPE, DIM, 8>(a, groups, device, stream);
     return launch_prompt_waves<TYPE, DIM, 4>(a, groups, device, stream);
 }
 template <int TYPE>

@@ -278,6 +278,7 @@ PROMPTS = [
     ([(0, 0, 500), (1, 300, 250)], 2, 32, 8, 128, 16, "q4", 0, False, 30.0, False, False, 64), ([(0, 0, 300), (1, 700, 333), (2, 3, 70)], 3, 24, 8, 96, 16, "q8", 100, True, 20.0, True, True, 0),
     ([(0, 0, 1100)], 1, 16, 8, 64, 32, "q8", 0, False, 0.0, False, False, 0), ([(0, 50, 520), (-1, 5, 30), (1, 0, 90)], 2, 28, 7, 128, 16, "f16", 0, False, 8.0, True, False, 0),
     ([(0, 0, 300), (1, 60, 120)], 2, 48, 12, 96, 16, "f16", 70, False, 0.0, False, True, 0), ([(0, 0, 600)], 1, 32, 16, 96, 64, "q4", 0, True, 0.0, False, False, 0),
+    ([(0, 0, 2100)], 1, 8, 4, 64, 16, "q8", 0, False, 25.0, False, False, 100), ([(0, 30, 2050)], 1, 8, 4, 128, 64, "q4", 0, True, 0.0, False, False, 0),
     ([(0, 9, 600), (1, 0, 50)], 2, 32, 16, 64, 16, "q4", 0, False, 50.0, True, False, 0), ([(0, 0, 560)], 1, 32, 8, 128, 128, "q8", 0, False, 0.0, True, False, 30)]
 
 
